@@ -145,6 +145,14 @@ _DNN = {
                                        c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]),
     "grxdnnSetCycleProbe": (c_int, [c_void_p, c_void_p, c_int]),
     "grxdnnAttentionCycleSlotsNeeded": (c_int, [c_void_p, c_int, c_int, c_int]),
+    "grxdnnPagedCacheAppend": (c_int, [c_void_p] * 13),
+    "grxdnnPagedAttentionGetWorkspaceSize": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+                                                     POINTER(c_size_t)]),
+    "grxdnnPagedAttentionForward": (c_int, [c_void_p] * 11 + [c_float] + [c_void_p] * 5 + [c_size_t]),
+    "grxdnnPagedCacheEvict": (c_int, [c_void_p] * 10 + [c_int, c_int] + [c_void_p] * 6),
+    "grxdnnTokenLogProbGetWorkspaceSize": (c_int, [c_void_p, c_void_p, c_int, POINTER(c_size_t)]),
+    "grxdnnTokenLogProbForward": (c_int, [c_void_p] * 7 + [c_int, c_void_p, c_void_p, c_void_p, c_size_t]),
+    "grxdnnTokenLogProbBackward": (c_int, [c_void_p] * 10),
 }
 EXPORTS = {"libgrxrt.so": _RT, "libgrxblas.so": _BLAS, "libgrxdnn.so": _DNN}
 
@@ -384,6 +392,41 @@ class Dnn:
 
     def gelu(self, mode: int, xd, x, yd, y) -> int:
         return self.L.grxdnnGeluForward(self.h, mode, xd.d, x, yd.d, y)
+
+    def paged_append(self, kd, k, vd, v, kcd, kc, vcd, vc, td, table, lengths, counts=None) -> int:
+        return self.L.grxdnnPagedCacheAppend(self.h, kd.d, k, vd.d, v, kcd.d, kc, vcd.d, vc, td.d, table,
+                                             lengths, counts)
+
+    def paged_attention_workspace(self, qd, kcd, td, wd=None) -> int:
+        n = c_size_t(0)
+        check(self.L.grxdnnPagedAttentionGetWorkspaceSize(self.h, qd.d, kcd.d, td.d, wd.d if wd else None,
+                                                          ctypes.byref(n)), "paged attention workspace")
+        return n.value
+
+    def paged_attention(self, ad, qd, q, kcd, kc, vcd, vc, td, table, lengths, decay, wd, w, od, o, ws,
+                        ws_bytes) -> int:
+        """wd and w: None where no weights are accumulated."""
+        return self.L.grxdnnPagedAttentionForward(self.h, ad.d, qd.d, q, kcd.d, kc, vcd.d, vc, td.d, table,
+                                                  lengths, decay, wd.d if wd else None, w, od.d, o, ws, ws_bytes)
+
+    def paged_evict(self, kcd, kc, vcd, vc, td, table, lengths, wd, w, budget, recent, kept, ntd, new_table,
+                    new_lengths, nwd, new_w) -> int:
+        return self.L.grxdnnPagedCacheEvict(self.h, kcd.d, kc, vcd.d, vc, td.d, table, lengths, wd.d, w, budget,
+                                            recent, kept, ntd.d, new_table, new_lengths, nwd.d, new_w)
+
+    def token_logprob_workspace(self, xd, top: int) -> int:
+        n = c_size_t(0)
+        check(self.L.grxdnnTokenLogProbGetWorkspaceSize(self.h, xd.d, top, ctypes.byref(n)),
+              "token logprob workspace")
+        return n.value
+
+    def token_logprob(self, xd, x, tokens, logprob, lse, entropy, top, top_logprob, top_index, ws, ws_bytes) -> int:
+        return self.L.grxdnnTokenLogProbForward(self.h, xd.d, x, tokens, logprob, lse, entropy, top, top_logprob,
+                                                top_index, ws, ws_bytes)
+
+    def token_logprob_backward(self, xd, x, tokens, lse, entropy, dlogprob, dentropy, dxd, dx) -> int:
+        return self.L.grxdnnTokenLogProbBackward(self.h, xd.d, x, tokens, lse, entropy, dlogprob, dentropy, dxd.d,
+                                                 dx)
 
 
 class Stream:

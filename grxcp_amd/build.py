@@ -6,7 +6,8 @@ Outputs, next to this file in ``lib/``:
 
 * ``libgrxrt.so``   runtime subset over HIP (grx_runtime.h)
 * ``libgrxblas.so`` grxBLAS host library + GEMM / level-1/2 kernels (grxblas.h)
-* ``libgrxdnn.so``  grxDNN host library + norm / attention kernels (grxdnn.h)
+* ``libgrxdnn.so``  grxDNN host library + norm / softmax / attention / paged-cache /
+  log-probability kernels (grxdnn.h)
 
 Host ``.cpp`` files are compiled with g++ against the HIP runtime API headers;
 ``.hip`` kernel files with ``hipcc --offload-arch=gfx950``. Every HIP
@@ -47,7 +48,8 @@ LIBS = {
     "libgrxblas.so": (["grxblas.cpp", "kernels/gemm_mfma.hip", "kernels/sgemm.hip",
                        "kernels/noalloc_scratch.hip"], ["grxrt"]),
     "libgrxdnn.so": (["grxdnn.cpp", "kernels/norms.hip", "kernels/softmax_gelu.hip",
-                      "kernels/attention.hip"], ["grxrt"]),
+                      "kernels/attention.hip", "kernels/paged_cache.hip",
+                      "kernels/paged_attention.hip", "kernels/token_logprob.hip"], ["grxrt"]),
 }
 
 

@@ -20,6 +20,7 @@
 #include <cstring>
 #include <mutex>
 #include <new>
+#include <utility>
 
 #include "hip_status.h"
 #include "launch.h"
@@ -305,6 +306,78 @@ grxdnnStatus_t row_common(grxdnnHandle_t handle, grxdnnTensorDescriptor_t xDesc,
   return GRXDNN_STATUS_SUCCESS;
 }
 
+bool half_type(grxDataType_t t) { return t == GRX_R_16BF || t == GRX_R_16F; }
+
+// 16-byte vector access along the last dimension: contiguous, rows on 16 bytes.
+bool half_rows(const grxdnnTensorStruct& t) {
+  if (t.strides[t.nb - 1] != 1) return false;
+  for (int i = 0; i < t.nb - 1; ++i)
+    if (t.dims[i] > 1 && t.strides[i] % 8 != 0) return false;
+  return true;
+}
+
+// A table of pages: [B, W] ints, rows of any pitch.
+bool table_shape(const grxdnnTensorStruct& t) {
+  return t.nb == 2 && t.type == GRX_R_32I && t.dims[1] >= 1 && (t.dims[1] == 1 || t.strides[1] == 1);
+}
+
+// fp32 [B, heads, S] of S >= slots with contiguous slots.
+bool weights_shape(const grxdnnTensorStruct& t, int B, int heads, int64_t slots) {
+  return t.nb == 3 && t.type == GRX_R_32F && t.dims[0] == B && t.dims[1] == heads && t.dims[2] >= slots &&
+         (t.dims[2] <= 1 || t.strides[2] == 1);
+}
+
+// The pools and the table of a paged call, but for their pointers.
+grxdnnStatus_t paged_cache(grxdnnTensorDescriptor_t kDesc, grxdnnTensorDescriptor_t vDesc,
+                           grxdnnTensorDescriptor_t tableDesc, bool written, grxk::PagedCache* c) {
+  if (!kDesc || !vDesc || !tableDesc || !kDesc->set || !vDesc->set || !tableDesc->set)
+    return GRXDNN_STATUS_INVALID_VALUE;
+  if (kDesc->nb != 4 || !same_shape(*kDesc, *vDesc) || !table_shape(*tableDesc))
+    return GRXDNN_STATUS_INVALID_VALUE;
+  for (int i = 0; i < 4; ++i)
+    if (kDesc->dims[i] < 1) return GRXDNN_STATUS_INVALID_VALUE;
+  if (!half_type(kDesc->type) || vDesc->type != kDesc->type) return GRXDNN_STATUS_NOT_SUPPORTED;
+  c->pages = kDesc->dims[0];
+  c->heads = kDesc->dims[1];
+  c->page = kDesc->dims[2];
+  c->D = kDesc->dims[3];
+  c->B = tableDesc->dims[0];
+  c->W = tableDesc->dims[1];
+  c->table_rs = tableDesc->strides[0];
+  if (c->D != 64 && c->D != 128) return GRXDNN_STATUS_NOT_SUPPORTED;
+  if ((int64_t)c->W * c->page > INT_MAX - 255) return GRXDNN_STATUS_NOT_SUPPORTED;
+  // (sequence, head) pairs are counted in 32 bits
+  if ((int64_t)c->B * c->heads > INT_MAX / 4) return GRXDNN_STATUS_NOT_SUPPORTED;
+  if (!half_rows(*kDesc) || !half_rows(*vDesc)) return GRXDNN_STATUS_NOT_SUPPORTED;
+  if (written && (!no_overlap(*kDesc) || !no_overlap(*vDesc))) return GRXDNN_STATUS_INVALID_VALUE;
+  c->k_sp = kDesc->strides[0]; c->k_sh = kDesc->strides[1]; c->k_ss = kDesc->strides[2];
+  c->v_sp = vDesc->strides[0]; c->v_sh = vDesc->strides[1]; c->v_ss = vDesc->strides[2];
+  return GRXDNN_STATUS_SUCCESS;
+}
+
+Span bytes_at(const void* p, int64_t n) { return {(uintptr_t)p, (uintptr_t)p + (uintptr_t)n}; }
+
+// Logits of softmax's layout: rows, their pitch and the element type.
+grxdnnStatus_t logit_rows(const grxdnnTensorStruct& x, grxk::NormType* nt, int64_t* rows, int64_t* pitch) {
+  switch (x.type) {
+    case GRX_R_16BF: *nt = grxk::NormType::BF16; break;
+    case GRX_R_16F:  *nt = grxk::NormType::F16; break;
+    case GRX_R_32F:  *nt = grxk::NormType::F32; break;
+    default: return GRXDNN_STATUS_NOT_SUPPORTED;
+  }
+  const int vocab = x.dims[x.nb - 1];
+  *rows = 1;
+  for (int i = 0; i < x.nb - 1; ++i)
+    if (x.dims[i] == 0) *rows = 0;
+  if (vocab <= 0) return *rows ? GRXDNN_STATUS_INVALID_VALUE : GRXDNN_STATUS_SUCCESS;
+  if (vocab > (1 << 24)) return GRXDNN_STATUS_NOT_SUPPORTED;
+  if (x.strides[x.nb - 1] != 1) return GRXDNN_STATUS_NOT_SUPPORTED;
+  if (*rows && !row_layout(x, rows, pitch)) return GRXDNN_STATUS_NOT_SUPPORTED;
+  return GRXDNN_STATUS_SUCCESS;
+}
+
+size_t element_size(grxk::NormType t) { return t == grxk::NormType::F32 ? 4 : 2; }
+
 }  // namespace
 
 // The C API is the only thing these libraries export (built with
@@ -551,6 +624,274 @@ int grxdnnAttentionCycleSlotsNeeded(grxdnnHandle_t handle, int batch, int heads,
   if (batch <= 0 || heads <= 0 || seqLen <= 0) return 0;
   const int64_t s = grxk::attention_probe_slots(batch, heads, seqLen);
   return s > INT_MAX ? INT_MAX : (int)s;
+}
+
+grxdnnStatus_t grxdnnPagedCacheAppend(grxdnnHandle_t handle, grxdnnTensorDescriptor_t kDesc, const void* k,
+                                      grxdnnTensorDescriptor_t vDesc, const void* v,
+                                      grxdnnTensorDescriptor_t kCacheDesc, void* kCache,
+                                      grxdnnTensorDescriptor_t vCacheDesc, void* vCache,
+                                      grxdnnTensorDescriptor_t tableDesc, const int* table,
+                                      const int* lengths, const int* counts) {
+  if (!handle) return GRXDNN_STATUS_NOT_INITIALIZED;
+  if (!kDesc || !vDesc || !kDesc->set || !vDesc->set) return GRXDNN_STATUS_INVALID_VALUE;
+  grxk::PagedAppendDesc d{};
+  grxdnnStatus_t s = paged_cache(kCacheDesc, vCacheDesc, tableDesc, true, &d.c);
+  if (s != GRXDNN_STATUS_SUCCESS) return s;
+  if (kDesc->nb != 4 || !same_shape(*kDesc, *vDesc) || kDesc->dims[0] != d.c.B ||
+      kDesc->dims[1] != d.c.heads || kDesc->dims[3] != d.c.D)
+    return GRXDNN_STATUS_INVALID_VALUE;
+  if (kDesc->type != kCacheDesc->type || vDesc->type != kCacheDesc->type) return GRXDNN_STATUS_NOT_SUPPORTED;
+  d.T = kDesc->dims[2];
+  if (d.c.B == 0 || d.T == 0) return GRXDNN_STATUS_SUCCESS;
+  if (!half_rows(*kDesc) || !half_rows(*vDesc)) return GRXDNN_STATUS_NOT_SUPPORTED;
+  if (!k || !v || !kCache || !vCache || !table || !lengths) return GRXDNN_STATUS_INVALID_VALUE;
+  if (may_alias(*kCacheDesc, kCache, *vCacheDesc, vCache)) return GRXDNN_STATUS_INVALID_VALUE;
+  for (const auto& [cd, cp] : {std::pair{kCacheDesc, kCache}, std::pair{vCacheDesc, vCache}}) {
+    const Span c = span_of(*cd, cp, 2);
+    if (intersect(c, span_of(*kDesc, k, 2)) || intersect(c, span_of(*vDesc, v, 2)) ||
+        intersect(c, span_of(*tableDesc, table, 4)) || intersect(c, bytes_at(lengths, 4ll * d.c.B)) ||
+        (counts && intersect(c, bytes_at(counts, 4ll * d.c.B))))
+      return GRXDNN_STATUS_INVALID_VALUE;
+  }
+  if (!aligned16(k) || !aligned16(v) || !aligned16(kCache) || !aligned16(vCache))
+    return GRXDNN_STATUS_NOT_SUPPORTED;
+  s = ensure_device(*handle);
+  if (s != GRXDNN_STATUS_SUCCESS) return s;
+  d.c.k = kCache; d.c.v = vCache; d.c.table = table; d.c.lengths = lengths;
+  d.k = k; d.k_sb = kDesc->strides[0]; d.k_sh = kDesc->strides[1]; d.k_st = kDesc->strides[2];
+  d.v = v; d.v_sb = vDesc->strides[0]; d.v_sh = vDesc->strides[1]; d.v_st = vDesc->strides[2];
+  d.counts = counts;
+  return from_hip(grxk::launch_paged_append(d, handle->stream));
+}
+
+grxdnnStatus_t grxdnnPagedAttentionGetWorkspaceSize(grxdnnHandle_t handle, grxdnnTensorDescriptor_t qDesc,
+                                                    grxdnnTensorDescriptor_t kCacheDesc,
+                                                    grxdnnTensorDescriptor_t tableDesc,
+                                                    grxdnnTensorDescriptor_t weightsDesc, size_t* bytes) {
+  if (!handle) return GRXDNN_STATUS_NOT_INITIALIZED;
+  if (!qDesc || !qDesc->set || !bytes) return GRXDNN_STATUS_INVALID_VALUE;
+  grxk::PagedCache c{};
+  const grxdnnStatus_t s = paged_cache(kCacheDesc, kCacheDesc, tableDesc, false, &c);
+  if (s != GRXDNN_STATUS_SUCCESS) return s;
+  if (weightsDesc && !weightsDesc->set) return GRXDNN_STATUS_INVALID_VALUE;
+  if (qDesc->nb != 4 || qDesc->dims[0] != c.B || qDesc->dims[1] < 1 || qDesc->dims[1] % c.heads != 0 ||
+      qDesc->dims[3] != c.D)
+    return GRXDNN_STATUS_INVALID_VALUE;
+  *bytes = c.B == 0 ? 0 : grxk::paged_attention_workspace(c.B, qDesc->dims[1], c.heads, c.D, c.W, c.page,
+                                                          weightsDesc != nullptr);
+  return GRXDNN_STATUS_SUCCESS;
+}
+
+grxdnnStatus_t grxdnnPagedAttentionForward(grxdnnHandle_t handle, grxdnnAttentionDescriptor_t attnDesc,
+                                           grxdnnTensorDescriptor_t qDesc, const void* q,
+                                           grxdnnTensorDescriptor_t kCacheDesc, const void* kCache,
+                                           grxdnnTensorDescriptor_t vCacheDesc, const void* vCache,
+                                           grxdnnTensorDescriptor_t tableDesc, const int* table,
+                                           const int* lengths, float weightDecay,
+                                           grxdnnTensorDescriptor_t weightsDesc, float* weights,
+                                           grxdnnTensorDescriptor_t oDesc, void* o, void* workspace,
+                                           size_t workspaceBytes) {
+  if (!handle) return GRXDNN_STATUS_NOT_INITIALIZED;
+  if (!attnDesc || !qDesc || !oDesc || !attnDesc->set || !qDesc->set || !oDesc->set)
+    return GRXDNN_STATUS_INVALID_VALUE;
+  if ((weightsDesc != nullptr) != (weights != nullptr) || (weightsDesc && !weightsDesc->set))
+    return GRXDNN_STATUS_INVALID_VALUE;
+  grxk::PagedAttnDesc d{};
+  grxdnnStatus_t s = paged_cache(kCacheDesc, vCacheDesc, tableDesc, false, &d.c);
+  if (s != GRXDNN_STATUS_SUCCESS) return s;
+  if (qDesc->nb != 4 || !same_shape(*qDesc, *oDesc) || qDesc->dims[0] != d.c.B || qDesc->dims[1] < 1 ||
+      qDesc->dims[1] % d.c.heads != 0 || qDesc->dims[3] != d.c.D)
+    return GRXDNN_STATUS_INVALID_VALUE;
+  if (weights) {
+    if (!weights_shape(*weightsDesc, d.c.B, d.c.heads, (int64_t)d.c.W * d.c.page))
+      return GRXDNN_STATUS_INVALID_VALUE;
+    if (!std::isfinite(weightDecay) || weightDecay < 0.0f) return GRXDNN_STATUS_INVALID_VALUE;
+  }
+  if (qDesc->type != kCacheDesc->type || oDesc->type != kCacheDesc->type) return GRXDNN_STATUS_NOT_SUPPORTED;
+  d.H = qDesc->dims[1];
+  // one query per sequence; (sequence, query head) pairs are counted in 32 bits
+  if (qDesc->dims[2] != 1 || d.H / d.c.heads > 1024 || (int64_t)d.c.B * d.H > INT_MAX / 4)
+    return GRXDNN_STATUS_NOT_SUPPORTED;
+  if (d.c.B == 0) return GRXDNN_STATUS_SUCCESS;
+  if (!half_rows(*qDesc) || !half_rows(*oDesc)) return GRXDNN_STATUS_NOT_SUPPORTED;
+  if (!no_overlap(*oDesc) || (weights && !no_overlap(*weightsDesc))) return GRXDNN_STATUS_INVALID_VALUE;
+  if (!q || !kCache || !vCache || !table || !lengths || !o) return GRXDNN_STATUS_INVALID_VALUE;
+  const size_t need = grxk::paged_attention_workspace(d.c.B, d.H, d.c.heads, d.c.D, d.c.W, d.c.page,
+                                                      weights != nullptr);
+  if (workspaceBytes < need || (need && !workspace)) return GRXDNN_STATUS_INVALID_VALUE;
+  if (may_alias(*oDesc, o, *qDesc, q) && !(o == q && same_strides(*oDesc, *qDesc)))
+    return GRXDNN_STATUS_INVALID_VALUE;
+  // What is written, against everything else that the call reads or writes.
+  const Span so = span_of(*oDesc, o, 2), sw = weights ? span_of(*weightsDesc, weights, 4) : Span{0, 0};
+  const Span ss = need ? bytes_at(workspace, (int64_t)need) : Span{0, 0};
+  const Span in[] = {span_of(*kCacheDesc, kCache, 2), span_of(*vCacheDesc, vCache, 2),
+                     span_of(*tableDesc, table, 4), bytes_at(lengths, 4ll * d.c.B)};
+  for (const Span& x : in)
+    if (intersect(so, x) || (weights && intersect(sw, x)) || (need && intersect(ss, x)))
+      return GRXDNN_STATUS_INVALID_VALUE;
+  const Span sq = span_of(*qDesc, q, 2);
+  if (weights && (intersect(sw, so) || intersect(sw, sq))) return GRXDNN_STATUS_INVALID_VALUE;
+  if (need && (intersect(ss, so) || intersect(ss, sq) || (weights && intersect(ss, sw))))
+    return GRXDNN_STATUS_INVALID_VALUE;
+  if (!aligned16(q) || !aligned16(kCache) || !aligned16(vCache) || !aligned16(o) ||
+      (need && !aligned16(workspace)))
+    return GRXDNN_STATUS_NOT_SUPPORTED;
+  s = ensure_device(*handle);
+  if (s != GRXDNN_STATUS_SUCCESS) return s;
+  d.c.k = const_cast<void*>(kCache); d.c.v = const_cast<void*>(vCache);
+  d.c.table = table; d.c.lengths = lengths;
+  d.scale = attnDesc->scale;
+  d.q = q; d.q_sb = qDesc->strides[0]; d.q_sh = qDesc->strides[1];
+  d.o = o; d.o_sb = oDesc->strides[0]; d.o_sh = oDesc->strides[1];
+  d.decay = weightDecay;
+  if (weights) {
+    d.weights = weights;
+    d.w_sb = weightsDesc->strides[0];
+    d.w_sh = weightsDesc->strides[1];
+  }
+  d.ws = workspace;
+  return from_hip(grxk::launch_paged_attention(
+      qDesc->type == GRX_R_16BF ? grxk::AttnType::BF16 : grxk::AttnType::F16, d, handle->stream));
+}
+
+grxdnnStatus_t grxdnnPagedCacheEvict(grxdnnHandle_t handle, grxdnnTensorDescriptor_t kCacheDesc, void* kCache,
+                                     grxdnnTensorDescriptor_t vCacheDesc, void* vCache,
+                                     grxdnnTensorDescriptor_t tableDesc, const int* table, const int* lengths,
+                                     grxdnnTensorDescriptor_t weightsDesc, const float* weights, int budget,
+                                     int recent, int* kept, grxdnnTensorDescriptor_t newTableDesc,
+                                     const int* newTable, int* newLengths,
+                                     grxdnnTensorDescriptor_t newWeightsDesc, float* newWeights) {
+  if (!handle) return GRXDNN_STATUS_NOT_INITIALIZED;
+  if (!weightsDesc || !newTableDesc || !newWeightsDesc || !weightsDesc->set || !newTableDesc->set ||
+      !newWeightsDesc->set)
+    return GRXDNN_STATUS_INVALID_VALUE;
+  grxk::PagedEvictDesc d{};
+  grxdnnStatus_t s = paged_cache(kCacheDesc, vCacheDesc, tableDesc, true, &d.c);
+  if (s != GRXDNN_STATUS_SUCCESS) return s;
+  if (budget < 1 || recent < 0 || recent > budget) return GRXDNN_STATUS_INVALID_VALUE;
+  if (!table_shape(*newTableDesc) || newTableDesc->dims[0] != d.c.B ||
+      (int64_t)newTableDesc->dims[1] * d.c.page < budget)
+    return GRXDNN_STATUS_INVALID_VALUE;
+  if ((int64_t)newTableDesc->dims[1] * d.c.page > INT_MAX - 255) return GRXDNN_STATUS_NOT_SUPPORTED;
+  if (!weights_shape(*weightsDesc, d.c.B, d.c.heads, (int64_t)d.c.W * d.c.page) ||
+      !weights_shape(*newWeightsDesc, d.c.B, d.c.heads, budget))
+    return GRXDNN_STATUS_INVALID_VALUE;
+  if (d.c.B == 0) return GRXDNN_STATUS_SUCCESS;
+  if (!no_overlap(*newWeightsDesc)) return GRXDNN_STATUS_INVALID_VALUE;
+  if (!kCache || !vCache || !table || !lengths || !weights || !kept || !newTable || !newLengths || !newWeights)
+    return GRXDNN_STATUS_INVALID_VALUE;
+  if (may_alias(*kCacheDesc, kCache, *vCacheDesc, vCache)) return GRXDNN_STATUS_INVALID_VALUE;
+  // Each written array against everything else; the pools are read and written.
+  const Span spans[] = {span_of(*kCacheDesc, kCache, 2), span_of(*vCacheDesc, vCache, 2),
+                        bytes_at(kept, 4ll * d.c.B * d.c.heads * budget), bytes_at(newLengths, 4ll * d.c.B),
+                        span_of(*newWeightsDesc, newWeights, 4),
+                        // only read from here on
+                        span_of(*tableDesc, table, 4), span_of(*newTableDesc, newTable, 4),
+                        span_of(*weightsDesc, weights, 4), bytes_at(lengths, 4ll * d.c.B)};
+  for (int i = 0; i < 5; ++i)
+    for (int j = i + 1; j < 9; ++j) {
+      if (i == 0 && j == 1) continue;                      // the pools: element by element, above
+      if (i == 3 && j == 8 && newLengths == lengths) continue;   // in place
+      if (intersect(spans[i], spans[j])) return GRXDNN_STATUS_INVALID_VALUE;
+    }
+  if (!aligned16(kCache) || !aligned16(vCache)) return GRXDNN_STATUS_NOT_SUPPORTED;
+  s = ensure_device(*handle);
+  if (s != GRXDNN_STATUS_SUCCESS) return s;
+  d.c.k = kCache; d.c.v = vCache; d.c.table = table; d.c.lengths = lengths;
+  d.weights = weights; d.w_sb = weightsDesc->strides[0]; d.w_sh = weightsDesc->strides[1];
+  d.budget = budget; d.recent = recent; d.kept = kept;
+  d.new_table = newTable; d.new_table_rs = newTableDesc->strides[0]; d.new_W = newTableDesc->dims[1];
+  d.new_lengths = newLengths;
+  d.new_weights = newWeights; d.nw_sb = newWeightsDesc->strides[0]; d.nw_sh = newWeightsDesc->strides[1];
+  d.nw_slots = newWeightsDesc->dims[2];
+  return from_hip(grxk::launch_paged_evict(d, handle->stream));
+}
+
+grxdnnStatus_t grxdnnTokenLogProbGetWorkspaceSize(grxdnnHandle_t handle, grxdnnTensorDescriptor_t xDesc,
+                                                  int topCount, size_t* bytes) {
+  if (!handle) return GRXDNN_STATUS_NOT_INITIALIZED;
+  if (!xDesc || !xDesc->set || !bytes || topCount < 0) return GRXDNN_STATUS_INVALID_VALUE;
+  grxk::NormType nt{};
+  int64_t rows = 0, pitch = 0;
+  const grxdnnStatus_t s = logit_rows(*xDesc, &nt, &rows, &pitch);
+  if (s != GRXDNN_STATUS_SUCCESS) return s;
+  const int vocab = xDesc->dims[xDesc->nb - 1];
+  if (rows && topCount > vocab) return GRXDNN_STATUS_INVALID_VALUE;
+  if (topCount > 64) return GRXDNN_STATUS_NOT_SUPPORTED;
+  *bytes = rows ? grxk::token_logprob_workspace(nt, rows, vocab, topCount) : 0;
+  return GRXDNN_STATUS_SUCCESS;
+}
+
+grxdnnStatus_t grxdnnTokenLogProbForward(grxdnnHandle_t handle, grxdnnTensorDescriptor_t xDesc, const void* x,
+                                         const int* tokens, float* logProb, float* logSumExp, float* entropy,
+                                         int topCount, float* topLogProb, int* topIndex, void* workspace,
+                                         size_t workspaceBytes) {
+  size_t need = 0;
+  grxdnnStatus_t s = grxdnnTokenLogProbGetWorkspaceSize(handle, xDesc, topCount, &need);
+  if (s != GRXDNN_STATUS_SUCCESS) return s;
+  if ((tokens != nullptr) != (logProb != nullptr)) return GRXDNN_STATUS_INVALID_VALUE;
+  if (topCount ? !topLogProb || !topIndex : topLogProb || topIndex) return GRXDNN_STATUS_INVALID_VALUE;
+  grxk::NormType nt{};
+  grxk::TokenLogProbDesc d{};
+  (void)logit_rows(*xDesc, &nt, &d.rows, &d.x_row_stride);
+  if (d.rows == 0) return GRXDNN_STATUS_SUCCESS;
+  if (!x || !logSumExp) return GRXDNN_STATUS_INVALID_VALUE;
+  if (workspaceBytes < need || (need && !workspace)) return GRXDNN_STATUS_INVALID_VALUE;
+  // Each written array against the inputs and the other written ones.
+  const Span spans[] = {logProb ? bytes_at(logProb, 4 * d.rows) : Span{0, 0},
+                        bytes_at(logSumExp, 4 * d.rows),
+                        entropy ? bytes_at(entropy, 4 * d.rows) : Span{0, 0},
+                        topCount ? bytes_at(topLogProb, 4 * d.rows * topCount) : Span{0, 0},
+                        topCount ? bytes_at(topIndex, 4 * d.rows * topCount) : Span{0, 0},
+                        need ? bytes_at(workspace, (int64_t)need) : Span{0, 0},
+                        span_of(*xDesc, x, element_size(nt)),
+                        tokens ? bytes_at(tokens, 4 * d.rows) : Span{0, 0}};
+  for (int i = 0; i < 6; ++i)
+    for (int j = i + 1; j < 8; ++j)
+      if (intersect(spans[i], spans[j])) return GRXDNN_STATUS_INVALID_VALUE;
+  if (need && !aligned16(workspace)) return GRXDNN_STATUS_NOT_SUPPORTED;
+  s = ensure_device(*handle);
+  if (s != GRXDNN_STATUS_SUCCESS) return s;
+  d.vocab = xDesc->dims[xDesc->nb - 1];
+  d.x = x; d.tokens = tokens; d.logprob = logProb; d.lse = logSumExp; d.entropy = entropy;
+  d.top = topCount; d.top_logprob = topLogProb; d.top_index = topIndex;
+  d.ws = workspace;
+  return from_hip(grxk::launch_token_logprob(nt, d, handle->stream));
+}
+
+grxdnnStatus_t grxdnnTokenLogProbBackward(grxdnnHandle_t handle, grxdnnTensorDescriptor_t xDesc, const void* x,
+                                          const int* tokens, const float* logSumExp, const float* entropy,
+                                          const float* dLogProb, const float* dEntropy,
+                                          grxdnnTensorDescriptor_t dxDesc, void* dx) {
+  if (!handle) return GRXDNN_STATUS_NOT_INITIALIZED;
+  if (!xDesc || !dxDesc || !xDesc->set || !dxDesc->set) return GRXDNN_STATUS_INVALID_VALUE;
+  if (!same_shape(*xDesc, *dxDesc)) return GRXDNN_STATUS_INVALID_VALUE;
+  if ((tokens != nullptr) != (dLogProb != nullptr) || (entropy != nullptr) != (dEntropy != nullptr) ||
+      (!tokens && !entropy))
+    return GRXDNN_STATUS_INVALID_VALUE;
+  if (xDesc->type != dxDesc->type) return GRXDNN_STATUS_NOT_SUPPORTED;
+  grxk::NormType nt{};
+  grxk::TokenLogProbGradDesc d{};
+  int64_t rows = 0;
+  grxdnnStatus_t s = logit_rows(*xDesc, &nt, &d.rows, &d.x_row_stride);
+  if (s != GRXDNN_STATUS_SUCCESS) return s;
+  s = logit_rows(*dxDesc, &nt, &rows, &d.dx_row_stride);
+  if (s != GRXDNN_STATUS_SUCCESS) return s;
+  if (d.rows == 0) return GRXDNN_STATUS_SUCCESS;
+  if (!x || !logSumExp || !dx) return GRXDNN_STATUS_INVALID_VALUE;
+  if (!no_overlap(*dxDesc)) return GRXDNN_STATUS_INVALID_VALUE;
+  const Span out = span_of(*dxDesc, dx, element_size(nt));
+  if (intersect(out, span_of(*xDesc, x, element_size(nt))) && !(dx == x && same_strides(*dxDesc, *xDesc)))
+    return GRXDNN_STATUS_INVALID_VALUE;
+  for (const void* p : {(const void*)tokens, (const void*)logSumExp, (const void*)entropy,
+                        (const void*)dLogProb, (const void*)dEntropy})
+    if (p && intersect(out, bytes_at(p, 4 * d.rows))) return GRXDNN_STATUS_INVALID_VALUE;
+  s = ensure_device(*handle);
+  if (s != GRXDNN_STATUS_SUCCESS) return s;
+  d.vocab = xDesc->dims[xDesc->nb - 1];
+  d.x = x; d.tokens = tokens; d.lse = logSumExp; d.entropy = entropy;
+  d.dlogprob = dLogProb; d.dentropy = dEntropy; d.dx = dx;
+  return from_hip(grxk::launch_token_logprob_grad(nt, d, handle->stream));
 }
 
 }  // extern "C"

@@ -142,6 +142,80 @@ hipError_t launch_attention(AttnType t, const AttnDesc& d, hipStream_t s);
 // (workgroups x waves per workgroup; slot = blockIdx * waves + wave).
 int64_t attention_probe_slots(int B, int H, int S);
 
+// The paged key-value cache: two pools of [pages, heads, page, D] and the table
+// that names the pages of B sequences.
+struct PagedCache {
+  void* k; int64_t k_sp, k_sh, k_ss;         // strides (elements) of page, head, slot
+  void* v; int64_t v_sp, v_sh, v_ss;
+  int pages, heads, page, D;
+  int B, W;
+  const int* table; int64_t table_rs;
+  const int* lengths;
+};
+struct PagedAppendDesc {
+  PagedCache c;
+  const void* k; int64_t k_sb, k_sh, k_st;   // new rows [B, heads, T, D]
+  const void* v; int64_t v_sb, v_sh, v_st;
+  int T;
+  const int* counts;                         // may be null: T each
+};
+hipError_t launch_paged_append(const PagedAppendDesc& d, hipStream_t s);
+
+struct PagedAttnDesc {
+  PagedCache c;
+  int H;                                     // query heads, a multiple of c.heads
+  float scale;
+  const void* q; int64_t q_sb, q_sh;
+  void* o;       int64_t o_sb, o_sh;
+  float* weights; int64_t w_sb, w_sh;        // may be null
+  float decay;
+  void* ws;
+};
+hipError_t launch_paged_attention(AttnType t, const PagedAttnDesc& d, hipStream_t s);
+// Workspace bytes of a call: B sequences of W * page slots, H query heads on
+// `heads` key heads, with or without the slots' weights.
+size_t paged_attention_workspace(int B, int H, int heads, int D, int W, int page, bool weights);
+
+struct PagedEvictDesc {
+  PagedCache c;
+  const float* weights; int64_t w_sb, w_sh;
+  int budget, recent;
+  int* kept;                                 // [B, heads, budget]
+  const int* new_table; int64_t new_table_rs; int new_W;
+  int* new_lengths;
+  float* new_weights; int64_t nw_sb, nw_sh; int nw_slots;
+};
+hipError_t launch_paged_evict(const PagedEvictDesc& d, hipStream_t s);
+
+// Log probabilities of tokens over rows of logits, and their gradient.
+struct TokenLogProbDesc {
+  int64_t rows;
+  int vocab;
+  int64_t x_row_stride;                      // elements
+  const void* x;
+  const int* tokens; float* logprob;         // both may be null
+  float* lse;
+  float* entropy;                            // may be null
+  int top;
+  float* top_logprob; int* top_index;
+  void* ws;
+};
+size_t token_logprob_workspace(NormType t, int64_t rows, int vocab, int top);
+hipError_t launch_token_logprob(NormType t, const TokenLogProbDesc& d, hipStream_t s);
+struct TokenLogProbGradDesc {
+  int64_t rows;
+  int vocab;
+  int64_t x_row_stride, dx_row_stride;       // elements
+  const void* x;
+  const int* tokens;
+  const float* lse;
+  const float* entropy;
+  const float* dlogprob;                     // null without tokens
+  const float* dentropy;                     // null: no entropy term
+  void* dx;
+};
+hipError_t launch_token_logprob_grad(NormType t, const TokenLogProbGradDesc& d, hipStream_t s);
+
 }  // namespace grxk
 
 #endif  // GRXCP_LAUNCH_H

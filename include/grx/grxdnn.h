@@ -1,4 +1,4 @@
-/* grxdnn.h -- grxDNN forward primitives, MI355X (gfx950) build.
+/* grxdnn.h -- grxDNN primitives, MI355X (gfx950) build.
  *
  * The reference plans grxDNN but ships no code for it: a CMake slot
  * (ref: src/libs/CMakeLists.txt:12), an architecture entry naming grxdnn.h
@@ -167,6 +167,155 @@ grxdnnStatus_t grxdnnSetCycleProbe(grxdnnHandle_t handle, grxCycleSlot* slots,
                                    int capacity);
 int            grxdnnAttentionCycleSlotsNeeded(grxdnnHandle_t handle, int batch,
                                                int heads, int seqLen);
+
+/* ---- paged key-value cache --------------------------------------------------
+ *
+ * Keys and values of running sequences lie in two pools, each described by a
+ * 4-d descriptor [pages, Hkv, P, D]: pages of P slots for Hkv heads of D values
+ * (any strides: [pages, P, Hkv, D] memory is a view of it). A page table, 2-d
+ * [B, W] GRX_R_32I with innermost stride 1, names the pages of each of B
+ * sequences: slot j of sequence b is row j % P of page table[b][j / P], and a
+ * sequence has room for W * P slots (at most 2^31 - 256). lengths: B ints, the
+ * slots of each sequence that hold tokens; below 0 counts as 0, above W * P as
+ * W * P. Tables, lengths and counts are device memory, read when the kernels
+ * run: a captured call follows their contents on every replay.
+ *
+ * Table entries of pages that a call does not reach are not read. An entry
+ * outside [0, pages) that it does reach is never followed: a row written there
+ * is dropped, and a row read there is as if the slot were not in the sequence.
+ * Two sequences may share pages that are only read.
+ *
+ * Types GRX_R_16BF or GRX_R_16F, one for all key, value, query and output
+ * tensors; D is 64 or 128; innermost stride 1, the other strides multiples of 8
+ * elements, pointers 16-byte aligned (else NOT_SUPPORTED). The two pools have
+ * one shape and share no element; written tensors must not share elements of
+ * their own or with what the call reads (INVALID_VALUE where the descriptors
+ * show it; pages that two written table entries name are the caller's matter:
+ * such rows hold one of the values written).
+ * (New: planned by ref docs/designs/grxcp_roadmap.md:864-877, "attention".) */
+
+/* New rows behind the tokens that a cache holds: for every sequence b, head h
+ * and t < counts[b],
+ *   cache[slot lengths[b] + t of b, head h] = new[b, h, t, :]   (keys and values)
+ * k, v: [B, Hkv, T, D]. counts: B ints within 0 .. T (others are clamped), or
+ * NULL for T each. Rows past a sequence's room are dropped. lengths is not
+ * changed: the caller adds counts to it. */
+grxdnnStatus_t grxdnnPagedCacheAppend(grxdnnHandle_t handle,
+                                      grxdnnTensorDescriptor_t kDesc, const void* k,
+                                      grxdnnTensorDescriptor_t vDesc, const void* v,
+                                      grxdnnTensorDescriptor_t kCacheDesc, void* kCache,
+                                      grxdnnTensorDescriptor_t vCacheDesc, void* vCache,
+                                      grxdnnTensorDescriptor_t tableDesc, const int* table,
+                                      const int* lengths, const int* counts);
+
+/* Attention of one new token per sequence over its slots (the token's own key
+ * and value included, appended before):
+ *   s[b,h,j] = softmaxScale * <q[b,h,0,:], K[slot j of b, head h / G, :]>,  j < lengths[b]
+ *   p[b,h,:] = softmax(s[b,h,:]),  o[b,h,0,:] = sum_j p[b,h,j] V[slot j of b, head h / G, :]
+ * q, o: [B, H, 1, D], H = G * Hkv query heads in groups of G = 1 .. 1024. The
+ * descriptor's causal flag makes no difference: the new token is the last one.
+ * Scores, softmax and sums are fp32 and the weights of the values are rounded
+ * to the value type (as in grxdnnAttentionForward); o is rounded once. o may be
+ * q itself (same pointer and strides). A sequence of no slots gives o = 0; one
+ * whose scores are all -inf gives NaN, as the formula does. Slots at or past
+ * lengths[b] are not read, whatever their pages hold.
+ *
+ * weights (optional, both arguments or neither NULL): what the slots received,
+ * [B, Hkv, S] GRX_R_32F, S >= W * P, innermost stride 1:
+ *   weights[b,g,j] = weightDecay * weights[b,g,j] + sum_{h in group g} p[b,h,j],  j < lengths[b]
+ * with entries at or past lengths[b] left as they are. weightDecay: finite and
+ * >= 0; with 0 the old weights are not read.
+ *
+ * workspace: device memory of at least the size that
+ * grxdnnPagedAttentionGetWorkspaceSize gives for the same descriptors (a
+ * smaller one is INVALID_VALUE; 16-byte aligned; its contents before the call
+ * do not matter). Calls that may run at the same time, captured graphs
+ * included, need workspaces of their own. */
+grxdnnStatus_t grxdnnPagedAttentionGetWorkspaceSize(grxdnnHandle_t handle,
+                                                    grxdnnTensorDescriptor_t qDesc,
+                                                    grxdnnTensorDescriptor_t kCacheDesc,
+                                                    grxdnnTensorDescriptor_t tableDesc,
+                                                    grxdnnTensorDescriptor_t weightsDesc,
+                                                    size_t* bytes);
+grxdnnStatus_t grxdnnPagedAttentionForward(grxdnnHandle_t handle,
+                                           grxdnnAttentionDescriptor_t attnDesc,
+                                           grxdnnTensorDescriptor_t qDesc, const void* q,
+                                           grxdnnTensorDescriptor_t kCacheDesc, const void* kCache,
+                                           grxdnnTensorDescriptor_t vCacheDesc, const void* vCache,
+                                           grxdnnTensorDescriptor_t tableDesc, const int* table,
+                                           const int* lengths, float weightDecay,
+                                           grxdnnTensorDescriptor_t weightsDesc, float* weights,
+                                           grxdnnTensorDescriptor_t oDesc, void* o,
+                                           void* workspace, size_t workspaceBytes);
+
+/* The slots of each sequence and head that matter, into pages of their own. Of
+ * n = lengths[b] slots with weights[b,h,:] (as grxdnnPagedAttentionForward
+ * accumulates them) head h of sequence b keeps all if n <= budget, else the
+ * newest `recent` ones (0 <= recent <= budget) and, of the others, the
+ * budget - recent of largest weight; of equal weights the lower slots stay, -0
+ * equals 0 and NaN counts as largest. With m = min(n, budget), in slot order:
+ *   kept[b,h,i]       = slot of the i-th one,       -1 for i >= m
+ *   row i of the sequence in newTable = that slot's key and value,  i < m
+ *   newWeights[b,h,i] = its weight,                  0 for i >= m
+ *   newLengths[b]     = m
+ * table, newTable: [B, W] and [B, W2] (any W2 * P >= budget) over the same pools;
+ * pages named by newTable must not be pages that any sequence of the call
+ * reads (a page may be shared by sequences: their rows are copied out of it).
+ * The pages of table are the caller's again afterwards. kept: packed
+ * [B, Hkv, budget] ints. weights, newWeights: [B, Hkv, S], S >= W * P and
+ * [B, Hkv, S2], S2 >= budget, GRX_R_32F, innermost stride 1. newLengths may be
+ * lengths itself. budget >= 1. */
+grxdnnStatus_t grxdnnPagedCacheEvict(grxdnnHandle_t handle,
+                                     grxdnnTensorDescriptor_t kCacheDesc, void* kCache,
+                                     grxdnnTensorDescriptor_t vCacheDesc, void* vCache,
+                                     grxdnnTensorDescriptor_t tableDesc, const int* table,
+                                     const int* lengths,
+                                     grxdnnTensorDescriptor_t weightsDesc, const float* weights,
+                                     int budget, int recent, int* kept,
+                                     grxdnnTensorDescriptor_t newTableDesc, const int* newTable,
+                                     int* newLengths,
+                                     grxdnnTensorDescriptor_t newWeightsDesc, float* newWeights);
+
+/* ---- log probabilities of tokens ---------------------------------------------
+ * x: logits [..., V] under softmax's layout rules and types (rows flatten to one
+ * row stride; GRX_R_16BF, GRX_R_16F, GRX_R_32F; V = 1 .. 2^24). For row r of the R:
+ *   logSumExp[r] = log sum_j exp(x[r,j])
+ *   logProb[r]   = x[r, tokens[r]] - logSumExp[r]    (from the row's maximum, not the
+ *                                                     rounded logSumExp; 0 where tokens[r] is
+ *                                                     outside [0, V): a padded row)
+ *   entropy[r]   = - sum_j p[r,j] log p[r,j],  p = softmax(x[r,:]),  0 log 0 = 0
+ *   topLogProb[r,i], topIndex[r,i]: the i-th largest x[r,j] - logSumExp[r] and its j,
+ *                  i < topCount; of equal ones the lower j comes first, -0 equals 0, NaN is largest
+ * Device arrays, packed: tokens and topIndex 32-bit ints, the others fp32; sums
+ * are fp32. entropy may be NULL, tokens and logProb may both be NULL; topCount
+ * is 0 .. min(V, 64), the two top arrays NULL if 0. -inf (a masked token) has
+ * p = 0. A row of only -inf has logSumExp -inf and NaN for the rest; one with NaN
+ * or +inf in it is NaN throughout (inf - inf, as in softmax) but for topIndex and
+ * the 0 of a padded row.
+ * workspace: as for grxdnnPagedAttentionForward. */
+grxdnnStatus_t grxdnnTokenLogProbGetWorkspaceSize(grxdnnHandle_t handle,
+                                                  grxdnnTensorDescriptor_t xDesc, int topCount,
+                                                  size_t* bytes);
+grxdnnStatus_t grxdnnTokenLogProbForward(grxdnnHandle_t handle,
+                                         grxdnnTensorDescriptor_t xDesc, const void* x,
+                                         const int* tokens, float* logProb, float* logSumExp,
+                                         float* entropy, int topCount, float* topLogProb,
+                                         int* topIndex, void* workspace, size_t workspaceBytes);
+
+/* The gradient of the log probabilities and entropies in the logits, from the
+ * forward call's logSumExp and entropy:
+ *   dx[r,j] = dLogProb[r] (1[j = tokens[r]] - p[r,j])         (0 without a token)
+ *           - dEntropy[r] p[r,j] (log p[r,j] + entropy[r])    (0 where p = 0)
+ * with p[r,j] = exp(x[r,j] - logSumExp[r]). tokens and dLogProb, or entropy and
+ * dEntropy, may be NULL together (that term is left out), not all four. dx: a
+ * descriptor of x's shape and type; fp32 arithmetic, rounded once; dx may be x
+ * itself (same pointer and strides). topLogProb has no gradient here. */
+grxdnnStatus_t grxdnnTokenLogProbBackward(grxdnnHandle_t handle,
+                                          grxdnnTensorDescriptor_t xDesc, const void* x,
+                                          const int* tokens, const float* logSumExp,
+                                          const float* entropy, const float* dLogProb,
+                                          const float* dEntropy,
+                                          grxdnnTensorDescriptor_t dxDesc, void* dx);
 
 #ifdef __cplusplus
 }  /* extern "C" */
