@@ -37,10 +37,11 @@ HIP_FLAGS = ["-O3", "-std=c++17", "-fPIC", "-fvisibility=hidden", f"--offload-ar
 HOST_FLAGS = ["-O2", "-std=c++17", "-fPIC", "-fvisibility=hidden", "-Wall", "-Wextra", "-D__HIP_PLATFORM_AMD__",
               "-I", os.path.join(ROCM, "include")]
 
-# Per-file extra flags. Attention keeps its MFMA results (scores and O) in
-# VGPRs, where the softmax VALU work reads them without AGPR copies.
+# Per-file extra flags. The attention kernels keep their MFMA results (scores and
+# O) in VGPRs, where the softmax VALU work reads them without AGPR copies.
 EXTRA = {
     "kernels/attention.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
+    "kernels/paged_attention.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
 }
 
 LIBS = {

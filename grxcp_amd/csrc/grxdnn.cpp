@@ -866,8 +866,7 @@ grxdnnStatus_t grxdnnTokenLogProbBackward(grxdnnHandle_t handle, grxdnnTensorDes
   if (!handle) return GRXDNN_STATUS_NOT_INITIALIZED;
   if (!xDesc || !dxDesc || !xDesc->set || !dxDesc->set) return GRXDNN_STATUS_INVALID_VALUE;
   if (!same_shape(*xDesc, *dxDesc)) return GRXDNN_STATUS_INVALID_VALUE;
-  if ((tokens != nullptr) != (dLogProb != nullptr) || (entropy != nullptr) != (dEntropy != nullptr) ||
-      (!tokens && !entropy))
+  if ((tokens != nullptr) != (dLogProb != nullptr) || (dEntropy && !entropy) || (!tokens && !dEntropy))
     return GRXDNN_STATUS_INVALID_VALUE;
   if (xDesc->type != dxDesc->type) return GRXDNN_STATUS_NOT_SUPPORTED;
   grxk::NormType nt{};
@@ -889,7 +888,7 @@ grxdnnStatus_t grxdnnTokenLogProbBackward(grxdnnHandle_t handle, grxdnnTensorDes
   s = ensure_device(*handle);
   if (s != GRXDNN_STATUS_SUCCESS) return s;
   d.vocab = xDesc->dims[xDesc->nb - 1];
-  d.x = x; d.tokens = tokens; d.lse = logSumExp; d.entropy = entropy;
+  d.x = x; d.tokens = tokens; d.lse = logSumExp; d.entropy = dEntropy ? entropy : nullptr;
   d.dlogprob = dLogProb; d.dentropy = dEntropy; d.dx = dx;
   return from_hip(grxk::launch_token_logprob_grad(nt, d, handle->stream));
 }

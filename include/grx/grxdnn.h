@@ -306,8 +306,9 @@ grxdnnStatus_t grxdnnTokenLogProbForward(grxdnnHandle_t handle,
  * forward call's logSumExp and entropy:
  *   dx[r,j] = dLogProb[r] (1[j = tokens[r]] - p[r,j])         (0 without a token)
  *           - dEntropy[r] p[r,j] (log p[r,j] + entropy[r])    (0 where p = 0)
- * with p[r,j] = exp(x[r,j] - logSumExp[r]). tokens and dLogProb, or entropy and
- * dEntropy, may be NULL together (that term is left out), not all four. dx: a
+ * with p[r,j] = exp(x[r,j] - logSumExp[r]). tokens and dLogProb may be NULL
+ * together, and dEntropy may be (entropy is then not read): that term is left
+ * out; not both. dx: a
  * descriptor of x's shape and type; fp32 arithmetic, rounded once; dx may be x
  * itself (same pointer and strides). topLogProb has no gradient here. */
 grxdnnStatus_t grxdnnTokenLogProbBackward(grxdnnHandle_t handle,

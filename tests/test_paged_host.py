@@ -109,7 +109,8 @@ def test_valid_calls_reach_the_device_check(dnn):
     assert logprob(dnn) == OK
     assert logprob(dnn, tokens=None, logprob=None, entropy=None, top=0, top_logprob=None, top_index=None) == OK
     assert gradient(dnn) == OK
-    assert gradient(dnn, entropy=None, dentropy=None) == OK and gradient(dnn, tokens=None, dlogprob=None) == OK
+    assert gradient(dnn, entropy=None, dentropy=None) == OK and gradient(dnn, dentropy=None) == OK
+    assert gradient(dnn, tokens=None, dlogprob=None) == OK
     # [pages, page, heads, d] memory, q and o as rows of a packed projection, o over q
     tok = T(BF16, POOL, [4096, 64, 256, 1])
     assert append(dnn, kcd=tok, vcd=tok) == OK
@@ -155,7 +156,7 @@ def test_missing_and_unset_descriptors(dnn, call, names):
     (attend, ["q", "kc", "vc", "table", "lengths", "o", "w"]),
     (evict, ["kc", "vc", "table", "lengths", "w", "kept", "new_table", "new_lengths", "new_w"]),
     (logprob, ["x", "tokens", "logprob", "lse", "top_logprob", "top_index"]),
-    (gradient, ["x", "tokens", "lse", "entropy", "dlogprob", "dentropy", "dx"])])
+    (gradient, ["x", "tokens", "lse", "entropy", "dlogprob", "dx"])])
 def test_null_pointers(dnn, call, names):
     for n in names:
         assert call(dnn, **{n: None}) == INVALID, n
@@ -282,8 +283,9 @@ def test_overlaps_are_refused(dnn):
 
 def test_optional_pairs(dnn):
     assert gradient(dnn, tokens=None) == INVALID and gradient(dnn, dlogprob=None) == INVALID
-    assert gradient(dnn, entropy=None) == INVALID and gradient(dnn, dentropy=None) == INVALID
+    assert gradient(dnn, entropy=None) == INVALID
     assert gradient(dnn, tokens=None, dlogprob=None, entropy=None, dentropy=None) == INVALID
+    assert gradient(dnn, tokens=None, dlogprob=None, dentropy=None) == INVALID
     assert logprob(dnn, tokens=None) == INVALID and logprob(dnn, logprob=None) == INVALID
 
 
