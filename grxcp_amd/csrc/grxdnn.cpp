@@ -677,8 +677,7 @@ grxdnnStatus_t grxdnnPagedAttentionGetWorkspaceSize(grxdnnHandle_t handle, grxdn
   if (qDesc->nb != 4 || qDesc->dims[0] != c.B || qDesc->dims[1] < 1 || qDesc->dims[1] % c.heads != 0 ||
       qDesc->dims[3] != c.D)
     return GRXDNN_STATUS_INVALID_VALUE;
-  *bytes = c.B == 0 ? 0 : grxk::paged_attention_workspace(c.B, qDesc->dims[1], c.heads, c.D, c.W, c.page,
-                                                          weightsDesc != nullptr);
+  *bytes = c.B == 0 ? 0 : grxk::paged_attention_workspace(c, qDesc->dims[1], weightsDesc != nullptr);
   return GRXDNN_STATUS_SUCCESS;
 }
 
@@ -716,8 +715,8 @@ grxdnnStatus_t grxdnnPagedAttentionForward(grxdnnHandle_t handle, grxdnnAttentio
   if (!half_rows(*qDesc) || !half_rows(*oDesc)) return GRXDNN_STATUS_NOT_SUPPORTED;
   if (!no_overlap(*oDesc) || (weights && !no_overlap(*weightsDesc))) return GRXDNN_STATUS_INVALID_VALUE;
   if (!q || !kCache || !vCache || !table || !lengths || !o) return GRXDNN_STATUS_INVALID_VALUE;
-  const size_t need = grxk::paged_attention_workspace(d.c.B, d.H, d.c.heads, d.c.D, d.c.W, d.c.page,
-                                                      weights != nullptr);
+  if (!grxk::paged_attention_fits(d.c, d.H)) return GRXDNN_STATUS_NOT_SUPPORTED;
+  const size_t need = grxk::paged_attention_workspace(d.c, d.H, weights != nullptr);
   if (workspaceBytes < need || (need && !workspace)) return GRXDNN_STATUS_INVALID_VALUE;
   if (may_alias(*oDesc, o, *qDesc, q) && !(o == q && same_strides(*oDesc, *qDesc)))
     return GRXDNN_STATUS_INVALID_VALUE;

@@ -43,12 +43,14 @@ namespace {
 
 constexpr int kWaves = 4;
 constexpr int kTile = 32;                 // slots of a wave's tile
-constexpr int kUnit = kWaves * kTile;     // slots of a unit
 constexpr float kLowest = -__FLT_MAX__;
 constexpr uint32_t kAbsent = 0x7fc0dead;  // a score of no slot (a NaN that no arithmetic gives)
 typedef __attribute__((address_space(3))) void* lds_ptr_t;
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) s16x4* lds_s16x4_t;
+
+// Workgroups that share a CU: registers (D = 64 has half the accumulators) and LDS.
+template <int D, int NT> constexpr int wgs_per_cu() { return D == 64 && NT == 1 ? 3 : 2; }
 
 template <int N> struct Buf { static constexpr int value = N; };
 
@@ -81,8 +83,8 @@ constexpr float kLazy = 4.0f;
 
 struct DParams {
   PagedView view;
-  const uint8_t* k; int64_t k_sp, k_sh, k_ss;   // byte strides of page, head, slot
-  const uint8_t* v; int64_t v_sp, v_sh, v_ss;
+  const uint8_t* k; uint32_t k_sp, k_sh, k_ss;   // strides of page, head, slot in 16-byte chunks
+  const uint8_t* v; uint32_t v_sp, v_sh, v_ss;
   const uint8_t* q; int64_t q_sb, q_sh;
   uint8_t* o; int64_t o_sb, o_sh;
   float* w; int64_t w_sb, w_sh;
@@ -92,8 +94,10 @@ struct DParams {
   float* scores;       // [B, H, slots], or null: no weights asked for
   int64_t slots;
   int B, H, heads, group;
+  int hw;              // key heads of a workgroup: 1, 2 or 4 waves' worth
+  int shift;           // a unit is 2^shift slots: kTile for each of a head's waves
   int gtiles;          // tiles of 16 * NT query heads in a group
-  int items;           // (key head, tile) pairs of a sequence
+  int items;           // (hw key heads, tile) pairs of a sequence
   int rows;            // query heads of a tile
   int wgs;             // workgroups of decode_split
   int whole;           // one workgroup per item, nothing to join
@@ -102,27 +106,44 @@ struct DParams {
 
 // ---- who does what -----------------------------------------------------------
 
-__device__ __forceinline__ int units_of(int len) { return max(1, (len + kUnit - 1) / kUnit); }
-
-__device__ __forceinline__ int64_t wave_sum64(int64_t v) {
-#pragma unroll
-  for (int o = 32; o; o >>= 1) v += __shfl_xor((long long)v, o);
-  return v;
+__device__ __forceinline__ uint32_t units_of(const DParams& p, int len) {
+  return max(1u, ((uint32_t)len + (1u << p.shift) - 1) >> p.shift);
 }
 
-// Units of one head of the sequences before b (b = B: of all).
-__device__ __forceinline__ int64_t units_before(const DParams& p, int b, int lane) {
-  int64_t s = 0;
-  for (int i = lane; i < b; i += 64) s += units_of(clamp_length(p.view.lengths[i], p.view.room));
-  return wave_sum64(s);
+// Sums over the wave in the ALU: rows of 16 lanes, then across them (all lanes get
+// the total of `total`; `upto` is each lane's sum of the lanes up to it).
+template <int CTRL, int ROWS> __device__ __forceinline__ uint32_t dpp_add(uint32_t v) {
+  return v + (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xf, false);
+}
+__device__ __forceinline__ uint32_t wave_upto(uint32_t v) {
+  v = dpp_add<0x111, 0xf>(v);        // row_shr 1, 2, 4, 8
+  v = dpp_add<0x112, 0xf>(v);
+  v = dpp_add<0x114, 0xf>(v);
+  v = dpp_add<0x118, 0xf>(v);
+  v = dpp_add<0x142, 0xa>(v);        // row_bcast 15: a row's last lane to the next row
+  return dpp_add<0x143, 0xc>(v);     // row_bcast 31: lane 31 to the upper half
+}
+__device__ __forceinline__ uint32_t wave_total(uint32_t v) {
+  return (uint32_t)__builtin_amdgcn_readlane((int)wave_upto(v), 63);
 }
 
-// Of `total` units share w of n is [total w / n, total (w + 1) / n): one to each
-// workgroup, but none is empty.
-__device__ __forceinline__ int64_t shares(const DParams& p, int64_t total) { return min((int64_t)p.wgs, total); }
-// The share that holds unit u.
-__device__ __forceinline__ int share_of(int64_t u, int64_t total, int64_t n) {
-  return (int)((uint64_t)((u + 1) * n - 1) / (uint64_t)total);
+// `total` units in `n` shares, none empty: the first `more` have `per` + 1 units, the
+// others `per`.
+struct Shares {
+  uint32_t n, per, more;
+  __device__ __forceinline__ uint32_t begin(uint32_t w) const { return w * per + min(w, more); }
+  // the share that holds unit u
+  __device__ __forceinline__ uint32_t of(uint32_t u) const {
+    const uint32_t big = more * (per + 1);
+    return u < big ? u / (per + 1) : more + (u - big) / per;
+  }
+};
+__device__ __forceinline__ Shares shares(const DParams& p, uint32_t total) {
+  Shares s;
+  s.n = min((uint32_t)p.wgs, total);
+  s.per = total / s.n;
+  s.more = total - s.per * s.n;
+  return s;
 }
 
 // ---- the split -----------------------------------------------------------------
@@ -136,8 +157,11 @@ __device__ __forceinline__ uint32_t lds_addr(const void* p) { return (uint32_t)(
 // assembly so that the compiler does not make every LDS read wait for it: the
 // tile loop waits itself, before the tile is used. M0 holds the LDS address and
 // needs a wait state before the load that reads it.
-__device__ __forceinline__ void dma16(const uint8_t* src, uint32_t lds) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(src) : "memory");
+template <bool ONCE> __device__ __forceinline__ void dma16(const uint8_t* src, uint32_t lds) {
+  if constexpr (ONCE)
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off nt" ::"s"(lds), "v"(src) : "memory");
+  else
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(src) : "memory");
 }
 
 // 16-byte chunk of a V row in LDS: chunk ^ vswz(row).
@@ -154,8 +178,8 @@ template <class Op> __device__ __forceinline__ float over_query(float v, Op op) 
   return op(__uint_as_float(b[0]), __uint_as_float(b[1]));
 }
 
-template <AttnType T, int D, int NT>
-__global__ __launch_bounds__(64 * kWaves, 2) void decode_split(DParams p) {
+template <AttnType T, int D, int NT, bool ONCE>
+__global__ __launch_bounds__(64 * kWaves, (wgs_per_cu<D, NT>())) void decode_split(DParams p) {
   using IO = PIo<T>;
   constexpr int F = D / 32;          // contraction steps of a score
   constexpr int DT = D / 16;         // tiles of the head dimension
@@ -172,62 +196,69 @@ __global__ __launch_bounds__(64 * kWaves, 2) void decode_split(DParams p) {
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
 
   // The share: sequence b, item `it` of it, from unit `i` on, `left` units.
-  int b = 0, it = 0, i = 0;
-  int64_t left;
+  uint32_t b = 0, it = 0, i = 0, share = blockIdx.x, left;
+  // Lengths of the first 64 sequences stay in the lanes; the others' are read again.
+  const int len64 = lane < p.B ? clamp_length(p.view.lengths[lane], p.view.room) : 0;
   if (p.whole) {
     b = blockIdx.x / p.items;
     it = blockIdx.x - b * p.items;
-    left = units_of(clamp_length(p.view.lengths[b], p.view.room));
+    left = 1;
   } else {
-    const int64_t total = units_before(p, p.B, lane) * p.items;
-    const int64_t parts = shares(p, total);
-    if (blockIdx.x >= parts) return;
-    const int64_t u0 = total * blockIdx.x / parts;
-    left = total * (blockIdx.x + 1) / parts - u0;
-    int64_t base = 0;                // units of the sequences before this 64
+    const uint32_t first64 = lane < p.B ? units_of(p, len64) : 0;
+    uint32_t total = first64;
+    for (int x = lane + 64; x < p.B; x += 64) total += units_of(p, clamp_length(p.view.lengths[x], p.view.room));
+    const Shares sh = shares(p, wave_total(total) * p.items);
+    if (blockIdx.x >= sh.n) return;
+    // Neighbouring shares go to one XCD (workgroups are dealt over the eight in turn).
+    if (sh.n == p.wgs) share = (blockIdx.x & 7) * (p.wgs >> 3) + (blockIdx.x >> 3);
+    const uint32_t u0 = sh.begin(share);
+    left = sh.begin(share + 1) - u0;
+    uint32_t base = 0;               // units of the sequences before this 64
     for (int b0 = 0;; b0 += 64) {
-      const int mine = b0 + lane < p.B ? units_of(clamp_length(p.view.lengths[b0 + lane], p.view.room)) : 0;
-      int64_t upto = mine;
-#pragma unroll
-      for (int o = 1; o < 64; o <<= 1) {
-        const int64_t below = __shfl_up((long long)upto, o);
-        if (lane >= o) upto += below;
-      }
+      const uint32_t mine = b0 == 0 ? first64
+                            : b0 + lane < p.B ? units_of(p, clamp_length(p.view.lengths[b0 + lane], p.view.room)) : 0;
+      const uint32_t upto = wave_upto(mine);
       const uint64_t past = __ballot((base + upto) * p.items > u0);
       if (past) {                    // u0 < total: some sequence ends past it
         const int at = __ffsll((unsigned long long)past) - 1;
         b = b0 + at;
-        const int64_t first = (base + __shfl((long long)(upto - mine), at)) * p.items;
-        const int n = __shfl(mine, at);
-        it = (int)((u0 - first) / n);
-        i = (int)((u0 - first) - (int64_t)it * n);
+        const uint32_t n = (uint32_t)__builtin_amdgcn_readlane((int)mine, at);
+        const uint32_t first = (base + (uint32_t)__builtin_amdgcn_readlane((int)upto, at) - n) * p.items;
+        it = (u0 - first) / n;
+        i = (u0 - first) - it * n;
         break;
       }
-      base += __shfl((long long)upto, 63);
+      base += (uint32_t)__builtin_amdgcn_readlane((int)upto, 63);
     }
   }
   b = __builtin_amdgcn_readfirstlane(b);
   it = __builtin_amdgcn_readfirstlane(it);
   i = __builtin_amdgcn_readfirstlane(i);
+  left = __builtin_amdgcn_readfirstlane(left);
 
   uint8_t* vt = smem + wave * 2 * kStage * 16;
   const int kk = lane & 31;
   const bool second = lane >= 32;    // this half of the wave finds the V rows
+  const int of = kWaves / p.hw;      // waves of a key head
+  const int hd = wave / of, sub = wave - hd * of;
+  const uint32_t sp = second ? p.v_sp : p.k_sp, ss = second ? p.v_ss : p.k_ss;
 
   while (left > 0) {
-    const int len = __builtin_amdgcn_readfirstlane(clamp_length(p.view.lengths[b], p.view.room));
-    const int n = units_of(len);
-    const int take = (int)min(left, (int64_t)(n - i));
-    const int h = it / p.gtiles, q0 = (it - h * p.gtiles) * 16 * NT;   // key head, first query head of the group
-    const int* table = p.view.table + b * p.view.table_rs;
-    const uint8_t* base = second ? p.v + h * p.v_sh : p.k + h * p.k_sh;
-    const int64_t sp = second ? p.v_sp : p.k_sp, ss = second ? p.v_ss : p.k_ss;
+    const int len = b < 64 ? __builtin_amdgcn_readlane(len64, b)
+                           : __builtin_amdgcn_readfirstlane(clamp_length(p.view.lengths[b], p.view.room));
+    const uint32_t n = units_of(p, len);
+    if (p.whole) left = n;
+    const uint32_t take = min(left, n - i);
+    const int hg = (int)it / p.gtiles, q0 = ((int)it - hg * p.gtiles) * 16 * NT;   // first query head of the group
+    const int h = hg * p.hw + hd;                                       // the wave's key head
+    const int* table = p.view.table + (int64_t)b * p.view.table_rs;
+    const uint8_t* base = second ? p.v + 16ull * h * p.v_sh : p.k + 16ull * h * p.k_sh;
 
     i32x4 qf[NT][F];
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
       const int r = q0 + 16 * t + l16;
-      const uint8_t* src = r < p.group ? p.q + b * p.q_sb + (h * p.group + r) * p.q_sh : (const uint8_t*)zero_row;
+      const uint8_t* src = r < p.group ? p.q + (int64_t)b * p.q_sb + (h * p.group + r) * p.q_sh : (const uint8_t*)zero_row;
 #pragma unroll
       for (int f = 0; f < F; ++f) qf[t][f] = *(const i32x4*)(src + 64 * f + 16 * g);
     }
@@ -244,8 +275,9 @@ __global__ __launch_bounds__(64 * kWaves, 2) void decode_split(DParams p) {
 
     i32x4 kf[2][2][F];
     uint32_t live[2];
-    int key = i * kUnit + wave * kTile;                                // the wave's first slot
-    const int end = min(len, (i + take) * kUnit);
+    const int step = 1 << p.shift;
+    int key = (int)(i << p.shift) + sub * kTile;                        // the wave's first slot
+    const int end = (int)min((uint32_t)len, (i + take) << p.shift);
     auto entry = [&](int key0) __attribute__((always_inline)) {
       const int j = key0 + kk;
       return j < end ? table[div_page(p.view.div, j)] : -1;
@@ -256,20 +288,24 @@ __global__ __launch_bounds__(64 * kWaves, 2) void decode_split(DParams p) {
       const int j = key0 + kk;
       const int page = j < end ? checked_page(e, p.view.pages) : -1;
       const int row = j - div_page(p.view.div, j) * p.view.page;
-      rows[wave][second][kk] = (uint64_t)(page >= 0 ? base + page * sp + row * ss : (const uint8_t*)zero_row);
+      rows[wave][second][kk] = (uint64_t)(
+          page >= 0 ? base + 16 * ((uint64_t)(uint32_t)page * sp + (uint64_t)(uint32_t)row * ss) : (const uint8_t*)zero_row);
       live[BUF] = (uint32_t)__ballot(page >= 0);
       __builtin_amdgcn_wave_barrier();
 #pragma unroll
       for (int kt = 0; kt < 2; ++kt) {
         const uint8_t* src = (const uint8_t*)rows[wave][0][16 * kt + l16] + 16 * g;
 #pragma unroll
-        for (int f = 0; f < F; ++f) kf[BUF][kt][f] = *(const i32x4*)(src + 64 * f);
+        for (int f = 0; f < F; ++f) {
+          if constexpr (ONCE) kf[BUF][kt][f] = __builtin_nontemporal_load((const i32x4*)(src + 64 * f));
+          else kf[BUF][kt][f] = *(const i32x4*)(src + 64 * f);
+        }
       }
 #pragma unroll
       for (int x = 0; x < kTile / RPI; ++x) {
         const int r = RPI * x + lane / CH;
         const uint8_t* src = (const uint8_t*)rows[wave][1][r] + 16 * ((lane % CH) ^ vswz<D>(r));
-        dma16(src, lds_addr(vt + (BUF * kStage + 64 * x) * 16));
+        dma16<ONCE>(src, lds_addr(vt + (BUF * kStage + 64 * x) * 16));
       }
     };
     auto compute = [&](auto buf, int key0) __attribute__((always_inline)) {
@@ -352,29 +388,29 @@ __global__ __launch_bounds__(64 * kWaves, 2) void decode_split(DParams p) {
       }
     };
     int e = entry(key);
-    int next = entry(key + kUnit);
+    int next = entry(key + step);
     if (key < end) issue(Buf<0>{}, key, e);
     while (key < end) {
       wait_all();
-      if (key + kUnit < end) {
-        issue(Buf<1>{}, key + kUnit, next);
-        next = entry(key + 2 * kUnit);
+      if (key + step < end) {
+        issue(Buf<1>{}, key + step, next);
+        next = entry(key + 2 * step);
       }
       compute(Buf<0>{}, key);
-      key += kUnit;
+      key += step;
       if (key >= end) break;
       wait_all();
-      if (key + kUnit < end) {
-        issue(Buf<0>{}, key + kUnit, next);
-        next = entry(key + 2 * kUnit);
+      if (key + step < end) {
+        issue(Buf<0>{}, key + step, next);
+        next = entry(key + 2 * step);
       }
       compute(Buf<1>{}, key);
-      key += kUnit;
+      key += step;
     }
 
-    // The waves' results meet: rows of 16 query heads at a time.
+    // The results of a key head's waves meet: 16 query heads at a time.
     const bool whole = take == n;
-    const int64_t part = p.whole ? blockIdx.x : (int64_t)b * p.items + it + blockIdx.x;
+    const int64_t part = p.whole ? share : (int64_t)b * p.items + it + share;
     float* mo = (float*)smem;
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
@@ -388,39 +424,38 @@ __global__ __launch_bounds__(64 * kWaves, 2) void decode_split(DParams p) {
         ml[wave][1][l16] = sum;
       }
       __syncthreads();
-      constexpr int E = D / 16;      // values of a thread
+      constexpr int E = D / 16;      // values of a thread, of 16 to a row
       const int r = tid >> 4, d0 = (tid & 15) * E;
-      float top = ml[0][0][r];
-#pragma unroll
-      for (int x = 1; x < kWaves; ++x) top = fmaxf(top, ml[x][0][r]);
-      float lsum = 0.0f, acc[E];
-#pragma unroll
-      for (int y = 0; y < E; ++y) acc[y] = 0.0f;
-#pragma unroll
-      for (int x = 0; x < kWaves; ++x) {
-        const float f = top == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ml[x][0][r] - top);
-        lsum = fmaf(f, ml[x][1][r], lsum);
-#pragma unroll
-        for (int y = 0; y < E; ++y) acc[y] = fmaf(f, mo[(x * 16 + r) * kPitch + d0 + y], acc[y]);
-      }
       const int row = 16 * t + r;    // in the tile
-      if (q0 + row < p.group) {
+      if (q0 + row >= p.group) continue;
+      for (int y = 0; y < p.hw; ++y) {
+        float top = -INFINITY;
+        for (int x = y * of; x < (y + 1) * of; ++x) top = fmaxf(top, ml[x][0][r]);
+        float lsum = 0.0f, acc[E];
+#pragma unroll
+        for (int e = 0; e < E; ++e) acc[e] = 0.0f;
+        for (int x = y * of; x < (y + 1) * of; ++x) {
+          const float f = __builtin_amdgcn_exp2f(ml[x][0][r] - fmaxf(top, kLowest));
+          lsum = fmaf(f, ml[x][1][r], lsum);
+#pragma unroll
+          for (int e = 0; e < E; ++e) acc[e] = fmaf(f, mo[(x * 16 + r) * kPitch + d0 + e], acc[e]);
+        }
+        const int64_t at = (part * p.hw + y) * p.rows + row;
         if (whole) {
           const float inv = top == -INFINITY ? 0.0f : 1.0f / lsum;   // no slot: 0; only -inf scores: 0 * inf
           uint32_t out[E / 2];
 #pragma unroll
-          for (int y = 0; y < E / 2; ++y) out[y] = IO::pack2(acc[2 * y] * inv, acc[2 * y + 1] * inv);
-          uint8_t* to = p.o + b * p.o_sb + (h * p.group + q0 + row) * p.o_sh + 2 * d0;
+          for (int e = 0; e < E / 2; ++e) out[e] = IO::pack2(acc[2 * e] * inv, acc[2 * e + 1] * inv);
+          uint8_t* to = p.o + (int64_t)b * p.o_sb + ((hg * p.hw + y) * p.group + q0 + row) * p.o_sh + 2 * d0;
           if constexpr (E == 8) *(u32x4*)to = u32x4{out[0], out[1], out[2], out[3]};
           else *(u32x2*)to = u32x2{out[0], out[1]};
         } else {
-          float* to = p.po + (part * p.rows + row) * D + d0;
 #pragma unroll
-          for (int y = 0; y < E; y += 4) *(f32x4*)(to + y) = f32x4{acc[y], acc[y + 1], acc[y + 2], acc[y + 3]};
+          for (int e = 0; e < E; e += 4) *(f32x4*)(p.po + at * D + d0 + e) = f32x4{acc[e], acc[e + 1], acc[e + 2], acc[e + 3]};
         }
         if (d0 == 0 && (!whole || p.scores)) {
-          p.ml[(part * p.rows + row) * 2] = top;
-          p.ml[(part * p.rows + row) * 2 + 1] = lsum;
+          p.ml[2 * at] = top;
+          p.ml[2 * at + 1] = lsum;
         }
       }
     }
@@ -443,106 +478,193 @@ struct Parts {
   int64_t first;
   int count;
 };
-__device__ __forceinline__ Parts parts_of(const DParams& p, int b, int it, int64_t before, int64_t total, int n) {
+__device__ __forceinline__ Parts parts_of(const DParams& p, const Shares& sh, uint32_t before, uint32_t n, int b, int it) {
   const int64_t item = (int64_t)b * p.items + it;
   if (p.whole) return {item, 1};
-  const int64_t u = before * p.items + (int64_t)it * n;
-  const int64_t wgs = shares(p, total);
-  const int w0 = share_of(u, total, wgs), w1 = share_of(u + n - 1, total, wgs);
-  return {item + w0, w1 - w0 + 1};
+  const uint32_t u = before + it * n, w0 = sh.of(u), w1 = sh.of(u + n - 1);
+  return {item + w0, (int)(w1 - w0) + 1};
 }
 
-// Workgroups below `heads` of the grid add up the parts of one query head's O; the
-// others give 1024 slots of a key head their weights.
+// The parts of a query head's O from part `y0` on in steps of `by`, added up by lanes
+// of V values each: acc, maximum and sum over them.
+template <int V>
+__device__ __forceinline__ void add_parts(const float* ml, const float* po, int64_t each, int D, int count, int y0,
+                                          int by, float (&acc)[V], float& m, float& l) {
+  typedef float vec __attribute__((ext_vector_type(V)));
+#pragma unroll
+  for (int e = 0; e < V; ++e) acc[e] = 0.0f;
+  m = -INFINITY;
+  l = 0.0f;
+  for (int y = y0; y < count; y += 4 * by) {
+    vec v[4];
+    float pm[4], pl[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {            // all loads first; a part too far counts as one of no slot
+      const int64_t at = min(y + u * by, count - 1) * each;
+      v[u] = *(const vec*)(po + at * D);
+      pm[u] = y + u * by < count ? ml[2 * at] : -INFINITY;
+      pl[u] = ml[2 * at + 1];
+    }
+    const float top = fmaxf(fmaxf(m, fmaxf(pm[0], pm[1])), fmaxf(pm[2], pm[3]));
+    const float from = fmaxf(top, kLowest);  // -inf - from is -inf
+    const float f = __builtin_amdgcn_exp2f(m - from);
+    m = top;
+    l *= f;
+#pragma unroll
+    for (int e = 0; e < V; ++e) acc[e] *= f;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const float w = __builtin_amdgcn_exp2f(pm[u] - from);
+      l = fmaf(w, pl[u], l);
+#pragma unroll
+      for (int e = 0; e < V; ++e) acc[e] = fmaf(w, ((const float*)&v[u])[e], acc[e]);
+    }
+  }
+}
+
+// For sequence blockIdx.y: workgroups below `outs` add up the parts of `apiece` query
+// heads' O (4: a wave each, 1: the workgroup together), the others give 1024 slots of
+// a key head their weights.
 template <AttnType T, int D>
-__global__ __launch_bounds__(256) void decode_join(DParams p, int64_t outs, int64_t chunks, int64_t jobs) {
+__global__ __launch_bounds__(256) void decode_join(DParams p, uint32_t outs, int apiece, uint32_t chunks) {
   using IO = PIo<T>;
   constexpr int LD = D / 4, NP = 256 / LD;   // lanes of a part, parts at a time
-  __shared__ float red[NP][D], top4[4], lred[NP];
+  __shared__ float red[NP][D], mred[NP], lred[NP];
   __shared__ float stat[1024][2];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int64_t total = p.whole ? 0 : units_before(p, p.B, lane) * p.items;
-  for (int64_t job = blockIdx.x; job < jobs; job += gridDim.x) {
-    const bool weights = job >= outs;
-    const int64_t bh = weights ? (job - outs) / chunks : job;
-    const int b = (int)(bh / (weights ? p.heads : p.H));
-    const int head = (int)(bh - (int64_t)b * (weights ? p.heads : p.H));
-    const int len = clamp_length(p.view.lengths[b], p.view.room), n = units_of(len);
-    const int64_t before = p.whole ? 0 : units_before(p, b, lane);
-    if (!weights) {
-      const int h = head / p.group, r = head - h * p.group;
-      const int gt = r / p.rows, row = r - gt * p.rows;
-      const Parts x = parts_of(p, b, h * p.gtiles + gt, before, total, n);
-      if (x.count == 1) continue;            // decode_split had all of it
-      const float* ml = p.ml + (x.first * p.rows + row) * 2;
-      const float* po = p.po + (x.first * p.rows + row) * D;
-      float top = -INFINITY;
-      for (int y = tid; y < x.count; y += 256) top = fmaxf(top, ml[(int64_t)y * p.rows * 2]);
-      top = wave_max(top);
-      __syncthreads();
-      if (lane == 0) top4[wave] = top;
-      __syncthreads();
-      top = fmaxf(fmaxf(top4[0], top4[1]), fmaxf(top4[2], top4[3]));
-      const int part = tid / LD, d = (tid % LD) * 4;
-      f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
-      float l = 0.0f;
-      for (int y = part; y < x.count; y += NP) {
-        const float* s = ml + (int64_t)y * p.rows * 2;
-        const float f = top == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(s[0] - top);
-        l = fmaf(f, s[1], l);
-        acc += *(const f32x4*)(po + (int64_t)y * p.rows * D + d) * f;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const bool weights = blockIdx.x >= outs;
+  int head = weights ? (blockIdx.x - outs) / chunks : blockIdx.x;
+  if (!weights && apiece == 4) head = __builtin_amdgcn_readfirstlane(4 * head + (tid >> 6));
+  for (int b = blockIdx.y; b < p.B; b += gridDim.y) {
+    const int len = clamp_length(p.view.lengths[b], p.view.room);
+    const uint32_t n = units_of(p, len);
+    uint32_t before = 0, total = 0;          // units of all sequences, of those before b
+    if (!p.whole) {
+      for (int x = lane; x < p.B; x += 64) {
+        const uint32_t m = units_of(p, clamp_length(p.view.lengths[x], p.view.room));
+        total += m;
+        before += x < b ? m : 0;
       }
-      *(f32x4*)&red[part][d] = acc;
-      if (d == 0) lred[part] = l;
+      total = wave_total(total) * p.items;
+      before = wave_total(before) * p.items;
+    } else {
+      total = 1;
+    }
+    const Shares sh = shares(p, total);
+    if (!weights) {
+      if (head >= p.H) continue;             // (a wave that has none)
+      const int h = head / p.group, r = head - h * p.group;
+      const int gt = r / p.rows, row = r - gt * p.rows, each = p.hw * p.rows;
+      const Parts x = parts_of(p, sh, before, n, b, h / p.hw * p.gtiles + gt);
+      if (x.count == 1) continue;            // decode_split had all of it
+      const int64_t from = x.first * each + h % p.hw * p.rows + row;
+      const float* ml = p.ml + from * 2;
+      const float* po = p.po + from * D;
+      uint8_t* out = p.o + (int64_t)b * p.o_sb + (int64_t)head * p.o_sh;
+      float m, l;
+      if (apiece == 4) {
+        float acc[D / 64];
+        add_parts<D / 64>(ml, po + lane * (D / 64), each, D, x.count, 0, 1, acc, m, l);
+        const float inv = m == -INFINITY ? 0.0f : 1.0f / l;
+        const uint32_t w = IO::pack2(acc[0] * inv, acc[D / 64 - 1] * inv);
+        if constexpr (D == 128) *(uint32_t*)(out + 4 * lane) = w;
+        else *(uint16_t*)(out + 2 * lane) = (uint16_t)w;
+        continue;
+      }
+      const int part = tid / LD, d = (tid % LD) * 4;
+      float acc[4];
+      add_parts<4>(ml, po + d, each, D, x.count, part, NP, acc, m, l);
+      *(f32x4*)&red[part][d] = f32x4{acc[0], acc[1], acc[2], acc[3]};
+      if (d == 0) {
+        mred[part] = m;
+        lred[part] = l;
+      }
       __syncthreads();
       if (tid < D / 2) {
+        float top = mred[0];
+#pragma unroll
+        for (int y = 1; y < NP; ++y) top = fmaxf(top, mred[y]);
         float a0 = 0.0f, a1 = 0.0f, sum = 0.0f;
 #pragma unroll
         for (int y = 0; y < NP; ++y) {
-          a0 += red[y][2 * tid];
-          a1 += red[y][2 * tid + 1];
-          sum += lred[y];
+          const float f = __builtin_amdgcn_exp2f(mred[y] - fmaxf(top, kLowest));
+          a0 = fmaf(f, red[y][2 * tid], a0);
+          a1 = fmaf(f, red[y][2 * tid + 1], a1);
+          sum = fmaf(f, lred[y], sum);
         }
         const float inv = top == -INFINITY ? 0.0f : 1.0f / sum;
-        *(uint32_t*)(p.o + b * p.o_sb + head * p.o_sh + 4 * tid) = IO::pack2(a0 * inv, a1 * inv);
+        *(uint32_t*)(out + 4 * tid) = IO::pack2(a0 * inv, a1 * inv);
       }
       __syncthreads();
       continue;
     }
-    const int j0 = (int)((job - outs) % chunks) * 1024;
+    const int j0 = (int)((blockIdx.x - outs) % chunks) * 1024;
     if (j0 >= len) continue;
-    __syncthreads();
-    for (int r = tid; r < p.group; r += 256) {
-      const int gt = r / p.rows, row = r - gt * p.rows;
-      const Parts x = parts_of(p, b, head * p.gtiles + gt, before, total, n);
-      const float* ml = p.ml + (x.first * p.rows + row) * 2;
-      float top = -INFINITY, l = 0.0f;
-      for (int y = 0; y < x.count; ++y) top = fmaxf(top, ml[(int64_t)y * p.rows * 2]);
-      for (int y = 0; y < x.count; ++y) {
-        const float* s = ml + (int64_t)y * p.rows * 2;
-        if (top != -INFINITY) l = fmaf(__builtin_amdgcn_exp2f(s[0] - top), s[1], l);
-      }
-      stat[r][0] = top;
-      stat[r][1] = __builtin_amdgcn_exp2f(IO::kTop) / l;   // the sum has the weights' scale
-    }
-    __syncthreads();
+    // What the past steps gave the thread's four slots: it comes meanwhile.
     float* w = p.w + b * p.w_sb + head * p.w_sh;
     const float* sc = p.scores + ((int64_t)b * p.H + head * p.group) * p.slots;
-    for (int j = j0 + tid; j < min(len, j0 + 1024); j += 256) {
-      float a = 0.0f;
-      for (int r = 0; r < p.group; ++r) {
-        const float s = sc[(int64_t)r * p.slots + j];
-        if (__float_as_uint(s) != kAbsent) a = fmaf(__builtin_amdgcn_exp2f(s - stat[r][0]), stat[r][1], a);
-      }
-      w[j] = p.decay == 0.0f ? a : fmaf(p.decay, w[j], a);
+    float old[4], a[4];
+    int at[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      at[u] = min(j0 + 256 * u + tid, len - 1);
+      old[u] = p.decay == 0.0f ? 0.0f : w[at[u]];
+      a[u] = 0.0f;
     }
+    // Sixteen lanes to a query head's parts.
+    for (int r0 = 0; r0 < p.group; r0 += 16) {
+      const int r = r0 + (tid >> 4);
+      float m = -INFINITY, l = 0.0f;
+      if (r < p.group) {
+        const int gt = r / p.rows, row = r - gt * p.rows;
+        const Parts x = parts_of(p, sh, before, n, b, head / p.hw * p.gtiles + gt);
+        const float* ml = p.ml + (x.first * p.hw * p.rows + head % p.hw * p.rows + row) * 2;
+        for (int y = tid & 15; y < x.count; y += 16) {
+          const float* s = ml + (int64_t)y * p.hw * p.rows * 2;
+          const float top = fmaxf(m, s[0]), from = fmaxf(top, kLowest);
+          l = fmaf(__builtin_amdgcn_exp2f(s[0] - from), s[1], l * __builtin_amdgcn_exp2f(m - from));
+          m = top;
+        }
+      }
+#pragma unroll
+      for (int o = 1; o < 16; o <<= 1) {
+        const float om = __shfl_xor(m, o), ol = __shfl_xor(l, o);
+        const float top = fmaxf(m, om), from = fmaxf(top, kLowest);
+        l = fmaf(__builtin_amdgcn_exp2f(om - from), ol, l * __builtin_amdgcn_exp2f(m - from));
+        m = top;
+      }
+      if (r < p.group && (tid & 15) == 0) {
+        stat[r][0] = m;
+        stat[r][1] = __builtin_amdgcn_exp2f(IO::kTop) / l;   // the sum has the weights' scale
+      }
+    }
+    __syncthreads();
+#pragma unroll 2
+    for (int r = 0; r < p.group; ++r) {
+      float s[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) s[u] = sc[(int64_t)r * p.slots + at[u]];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const float x = __builtin_amdgcn_exp2f(s[u] - stat[r][0]) * stat[r][1];
+        a[u] += __float_as_uint(s[u]) == kAbsent ? 0.0f : x;
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+      if (j0 + 256 * u + tid < len) w[at[u]] = p.decay == 0.0f ? a[u] : fmaf(p.decay, old[u], a[u]);
+    __syncthreads();
   }
 }
 
 // ---- launch --------------------------------------------------------------------
 
+// Heads of a slot lie next to each other ([pages, P, Hkv, D] memory), rather than the
+// slots of a head.
+bool neighbours(int64_t head_stride, int64_t slot_stride) { return head_stride < slot_stride; }
+
 struct Plan {
-  int nt, gtiles, rows, wgs;
+  int nt, hw, gtiles, rows, wgs;
   bool whole;
   int64_t items, slots;
   size_t ml, po, scores;     // floats of the workspace, 16-byte multiples
@@ -555,30 +677,46 @@ int compute_units() {
   return std::max(8, cus / 8 * 8);
 }
 
-Plan plan_of(int B, int H, int heads, int D, int W, int page, bool weights) {
+Plan plan_of(int B, int H, int heads, int D, int W, int page, bool neighbours, bool weights) {
   Plan x{};
   const int group = H / heads;
   x.nt = group > 16 ? 2 : 1;
   x.gtiles = (group + 16 * x.nt - 1) / (16 * x.nt);
   x.rows = std::min(group, 16 * x.nt);
-  x.items = (int64_t)B * heads * x.gtiles;
-  x.slots = ((int64_t)W * page + kUnit - 1) / kUnit * kUnit;
-  x.whole = (int64_t)W * page <= 2 * kUnit && x.items <= (1 << 20);
-  x.wgs = x.whole ? (int)x.items : 2 * compute_units();
+  x.slots = ((int64_t)W * page + 127) / 128 * 128;
+  // A workgroup per (sequence, head) and no join where no sequence is long: up to 256
+  // slots always, up to 512 where there are workgroups enough to read as fast as the
+  // memory gives (a CU alone reads about 46 GB/s). us, split and joined / whole: 32 x 8
+  // heads of 300 slots 20.0 / 11.4, of 500 21.1 / 15.9, 16 x 8 of 500 14.6 / 14.2, but
+  // 4 x 8 of 500 10.9 / 12.4, 8 x 8 of 1000 14.4 / 23.0, 64 x 8 of 20 to 1000 35.8 / 38.2.
+  const int64_t room = (int64_t)W * page, each = (int64_t)B * heads * x.gtiles;
+  x.whole = (room <= 256 || (room <= 512 && each >= 128)) && each <= (1 << 20);
+  // Where the heads of a slot lie together, a workgroup takes up to four of them (a
+  // wave each), so that what it reads at a time does: 16 sequences of 8192, 8 heads of
+  // 128, 103 us with one head, 93 with four (90 where the slots of a head lie
+  // together). Not where that leaves few items, of many parts each: one sequence of
+  // 8000, 15.9 us with one head, 21.7 with four.
+  x.hw = 1;
+  if (!x.whole && neighbours)
+    for (int hw = 4; hw > 1 && x.hw == 1; hw /= 2)
+      if (heads % hw == 0 && (int64_t)B * (heads / hw) * x.gtiles >= 64) x.hw = hw;
+  x.items = (int64_t)B * (heads / x.hw) * x.gtiles;
+  x.wgs = x.whole ? (int)x.items : (D == 64 && x.nt == 1 ? 3 : 2) * compute_units();
   const size_t parts = x.whole ? (size_t)x.items : (size_t)x.items + x.wgs;
-  if (weights || !x.whole) x.ml = (parts * x.rows * 2 + 3) / 4 * 4;
-  if (!x.whole) x.po = parts * x.rows * D;
+  if (weights || !x.whole) x.ml = (parts * x.hw * x.rows * 2 + 3) / 4 * 4;
+  if (!x.whole) x.po = parts * x.hw * x.rows * D;
   if (weights) x.scores = (size_t)B * H * x.slots;
   return x;
 }
 
 template <AttnType T, int D>
 hipError_t run(const PagedAttnDesc& d, hipStream_t s) {
-  const Plan x = plan_of(d.c.B, d.H, d.c.heads, D, d.c.W, d.c.page, d.weights != nullptr);
+  const Plan x = plan_of(d.c.B, d.H, d.c.heads, D, d.c.W, d.c.page, neighbours(d.c.k_sh, d.c.k_ss),
+                         d.weights != nullptr);
   DParams p{};
   p.view = {d.c.table, d.c.table_rs, d.c.lengths, d.c.pages, d.c.page, d.c.W * d.c.page, page_div(d.c.page)};
-  p.k = (const uint8_t*)d.c.k; p.k_sp = 2 * d.c.k_sp; p.k_sh = 2 * d.c.k_sh; p.k_ss = 2 * d.c.k_ss;
-  p.v = (const uint8_t*)d.c.v; p.v_sp = 2 * d.c.v_sp; p.v_sh = 2 * d.c.v_sh; p.v_ss = 2 * d.c.v_ss;
+  p.k = (const uint8_t*)d.c.k; p.k_sp = d.c.k_sp / 8; p.k_sh = d.c.k_sh / 8; p.k_ss = d.c.k_ss / 8;
+  p.v = (const uint8_t*)d.c.v; p.v_sp = d.c.v_sp / 8; p.v_sh = d.c.v_sh / 8; p.v_ss = d.c.v_ss / 8;
   p.q = (const uint8_t*)d.q; p.q_sb = 2 * d.q_sb; p.q_sh = 2 * d.q_sh;
   p.o = (uint8_t*)d.o; p.o_sb = 2 * d.o_sb; p.o_sh = 2 * d.o_sh;
   p.w = d.weights; p.w_sb = d.w_sb; p.w_sh = d.w_sh;
@@ -589,25 +727,35 @@ hipError_t run(const PagedAttnDesc& d, hipStream_t s) {
   p.scores = d.weights ? ws + x.ml + x.po : nullptr;
   p.slots = x.slots;
   p.B = d.c.B; p.H = d.H; p.heads = d.c.heads; p.group = d.H / d.c.heads;
-  p.gtiles = x.gtiles; p.items = d.c.heads * x.gtiles; p.rows = x.rows; p.wgs = x.wgs; p.whole = x.whole;
+  p.hw = x.hw; p.shift = x.hw == 4 ? 5 : x.hw == 2 ? 6 : 7;
+  p.gtiles = x.gtiles; p.items = d.c.heads / x.hw * x.gtiles; p.rows = x.rows; p.wgs = x.wgs; p.whole = x.whole;
   p.c = d.scale * 1.4426950408889634f;
-  if (x.nt == 1) hipLaunchKernelGGL((decode_split<T, D, 1>), dim3(x.wgs), dim3(64 * kWaves), 0, s, p);
-  else hipLaunchKernelGGL((decode_split<T, D, 2>), dim3(x.wgs), dim3(64 * kWaves), 0, s, p);
+  const dim3 grid(x.wgs), threads(64 * kWaves);
+  auto go = [&](auto kern) { hipLaunchKernelGGL(kern, grid, threads, 0, s, p); };
+  if (x.nt == 1) go(decode_split<T, D, 1, true>);
+  else if (x.gtiles == 1) go(decode_split<T, D, 2, true>);
+  else go(decode_split<T, D, 2, false>);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess || (x.whole && !d.weights)) return e;
-  const int64_t outs = x.whole ? 0 : (int64_t)p.B * p.H;
-  const int64_t chunks = ((int64_t)d.c.W * d.c.page + 1023) / 1024;
-  const int64_t jobs = outs + (d.weights ? (int64_t)p.B * p.heads * chunks : 0);
-  hipLaunchKernelGGL((decode_join<T, D>), dim3((unsigned)std::min<int64_t>(jobs, 1 << 20)), dim3(256), 0, s, p, outs,
-                     chunks, jobs);
+  const int apiece = (int64_t)p.B * p.H >= 512 ? 4 : 1;
+  const int64_t outs = x.whole ? 0 : (p.H + apiece - 1) / apiece, chunks = ((int64_t)d.c.W * d.c.page + 1023) / 1024;
+  const int64_t jobs = outs + (d.weights ? p.heads * chunks : 0);
+  if (jobs > max_workgroups(256)) return hipErrorNotSupported;
+  hipLaunchKernelGGL((decode_join<T, D>), dim3((unsigned)jobs, (unsigned)std::min(p.B, 65535)), dim3(256), 0, s, p,
+                     (uint32_t)outs, apiece, (uint32_t)chunks);
   return hipGetLastError();
 }
 
 }  // namespace
 
-size_t paged_attention_workspace(int B, int H, int heads, int D, int W, int page, bool weights) {
-  const Plan x = plan_of(B, H, heads, D, W, page, weights);
+size_t paged_attention_workspace(const PagedCache& c, int H, bool weights) {
+  const Plan x = plan_of(c.B, H, c.heads, c.D, c.W, c.page, neighbours(c.k_sh, c.k_ss), weights);
   return (x.ml + x.po + x.scores) * sizeof(float);
+}
+
+bool paged_attention_fits(const PagedCache& c, int H) {
+  const Plan x = plan_of(c.B, H, c.heads, c.D, c.W, c.page, neighbours(c.k_sh, c.k_ss), false);
+  return (double)x.items * (x.slots / 32) < 0x1p31;
 }
 
 hipError_t launch_paged_attention(AttnType t, const PagedAttnDesc& d, hipStream_t s) {

@@ -172,9 +172,11 @@ struct PagedAttnDesc {
   void* ws;
 };
 hipError_t launch_paged_attention(AttnType t, const PagedAttnDesc& d, hipStream_t s);
-// Workspace bytes of a call: B sequences of W * page slots, H query heads on
-// `heads` key heads, with or without the slots' weights.
-size_t paged_attention_workspace(int B, int H, int heads, int D, int W, int page, bool weights);
+// Workspace bytes of a call with H query heads (c's pointers are not looked at),
+// with or without the slots' weights.
+size_t paged_attention_workspace(const PagedCache& c, int H, bool weights);
+// Whether the kernels can count the slots that the table has room for.
+bool paged_attention_fits(const PagedCache& c, int H);
 
 struct PagedEvictDesc {
   PagedCache c;
