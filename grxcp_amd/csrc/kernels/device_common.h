@@ -97,6 +97,20 @@ __device__ __forceinline__ float wave_max(float v) {
   return wave_reduce(v, [](float a, float b) { return fmaxf(a, b); });
 }
 
+// Each lane's sum of the lanes up to it, in the ALU: within rows of 16 lanes, then a
+// row's last lane to the next row, then lane 31 to the upper half.
+template <int CTRL, int ROWS> __device__ __forceinline__ uint32_t dpp_add(uint32_t v) {
+  return v + (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xf, false);
+}
+__device__ __forceinline__ uint32_t wave_upto(uint32_t v) {
+  v = dpp_add<0x111, 0xf>(v);   // row_shr 1, 2, 4, 8
+  v = dpp_add<0x112, 0xf>(v);
+  v = dpp_add<0x114, 0xf>(v);
+  v = dpp_add<0x118, 0xf>(v);
+  v = dpp_add<0x142, 0xa>(v);   // row_bcast 15
+  return dpp_add<0x143, 0xc>(v);   // row_bcast 31
+}
+
 // ---- cycle probe -------------------------------------------------------------
 // One grxCycleSlot per wave, written by lane 0 with an ordinary (vector)
 // global store. `core` = XCD id << 16 | CU-level hardware id bits, so slots

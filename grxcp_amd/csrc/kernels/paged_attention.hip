@@ -110,19 +110,6 @@ __device__ __forceinline__ uint32_t units_of(const DParams& p, int len) {
   return max(1u, ((uint32_t)len + (1u << p.shift) - 1) >> p.shift);
 }
 
-// Sums over the wave in the ALU: rows of 16 lanes, then across them (all lanes get
-// the total of `total`; `upto` is each lane's sum of the lanes up to it).
-template <int CTRL, int ROWS> __device__ __forceinline__ uint32_t dpp_add(uint32_t v) {
-  return v + (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xf, false);
-}
-__device__ __forceinline__ uint32_t wave_upto(uint32_t v) {
-  v = dpp_add<0x111, 0xf>(v);        // row_shr 1, 2, 4, 8
-  v = dpp_add<0x112, 0xf>(v);
-  v = dpp_add<0x114, 0xf>(v);
-  v = dpp_add<0x118, 0xf>(v);
-  v = dpp_add<0x142, 0xa>(v);        // row_bcast 15: a row's last lane to the next row
-  return dpp_add<0x143, 0xc>(v);     // row_bcast 31: lane 31 to the upper half
-}
 __device__ __forceinline__ uint32_t wave_total(uint32_t v) {
   return (uint32_t)__builtin_amdgcn_readlane((int)wave_upto(v), 63);
 }

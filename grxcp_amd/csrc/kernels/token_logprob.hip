@@ -4,8 +4,8 @@
 // New: the reference plans softmax for grxDNN (ref
 // docs/designs/grxcp_roadmap.md:864-877) and ships no code.
 //
-// Forward: one pass over the logits. A row, or a piece of it where rows are few,
-// goes to a workgroup; every thread keeps
+// Forward: one pass over the logits. A row, or a piece of it where rows are few, goes
+// to a wave; every lane keeps
 //   s = sum 2^(x log2 e - r),  t = sum 2^(x log2 e - r) (x log2 e - r)
 // over its elements with a reference r of its own that moves only when a batch's
 // maximum exceeds it by more than 8, so an element costs an unpack, half a max, two
@@ -15,17 +15,17 @@
 // log S - T / S from the sums moved to the row's maximum.
 // Products x log2 e are good to 2^-25 |x| (fma), which is enough within |x| <= 64:
 // a row whose maximum is outside, or whose sums are not finite, is read again with
-// x - max formed first (careful_sums).
+// x - max formed first.
 //
 // Alternatives: the same pass compares each batch's maximum with a threshold that K
 // elements already read reach, and only where it is higher looks at the elements: those
-// above go to a list in LDS. The first threshold is the K-th largest of the threads' (or
-// groups of four threads') maxima over the first batch; it is raised after batches 4,
-// 16, 64, ... from the list, so a row of random order pushes about K + 3 K + 3 K + ... of
-// its elements. Elements are ranked by value, then by lower index; as batches come in
-// index order an equal value later never outranks one in the list. A list that runs over (an
-// ordered row), NaN and +inf take the direct way: the largest element below the last one,
-// K times.
+// from it on go to a list in LDS. The first threshold is the K-th
+// largest of the 128 maxima of the wave's lanes' half batches; it is raised after batches
+// 2, 4, 8, ... to the list's K-th largest, so a wave lists about K of every doubling of
+// what it has read. Elements are ranked by value, then by lower index; as batches come in
+// index order an equal value in a later batch never outranks one in the list. A list that
+// runs over (an ordered row, one of equal values), NaN and +inf take the direct way: the
+// largest element below the last one, K times.
 //
 // Backward: one element-wise pass, bound by reading x and writing dx.
 
@@ -35,15 +35,16 @@
 #include "row_io.h"
 
 #include <algorithm>
+#include <climits>
 
 namespace grxk {
 namespace {
 
 constexpr float kLog2e = 1.4426950408889634f, kLog2eLow = 1.925963033e-8f, kLn2 = 0.6931471805599453f;
 constexpr float kLowest = -__FLT_MAX__;
-constexpr int kU = 4;         // chunks of a thread's batch
+constexpr int kU = 4;         // chunks of a thread (backward, and a forward batch of a whole row)
 constexpr int kMaxTop = 64;
-constexpr int kMaxPieces = 32;
+constexpr int kMaxPieces = 64, kMaxKeys = 1024;   // of a row, and what they list
 
 struct LParams {
   const uint8_t* x;
@@ -75,79 +76,122 @@ __device__ __forceinline__ float key_value(uint64_t k) {
 struct Sums {
   float m, s, t;
 };
-__device__ __forceinline__ Sums both(Sums a, Sums b) {
-  const float m = fmaxf(a.m, b.m);
-  const float fa = __builtin_amdgcn_exp2f((a.m - m) * kLog2e), fb = __builtin_amdgcn_exp2f((b.m - m) * kLog2e);
-  Sums r;
-  r.m = m;
-  r.s = fmaf(fa, a.s, fb * b.s);
-  // the weight of a part of no sum is 0 however far its maximum is
-  r.t = fa * a.t + fb * b.t;
-  r.t += a.s != 0.0f && fa != 0.0f ? fa * a.s * (a.m - m) : 0.0f;
-  r.t += b.s != 0.0f && fb != 0.0f ? fb * b.s * (b.m - m) : 0.0f;
-  return r;
-}
-__device__ __forceinline__ Sums wave_both(Sums v) {
-#pragma unroll
-  for (int o = 32; o; o >>= 1) v = both(v, {__shfl_xor(v.m, o), __shfl_xor(v.s, o), __shfl_xor(v.t, o)});
-  return v;
+// The same relative to m >= v.m. A part without a sum stays without one.
+__device__ __forceinline__ Sums moved(Sums v, float m) {
+  const float d = v.m - m, f = __builtin_amdgcn_exp2f(d * kLog2e);
+  const float t = fmaf(v.s, d, v.t);
+  return {m, v.s * f, v.s == 0.0f || f == 0.0f ? 0.0f : t * f};
 }
 
-// Number of the c keys that are larger than k.
+// Number of the first c keys that are larger than k. The list is read two keys at a
+// time; what lies behind its end (up to a multiple of 8) is not counted.
+typedef unsigned long long u64x2 __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ int rank_of(const uint64_t* keys, int c, uint64_t k) {
   int r = 0;
-#pragma unroll 4
-  for (int i = 0; i < c; ++i) r += keys[i] > k;
+  for (int i = 0; i < c; i += 8) {
+    u64x2 w[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) w[j] = ((const u64x2*)keys)[i / 2 + j];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      r += i + 2 * j < c && w[j][0] > k;
+      r += i + 2 * j + 1 < c && w[j][1] > k;
+    }
+  }
   return r;
 }
 
-template <int NW> __device__ __forceinline__ void sync() {
-  if constexpr (NW > 1) __syncthreads();
-  else __builtin_amdgcn_wave_barrier();
+// The largest key that K of the wave's keys reach, N of them to a lane, or one a little
+// below it: bit by bit from the top, as far down as keys of T differ. 0 if there are
+// fewer than K above 0.
+template <NormType T, int N> __device__ __forceinline__ uint32_t reached_by(const uint32_t (&key)[N], int K) {
+  constexpr int kLast = T == NormType::F32 ? 0 : T == NormType::BF16 ? 16 : 13;
+  uint32_t v = 0;
+  for (int bit = 31; bit >= kLast; --bit) {
+    const uint32_t t = v | (1u << bit);
+    int c = 0;
+#pragma unroll
+    for (int q = 0; q < N; ++q) c += __popcll(__ballot(key[q] >= t));
+    if (c >= K) v = t;
+    if (c == K) break;
+  }
+  return v;
+}
+// A bound's value; -inf for what is below every value.
+__device__ __forceinline__ float bound_value(uint32_t key) {
+  return key <= 0x007fffffu ? -INFINITY : key_value((uint64_t)key << 32);
+}
+// The next value above x (x is no NaN): of -0 as of 0.
+__device__ __forceinline__ float above(float x) {
+  const uint32_t u = order_key(__float_as_uint(x));
+  return x == INFINITY ? x : key_value((uint64_t)(u + 1) << 32);
 }
 
-template <int NW>
+// The list of a wave. A row may list all of its elements where it has fewer than K for
+// every lane.
+constexpr int kCap = 512;
 struct Shared {
-  static constexpr int kCap = NW == 1 ? 512 : 1024;   // keys of the list
-  Sums sums[NW];
-  uint64_t list[kCap], best[kMaxTop];
-  uint64_t groups[64 * NW];
-  uint64_t threshold;
-  int count;
+  __attribute__((aligned(16))) uint64_t list[kCap];
+  uint64_t best[kMaxTop];
 };
 
-// The list's K largest keys in order at its front, and the K-th as the threshold.
-template <int NW>
-__device__ __forceinline__ void shorten(Shared<NW>& sh, int top) {
-  const int tid = threadIdx.x;
-  sync<NW>();
-  const int c = min(sh.count, Shared<NW>::kCap);
-  for (int i = tid; i < c; i += 64 * NW) {
+// Of a list of c <= 64 N keys what reaches the bound that K of them reach; returns that
+// bound.
+template <NormType T, int N>
+__device__ __forceinline__ uint32_t refine(uint64_t* list, int& c, int top) {
+  const int lane = threadIdx.x;
+  uint64_t key[N];
+  uint32_t hi[N];
+#pragma unroll
+  for (int q = 0; q < N; ++q) {
+    key[q] = 64 * q + lane < c ? list[64 * q + lane] : 0;
+    hi[q] = (uint32_t)(key[q] >> 32);
+  }
+  const uint32_t bound = max(reached_by<T>(hi, top), 1u);
+  int to = 0;
+#pragma unroll
+  for (int q = 0; q < N; ++q) {
+    const uint64_t stay = __ballot(hi[q] >= bound);
+    if (hi[q] >= bound)
+      list[to + (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(stay >> 32),
+                                               __builtin_amdgcn_mbcnt_lo((uint32_t)stay, 0))] = key[q];
+    to += __popcll(stay);
+  }
+  c = to;
+  return bound;
+}
+template <NormType T>
+__device__ __forceinline__ uint32_t refine_list(uint64_t* list, int& c, int top) {
+  return c <= 64 ? refine<T, 1>(list, c, top) : refine<T, kCap / 64>(list, c, top);
+}
+
+// The K largest of a list of c keys, in order in `best`. Returns how many there are.
+template <NormType T>
+__device__ __forceinline__ int finish(Shared& sh, int top, int c) {
+  if (c > 64) refine_list<T>(sh.list, c, top);   // (a short list is ranked as it is)
+  __builtin_amdgcn_wave_barrier();
+  for (int i = threadIdx.x; i < c; i += 64) {
     const uint64_t k = sh.list[i];
     const int r = rank_of(sh.list, c, k);
     if (r < top) sh.best[r] = k;
   }
-  sync<NW>();
-  if (tid < min(c, top)) sh.list[tid] = sh.best[tid];
-  if (tid == 0 && c >= top) {
-    sh.threshold = sh.best[top - 1];
-    sh.count = top;
-  }
-  sync<NW>();
+  __builtin_amdgcn_wave_barrier();
+  return min(c, top);
 }
 
-// One piece of a row per workgroup of NW waves.
-template <NormType T, bool AL, int NW, bool TOP>
-__global__ __launch_bounds__(64 * NW) void logprob_pieces(LParams p) {
+// One row, or a piece of one, per wave.
+template <NormType T, bool AL, bool TOP>
+__global__ __launch_bounds__(64, AL ? 4 : 3) void logprob_pieces(LParams p) {
   using IO = Io<T>;
-  constexpr int V = IO::kVec, NT = 64 * NW;
+  constexpr int V = IO::kVec, NT = 64, U = kU;
   constexpr uint32_t kNone = T == NormType::F32 ? 0xff800000u : T == NormType::BF16 ? 0xff80ff80u : 0xfc00fc00u;
   const u32x4 none = {kNone, kNone, kNone, kNone};     // -inf: outside the row
-  __shared__ Shared<NW> sh;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  __shared__ Shared sh;
+  const int tid = threadIdx.x;
   const int64_t jobs = p.rows * p.pieces;
   for (int64_t job = blockIdx.x; job < jobs; job += gridDim.x) {
-    const int64_t row = p.pieces == 1 ? job : job / p.pieces;
+    // (pieces: of fewer than 2048 rows)
+    const int64_t row = p.pieces == 1 ? job : (uint32_t)job / (uint32_t)p.pieces;
     const int piece = p.pieces == 1 ? 0 : (int)(job - row * p.pieces);
     const uint8_t* x = p.x + row * p.x_rs * (int64_t)(16 / V);
     const RowChunks<T, AL> rc(x, p.vocab, p.align_mask);
@@ -157,37 +201,39 @@ __global__ __launch_bounds__(64 * NW) void logprob_pieces(LParams p) {
     auto has = [&](int c, int e) __attribute__((always_inline)) { return c < c1 && rc.any(c) && rc.has(c, e); };
 
     // Only the packed batch stays in registers between the passes over it.
-    auto hold = [&](u32x4 (&w)[kU]) __attribute__((always_inline)) {
+    auto hold = [&](u32x4 (&w)[U]) __attribute__((always_inline)) {
 #pragma unroll
-      for (int q = 0; q < kU; ++q) asm volatile("" : "+v"(w[q]));
+      for (int q = 0; q < U; ++q) asm volatile("" : "+v"(w[q]));
     };
-    if (tid == 0) sh.count = 0;
+    int listed = 0;                            // keys on the wave's list
     float m = -INFINITY, r = -1000.0f, s = 0.0f, t = 0.0f;
-    float limit = -INFINITY;                   // values above it may be alternatives
+    float limit = -INFINITY;                   // the wave's: values from it on may be alternatives
     bool over = false;                         // the list lost some
-    u32x4 raw[kU];
+    u32x4 raw[U];
 #pragma unroll
-    for (int q = 0; q < kU; ++q) raw[q] = load(c0 + tid + NT * q);
-    for (int c = c0 + tid, batch = 0;; c += kU * NT, ++batch) {
-      u32x4 cur[kU];
+    for (int q = 0; q < U; ++q) raw[q] = load(c0 + tid + NT * q);
+    for (int c = c0 + tid, batch = 0;; c += U * NT, ++batch) {
+      u32x4 cur[U];
 #pragma unroll
-      for (int q = 0; q < kU; ++q) cur[q] = raw[q];
+      for (int q = 0; q < U; ++q) cur[q] = raw[q];
       // (uniform: the first thread's next chunk)
-      const int next = c - tid + kU * NT;
+      const int next = c - tid + U * NT;
       const bool more = next < c1 && rc.any(next);
       if (more)
 #pragma unroll
-        for (int q = 0; q < kU; ++q) raw[q] = load(c + (kU + q) * NT);
-      float high[kU];
+        for (int q = 0; q < U; ++q) raw[q] = load(c + (U + q) * NT);
+      float high[U];
 #pragma unroll
-      for (int q = 0; q < kU; ++q) {
+      for (int q = 0; q < U; ++q) {
         float v[V];
         IO::unpack(cur[q], v);
         high[q] = v[0];
 #pragma unroll
         for (int e = 1; e < V; ++e) high[q] = fmaxf(high[q], v[e]);
       }
-      const float top = fmaxf(fmaxf(high[0], high[1]), fmaxf(high[2], high[3]));
+      float top = high[0];
+#pragma unroll
+      for (int q = 1; q < U; ++q) top = fmaxf(top, high[q]);
       m = fmaxf(m, top);
       const float top2 = top * kLog2e;
       if (top2 > r + 8.0f) {
@@ -199,7 +245,7 @@ __global__ __launch_bounds__(64 * NW) void logprob_pieces(LParams p) {
       hold(cur);
       float bs = 0.0f, bt = 0.0f;
 #pragma unroll
-      for (int q = 0; q < kU; ++q) {
+      for (int q = 0; q < U; ++q) {
         float v[V];
         IO::unpack(cur[q], v);
 #pragma unroll
@@ -212,76 +258,68 @@ __global__ __launch_bounds__(64 * NW) void logprob_pieces(LParams p) {
       if (__ballot(bt != bt)) {                // -inf among them: 0 * -inf stands for 0
         hold(cur);
         bt = 0.0f;
-#pragma unroll
-        for (int q = 0; q < kU; ++q) {
+#pragma unroll 1
+        for (int q = 0; q < U; ++q) {
           float v[V];
-          IO::unpack(cur[q], v);
+          IO::unpack(cur[0], v);
 #pragma unroll
           for (int e = 0; e < V; ++e) {
             const float d = fmaf(v[e], kLog2e, -r), w = __builtin_amdgcn_exp2f(d);
             bt += w == 0.0f ? 0.0f : w * d;
           }
+          const u32x4 w = cur[0];
+#pragma unroll
+          for (int u = 0; u + 1 < U; ++u) cur[u] = cur[u + 1];
+          cur[U - 1] = w;
         }
       }
       s += bs;
       t += bt;
       if constexpr (TOP) {
-        hold(cur);
-        uint64_t bound = 0;                    // first batch: keys from here on
         if (batch == 0) {
-          // The K-th largest of the threads' own largest keys, or of groups of four
-          // threads' where K is small; fewer than K such keys: every element is listed.
-          uint64_t best = 0;
+          const uint32_t key[2] = {order_key(__float_as_uint(fmaxf(high[0], high[1]))),
+                                   order_key(__float_as_uint(fmaxf(high[2], high[3])))};
+          limit = bound_value(reached_by<T>(key, p.top));
+        }
+        if (__ballot(top >= limit)) {
+          hold(cur);
+          // The thread's elements that go to the list, a bit each; -inf is also what lies
+          // outside the row.
+          uint32_t pass = 0;
 #pragma unroll
-          for (int q = kU - 1; q >= 0; --q) {
+          for (int q = U - 1; q >= 0; --q) {
             float v[V];
             IO::unpack(cur[q], v);
-            const int at = c + q * NT;
 #pragma unroll
-            for (int e = V - 1; e >= 0; --e)
-              if (has(at, e)) best = max(best, rank_key(v[e], rc.first(at) + e));
+            for (int e = V - 1; e >= 0; --e) pass = pass + pass + (v[e] >= limit ? 1u : 0u);
           }
-          const bool by4 = NW > 1 && p.top <= 16;
-          if (by4) {
-            best = max(best, (uint64_t)__shfl_xor((unsigned long long)best, 1));
-            best = max(best, (uint64_t)__shfl_xor((unsigned long long)best, 2));
-            if ((tid & 3) == 0) sh.groups[tid >> 2] = best;
-          } else {
-            sh.groups[tid] = best;
-          }
-          if (tid == 0) sh.threshold = 0;
-          sync<NW>();
-          const int n = by4 ? NT / 4 : NT;
-          if (tid < n) {
-            const uint64_t k = sh.groups[tid];
-            if (k && rank_of(sh.groups, n, k) == p.top - 1) sh.threshold = k;
-          }
-          sync<NW>();
-          bound = sh.threshold;
-          hold(cur);
-        }
+          if (limit == -INFINITY)
 #pragma unroll
-        for (int q = 0; q < kU; ++q) {
-          if (batch && !__ballot(high[q] > limit)) continue;
-          float v[V];
-          IO::unpack(cur[q], v);
-          const int at = c + q * NT;
+            for (int q = 0; q < U; ++q)
 #pragma unroll
-          for (int e = 0; e < V; ++e) {
-            const bool in = batch ? v[e] > limit : has(at, e) && rank_key(v[e], rc.first(at) + e) >= bound;
-            if (in) {
-              const int to = atomicAdd(&sh.count, 1);
-              if (to < sh.kCap) sh.list[to] = rank_key(v[e], rc.first(at) + e);
-            }
+              for (int e = 0; e < V; ++e)
+                if (!has(c + q * NT, e)) pass &= ~(1u << (V * q + e));
+          for (uint64_t any; (any = __ballot(pass != 0));) {
+            const uint32_t i = pass ? __ffs(pass) - 1 : 0;
+            const int at = listed + (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(any >> 32),
+                                                                   __builtin_amdgcn_mbcnt_lo((uint32_t)any, 0));
+            uint32_t w = cur[0][0];
+#pragma unroll
+            for (uint32_t u = 1; u < 4 * U; ++u) w = i / (V / 4) == u ? cur[u / 4][u % 4] : w;
+            float v[V];
+            IO::unpack(u32x4{w, w, w, w}, v);
+            const float x1 = V == 8 && (i & 1) ? v[1] : v[0];
+            if (pass && at < kCap) sh.list[at] = rank_key(x1, rc.first(c + (int)(i / V) * NT) + (int)(i % V));
+            pass &= pass - 1;
+            listed += __popcll(any);
           }
         }
-        if (batch == 0) limit = bound ? key_value(bound) : -INFINITY;
-        // after batches 0, 3, 15, 63, ... (the list's order does not depend on the waves')
-        if (more && ((batch + 1) & batch) == 0 && (__ffs(batch + 1) & 1)) {
-          sync<NW>();
-          over |= sh.count > sh.kCap;
-          shorten<NW>(sh, p.top);
-          limit = key_value(sh.threshold);
+        if (batch == 0) limit = above(limit);  // an equal value at a higher place ranks lower
+        // after batches 1, 3, 7, ...; of many alternatives after the first as well
+        if (more && ((batch + 1) & batch) == 0 && (batch || p.top > 16) && listed >= p.top) {
+          over |= listed > kCap;
+          listed = min(listed, kCap);
+          limit = fmaxf(limit, above(bound_value(refine_list<T>(sh.list, listed, p.top))));
         }
       }
       if (!more) break;
@@ -297,12 +335,9 @@ __global__ __launch_bounds__(64 * NW) void logprob_pieces(LParams p) {
       v.t = kLn2 * f * fmaf(s, off, t);
       if (m == -INFINITY) v = {kLowest, s, 0.0f};                    // s: 0, or NaN
     }
-    v = wave_both(v);
-    if (lane == 0) sh.sums[wave] = v;
-    sync<NW>();
-    v = sh.sums[0];
-#pragma unroll
-    for (int w = 1; w < NW; ++w) v = both(v, sh.sums[w]);
+    v = moved(v, wave_max(v.m));
+    v.s = wave_sum(v.s);
+    v.t = wave_sum(v.t);
     // NaN and +inf (S is not finite then), or a maximum of over 64.
     const bool odd = !(v.s < INFINITY) || (!(fabsf(v.m) <= 64.0f) && v.s != 0.0f);
     if (odd) {
@@ -317,21 +352,14 @@ __global__ __launch_bounds__(64 * NW) void logprob_pieces(LParams p) {
           t2 += w == 0.0f ? 0.0f : w * d;
         }
       }
-      const float sum = wave_sum(s2), tsum = wave_sum(t2);
-      sync<NW>();
-      if (lane == 0) sh.sums[wave] = {v.m, sum, tsum};
-      sync<NW>();
-      v.s = v.t = 0.0f;
-#pragma unroll
-      for (int w = 0; w < NW; ++w) {
-        v.s += sh.sums[w].s;
-        v.t += sh.sums[w].t;
-      }
+      v.s = wave_sum(s2);
+      v.t = wave_sum(t2);
     }
+    int found = 0;
     if constexpr (TOP) {
-      over |= sh.count > sh.kCap;
+      over |= listed > kCap;
       if (!over && v.s < INFINITY) {
-        shorten<NW>(sh, p.top);
+        found = finish<T>(sh, p.top, listed);
       } else {                                 // the largest below the last one, K times
         uint64_t last = ~0ull;
         for (int i = 0; i < p.top; ++i) {
@@ -347,17 +375,11 @@ __global__ __launch_bounds__(64 * NW) void logprob_pieces(LParams p) {
           }
 #pragma unroll
           for (int o = 32; o; o >>= 1) best = max(best, (uint64_t)__shfl_xor((unsigned long long)best, o));
-          sync<NW>();
-          if (lane == 0) sh.groups[wave] = best;
-          sync<NW>();
-          last = sh.groups[0];
-#pragma unroll
-          for (int w = 1; w < NW; ++w) last = max(last, sh.groups[w]);
-          if (tid == 0) sh.list[i] = last;
+          last = best;
+          if (tid == 0) sh.best[i] = last;
         }
-        sync<NW>();
-        if (tid == 0) sh.count = p.top;
-        sync<NW>();
+        found = p.top;
+        __builtin_amdgcn_wave_barrier();
       }
     }
     if (p.pieces > 1) {
@@ -369,8 +391,7 @@ __global__ __launch_bounds__(64 * NW) void logprob_pieces(LParams p) {
       }
       // (a piece of fewer elements: keys of none)
       if constexpr (TOP) {
-        const int n = min(sh.count, p.top);
-        for (int i = tid; i < p.top; i += NT) p.keys[job * p.top + i] = i < n ? sh.list[i] : 0;
+        for (int i = tid; i < p.top; i += NT) p.keys[job * p.top + i] = i < found ? sh.best[i] : 0;
       }
     } else {
       const float ls = logf(v.s);
@@ -384,12 +405,12 @@ __global__ __launch_bounds__(64 * NW) void logprob_pieces(LParams p) {
       }
       if constexpr (TOP)
         for (int i = tid; i < p.top; i += NT) {
-          const uint64_t k = sh.list[i];
+          const uint64_t k = sh.best[i];
           p.top_index[row * p.top + i] = key_place(k);
           p.top_logprob[row * p.top + i] = (key_value(k) - v.m) - ls;
         }
     }
-    sync<NW>();                                // the next row's list
+    __builtin_amdgcn_wave_barrier();           // the next row's list
   }
 }
 
@@ -397,7 +418,7 @@ __global__ __launch_bounds__(64 * NW) void logprob_pieces(LParams p) {
 template <NormType T>
 __global__ __launch_bounds__(256) void logprob_join(LParams p) {
   using IO = Io<T>;
-  __shared__ uint64_t list[kMaxPieces * kMaxTop], some[2 * kMaxTop + kMaxPieces];
+  __shared__ __attribute__((aligned(16))) uint64_t list[kMaxKeys], some[2 * kMaxTop + kMaxPieces];
   __shared__ uint64_t threshold;
   __shared__ int count;
   const int tid = threadIdx.x, lane = tid & 63;
@@ -409,7 +430,9 @@ __global__ __launch_bounds__(256) void logprob_join(LParams p) {
     const uint64_t* keys = p.keys + row * p.pieces * p.top;
     const int n = p.pieces * p.top;
     for (int i = tid; i < n; i += 256) list[i] = keys[i];
-    v = wave_both(v);
+    v = moved(v, wave_max(v.m));
+    v.s = wave_sum(v.s);
+    v.t = wave_sum(v.t);
     const float ls = logf(v.s);
     if (tid == 0) {
       p.lse[row] = v.m + ls;
@@ -433,12 +456,12 @@ __global__ __launch_bounds__(256) void logprob_join(LParams p) {
     if (tid < m && some[tid] && rank_of(some, m, some[tid]) == p.top - 1) threshold = some[tid];
     __syncthreads();
     const uint64_t bound = max((uint64_t)1, threshold);
-    uint64_t mine[kMaxPieces * kMaxTop / 256];
+    uint64_t mine[kMaxKeys / 256];
 #pragma unroll
-    for (int q = 0; q < kMaxPieces * kMaxTop / 256; ++q) mine[q] = tid + 256 * q < n ? list[tid + 256 * q] : 0;
+    for (int q = 0; q < kMaxKeys / 256; ++q) mine[q] = tid + 256 * q < n ? list[tid + 256 * q] : 0;
     __syncthreads();
 #pragma unroll
-    for (int q = 0; q < kMaxPieces * kMaxTop / 256; ++q)
+    for (int q = 0; q < kMaxKeys / 256; ++q)
       if (mine[q] >= bound) list[atomicAdd(&count, 1)] = mine[q];
     __syncthreads();
     const int c = count;
@@ -518,18 +541,21 @@ __global__ __launch_bounds__(256) void logprob_grad(GParams p) {
 bool on16(const void* q) { return (uintptr_t)q % 16 == 0; }
 
 struct Plan {
-  int nw, pieces, each;
+  int pieces, each;
   size_t sums, keys;     // bytes of the workspace
 };
 
+// A wave to a row, or to each of a row's pieces where rows are fewer than two waves to a
+// SIMD: of at least a batch, and not more than the join holds. us for 1, 2 and 4 waves to
+// a SIMD at least: 256 x 131072 bf16, 8 alternatives, - / 28.9 / 30.9; 2048 x 32000
+// without any 24.9 in one piece, 32.8 in four. Four waves to a row, a workgroup with
+// barriers: 40 us for 19 at 8192 x 4000, 84 for 86 at 4096 x 32001 fp32.
 Plan plan_of(NormType t, int64_t rows, int vocab, int top) {
   Plan x{};
   const int V = t == NormType::F32 ? 4 : 8;
   const int chunks = (vocab + V - 1) / V + 1;        // one more where rows are off 16 bytes
-  x.nw = chunks <= kU * 64 ? 1 : 4;
-  // Few rows: pieces of at least a batch, four workgroups to a CU.
-  const int batch = kU * 64 * x.nw, most = (chunks + batch - 1) / batch;
-  x.pieces = (int)std::max<int64_t>(1, std::min<int64_t>({(1024 + rows - 1) / rows, most, kMaxPieces}));
+  const int most = (chunks + kU * 64 - 1) / (kU * 64);
+  x.pieces = (int)std::min<int64_t>({(2048 + rows - 1) / rows, most, kMaxPieces, kMaxKeys / std::max(1, top)});
   x.each = (chunks + x.pieces - 1) / x.pieces;
   if (x.pieces > 1) {
     x.sums = (size_t)rows * x.pieces * 16;
@@ -548,12 +574,9 @@ hipError_t run_forward(const TokenLogProbDesc& d, const Plan& x, hipStream_t s) 
   p.top_logprob = d.top_logprob; p.top_index = d.top_index;
   p.sums = (float*)d.ws;
   p.keys = (uint64_t*)((uint8_t*)d.ws + x.sums);
-  const unsigned grid = (unsigned)std::min<int64_t>(d.rows * x.pieces, max_workgroups(64 * x.nw));
-  auto go = [&](auto kern) { hipLaunchKernelGGL(kern, dim3(grid), dim3(64 * x.nw), 0, s, p); };
-  if (x.nw == 1 && d.top) go(logprob_pieces<T, AL, 1, true>);
-  else if (x.nw == 1) go(logprob_pieces<T, AL, 1, false>);
-  else if (d.top) go(logprob_pieces<T, AL, 4, true>);
-  else go(logprob_pieces<T, AL, 4, false>);
+  const unsigned grid = (unsigned)std::min<int64_t>(d.rows * x.pieces, max_workgroups(64));
+  if (d.top) hipLaunchKernelGGL((logprob_pieces<T, AL, true>), dim3(grid), dim3(64), 0, s, p);
+  else hipLaunchKernelGGL((logprob_pieces<T, AL, false>), dim3(grid), dim3(64), 0, s, p);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess || x.pieces == 1) return e;
   hipLaunchKernelGGL(logprob_join<T>, dim3((unsigned)std::min<int64_t>(d.rows, max_workgroups(256))), dim3(256), 0, s, p);
