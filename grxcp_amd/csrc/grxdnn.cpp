@@ -316,6 +316,10 @@ bool half_rows(const grxdnnTensorStruct& t) {
   return true;
 }
 
+// Slots that a sequence may have room for: the kernels count them in 32 bits, up to a
+// tile's or a workgroup's worth past the last.
+constexpr int kMaxRoom = INT_MAX - 4095;
+
 // A table of pages: [B, W] ints, rows of any pitch.
 bool table_shape(const grxdnnTensorStruct& t) {
   return t.nb == 2 && t.type == GRX_R_32I && t.dims[1] >= 1 && (t.dims[1] == 1 || t.strides[1] == 1);
@@ -345,7 +349,7 @@ grxdnnStatus_t paged_cache(grxdnnTensorDescriptor_t kDesc, grxdnnTensorDescripto
   c->W = tableDesc->dims[1];
   c->table_rs = tableDesc->strides[0];
   if (c->D != 64 && c->D != 128) return GRXDNN_STATUS_NOT_SUPPORTED;
-  if ((int64_t)c->W * c->page > INT_MAX - 255) return GRXDNN_STATUS_NOT_SUPPORTED;
+  if ((int64_t)c->W * c->page > kMaxRoom) return GRXDNN_STATUS_NOT_SUPPORTED;
   // (sequence, head) pairs are counted in 32 bits
   if ((int64_t)c->B * c->heads > INT_MAX / 4) return GRXDNN_STATUS_NOT_SUPPORTED;
   if (!half_rows(*kDesc) || !half_rows(*vDesc)) return GRXDNN_STATUS_NOT_SUPPORTED;
@@ -771,7 +775,7 @@ grxdnnStatus_t grxdnnPagedCacheEvict(grxdnnHandle_t handle, grxdnnTensorDescript
   if (!table_shape(*newTableDesc) || newTableDesc->dims[0] != d.c.B ||
       (int64_t)newTableDesc->dims[1] * d.c.page < budget)
     return GRXDNN_STATUS_INVALID_VALUE;
-  if ((int64_t)newTableDesc->dims[1] * d.c.page > INT_MAX - 255) return GRXDNN_STATUS_NOT_SUPPORTED;
+  if ((int64_t)newTableDesc->dims[1] * d.c.page > kMaxRoom) return GRXDNN_STATUS_NOT_SUPPORTED;
   if (!weights_shape(*weightsDesc, d.c.B, d.c.heads, (int64_t)d.c.W * d.c.page) ||
       !weights_shape(*newWeightsDesc, d.c.B, d.c.heads, budget))
     return GRXDNN_STATUS_INVALID_VALUE;

@@ -34,24 +34,37 @@ struct AppendParams {
   const u32x4* kn; int64_t kn_sb, kn_sh, kn_st;   // chunks
   const u32x4* vn; int64_t vn_sb, vn_sh, vn_st;
   const int* counts;
-  int B, heads, T, chunks;                        // 16-byte chunks of a row
+  PageDiv by_heads;
+  int B, T, heads, tokens;    // tokens: of a tile
 };
 
-// One 16-byte chunk of a key and of a value per thread.
+// Tiles of `tokens` new tokens of one sequence (blockIdx.y), their heads side by side: a
+// thread copies a 16-byte chunk of a key and of a value of a row. Bound by memory, each row
+// read and written once. The rows are written to stay in the caches: the next attention
+// reads them. us, 8 x 4000 tokens of 8 heads of 128: 51.5 (5.1 TB/s); with four rows a
+// thread, all loaded before the first is stored, 53.6; that and stores past the caches 50.5
+// (but 8 x 2250 30.6 for 28.2); 64 tokens 4.9, 256 tokens 4.9.
+template <int C>       // chunks of a row
 __global__ __launch_bounds__(256) void paged_append(AppendParams p) {
-  const int64_t total = (int64_t)p.B * p.T * p.heads * p.chunks;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
-    const int c = (int)(i % p.chunks);
-    int64_t r = i / p.chunks;
-    const int h = (int)(r % p.heads);
-    r /= p.heads;
-    const int t = (int)(r % p.T), b = (int)(r / p.T);
-    if (p.counts && t >= p.counts[b]) continue;
-    const int64_t slot = (int64_t)clamp_length(p.view.lengths[b], p.view.room) + t;
-    int page, row;
-    if (slot >= p.view.room || !find_slot(p.view, b, (int)slot, &page, &row)) continue;
-    p.k.row(page, h, row)[c] = p.kn[b * p.kn_sb + h * p.kn_sh + t * p.kn_st + c];
-    p.v.row(page, h, row)[c] = p.vn[b * p.vn_sb + h * p.vn_sh + t * p.vn_st + c];
+  constexpr int R = 256 / C;
+  const int c = threadIdx.x % C, first = threadIdx.x / C;
+  const int rows = p.tokens * p.heads;
+  for (int b = blockIdx.y; b < p.B; b += gridDim.y) {
+    const int n = clamp_length(p.view.lengths[b], p.view.room);
+    const int T = min(p.counts ? min(p.counts[b], p.T) : p.T, p.view.room - n);   // the others have no place
+    for (int64_t t0 = (int64_t)blockIdx.x * p.tokens; t0 < T; t0 += (int64_t)gridDim.x * p.tokens) {
+      for (int r = first; r < rows; r += R) {
+        const int i = div_page(p.by_heads, r), h = r - i * p.heads;
+        const int64_t t = t0 + i;
+        if (t >= T) break;
+        int page, row;
+        if (!find_slot(p.view, b, n + (int)t, &page, &row)) continue;
+        const u32x4 key = __builtin_nontemporal_load(p.kn + b * p.kn_sb + h * p.kn_sh + t * p.kn_st + c);
+        const u32x4 value = __builtin_nontemporal_load(p.vn + b * p.vn_sb + h * p.vn_sh + t * p.vn_st + c);
+        p.k.row(page, h, row)[c] = key;
+        p.v.row(page, h, row)[c] = value;
+      }
+    }
   }
 }
 
@@ -64,95 +77,165 @@ struct EvictParams {
   float* nw; int64_t nw_sb, nw_sh; int nw_slots;
   int* kept;
   int* new_lengths;
-  int B, heads, budget, recent, chunks;
+  int B, heads, budget, recent;
 };
 
-__device__ __forceinline__ uint32_t key_at(const float* w, int j) { return order_key(__float_as_uint(w[j])); }
+constexpr int kWaves = 16;    // of a selecting workgroup
+constexpr int kU = 4;         // rows of a copying thread, all loaded before the first is stored
 
-// Sum of v over the 256 threads, in every thread.
-__device__ __forceinline__ int block_sum(int v, int* red) {
-#pragma unroll
-  for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o);
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
-  __syncthreads();
-  return red[0] + red[1] + red[2] + red[3];
-}
-
-// Which slots a head keeps: one workgroup per (sequence, head). The key of the
-// last slot that stays is found bit by bit from the top.
-__global__ __launch_bounds__(256) void evict_select(EvictParams p) {
-  __shared__ int red[4];
+// Which slots a head keeps: one workgroup per (sequence, head). Wave w has the slots
+// from 64 E w on, E to a lane, 64 neighbours at a time; E <= N of them in registers
+// (N = 0: read again in every pass).
+//  * The key of the last slot that stays is found from the top, two bits a step: how
+//    many slots reach each of three keys, summed over the waves. Weights that differ
+//    are told apart long before the last bit: the steps end when exactly as many slots
+//    reach a key as stay.
+//  * Where every slot goes follows from the numbers of kept ones and of ties in the
+//    waves before and ballots within the wave: no loop over the slots with a barrier.
+// 128 heads of 6000 to 8192 slots to 2048: 21.7 us, bound by instruction issue on the 128
+// CUs that have one; a binary search over passes through memory, 256 threads, took 187.
+template <int N>
+__global__ __launch_bounds__(64 * kWaves) void evict_select(EvictParams p) {
+  __shared__ int sums[2][3][kWaves], above_of[kWaves], ties_of[kWaves];
   const int bh = blockIdx.x, b = bh / p.heads, h = bh - b * p.heads, tid = threadIdx.x;
+  const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int n = clamp_length(p.view.lengths[b], p.view.room), m = min(n, p.budget);
   const int old = n <= p.budget ? 0 : max(0, n - p.recent);   // slots that the weights decide on
   const int want = n <= p.budget ? 0 : p.budget - p.recent;   // how many of them stay
   const float* w = p.w + b * p.w_sb + h * p.w_sh;
-  uint32_t last = 0;       // largest key that at least `want` slots reach
-  for (int bit = 31; bit >= 0; --bit) {
-    const uint32_t t = last | (1u << bit);
-    int c = 0;
-    for (int j = tid; j < old; j += 256) c += key_at(w, j) >= t;
-    if (block_sum(c, red) >= want) last = t;
+  const int E = (n + 64 * kWaves - 1) / (64 * kWaves), first = 64 * E * wave + lane;
+  // A slot's key, 0 (which no weight has) where the weights do not decide.
+  auto key_of = [&](int q) __attribute__((always_inline)) {
+    const int j = first + 64 * q;
+    return j < old ? order_key(__float_as_uint(w[j])) : 0;
+  };
+  uint32_t mine[N ? N : 1];
+  if constexpr (N > 0)
+#pragma unroll
+    for (int q = 0; q < N; ++q) mine[q] = q < E ? key_of(q) : 0;
+  // f(slot, key) for every row of 64 slots of the wave
+  auto each = [&](auto f) __attribute__((always_inline)) {
+    if constexpr (N > 0) {
+#pragma unroll
+      for (int q = 0; q < (N ? N : 1); ++q)
+        if (q < E) f(first + 64 * q, mine[q]);
+    } else {
+      for (int q = 0; q < E; ++q) f(first + 64 * q, key_of(q));
+    }
+  };
+
+  uint32_t last = 0;       // slots whose key reaches it stay, or (ties) those above it and some of it
+  bool ties = want > 0;
+  for (int bit = 30, turn = 0; bit >= 0 && ties; bit -= 2, turn ^= 1) {
+    uint32_t c[3] = {0, 0, 0};
+    each([&](int, uint32_t key) __attribute__((always_inline)) {
+#pragma unroll
+      for (uint32_t d = 0; d < 3; ++d) c[d] += key >= (last | (d + 1) << bit);
+    });
+#pragma unroll
+    for (int d = 0; d < 3; ++d) {
+      c[d] = wave_upto(c[d]);
+      if (lane == 63) sums[turn][d][wave] = (int)c[d];
+    }
+    // One barrier a step: a wave that is a step ahead writes the other turn's sums.
+    __syncthreads();
+    uint32_t got = lane < 3 * kWaves ? (uint32_t)sums[turn][lane / kWaves][lane % kWaves] : 0;
+    got = dpp_add<0x111, 0xf>(got);    // row_shr 1, 2, 4, 8: lanes 15, 31, 47 get their 16's sum
+    got = dpp_add<0x112, 0xf>(got);
+    got = dpp_add<0x114, 0xf>(got);
+    got = dpp_add<0x118, 0xf>(got);
+    static_assert(kWaves == 16, "a row of lanes per sum");
+#pragma unroll
+    for (int d = 2; d >= 0; --d) {
+      const int s = __builtin_amdgcn_readlane((int)got, 16 * d + 15);
+      if (s >= want) {
+        last |= (uint32_t)(d + 1) << bit;
+        ties = s != want;
+        break;
+      }
+    }
   }
-  int c = 0;
-  for (int j = tid; j < old; j += 256) c += key_at(w, j) > last;
-  int ties = want - block_sum(c, red);                        // lowest slots with the last key
+  // What stays: newer slots, old ones above `last`, and of those at it all or, where
+  // more than fit tie, the lowest.
+  auto above = [&](int j, uint32_t key) __attribute__((always_inline)) {
+    return j < old ? want && (ties ? key > last : key >= last) : j < n;
+  };
+  auto tied = [&](int j, uint32_t key) __attribute__((always_inline)) { return ties && j < old && key == last; };
+  int up = 0, at = 0;
+  each([&](int j, uint32_t key) __attribute__((always_inline)) {
+    up += __popcll(__ballot(above(j, key)));
+    at += __popcll(__ballot(tied(j, key)));
+  });
+  if (lane == 0) {
+    above_of[wave] = up;
+    ties_of[wave] = at;
+  }
+  __syncthreads();
+  int total = 0;
+#pragma unroll
+  for (int x = 0; x < kWaves; ++x) total += above_of[x];
+  int room = m - total, to = 0;      // ties that stay
+#pragma unroll
+  for (int x = 0; x < kWaves; ++x)
+    if (x < wave) {
+      const int some = min(room, ties_of[x]);
+      to += above_of[x] + some;
+      room -= some;
+    }
   int* kept = p.kept + (int64_t)bh * p.budget;
   float* nw = p.nw + b * p.nw_sb + h * p.nw_sh;
-  // In slot order, 256 slots at a time: tied ones before, kept ones before.
-  __shared__ int before[2][4];
-  int at = 0;
-  for (int j0 = 0; j0 < n; j0 += 256) {
-    const int j = j0 + tid;
-    const uint32_t key = j < old ? key_at(w, j) : 0;
-    const bool tie = j < old && key == last;
-    const uint64_t tmask = __ballot(tie), below = (1ull << (tid & 63)) - 1;
-    __syncthreads();
-    if ((tid & 63) == 0) before[0][tid >> 6] = __popcll(tmask);
-    __syncthreads();
-    int rank = __popcll(tmask & below);
-    for (int i = 0; i < tid >> 6; ++i) rank += before[0][i];
-    const bool stay = j < n && (j >= old || key > last || (tie && rank < ties));
-    ties -= before[0][0] + before[0][1] + before[0][2] + before[0][3];
-    const uint64_t smask = __ballot(stay);
-    if ((tid & 63) == 0) before[1][tid >> 6] = __popcll(smask);
-    __syncthreads();
-    int to = at + __popcll(smask & below);
-    for (int i = 0; i < tid >> 6; ++i) to += before[1][i];
+  const uint64_t below = (1ull << lane) - 1;
+  each([&](int j, uint32_t key) __attribute__((always_inline)) {
+    const uint64_t tie = __ballot(tied(j, key));
+    const bool stay = above(j, key) || (tied(j, key) && __popcll(tie & below) < room);
+    const uint64_t all = __ballot(stay);
     if (stay) {
-      kept[to] = j;
-      nw[to] = w[j];
+      const int i = to + __popcll(all & below);
+      kept[i] = j;
+      nw[i] = w[j];
     }
-    at += before[1][0] + before[1][1] + before[1][2] + before[1][3];
-  }
-  for (int i = m + tid; i < p.budget; i += 256) kept[i] = -1;
-  for (int i = m + tid; i < p.nw_slots; i += 256) nw[i] = 0.0f;
+    room -= min(room, __popcll(tie));
+    to += __popcll(all);
+  });
+  for (int i = m + tid; i < p.budget; i += 64 * kWaves) kept[i] = -1;
+  for (int i = m + tid; i < p.nw_slots; i += 64 * kWaves) nw[i] = 0.0f;
 }
 
-// The kept rows into the new pages, a 16-byte chunk of a key and of a value per
-// thread; the new lengths (after every reader of lengths, which they may replace).
+// The kept rows of (sequence, head) blockIdx.y into the new pages: a thread copies a
+// 16-byte chunk of a key and of a value of kU rows. Bound by memory (128 heads of 2048 kept
+// rows of 128 from 4 KB pages, a quarter of each: 268 MB in 56 us). The new lengths after every reader of
+// lengths, which they may replace.
+template <int C>
 __global__ __launch_bounds__(256) void evict_copy(EvictParams p) {
-  const int64_t total = (int64_t)p.B * p.heads * p.budget * p.chunks;
-  const int64_t first = (int64_t)blockIdx.x * 256 + threadIdx.x, step = (int64_t)gridDim.x * 256;
-  for (int64_t i = first; i < total; i += step) {
-    const int c = (int)(i % p.chunks);
-    const int64_t r = i / p.chunks;
-    const int slot = p.kept[r];
-    if (slot < 0) continue;
-    const int to = (int)(r % p.budget);
-    const int bh = (int)(r / p.budget), b = bh / p.heads, h = bh - b * p.heads;
-    int page, row, new_page, new_row;
-    if (!find_slot(p.view, b, slot, &page, &row) || !find_slot(p.to, b, to, &new_page, &new_row)) continue;
-    p.k.row(new_page, h, new_row)[c] = p.k.row(page, h, row)[c];
-    p.v.row(new_page, h, new_row)[c] = p.v.row(page, h, row)[c];
+  constexpr int R = 256 / C;
+  const int c = threadIdx.x % C, first = threadIdx.x / C;
+  for (int bh = blockIdx.y; bh < p.B * p.heads; bh += gridDim.y) {
+    const int b = bh / p.heads, h = bh - b * p.heads;
+    const int* kept = p.kept + (int64_t)bh * p.budget;
+    for (int r0 = blockIdx.x * R * kU + first; r0 < p.budget; r0 += gridDim.x * R * kU) {
+      u32x4 kv[kU][2];
+      int slot[kU], page[kU], row[kU], new_page[kU], new_row[kU];
+#pragma unroll
+      for (int u = 0; u < kU; ++u) slot[u] = r0 + R * u < p.budget ? kept[r0 + R * u] : -1;
+#pragma unroll
+      for (int u = 0; u < kU; ++u) {
+        const bool from = find_slot(p.view, b, max(slot[u], 0), &page[u], &row[u]);
+        const bool to = find_slot(p.to, b, min(r0 + R * u, p.budget - 1), &new_page[u], &new_row[u]);
+        page[u] = ((slot[u] >= 0) & from & to) ? page[u] : -1;
+        if (page[u] < 0) continue;
+        kv[u][0] = __builtin_nontemporal_load(p.k.row(page[u], h, row[u]) + c);
+        kv[u][1] = __builtin_nontemporal_load(p.v.row(page[u], h, row[u]) + c);
+      }
+#pragma unroll
+      for (int u = 0; u < kU; ++u) {
+        if (page[u] < 0) continue;
+        __builtin_nontemporal_store(kv[u][0], p.k.row(new_page[u], h, new_row[u]) + c);
+        __builtin_nontemporal_store(kv[u][1], p.v.row(new_page[u], h, new_row[u]) + c);
+      }
+    }
+    if (h == 0 && blockIdx.x == 0 && threadIdx.x == 0)
+      p.new_lengths[b] = min(clamp_length(p.view.lengths[b], p.view.room), p.budget);
   }
-  for (int64_t b = first; b < p.B; b += step)
-    p.new_lengths[b] = min(clamp_length(p.view.lengths[b], p.view.room), p.budget);
-}
-
-unsigned blocks(int64_t threads) {
-  return (unsigned)std::max<int64_t>(1, std::min<int64_t>((threads + 255) / 256, 1 << 20));
 }
 
 }  // namespace
@@ -165,9 +248,15 @@ hipError_t launch_paged_append(const PagedAppendDesc& d, hipStream_t s) {
   p.kn = (const u32x4*)d.k; p.kn_sb = d.k_sb / 8; p.kn_sh = d.k_sh / 8; p.kn_st = d.k_st / 8;
   p.vn = (const u32x4*)d.v; p.vn_sb = d.v_sb / 8; p.vn_sh = d.v_sh / 8; p.vn_st = d.v_st / 8;
   p.counts = d.counts;
-  p.B = d.c.B; p.heads = d.c.heads; p.T = d.T; p.chunks = d.c.D / 8;
-  const int64_t total = (int64_t)p.B * p.T * p.heads * p.chunks;
-  hipLaunchKernelGGL(paged_append, dim3(blocks(total)), dim3(256), 0, s, p);
+  p.B = d.c.B; p.heads = d.c.heads; p.T = d.T;
+  p.by_heads = page_div(p.heads);
+  const int chunks = d.c.D / 8;
+  p.tokens = (int)std::max<int64_t>(1, 256 / ((int64_t)p.heads * chunks));
+  const int64_t tiles = ((int64_t)p.T + p.tokens - 1) / p.tokens;
+  const dim3 grid((unsigned)std::min<int64_t>(tiles, 1 << 20), (unsigned)std::min(p.B, 65535));
+  auto go = [&](auto kern) { hipLaunchKernelGGL(kern, grid, dim3(256), 0, s, p); };
+  if (chunks == 16) go(paged_append<16>);
+  else go(paged_append<8>);
   return hipGetLastError();
 }
 
@@ -184,13 +273,20 @@ hipError_t launch_paged_evict(const PagedEvictDesc& d, hipStream_t s) {
   p.nw = d.new_weights; p.nw_sb = d.nw_sb; p.nw_sh = d.nw_sh; p.nw_slots = d.nw_slots;
   p.kept = d.kept;
   p.new_lengths = d.new_lengths;
-  p.B = d.c.B; p.heads = d.c.heads; p.budget = d.budget; p.recent = d.recent; p.chunks = d.c.D / 8;
-  if ((int64_t)p.B * p.heads > max_workgroups(256)) return hipErrorNotSupported;
-  hipLaunchKernelGGL(evict_select, dim3((unsigned)(p.B * p.heads)), dim3(256), 0, s, p);
-  hipError_t e = hipGetLastError();
+  p.B = d.c.B; p.heads = d.c.heads; p.budget = d.budget; p.recent = d.recent;
+  const int64_t heads = (int64_t)p.B * p.heads;
+  if (heads > max_workgroups(64 * kWaves)) return hipErrorNotSupported;
+  const dim3 all((unsigned)heads), threads(64 * kWaves);
+  const int each = (p.view.room + 64 * kWaves - 1) / (64 * kWaves);
+  if (each <= 8) hipLaunchKernelGGL(evict_select<8>, all, threads, 0, s, p);
+  else if (each <= 32) hipLaunchKernelGGL(evict_select<32>, all, threads, 0, s, p);
+  else hipLaunchKernelGGL(evict_select<0>, all, threads, 0, s, p);
+  const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
-  const int64_t total = (int64_t)p.B * p.heads * p.budget * p.chunks;
-  hipLaunchKernelGGL(evict_copy, dim3(blocks(total)), dim3(256), 0, s, p);
+  const int chunks = d.c.D / 8, rows = 256 / chunks * kU;
+  const dim3 grid((unsigned)((p.budget + rows - 1) / rows), (unsigned)std::min<int64_t>(heads, 65535));
+  if (chunks == 16) hipLaunchKernelGGL(evict_copy<16>, grid, dim3(256), 0, s, p);
+  else hipLaunchKernelGGL(evict_copy<8>, grid, dim3(256), 0, s, p);
   return hipGetLastError();
 }
 

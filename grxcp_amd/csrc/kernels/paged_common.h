@@ -45,13 +45,17 @@ GRX_HD int clamp_length(int n, int room) { return n < 0 ? 0 : n > room ? room : 
 // The page that a table entry names, or -1 for one that no pool has.
 GRX_HD int checked_page(int entry, int pages) { return (uint32_t)entry < (uint32_t)pages ? entry : -1; }
 
-// Slot `slot` (>= 0) of sequence b: its page and row in it. False where the
-// sequence has no room for it or its entry names no page.
+// Slot `slot` (>= 0) of sequence b: its page and row in it. False, and page -1, where
+// the sequence has no room for it or its entry names no page. Without a branch (a slot
+// without room reads the row's last entry): the compiler (ROCm 7.2) lost the assignment
+// in "if (!find_slot(a) || !find_slot(b)) x[u] = -1" over an unrolled array when this was
+// one, and rows went to page -1. Callers join its results with & and selects.
 GRX_HD bool find_slot(const PagedView& v, int b, int slot, int* page, int* row) {
-  if (slot >= v.room) return false;
-  const int i = div_page(v.div, slot);
-  *page = checked_page(v.table[b * v.table_rs + i], v.pages);
-  *row = slot - i * v.page;
+  const int in = slot < v.room ? slot : v.room - 1;
+  const int i = div_page(v.div, in);
+  const int at = checked_page(v.table[b * v.table_rs + i], v.pages);
+  *page = slot < v.room ? at : -1;
+  *row = in - i * v.page;
   return *page >= 0;
 }
 

@@ -175,7 +175,7 @@ int            grxdnnAttentionCycleSlotsNeeded(grxdnnHandle_t handle, int batch,
  * (any strides: [pages, P, Hkv, D] memory is a view of it). A page table, 2-d
  * [B, W] GRX_R_32I with innermost stride 1, names the pages of each of B
  * sequences: slot j of sequence b is row j % P of page table[b][j / P], and a
- * sequence has room for W * P slots (at most 2^31 - 256). lengths: B ints, the
+ * sequence has room for W * P slots (at most 2^31 - 4096). lengths: B ints, the
  * slots of each sequence that hold tokens; below 0 counts as 0, above W * P as
  * W * P. Tables, lengths and counts are device memory, read when the kernels
  * run: a captured call follows their contents on every replay.

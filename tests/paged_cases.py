@@ -19,6 +19,13 @@ def ints(values):
     return torch.tensor(values, dtype=torch.int32, device="cuda")
 
 
+def guarded(pages, page, heads, d, dtype, tokmajor=False, fill=math.nan):
+    """A pool of `pages` pages with one more on either side: [pages + 2, heads, page, d]."""
+    shape = (pages + 2, page, heads, d) if tokmajor else (pages + 2, heads, page, d)
+    p = torch.full(shape, fill, dtype=dtype, device="cuda")
+    return p.transpose(1, 2) if tokmajor else p
+
+
 class Cache:
     """Pools whose every slot holds `fill` (NaN: what no call may read) but for the
     first lengths[b] slots of each sequence. tokmajor: memory is [pages, page, heads,
@@ -31,9 +38,8 @@ class Cache:
         self.dtype, self.heads, self.page, self.d = dtype, heads, page, d
         self.width = max(1, -(-max([room or 0, *lengths]) // page))
         total = b * self.width + spare
-        shape = (total, page, heads, d) if tokmajor else (total, heads, page, d)
-        pools = [torch.full(shape, fill, dtype=dtype, device="cuda") for _ in range(2)]
-        self.k, self.v = (p.transpose(1, 2) if tokmajor else p for p in pools)
+        self.guarded = [guarded(total, page, heads, d, dtype, tokmajor, fill) for _ in range(2)]
+        self.k, self.v = (p[1:-1] for p in self.guarded)
         order = torch.randperm(total, generator=gen)
         self.spare = order[b * self.width:]
         table = order[: b * self.width].reshape(b, self.width).int()

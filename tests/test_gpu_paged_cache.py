@@ -6,7 +6,7 @@ import torch
 
 import grxcp_amd as g
 from helpers import say
-from paged_cases import Cache, append, desc, evict, evict_ref, ints
+from paged_cases import Cache, append, desc, evict, evict_ref, guarded, ints
 
 pytestmark = pytest.mark.gpu
 BF16, F16 = torch.bfloat16, torch.float16
@@ -14,6 +14,10 @@ BF16, F16 = torch.bfloat16, torch.float16
 
 def bits(t):
     return t.cpu().contiguous().view(torch.int16)
+
+
+def guards_intact(pools):
+    return all(torch.isnan(p[[0, -1]].float()).all() for p in pools)
 
 
 # ---- append ------------------------------------------------------------------
@@ -46,6 +50,7 @@ def check_append(dnn, c, k, v, counts):
     say(f"append {tuple(k.shape)} to {c.n}")
     append(dnn, c, k, v, None if counts is None else ints(counts))
     assert torch.equal(bits(c.k), bits(want[0])) and torch.equal(bits(c.v), bits(want[1]))
+    assert guards_intact(c.guarded)
 
 
 @pytest.mark.parametrize("case", range(len(APPENDS)))
@@ -110,8 +115,9 @@ def check_evict(dnn, c, w, budget, recent, bad=(), width=None, slots=None, inpla
     b, pages = len(c.n), c.k.shape[0]
     width = width or -(-budget // c.page)
     grown = b * width
-    k = torch.cat([c.k.contiguous(), torch.full((grown, *c.k.shape[1:]), math.nan, dtype=c.dtype, device="cuda")])
-    v = torch.cat([c.v.contiguous(), torch.full((grown, *c.v.shape[1:]), math.nan, dtype=c.dtype, device="cuda")])
+    pools = [guarded(pages + grown, c.page, c.heads, c.d, c.dtype) for _ in range(2)]
+    k, v = (p[1:-1] for p in pools)
+    k[:pages], v[:pages] = c.k, c.v
     c.k, c.v = k, v
     new_table = ints(torch.randperm(grown).add(pages).reshape(b, width).tolist())
     for i, e in bad:
@@ -139,6 +145,7 @@ def check_evict(dnn, c, w, budget, recent, bad=(), width=None, slots=None, inpla
     assert new_lengths.tolist() == [min(n, budget) for n in c.n]
     assert torch.equal(new_w.cpu().view(torch.int32), want_w.view(torch.int32))
     assert torch.equal(bits(c.k), bits(want[0])) and torch.equal(bits(c.v), bits(want[1]))
+    assert guards_intact(pools)
     return new_table, new_w, new_lengths
 
 
