@@ -81,7 +81,6 @@ struct EvictParams {
 };
 
 constexpr int kWaves = 16;    // of a selecting workgroup
-constexpr int kU = 4;         // rows of a copying thread, all loaded before the first is stored
 
 // Which slots a head keeps: one workgroup per (sequence, head). Wave w has the slots
 // from 64 E w on, E to a lane, 64 neighbours at a time; E <= N of them in registers
@@ -198,12 +197,13 @@ __global__ __launch_bounds__(64 * kWaves) void evict_select(EvictParams p) {
     to += __popcll(all);
   });
   for (int i = m + tid; i < p.budget; i += 64 * kWaves) kept[i] = -1;
-  for (int i = m + tid; i < p.nw_slots; i += 64 * kWaves) nw[i] = 0.0f;
+  for (int64_t i = m + tid; i < p.nw_slots; i += 64 * kWaves) nw[i] = 0.0f;
 }
 
-// The kept rows of (sequence, head) blockIdx.y into the new pages: a thread copies a
-// 16-byte chunk of a key and of a value of kU rows. Bound by memory (128 heads of 2048 kept
-// rows of 128 from 4 KB pages, a quarter of each: 268 MB in 56 us). The new lengths after every reader of
+// The kept rows of (sequence, head) blockIdx.y into the new pages: a thread copies a 16-byte
+// chunk of a key and of a value of a row. Bound by memory: 128 heads of 2048 kept rows of
+// 256 bytes, a quarter of those that lie between them, 268 MB in 56 us; four rows a thread
+// took as long, and 1.6 us more in a call of 8 heads. The new lengths after every reader of
 // lengths, which they may replace.
 template <int C>
 __global__ __launch_bounds__(256) void evict_copy(EvictParams p) {
@@ -212,30 +212,26 @@ __global__ __launch_bounds__(256) void evict_copy(EvictParams p) {
   for (int bh = blockIdx.y; bh < p.B * p.heads; bh += gridDim.y) {
     const int b = bh / p.heads, h = bh - b * p.heads;
     const int* kept = p.kept + (int64_t)bh * p.budget;
-    for (int r0 = blockIdx.x * R * kU + first; r0 < p.budget; r0 += gridDim.x * R * kU) {
-      u32x4 kv[kU][2];
-      int slot[kU], page[kU], row[kU], new_page[kU], new_row[kU];
-#pragma unroll
-      for (int u = 0; u < kU; ++u) slot[u] = r0 + R * u < p.budget ? kept[r0 + R * u] : -1;
-#pragma unroll
-      for (int u = 0; u < kU; ++u) {
-        const bool from = find_slot(p.view, b, max(slot[u], 0), &page[u], &row[u]);
-        const bool to = find_slot(p.to, b, min(r0 + R * u, p.budget - 1), &new_page[u], &new_row[u]);
-        page[u] = ((slot[u] >= 0) & from & to) ? page[u] : -1;
-        if (page[u] < 0) continue;
-        kv[u][0] = __builtin_nontemporal_load(p.k.row(page[u], h, row[u]) + c);
-        kv[u][1] = __builtin_nontemporal_load(p.v.row(page[u], h, row[u]) + c);
-      }
-#pragma unroll
-      for (int u = 0; u < kU; ++u) {
-        if (page[u] < 0) continue;
-        __builtin_nontemporal_store(kv[u][0], p.k.row(new_page[u], h, new_row[u]) + c);
-        __builtin_nontemporal_store(kv[u][1], p.v.row(new_page[u], h, new_row[u]) + c);
-      }
+    for (int64_t r = (int64_t)blockIdx.x * R + first; r < p.budget; r += (int64_t)gridDim.x * R) {
+      const int slot = kept[r];
+      int page, row, new_page, new_row;
+      const bool from = find_slot(p.view, b, max(slot, 0), &page, &row);
+      const bool to = find_slot(p.to, b, (int)r, &new_page, &new_row);
+      if (!((slot >= 0) & from & to)) continue;
+      const u32x4 key = __builtin_nontemporal_load(p.k.row(page, h, row) + c);
+      const u32x4 value = __builtin_nontemporal_load(p.v.row(page, h, row) + c);
+      __builtin_nontemporal_store(key, p.k.row(new_page, h, new_row) + c);
+      __builtin_nontemporal_store(value, p.v.row(new_page, h, new_row) + c);
     }
     if (h == 0 && blockIdx.x == 0 && threadIdx.x == 0)
       p.new_lengths[b] = min(clamp_length(p.view.lengths[b], p.view.room), p.budget);
   }
+}
+
+// x by y workgroups, which loop where that is more than a million.
+dim3 tiles_by(int64_t x, int64_t y) {
+  y = std::min<int64_t>(y, 65535);
+  return dim3((unsigned)std::min(x, std::max<int64_t>(1, (1 << 20) / y)), (unsigned)y);
 }
 
 }  // namespace
@@ -253,7 +249,7 @@ hipError_t launch_paged_append(const PagedAppendDesc& d, hipStream_t s) {
   const int chunks = d.c.D / 8;
   p.tokens = (int)std::max<int64_t>(1, 256 / ((int64_t)p.heads * chunks));
   const int64_t tiles = ((int64_t)p.T + p.tokens - 1) / p.tokens;
-  const dim3 grid((unsigned)std::min<int64_t>(tiles, 1 << 20), (unsigned)std::min(p.B, 65535));
+  const dim3 grid = tiles_by(tiles, p.B);
   auto go = [&](auto kern) { hipLaunchKernelGGL(kern, grid, dim3(256), 0, s, p); };
   if (chunks == 16) go(paged_append<16>);
   else go(paged_append<8>);
@@ -283,8 +279,8 @@ hipError_t launch_paged_evict(const PagedEvictDesc& d, hipStream_t s) {
   else hipLaunchKernelGGL(evict_select<0>, all, threads, 0, s, p);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
-  const int chunks = d.c.D / 8, rows = 256 / chunks * kU;
-  const dim3 grid((unsigned)((p.budget + rows - 1) / rows), (unsigned)std::min<int64_t>(heads, 65535));
+  const int chunks = d.c.D / 8, rows = 256 / chunks;
+  const dim3 grid = tiles_by((p.budget + (int64_t)rows - 1) / rows, heads);
   if (chunks == 16) hipLaunchKernelGGL(evict_copy<16>, grid, dim3(256), 0, s, p);
   else hipLaunchKernelGGL(evict_copy<8>, grid, dim3(256), 0, s, p);
   return hipGetLastError();
