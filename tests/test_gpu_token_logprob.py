@@ -255,7 +255,6 @@ def test_backward_of_masked_and_padded_rows(dnn):
     x[0, 5:300] = -math.inf
     x[1, :599] = -math.inf
     check_backward(dnn, x, [0, 599, 3, 4], True, gen)
-    assert torch.equal(torch.isfinite(x), torch.isfinite(x))
     x[2, 7], x[3] = math.nan, math.inf
     dx = torch.full_like(x, math.nan)
     lse, dl = torch.zeros(4, device="cuda"), torch.ones(4, device="cuda")
