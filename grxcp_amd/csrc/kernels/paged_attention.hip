@@ -5,18 +5,19 @@
 // docs/designs/grxcp_roadmap.md:864-877) and ships no code.
 //
 // Every key and value is read once, for the whole group of query heads that share
-// it, so the call is bound by reading the cache: 4 flops per query head and byte
-// pair. What carries that:
+// it (32 of them at a time), so the call is bound by reading the cache: 4 flops per
+// query head and byte pair. What carries that:
 //
-//  * the cache of all sequences and key heads is one list of units of 128 slots of
-//    one head, which the workgroups divide evenly (decode_split): whatever the
-//    sequences' lengths, every CU reads the same share. The lengths are device
-//    data, so each workgroup finds its share by a scan of them. A share that ends
-//    inside a sequence leaves a partial result (O without its division, running
-//    maximum, sum) and decode_join adds those up, in the order of the slots;
-//  * a unit's four tiles of 32 slots go to the workgroup's four waves, each with a
-//    running maximum, sum and O of its own: no barrier until a share's part of a
-//    sequence ends and the four meet in LDS;
+//  * the cache of all sequences and key heads is one list of units, of a tile of 32
+//    slots for each of the workgroup's four waves: 128 slots of one key head, 64 of
+//    two or 32 of four (plan_of says when). The workgroups divide it evenly
+//    (decode_split): whatever the sequences' lengths, every CU reads the same share.
+//    The lengths are device data, so each workgroup finds its share by a scan of
+//    them. A share that ends inside a sequence leaves a partial result (O without its
+//    division, running maximum, sum) and decode_join adds those up, in the order of
+//    the slots. Where no sequence is long a workgroup takes a whole one instead;
+//  * each wave has a running maximum, sum and O of its own: no barrier until a
+//    share's part of a sequence ends and a head's waves meet in LDS;
 //  * scores are S^T = K Q^T (v_mfma_16x16x32), 16 query heads at a time, the K rows
 //    in registers straight from memory. A group of fewer heads leaves columns
 //    empty: the matrix cores have the time (16 MFMAs per 16 KB of cache);
@@ -27,10 +28,19 @@
 //    (global_load_lds_dwordx4), chunks of 16 bytes XORed with the row so that a read
 //    of 8 rows touches every bank once;
 //  * the next tile's K and V are in flight while one is computed, and the page table
-//    is read a tile further ahead: 16 KB per wave and tile, 8 waves per CU;
+//    is read a tile further ahead: 16 KB per wave and tile, 8 waves per CU. Rows that
+//    nothing reads again are loaded past the caches (6.8 TB/s for 6.1 in a loop that
+//    only reads); those of a group of more than 32 heads are read once per 32;
 //  * slots that are not there (past the length, or on a page that does not exist)
 //    read a row of zeros in place of what their page holds, and their scores are
 //    -inf, so nothing stale reaches a sum.
+//
+// us for 32 query and 8 key heads of 128, bf16, pages of 16 slots: 48 sequences of 33 to
+// 4096 slots 77.5 (5.2 TB/s; 73 the split, 5 the join), 16 of 8192 93.6 (5.7), 2 of
+// 131072 with 4 key heads 90 (6.0), 64 of 500 26.9 (4.9), one of 201 6.7, one of 60 5.3.
+// 512 workgroups that fill a CU's registers start together, and each waits for lengths,
+// a table entry and its first tile in turn before the memory is busy; with the second
+// launch that is what a call has above its bytes.
 
 #include "../launch.h"
 #include "device_common.h"
@@ -724,6 +734,9 @@ hipError_t run(const PagedAttnDesc& d, hipStream_t s) {
   else go(decode_split<T, D, 2, false>);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess || (x.whole && !d.weights)) return e;
+  // A wave to a query head, or the workgroup: few heads have many parts each. us, wave /
+  // workgroup: 128 sequences of 800, 32 heads, 79.5 / 87.1; 16 of 8192 93.8 / 93.6; 2 of
+  // 131072 97.7 / 89.7; one of 8000 22.6 / 15.0.
   const int apiece = (int64_t)p.B * p.H >= 512 ? 4 : 1;
   const int64_t outs = x.whole ? 0 : (p.H + apiece - 1) / apiece, chunks = ((int64_t)d.c.W * d.c.page + 1023) / 1024;
   const int64_t jobs = outs + (d.weights ? p.heads * chunks : 0);

@@ -28,6 +28,11 @@
 // largest element below the last one, K times.
 //
 // Backward: one element-wise pass, bound by reading x and writing dx.
+//
+// us: 32 rows of 131072 bf16 with 8 alternatives 14.1 (8.4 MB: two launches, 10 and 4, of
+// which most is waiting), 256 rows 28.9 (2.3 TB/s), 2048 x 32000 without any 24.9 (5.3),
+// 4096 x 32001 fp32 86 (6.1); the gradient of 8192 x 65536 bf16 with entropy 345 (6.2), of
+// 500 x 50001 fp16 21.5 (4.7).
 
 #include "../launch.h"
 #include "device_common.h"
@@ -503,6 +508,7 @@ __global__ __launch_bounds__(256) void logprob_grad(GParams p) {
     const float g = given ? p.dlogprob[row] : 0.0f;
     const float gh = ENT ? p.dentropy[row] : 0.0f;
     const float c0 = ENT ? fmaf(gh, p.entropy[row], g) : g;
+    const bool some = given || gh != 0.0f;   // else the row has no gradient, whatever is in it
     const RowChunks<T, AL> rc(x, p.vocab, V - 1);
     const int first = blockIdx.x * 256 * kU + threadIdx.x;
     u32x4 raw[kU];
@@ -522,14 +528,13 @@ __global__ __launch_bounds__(256) void logprob_grad(GParams p) {
         if constexpr (ENT) lp = lp < -200.0f ? -200.0f : lp;
         const float w = __builtin_amdgcn_exp2f(lp * kLog2e);
         const float a = ENT ? fmaf(gh, lp, c0) : c0;
-        // without a token and an entropy the row has no gradient, whatever is in it
-        v[e] = ENT || given ? -(w * a) : 0.0f;
+        v[e] = some ? -(w * a) : 0.0f;
       }
-      const int at = token - rc.first(c);
-      if (given && (uint32_t)at < (uint32_t)V) {
+      const uint32_t at = (uint32_t)token - (uint32_t)rc.first(c);
+      if (given && at < (uint32_t)V) {
 #pragma unroll
         for (int e = 0; e < V; ++e)
-          if (e == at) v[e] += g;
+          if ((uint32_t)e == at) v[e] += g;
       }
       rc.store(dx, c, IO::pack(v));
     }

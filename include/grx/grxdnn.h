@@ -306,11 +306,12 @@ grxdnnStatus_t grxdnnTokenLogProbForward(grxdnnHandle_t handle,
  * forward call's logSumExp and entropy:
  *   dx[r,j] = dLogProb[r] (1[j = tokens[r]] - p[r,j])         (0 without a token)
  *           - dEntropy[r] p[r,j] (log p[r,j] + entropy[r])    (0 where p = 0)
- * with p[r,j] = exp(x[r,j] - logSumExp[r]). tokens and dLogProb may be NULL
- * together, and dEntropy may be (entropy is then not read): that term is left
- * out; not both. dx: a
- * descriptor of x's shape and type; fp32 arithmetic, rounded once; dx may be x
- * itself (same pointer and strides). topLogProb has no gradient here. */
+ * with p[r,j] = exp(x[r,j] - logSumExp[r]) (below 2^-126: 0). A row without a token
+ * whose dEntropy is 0 or left out gets 0 whatever it holds: padding. tokens and
+ * dLogProb may be NULL together, and dEntropy may be (entropy is then not read):
+ * that term is left out; not both. dx: a descriptor of x's shape and type; fp32
+ * arithmetic, rounded once; dx may be x itself (same pointer and strides).
+ * topLogProb has no gradient here. */
 grxdnnStatus_t grxdnnTokenLogProbBackward(grxdnnHandle_t handle,
                                           grxdnnTensorDescriptor_t xDesc, const void* x,
                                           const int* tokens, const float* logSumExp,

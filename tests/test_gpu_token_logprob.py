@@ -261,6 +261,12 @@ def test_backward_of_masked_and_padded_rows(dnn):
     lse[2:] = math.nan
     backward(dnn, x, ints([0, 599, -1, 600]), lse, None, dl, None, dx)
     assert (dx[2:] == 0).all() and torch.isfinite(dx).all()
+    # with an entropy term for the first rows only
+    dx.fill_(math.nan)
+    H = torch.full_like(lse, math.nan)
+    H[:2] = 1.0
+    backward(dnn, x, ints([0, 599, -1, 600]), lse, H, dl, torch.tensor([0.5, 0.5, 0.0, -0.0], device="cuda"), dx)
+    assert (dx[2:] == 0).all() and torch.isfinite(dx).all()
 
 
 def test_gradient_against_differences(dnn):
