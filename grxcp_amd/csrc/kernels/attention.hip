@@ -820,12 +820,6 @@ int split_blocks(int cus, int64_t heads, int S, int D, bool causal) {
   return qw;
 }
 
-// GRXDNN_LOG set (and not "0"): one line on stderr per attention call.
-bool log_launches() {
-  const char* v = std::getenv("GRXDNN_LOG");
-  return v && *v && !(v[0] == '0' && v[1] == 0);
-}
-
 template <AttnType T, int D>
 hipError_t run(const AttnDesc& d, hipStream_t s) {
   AParams p{};
@@ -854,7 +848,7 @@ hipError_t run(const AttnDesc& d, hipStream_t s) {
   int qw = d.probe ? 0 : split_blocks(cus, (int64_t)d.B * d.H, d.S, D, p.causal);
   const int64_t items = qw ? (int64_t)p.heads * ((d.S + 32 * qw - 1) / (32 * qw)) : 0;
   if (items > max_workgroups(64 * kNW)) qw = 0;
-  if (log_launches())
+  if (log_dnn_launches())
     std::fprintf(stderr, "grxdnn: attention %s b=%d h=%d s=%d d=%d causal=%d kernel=%s\n",
                  T == AttnType::BF16 ? "bf16" : "f16", d.B, d.H, d.S, D, (int)p.causal,
                  qw == 4 ? "split4" : qw == 2 ? "split2" : "fwd");

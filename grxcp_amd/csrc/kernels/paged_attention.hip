@@ -47,6 +47,7 @@
 #include "paged_common.h"
 
 #include <algorithm>
+#include <cstdio>
 
 namespace grxk {
 namespace {
@@ -727,6 +728,10 @@ hipError_t run(const PagedAttnDesc& d, hipStream_t s) {
   p.hw = x.hw; p.shift = x.hw == 4 ? 5 : x.hw == 2 ? 6 : 7;
   p.gtiles = x.gtiles; p.items = d.c.heads / x.hw * x.gtiles; p.rows = x.rows; p.wgs = x.wgs; p.whole = x.whole;
   p.c = d.scale * 1.4426950408889634f;
+  if (log_dnn_launches())
+    std::fprintf(stderr, "grxdnn: paged attention %s b=%d h=%d hkv=%d d=%d page=%d room=%d weights=%d kernel=%s%d\n",
+                 T == AttnType::BF16 ? "bf16" : "f16", p.B, p.H, p.heads, D, p.view.page, p.view.room,
+                 (int)(d.weights != nullptr), x.whole ? "whole" : "split", x.hw);
   const dim3 grid(x.wgs), threads(64 * kWaves);
   auto go = [&](auto kern) { hipLaunchKernelGGL(kern, grid, threads, 0, s, p); };
   if (x.nt == 1) go(decode_split<T, D, 1, true>);

@@ -7,9 +7,17 @@
 #include <hip/hip_runtime_api.h>
 #include <stdint.h>
 
+#include <cstdlib>
+
 #include <grx/grx_cycles.h>
 
 namespace grxk {
+
+// GRXDNN_LOG set (and not "0"): one line on stderr per attention call.
+inline bool log_dnn_launches() {
+  const char* v = std::getenv("GRXDNN_LOG");
+  return v && *v && !(v[0] == '0' && v[1] == 0);
+}
 
 // HIP takes fewer than 2^32 threads along a launch's x dimension.
 inline int64_t max_workgroups(int threads) { return 0xffffffffll / threads; }

@@ -332,3 +332,23 @@ def test_same_bits_every_time(dnn):
         attend(dnn, c, q, o, 128 ** -0.5, w)
         outs.append((o, w))
     assert all(torch.equal(o, outs[0][0]) and torch.equal(w, outs[0][1]) for o, w in outs)
+
+
+@pytest.mark.parametrize("b,H,heads,d,room,tokmajor,weights,kernel", [
+    (3, 8, 2, 64, 256, True, False, "whole1"), (40, 8, 4, 64, 512, True, True, "whole1"),
+    (3, 8, 2, 128, 512, True, False, "split1"),
+    (20, 4, 4, 64, 700, True, True, "split1"), (64, 4, 4, 64, 700, True, True, "split4"),
+    (20, 4, 4, 64, 700, False, True, "split1"), (40, 12, 6, 64, 600, True, False, "split2"),
+    (2, 66, 2, 128, 600, True, True, "split1"), (40, 132, 4, 64, 640, True, False, "split4"),
+])
+def test_every_kernel_choice(dnn, capfd, monkeypatch, b, H, heads, d, room, tokmajor, weights, kernel):
+    """The choice that GRXDNN_LOG names, on ragged lengths from none to the room's."""
+    gen = torch.Generator().manual_seed(20)
+    lengths = [0, 1, room] + torch.randint(0, room + 1, (max(0, b - 3),), generator=gen).tolist()
+    c = Cache(gen, BF16, lengths[:b], heads, 20 if room % 20 == 0 else 16, d, tokmajor, room=room)
+    capfd.readouterr()
+    monkeypatch.setenv("GRXDNN_LOG", "1")
+    check(dnn, c, query(gen, b, H, d, BF16), d ** -0.5, weights=weights, decay=0.5)
+    monkeypatch.delenv("GRXDNN_LOG")
+    log = [x for x in capfd.readouterr().err.splitlines() if x.startswith("grxdnn: paged attention ")]
+    assert len(log) == 1 and log[0].endswith(f"weights={int(weights)} kernel={kernel}"), log
