@@ -352,3 +352,34 @@ def test_every_kernel_choice(dnn, capfd, monkeypatch, b, H, heads, d, room, tokm
     monkeypatch.delenv("GRXDNN_LOG")
     log = [x for x in capfd.readouterr().err.splitlines() if x.startswith("grxdnn: paged attention ")]
     assert len(log) == 1 and log[0].endswith(f"weights={int(weights)} kernel={kernel}"), log
+
+
+@pytest.mark.parametrize("room", [8, 640])      # one launch, split and joined
+def test_more_sequences_than_a_grid_has_rows(dnn, room):
+    """70000 sequences over shared pages, most of them short; 40 are held to 64 bits, the
+    empty ones to 0."""
+    gen = torch.Generator().manual_seed(21)
+    b, heads, d, page, pages = 70000, 1, 64, 8, 90
+    k, v = (torch.randn((pages, heads, page, d), generator=gen).to(BF16) for _ in range(2))
+    table = torch.randint(0, pages, (b, room // page), generator=gen).int()
+    lengths = torch.randint(0, 9, (b,), generator=gen).int()
+    some = torch.cat([torch.randint(0, b, (35,), generator=gen), torch.tensor([0, 65534, 65535, 65536, b - 1])])
+    lengths[some] = torch.randint(1, room + 1, (40,), generator=gen).int()
+    q = query(gen, b, 2, d, BF16)
+    o, w = torch.full_like(q, math.nan), torch.zeros((b, heads, room), device="cuda")
+    kc, vc, tc, lc = (t.cuda() for t in (k, v, table, lengths))
+    kd, td, qd, wd = desc(kc), desc(tc), desc(q), desc(w)
+    ws = Workspace(dnn.paged_attention_workspace(qd, kd, td, wd))
+    say(f"paged attention of {b} sequences, room {room}")
+    g.check(dnn.paged_attention(g.AttnDesc(True, 0.125), qd, q.data_ptr(), kd, kc.data_ptr(), kd, vc.data_ptr(), td,
+                                tc.data_ptr(), lc.data_ptr(), 1.0, wd, w.data_ptr(), qd, o.data_ptr(), ws.p, ws.size))
+    torch.cuda.synchronize()
+    for i in some.tolist():
+        n = lengths[i].item()
+        K, V = (t[table[i].long()].transpose(0, 1).reshape(heads, room, d)[:, :n] for t in (k, v))
+        ref, p, bound, pbound = attention_ref(q[i, :, 0].cpu(), K, V, 0.125)
+        assert within(o[i, :, 0], ref, bound), i
+        assert ((w[i, 0, :n].cpu().double() - p.sum(0)).abs() <= pbound.sum(0) + 2.0 ** -21 * p.sum(0)).all(), i
+    assert (o[lengths == 0] == 0).all() and torch.isfinite(o).all()
+    # every query's weights sum to 1 within their fp32 roundings
+    assert torch.allclose(w.sum((1, 2)).cpu(), 2.0 * (lengths > 0), rtol=2.0 ** -14, atol=0)

@@ -265,3 +265,55 @@ def test_evict_after_append_and_capture(gpu):
             same = bits(a) if a.dtype == F16 else a.cpu(), bits(b) if b.dtype == F16 else b.cpu()
             assert torch.equal(*same), rep
     dnn.close()
+
+
+def test_more_sequences_than_a_grid_has_rows(dnn):
+    """70000 sequences of up to 6 slots: a token appended to each, then 3 slots kept."""
+    gen = torch.Generator().manual_seed(60)
+    b, heads, page, d, budget = 70000, 1, 2, 64, 3
+    old = torch.randint(0, 6, (b,), generator=gen).int().cuda()
+    order = torch.randperm(b * 5, generator=gen).int().cuda()
+    table, new_table = order[: 3 * b].view(b, 3), order[3 * b:].view(b, 2)
+    shape = (b * 5, heads, page, d)
+    k, v = (torch.zeros(shape, dtype=BF16, device="cuda") for _ in range(2))
+    # a row's values say whose and which it is: sequence and slot, exact in bf16
+    who, slots = torch.arange(b, device="cuda"), torch.arange(6, device="cuda")
+    rows = torch.stack([(who % 256)[:, None] + 0 * slots, (who // 256)[:, None] + 0 * slots, 0 * who[:, None] + slots], 2)
+    for j in range(6):
+        at = table[:, j // page].long()
+        live = j < old
+        k[at[live], 0, j % page, :3] = rows[live, j].to(BF16)
+        v[at[live], 0, j % page, 1:4] = rows[live, j].to(BF16)
+    kn, vn = (torch.zeros((b, heads, 1, d), dtype=BF16, device="cuda") for _ in range(2))
+    kn[:, 0, 0, :3] = rows[who, old.long()].to(BF16)
+    vn[:, 0, 0, 1:4] = rows[who, old.long()].to(BF16)
+    kd, td = desc(k), desc(table)
+    say("append to and eviction of 70000 sequences")
+    nd = desc(kn)
+    g.check(dnn.paged_append(nd, kn.data_ptr(), nd, vn.data_ptr(), kd, k.data_ptr(), kd, v.data_ptr(), td,
+                             table.data_ptr(), old.data_ptr()))
+    n = old + 1
+    w = torch.randint(0, 4, (b, heads, 6), generator=gen).float().cuda()
+    kept = torch.full((b, heads, budget), -7, dtype=torch.int32, device="cuda")
+    new_n, new_w = torch.empty_like(n), torch.full((b, heads, 4), math.nan, device="cuda")
+    g.check(dnn.paged_evict(kd, k.data_ptr(), kd, v.data_ptr(), td, table.data_ptr(), n.data_ptr(), desc(w),
+                            w.data_ptr(), budget, 1, kept.data_ptr(), desc(new_table), new_table.data_ptr(),
+                            new_n.data_ptr(), desc(new_w), new_w.data_ptr()))
+    torch.cuda.synchronize()
+    assert torch.equal(new_n, n.clamp(max=budget))
+    # order of the old ones by (weight, lower slot), the newest before all
+    rank = w[:, 0] * 8 - slots
+    rank[slots == (n - 1)[:, None]] = 100
+    rank[slots >= n[:, None]] = -100
+    want = rank.argsort(1, descending=True)[:, :budget]
+    want[torch.arange(budget, device="cuda") >= n[:, None]] = 99
+    want = want.sort(1).values
+    there = want < 99
+    assert torch.equal(kept[:, 0], want.masked_fill(~there, -1).int())
+    assert torch.equal(new_w[:, 0, :3], torch.where(there, w[:, 0].gather(1, want.clamp(max=5)), 0.0))
+    assert (new_w[:, 0, 3] == 0).all()
+    for i in range(budget):
+        here = there[:, i]
+        for pool, c in ((k, 0), (v, 1)):
+            got = pool[new_table[here, i // page].long(), 0, i % page, c:c + 3]
+            assert torch.equal(got, rows[who[here], want[here, i]].to(BF16)), (i, c)

@@ -346,3 +346,12 @@ def test_captured_forward_and_backward(gpu):
         backward(dnn, x, tokens, lse, H, dl, dH, eager)
         assert torch.equal(eager, dx), rep
     dnn.close()
+
+
+@pytest.mark.parametrize("dtype,vocab", [(BF16, 1 << 24), (F32, (1 << 24) - 3)])
+def test_the_largest_vocabulary(dnn, dtype, vocab):
+    gen = torch.Generator().manual_seed(50)
+    x = logits(gen, (2, vocab), dtype)
+    x[1, -1] = 25.0
+    check_forward(dnn, x, [vocab - 1, vocab], 64)
+    check_backward(dnn, x, [vocab - 1, vocab], True, gen)
