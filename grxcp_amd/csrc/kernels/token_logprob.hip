@@ -23,14 +23,17 @@
 // largest of the 128 maxima of the wave's lanes' half batches; it is raised after batches
 // 2, 4, 8, ... to the list's K-th largest, so a wave lists about K of every doubling of
 // what it has read. Elements are ranked by value, then by lower index; as batches come in
-// index order an equal value in a later batch never outranks one in the list. A list that
-// runs over (an ordered row, one of equal values), NaN and +inf take the direct way: the
-// largest element below the last one, K times.
+// index order an equal value in a later batch never outranks one in the list. A batch with
+// more such elements than that (a row that rises, a vocabulary mask's run of -inf) sets the
+// threshold from its own maxima again and lists, of what equals it, only the first few: us
+// of 2048 x 32000 bf16 with 8 alternatives, 39 in no order, 51 where all but 5 are -inf,
+// 110 rising. What no such step fits (NaN, +inf, a last batch that rises by hundreds) takes
+// the direct way: the largest element below the last one, K times.
 //
 // Backward: one element-wise pass, bound by reading x and writing dx.
 //
-// us: 32 rows of 131072 bf16 with 8 alternatives 14.1 (8.4 MB: two launches, 10 and 4, of
-// which most is waiting), 256 rows 28.9 (2.3 TB/s), 2048 x 32000 without any 24.9 (5.3),
+// us: 32 rows of 131072 bf16 with 8 alternatives 14.3 (8.4 MB: two launches, 11 and 4, of
+// which most is waiting), 256 rows 30.2 (2.2 TB/s), 2048 x 32000 without any 24.9 (5.3),
 // 4096 x 32001 fp32 86 (6.1); the gradient of 8192 x 65536 bf16 with entropy 345 (6.2), of
 // 500 x 50001 fp16 21.5 (4.7).
 
@@ -106,9 +109,9 @@ __device__ __forceinline__ int rank_of(const uint64_t* keys, int c, uint64_t k) 
   return r;
 }
 
-// The largest key that K of the wave's keys reach, N of them to a lane, or one a little
-// below it: bit by bit from the top, as far down as keys of T differ. 0 if there are
-// fewer than K above 0.
+// The largest key that K of the wave's keys reach, N of them to a lane, or one below it
+// that no more than these reach: bit by bit from the top, as far down as keys of T differ
+// (the rest is 0, or all ones below the keys of 0). 0 if there are fewer than K above 0.
 template <NormType T, int N> __device__ __forceinline__ uint32_t reached_by(const uint32_t (&key)[N], int K) {
   constexpr int kLast = T == NormType::F32 ? 0 : T == NormType::BF16 ? 16 : 13;
   uint32_t v = 0;
@@ -120,7 +123,7 @@ template <NormType T, int N> __device__ __forceinline__ uint32_t reached_by(cons
     if (c >= K) v = t;
     if (c == K) break;
   }
-  return v;
+  return v && v < 0x80000000u ? v | ((1u << kLast) - 1) : v;
 }
 // A bound's value; -inf for what is below every value.
 __device__ __forceinline__ float bound_value(uint32_t key) {
@@ -168,6 +171,21 @@ __device__ __forceinline__ uint32_t refine(uint64_t* list, int& c, int top) {
 template <NormType T>
 __device__ __forceinline__ uint32_t refine_list(uint64_t* list, int& c, int top) {
   return c <= 64 ? refine<T, 1>(list, c, top) : refine<T, kCap / 64>(list, c, top);
+}
+
+// Of a list of c keys what reaches `bound`.
+__device__ __forceinline__ void keep(uint64_t* list, int& c, uint32_t bound) {
+  int to = 0;
+#pragma unroll 1
+  for (int i = 0; i < c; i += 64) {
+    const uint64_t key = i + (int)threadIdx.x < c ? list[i + threadIdx.x] : 0;
+    const bool stay = (uint32_t)(key >> 32) >= bound;
+    const uint64_t all = __ballot(stay);
+    if (stay)
+      list[to + (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(all >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)all, 0))] = key;
+    to += __popcll(all);
+  }
+  c = to;
 }
 
 // The K largest of a list of c keys, in order in `best`. Returns how many there are.
@@ -281,29 +299,74 @@ __global__ __launch_bounds__(64, AL ? 4 : 3) void logprob_pieces(LParams p) {
       s += bs;
       t += bt;
       if constexpr (TOP) {
-        if (batch == 0) {
-          const uint32_t key[2] = {order_key(__float_as_uint(fmaxf(high[0], high[1]))),
-                                   order_key(__float_as_uint(fmaxf(high[2], high[3])))};
-          limit = bound_value(reached_by<T>(key, p.top));
-        }
-        if (__ballot(top >= limit)) {
-          hold(cur);
-          // The thread's elements that go to the list, a bit each; -inf is also what lies
-          // outside the row.
-          uint32_t pass = 0;
-#pragma unroll
-          for (int q = U - 1; q >= 0; --q) {
-            float v[V];
-            IO::unpack(cur[q], v);
-#pragma unroll
-            for (int e = V - 1; e >= 0; --e) pass = pass + pass + (v[e] >= limit ? 1u : 0u);
+        // What K of the batch's elements reach: the K-th largest of its parts' maxima. Parts
+        // of two chunks a lane where fewer than K of them fit the list.
+        auto reach = [&]() __attribute__((always_inline)) {
+          if ((kMaxTop - 1) * 2 * V <= kCap || p.top <= kCap / (2 * V)) {
+            const uint32_t key[2] = {order_key(__float_as_uint(fmaxf(high[0], high[1]))),
+                                     order_key(__float_as_uint(fmaxf(high[2], high[3])))};
+            return bound_value(reached_by<T>(key, p.top));
           }
-          if (limit == -INFINITY)
+          uint32_t key[U];
+#pragma unroll
+          for (int q = 0; q < U; ++q) key[q] = order_key(__float_as_uint(high[q]));
+          return bound_value(reached_by<T>(key, p.top));
+        };
+        bool fresh = batch == 0;               // K of the batch's own elements reach the limit
+        if (fresh) limit = reach();
+        if (__ballot(top >= limit)) {
+          // The thread's elements from `from` on, a bit each.
+          auto reaching = [&](float from) __attribute__((always_inline)) {
+            hold(cur);
+            uint32_t pass = 0;
+#pragma unroll
+            for (int q = U - 1; q >= 0; --q) {
+              float v[V];
+              IO::unpack(cur[q], v);
+#pragma unroll
+              for (int e = V - 1; e >= 0; --e) pass = pass + pass + (v[e] >= from ? 1u : 0u);
+            }
+            return pass;
+          };
+          auto all = [&](uint32_t n) __attribute__((always_inline)) {
+            return __builtin_amdgcn_readlane((int)wave_upto(n), 63);
+          };
+          uint32_t pass = reaching(limit);
+          if (limit == -INFINITY)              // which is also what lies outside the row
 #pragma unroll
             for (int q = 0; q < U; ++q)
 #pragma unroll
               for (int e = 0; e < V; ++e)
                 if (!has(c + q * NT, e)) pass &= ~(1u << (V * q + e));
+          // More than a batch in no order has, or than the list holds: a rising row, runs of
+          // equal values. (Thirty-two elements to a lane: few lanes cannot.)
+          const int most = min(2 * p.top + 32, kCap - listed);
+          if (__builtin_expect(32 * __popcll(__ballot(pass != 0)) > most && all(__popc(pass)) > most, 0)) {
+            const float to = fresh ? limit : reach();
+            if (to >= limit) {                 // K of this batch make it the limit
+              fresh = true;
+              limit = to;
+              keep(sh.list, listed, order_key(__float_as_uint(to)));
+              pass &= reaching(to);
+              // Those above it, and of those at it the first few that make K.
+              const uint32_t strict = pass & reaching(above(to));
+              const int want = max(0, p.top - all(__popc(strict)));
+              int before = 0;
+#pragma unroll 1
+              for (int q = 0; q < U; ++q) {
+                uint32_t f = (pass & ~strict) >> (V * q) & ((1u << V) - 1);
+                const int n = __popc(f), upto = (int)wave_upto((uint32_t)n);
+                const int stay = min(max(want - before - (upto - n), 0), n);
+#pragma unroll 1
+                for (int x = n; x > stay; --x) {
+                  const uint32_t last = 0x80000000u >> __clz(f);
+                  f ^= last;
+                  pass ^= last << (V * q);
+                }
+                before += __builtin_amdgcn_readlane(upto, 63);
+              }
+            }
+          }
           for (uint64_t any; (any = __ballot(pass != 0));) {
             const uint32_t i = pass ? __ffs(pass) - 1 : 0;
             const int at = listed + (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(any >> 32),
@@ -319,11 +382,11 @@ __global__ __launch_bounds__(64, AL ? 4 : 3) void logprob_pieces(LParams p) {
             listed += __popcll(any);
           }
         }
-        if (batch == 0) limit = above(limit);  // an equal value at a higher place ranks lower
+        over |= listed > kCap;
+        listed = min(listed, kCap);
+        if (fresh) limit = above(limit);       // an equal value at a higher place ranks lower
         // after batches 1, 3, 7, ...; of many alternatives after the first as well
-        if (more && ((batch + 1) & batch) == 0 && (batch || p.top > 16) && listed >= p.top) {
-          over |= listed > kCap;
-          listed = min(listed, kCap);
+        if (more && ((((batch + 1) & batch) == 0 && (batch || p.top > 16)) || listed > kCap / 2) && listed >= p.top) {
           limit = fmaxf(limit, above(bound_value(refine_list<T>(sh.list, listed, p.top))));
         }
       }
@@ -362,7 +425,6 @@ __global__ __launch_bounds__(64, AL ? 4 : 3) void logprob_pieces(LParams p) {
     }
     int found = 0;
     if constexpr (TOP) {
-      over |= listed > kCap;
       if (!over && v.s < INFINITY) {
         found = finish<T>(sh, p.top, listed);
       } else {                                 // the largest below the last one, K times

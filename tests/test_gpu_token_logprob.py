@@ -355,3 +355,23 @@ def test_the_largest_vocabulary(dnn, dtype, vocab):
     x[1, -1] = 25.0
     check_forward(dnn, x, [vocab - 1, vocab], 64)
     check_backward(dnn, x, [vocab - 1, vocab], True, gen)
+
+
+@pytest.mark.parametrize("vocab", [700, 33000, 200001])
+@pytest.mark.parametrize("kind", ["few", "lowest_first", "steps", "minus_one", "rising_negative", "late_half", "blocks"])
+@pytest.mark.parametrize("top", [5, 33, 64])
+def test_alternatives_behind_masks_and_in_runs(dnn, vocab, kind, top):
+    """Vocabulary masks that leave few tokens, runs of one value, values that rise or jump
+    far into a row, so that more elements pass a threshold at once than a list holds."""
+    gen = torch.Generator().manual_seed(vocab + top)
+    at = torch.arange(vocab)
+    n = torch.randn(vocab, generator=gen).mul(3)
+    few = torch.full((vocab,), -math.inf)
+    few[torch.randperm(vocab, generator=gen)[:7]] = n[:7]
+    x = {"few": few, "lowest_first": torch.where(at < vocab // 3, -3.3e38, n), "steps": (at // 900).float() / 8 - 20,
+         "minus_one": torch.where(at % 1000 == 999, -0.5, -1.0), "rising_negative": (at - vocab) / 128.0,
+         "late_half": torch.where((at > vocab // 2) & (at // 8 % 2 == 0), 5.0, n.clamp(max=4.0)),
+         "blocks": torch.where(at // 512 % 3 == 2, (at // 512).float() / 50, -7.0)}[kind]
+    for dtype in (F32, BF16, F16):
+        y = x.clamp(min=-65504.0) if dtype == F16 and kind == "lowest_first" else x
+        check_forward(dnn, y.to(dtype).expand(2, vocab).contiguous().cuda(), [0, vocab - 1], top)
