@@ -9,6 +9,7 @@
 #include "paged_common.h"
 
 #include <algorithm>
+#include <climits>
 
 namespace grxk {
 namespace {
@@ -88,14 +89,16 @@ constexpr int kWaves = 16;    // of a selecting workgroup
 //  * The key of the last slot that stays is found from the top, two bits a step: how
 //    many slots reach each of three keys, summed over the waves. Weights that differ
 //    are told apart long before the last bit: the steps end when exactly as many slots
-//    reach a key as stay.
+//    reach a key as stay, and once 64 or fewer lie between a key that too few reach and
+//    one that enough do, those go on in registers without a barrier.
 //  * Where every slot goes follows from the numbers of kept ones and of ties in the
 //    waves before and ballots within the wave: no loop over the slots with a barrier.
-// 128 heads of 6000 to 8192 slots to 2048: 21.7 us, bound by instruction issue on the 128
+// 128 heads of 6000 to 8192 slots to 2048: 19 us, bound by instruction issue on the 128
 // CUs that have one; a binary search over passes through memory, 256 threads, took 187.
 template <int N>
 __global__ __launch_bounds__(64 * kWaves) void evict_select(EvictParams p) {
-  __shared__ int sums[2][3][kWaves], above_of[kWaves], ties_of[kWaves];
+  __shared__ int sums[2][3][kWaves], above_of[kWaves], ties_of[kWaves], few_n;
+  __shared__ uint32_t few[64];
   const int bh = blockIdx.x, b = bh / p.heads, h = bh - b * p.heads, tid = threadIdx.x;
   const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int n = clamp_length(p.view.lengths[b], p.view.room), m = min(n, p.budget);
@@ -125,6 +128,8 @@ __global__ __launch_bounds__(64 * kWaves) void evict_select(EvictParams p) {
 
   uint32_t last = 0;       // slots whose key reaches it stay, or (ties) those above it and some of it
   bool ties = want > 0;
+  int upper = 0, lower = INT_MAX;     // slots that reach last + 4 << bit, and last
+  if (tid == 0) few_n = 0;
   for (int bit = 30, turn = 0; bit >= 0 && ties; bit -= 2, turn ^= 1) {
     uint32_t c[3] = {0, 0, 0};
     each([&](int, uint32_t key) __attribute__((always_inline)) {
@@ -149,9 +154,28 @@ __global__ __launch_bounds__(64 * kWaves) void evict_select(EvictParams p) {
       const int s = __builtin_amdgcn_readlane((int)got, 16 * d + 15);
       if (s >= want) {
         last |= (uint32_t)(d + 1) << bit;
+        lower = s;
         ties = s != want;
         break;
       }
+      upper = s;
+    }
+    if (ties && bit && lower - upper <= 64) {
+      // What is left between: each wave goes on by itself, a key to a lane.
+      each([&](int, uint32_t key) __attribute__((always_inline)) {
+        if ((key - last) >> bit) return;       // (as unsigned: below last too)
+        few[atomicAdd(&few_n, 1)] = key;
+      });
+      __syncthreads();
+      const uint32_t key = lane < lower - upper ? few[lane] : 0;
+      for (int low = bit - 1; low >= 0 && ties; --low) {
+        const int c = __popcll(__ballot(key >= (last | 1u << low)));
+        if (c >= want - upper) {
+          last |= 1u << low;
+          ties = c != want - upper;
+        }
+      }
+      break;
     }
   }
   // What stays: newer slots, old ones above `last`, and of those at it all or, where
