@@ -598,15 +598,17 @@ __global__ __launch_bounds__(256) void decode_join(DParams p, uint32_t outs, int
     }
     const int j0 = (int)((blockIdx.x - outs) % chunks) * 1024;
     if (j0 >= len) continue;
-    // What the past steps gave the thread's four slots: it comes meanwhile.
+    // What the past steps gave the thread's four slots, and the first head's scores: they
+    // come meanwhile.
     float* w = p.w + b * p.w_sb + head * p.w_sh;
     const float* sc = p.scores + ((int64_t)b * p.H + head * p.group) * p.slots;
-    float old[4], a[4];
+    float old[4], a[4], s[4], next[4];
     int at[4];
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
       at[u] = min(j0 + 256 * u + tid, len - 1);
       old[u] = p.decay == 0.0f ? 0.0f : w[at[u]];
+      s[u] = sc[at[u]];
       a[u] = 0.0f;
     }
     // Sixteen lanes to a query head's parts.
@@ -639,13 +641,13 @@ __global__ __launch_bounds__(256) void decode_join(DParams p, uint32_t outs, int
     __syncthreads();
 #pragma unroll 2
     for (int r = 0; r < p.group; ++r) {
-      float s[4];
 #pragma unroll
-      for (int u = 0; u < 4; ++u) s[u] = sc[(int64_t)r * p.slots + at[u]];
+      for (int u = 0; u < 4; ++u) next[u] = sc[(int64_t)min(r + 1, p.group - 1) * p.slots + at[u]];
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
         const float x = __builtin_amdgcn_exp2f(s[u] - stat[r][0]) * stat[r][1];
         a[u] += __float_as_uint(s[u]) == kAbsent ? 0.0f : x;
+        s[u] = next[u];
       }
     }
 #pragma unroll
