@@ -36,7 +36,7 @@
 //    -inf, so nothing stale reaches a sum.
 //
 // us for 32 query and 8 key heads of 128, bf16, pages of 16 slots: 48 sequences of 33 to
-// 4096 slots 77.5 (5.2 TB/s; 73 the split, 5 the join), 16 of 8192 93.6 (5.7), 2 of
+// 4096 slots 76 (5.3 TB/s; 72 the split, 5 the join), 16 of 8192 93.6 (5.7), 2 of
 // 131072 with 4 key heads 90 (6.0), 64 of 500 26.9 (4.9), one of 201 6.7, one of 60 5.3.
 // 512 workgroups that fill a CU's registers start together, and each waits for lengths,
 // a table entry and its first tile in turn before the memory is busy; with the second
@@ -60,7 +60,10 @@ typedef __attribute__((address_space(3))) void* lds_ptr_t;
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) s16x4* lds_s16x4_t;
 
-// Workgroups that share a CU: registers (D = 64 has half the accumulators) and LDS.
+// Workgroups that share a CU: registers (D = 64 has half the accumulators) and LDS. us at
+// D = 64, three / four (28 bytes of registers spilled, shares a quarter shorter): 24 x 16
+// heads of 500 to 3001 slots with weights 42.3 / 50.8, 16 x 16 of 8192 94.6 / 103.4; with two
+// tiles of query heads, two / three: 32 x 2 of 4000 22.8 / 26.4.
 template <int D, int NT> constexpr int wgs_per_cu() { return D == 64 && NT == 1 ? 3 : 2; }
 
 template <int N> struct Buf { static constexpr int value = N; };
