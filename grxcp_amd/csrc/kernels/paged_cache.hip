@@ -164,7 +164,8 @@ __global__ __launch_bounds__(64 * kWaves) void evict_select(EvictParams p) {
       // What is left between: each wave goes on by itself, a key to a lane.
       each([&](int, uint32_t key) __attribute__((always_inline)) {
         if ((key - last) >> bit) return;       // (as unsigned: below last too)
-        few[atomicAdd(&few_n, 1)] = key;
+        const int at = atomicAdd(&few_n, 1);
+        if (at < 64) few[at] = key;
       });
       __syncthreads();
       const uint32_t key = lane < lower - upper ? few[lane] : 0;
@@ -212,8 +213,9 @@ __global__ __launch_bounds__(64 * kWaves) void evict_select(EvictParams p) {
     const uint64_t tie = __ballot(tied(j, key));
     const bool stay = above(j, key) || (tied(j, key) && __popcll(tie & below) < room);
     const uint64_t all = __ballot(stay);
-    if (stay) {
-      const int i = to + __popcll(all & below);
+    const int i = to + __popcll(all & below);
+    // (weights that change while they are read must not lead out of the arrays)
+    if (stay && i < m) {
       kept[i] = j;
       nw[i] = w[j];
     }
