@@ -20,7 +20,7 @@
 //    share's part of a sequence ends and a head's waves meet in LDS;
 //  * scores are S^T = K Q^T (v_mfma_16x16x32), 16 query heads at a time, the K rows
 //    in registers straight from memory. A group of fewer heads leaves columns
-//    empty: the matrix cores have the time (16 MFMAs per 16 KB of cache);
+//    empty: the matrix cores have the time (24 MFMAs per 16 KB of cache);
 //  * O^T += V^T P^T: the scores' lanes hold P^T as the B operand wants it if the
 //    contraction runs over slots in the order 4g .. 4g+3, 16+4g .. 16+4g+3 (g: 16
 //    lanes), and the V^T operand comes from the row-major V tile in LDS by the
@@ -63,7 +63,7 @@ typedef __attribute__((address_space(3))) s16x4* lds_s16x4_t;
 // Workgroups that share a CU: registers (D = 64 has half the accumulators) and LDS. us at
 // D = 64, three / four (28 bytes of registers spilled, shares a quarter shorter): 24 x 16
 // heads of 500 to 3001 slots with weights 42.3 / 50.8, 16 x 16 of 8192 94.6 / 103.4; with two
-// tiles of query heads, two / three: 32 x 2 of 4000 22.8 / 26.4.
+// tiles of query heads, two / three: 32 x 2 of 4000 23.1 / 26.4.
 template <int D, int NT> constexpr int wgs_per_cu() { return D == 64 && NT == 1 ? 3 : 2; }
 
 template <int N> struct Buf { static constexpr int value = N; };
@@ -71,10 +71,23 @@ template <int N> struct Buf { static constexpr int value = N; };
 // What a slot that is not there is read from: D values of zero.
 __device__ __attribute__((aligned(256))) uint32_t zero_row[64];
 
+// split2: two weights x, y >= 0 as a + b in the value type, which the product with V takes
+// one after the other: a is cut off, b what that leaves. That keeps 16 bits (bf16) or 21
+// (f16) of a weight; rounding it once, 8 or 11, costs o up to as much as its own rounding
+// (and more where values cancel). b is not 0 where a is not, so that an infinite value
+// times either is the same infinity. us, rounded once / so: groups of up to 16 heads as
+// before (48 sequences of 33 to 4096 slots 76.1 / 76.0), 32 x 2 groups of 32 heads of 128,
+// 4000 slots, 36.8 / 38.0, 8 groups of 128 heads, 8000 slots, 32.3 / 34.3.
 template <AttnType T> struct PIo;
 template <> struct PIo<AttnType::BF16> {
   // The weights' scale: exp2 of a score is at most 2^4 (kLazy) times this.
   static constexpr float kTop = 0.0f;
+  __device__ static void split2(float x, float y, int& a, int& b) {
+    const uint32_t ux = __float_as_uint(x), uy = __float_as_uint(y);
+    a = (int)((uy & 0xffff0000u) | ux >> 16);
+    b = (int)pack_bf16x2(fmaf(x, 1.0f + 0x1p-20f, -__uint_as_float(ux & 0xffff0000u)),
+                         fmaf(y, 1.0f + 0x1p-20f, -__uint_as_float(uy & 0xffff0000u)));
+  }
   __device__ static f32x4 mma(i32x4 a, i32x4 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c,
                                                    0, 0, 0);
@@ -85,6 +98,14 @@ template <> struct PIo<AttnType::F16> {
   // Up to 2^15 of fp16's 65504, so that weights down to 2^-25 of the largest one keep
   // all of their bits: thousands of small ones may outweigh it together.
   static constexpr float kTop = 11.0f;
+  __device__ static void split2(float x, float y, int& a, int& b) {
+    typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+    const f16x2 h = __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_pkrtz(x, y));
+    const f16x2 rest = __builtin_bit_cast(f16x2, pack_f16x2(x - (float)h[0], y - (float)h[1]));
+    const _Float16 least = 0x1p-24f;
+    a = __builtin_bit_cast(int, h);
+    b = __builtin_bit_cast(int, __builtin_elementwise_max(rest, __builtin_elementwise_min(h, f16x2{least, least})));
+  }
   __device__ static f32x4 mma(i32x4 a, i32x4 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c,
                                                   0, 0, 0);
@@ -313,17 +334,21 @@ __global__ __launch_bounds__(64 * kWaves, (wgs_per_cu<D, NT>())) void decode_spl
       constexpr int BUF = decltype(buf)::value;
       const uint32_t mask = live[BUF];
       if (!mask && !p.scores) return;            // nothing to add and nothing to say
-      i32x4 pf[NT];
+      f32x4 scores[NT][2];                       // of all heads first: the keys' registers are free then
 #pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        f32x4 s[2];
+      for (int t = 0; t < NT; ++t)
 #pragma unroll
         for (int kt = 0; kt < 2; ++kt) {
-          s[kt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+          scores[t][kt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-          for (int f = 0; f < F; ++f) s[kt] = IO::mma(kf[BUF][kt][f], qf[t][f], s[kt]);
-          s[kt] *= p.c;
+          for (int f = 0; f < F; ++f) scores[t][kt] = IO::mma(kf[BUF][kt][f], qf[t][f], scores[t][kt]);
         }
+      i32x4 pf[NT], pr[NT];                      // the weights: leading bits, rest
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        f32x4 (&s)[2] = scores[t];
+        s[0] *= p.c;
+        s[1] *= p.c;
         if (mask != 0xffffffffu) {
 #pragma unroll
           for (int kt = 0; kt < 2; ++kt)
@@ -369,23 +394,40 @@ __global__ __launch_bounds__(64 * kWaves, (wgs_per_cu<D, NT>())) void decode_spl
             w[kt][r] = __builtin_amdgcn_exp2f((s[kt][r] - m[t]) + IO::kTop);
             l[t] += w[kt][r];
           }
-        pf[t] = i32x4{(int)IO::pack2(w[0][0], w[0][1]), (int)IO::pack2(w[0][2], w[0][3]),
-                      (int)IO::pack2(w[1][0], w[1][1]), (int)IO::pack2(w[1][2], w[1][3])};
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          int a, b;
+          IO::split2(w[x / 2][x % 2 * 2], w[x / 2][x % 2 * 2 + 1], a, b);
+          pf[t][x] = a;
+          pr[t][x] = b;
+        }
       }
       if (!mask) return;
       const uint8_t* v0 = vt + BUF * kStage * 16;
       const int r0 = 4 * g + (l16 >> 2), r1 = r0 + 16;
+      // Two tiles of the head dimension at a time: the products with the leading bits, then
+      // those with the rest, which wait for them.
 #pragma unroll
-      for (int d = 0; d < DT; ++d) {
-        const int c = 2 * d + ((lane >> 1) & 1);
-        const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-            (lds_s16x4_t)(v0 + r0 * 2 * D + 16 * (c ^ vswz<D>(r0)) + 8 * (lane & 1)));
-        const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-            (lds_s16x4_t)(v0 + r1 * 2 * D + 16 * (c ^ vswz<D>(r1)) + 8 * (lane & 1)));
-        const u32x2 w0 = __builtin_bit_cast(u32x2, a), w1 = __builtin_bit_cast(u32x2, x);
-        const i32x4 vf = {(int)w0.x, (int)w0.y, (int)w1.x, (int)w1.y};
+      for (int d0 = 0; d0 < DT; d0 += 2) {
+        i32x4 vf[2];
 #pragma unroll
-        for (int t = 0; t < NT; ++t) o[t][d] = IO::mma(vf, pf[t], o[t][d]);
+        for (int x = 0; x < 2; ++x) {
+          const int c = 2 * (d0 + x) + ((lane >> 1) & 1);
+          const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+              (lds_s16x4_t)(v0 + r0 * 2 * D + 16 * (c ^ vswz<D>(r0)) + 8 * (lane & 1)));
+          const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+              (lds_s16x4_t)(v0 + r1 * 2 * D + 16 * (c ^ vswz<D>(r1)) + 8 * (lane & 1)));
+          const u32x2 w0 = __builtin_bit_cast(u32x2, a), w1 = __builtin_bit_cast(u32x2, b);
+          vf[x] = i32x4{(int)w0.x, (int)w0.y, (int)w1.x, (int)w1.y};
+        }
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+          for (int x = 0; x < 2; ++x) o[t][d0 + x] = IO::mma(vf[x], pf[t], o[t][d0 + x]);
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+          for (int x = 0; x < 2; ++x) o[t][d0 + x] = IO::mma(vf[x], pr[t], o[t][d0 + x]);
       }
     };
     int e = entry(key);

@@ -214,11 +214,11 @@ grxdnnStatus_t grxdnnPagedCacheAppend(grxdnnHandle_t handle,
  *   p[b,h,:] = softmax(s[b,h,:]),  o[b,h,0,:] = sum_j p[b,h,j] V[slot j of b, head h / G, :]
  * q, o: [B, H, 1, D], H = G * Hkv query heads in groups of G = 1 .. 1024. The
  * descriptor's causal flag makes no difference: the new token is the last one.
- * Scores, softmax and sums are fp32 and the weights of the values are rounded
- * to the value type (as in grxdnnAttentionForward); o is rounded once. o may be
- * q itself (same pointer and strides). A sequence of no slots gives o = 0; one
- * whose scores are all -inf gives NaN, as the formula does. Slots at or past
- * lengths[b] are not read, whatever their pages hold.
+ * Scores, softmax and sums are fp32, the weights of the values keep 16 bits (bf16)
+ * or 21 (f16), and o is rounded once. o may be q itself (same pointer and
+ * strides). A sequence of no slots gives o = 0; one whose scores are all -inf
+ * gives NaN, as the formula does. Slots at or past lengths[b] are not read,
+ * whatever their pages hold.
  *
  * weights (optional, both arguments or neither NULL): what the slots received,
  * [B, Hkv, S] GRX_R_32F, S >= W * P, innermost stride 1:

@@ -6,7 +6,7 @@ import torch
 
 import grxcp_amd as g
 from helpers import say
-from paged_cases import Cache, Workspace, attend, attention_ref, desc, ints
+from paged_cases import HALF_STEP, Cache, Workspace, attend, attention_ref, desc, ints
 
 pytestmark = pytest.mark.gpu
 BF16, F16 = torch.bfloat16, torch.float16
@@ -383,3 +383,47 @@ def test_more_sequences_than_a_grid_has_rows(dnn, room):
     assert (o[lengths == 0] == 0).all() and torch.isfinite(o).all()
     # every query's weights sum to 1 within their fp32 roundings
     assert torch.allclose(w.sum((1, 2)).cpu(), 2.0 * (lengths > 0), rtol=2.0 ** -14, atol=0)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("H,heads,room", [(4, 2, 64), (40, 1, 64), (4, 2, 6000), (64, 2, 6000)])
+def test_values_are_weighted_by_more_than_16_bits(dnn, dtype, H, heads, room):
+    """Values of either sign that nearly cancel: o's one rounding is small there, and what
+    16-bit weights would cost stands far above it. As attention_ref, but for the weights,
+    which are held to 2^-15."""
+    gen = torch.Generator().manual_seed(22)
+    c = Cache(gen, dtype, [5, 16, 40, 3], heads, 16, 64, True, room=room)
+    q, scale = query(gen, 4, H, 64, dtype), 0.125 / 8
+    o = torch.full_like(q, math.nan)
+    say(f"weights of the values, {dtype}, {H} on {heads} heads, room {room}")
+    attend(dnn, c, q, o, scale)
+    for i, n in enumerate(c.n):
+        k, v = (t[i].double().repeat_interleave(H // heads, 0) for t in (c.K, c.V))
+        qi = q[i, :, 0].cpu().double()
+        ref, p, _, _ = attention_ref(q[i, :, 0].cpu(), c.K[i], c.V[i], scale)
+        size = torch.matmul(k.abs(), qi.abs()[:, :, None])[..., 0] * scale
+        rel = 2 * (64 + 3) * 2.0 ** -24 * size.amax(1, keepdim=True) + 2.0 ** -18
+        u = HALF_STEP[dtype]
+        mass = torch.matmul(p[:, None], v.abs())[:, 0]
+        assert within(o[i, :, 0], ref, u * ref.abs() + (1 + u) * (2.0 ** -15 + rel) * mass + 2.0 ** -25), i
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("room", [80, 800])
+def test_an_infinite_value_shows_whatever_it_weighs(dnn, dtype, room):
+    """Infinite values of slots that weigh much, little, and as much as the heaviest (a power
+    of two: no bits behind the first)."""
+    gen = torch.Generator().manual_seed(23)
+    c = Cache(gen, dtype, [70, 70, 1, 70], 2, 16, 64, True, room=room)
+    for t in (c.K[0], c.K[3]):
+        t[:] = 0.0
+    c.K[3][:, 40:, 0] = -80 * math.log(2)                 # scores of -10 log 2, about 2^-10
+    c.V[0][0, 3, 5], c.V[0][1, 69, 6] = math.inf, -math.inf
+    c.V[1][0, :, 5] = math.inf
+    c.V[1][1, 33, 7] = -math.inf
+    c.V[2][1, 0, 9] = math.inf
+    c.V[3][0, 50, 5], c.V[3][1, 1, 6] = -math.inf, math.inf
+    c.store()
+    q = query(gen, 4, 4, 64, dtype)
+    q[..., 0] = 1.0
+    check(dnn, c, q, 0.125)
