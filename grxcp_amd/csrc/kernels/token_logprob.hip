@@ -406,8 +406,9 @@ __global__ __launch_bounds__(64, AL ? 4 : 3) void logprob_pieces(LParams p) {
     v = moved(v, wave_max(v.m));
     v.s = wave_sum(v.s);
     v.t = wave_sum(v.t);
-    // NaN and +inf (S is not finite then), or a maximum of over 64.
-    const bool odd = !(v.s < INFINITY) || (!(fabsf(v.m) <= 64.0f) && v.s != 0.0f);
+    // NaN and +inf (S is not finite then), or a maximum of over 64. (S may be 0 there: r does
+    // not move for elements below -992 / log2 e, whose 2^(x log2 e - r) may all be too small.)
+    const bool odd = !(v.s < INFINITY) || (__ballot(m != -INFINITY) && !(fabsf(v.m) <= 64.0f));
     if (odd) {
       float s2 = 0.0f, t2 = 0.0f;
       for (int c = c0 + tid; c < c1 && rc.any(c); c += NT) {

@@ -375,3 +375,17 @@ def test_alternatives_behind_masks_and_in_runs(dnn, vocab, kind, top):
     for dtype in (F32, BF16, F16):
         y = x.clamp(min=-65504.0) if dtype == F16 and kind == "lowest_first" else x
         check_forward(dnn, y.to(dtype).expand(2, vocab).contiguous().cuda(), [0, vocab - 1], top)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("vocab", [700, 40000])       # a row in one piece, in several
+def test_rows_far_below_zero(dnn, dtype, vocab):
+    """Finite rows whose logits all lie around -1126 log 2 = -780.5, where powers of two
+    relative to 2^-1000 leave fp32: equal ones, spread ones, and one among -inf."""
+    gen = torch.Generator().manual_seed(51)
+    at = torch.arange(-800.0, -680.0, 0.5)[:, None]
+    one = torch.full((len(at), vocab), -math.inf)
+    one[torch.arange(len(at)), torch.randint(0, vocab, (len(at),), generator=gen)] = at[:, 0]
+    spread = at + torch.randn((len(at), vocab), generator=gen)
+    for x in (at.expand(-1, vocab), spread, one):
+        check_forward(dnn, x.to(dtype).contiguous().cuda(), [r % vocab for r in range(len(at))], 3)
