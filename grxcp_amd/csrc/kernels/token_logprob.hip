@@ -13,9 +13,12 @@
 // lane operations against the 64 a CU does in a cycle, which is 8 TB/s of bf16, little
 // above what the memory gives. Then log sum exp = max + log S and entropy =
 // log S - T / S from the sums moved to the row's maximum.
-// Products x log2 e are good to 2^-25 |x| (fma), which is enough within |x| <= 64:
-// a row whose maximum is outside, or whose sums are not finite, is read again with
-// x - max formed first.
+// x log2 e - r is one fma: off by half a step of itself. What the rounded log2 e is off by
+// and what r is cancel when the sums move to the maximum, as 2^(r - max log2 e) takes the
+// same two numbers: an element is off by 2^-26 |x - max| for it, whatever |x| is. A row
+// whose maximum is outside -64 .. 64, far within where r stays harmless, or whose sums are
+// not finite, is read again with x - max formed first. As e^0 is among them, S is at least
+// 1 and T at most 0: held to that, no probability is above 1 and no entropy below 0.
 //
 // Alternatives: the same pass compares each batch's maximum with a threshold that K
 // elements already read reach, and only where it is higher looks at the elements: those
@@ -48,7 +51,7 @@
 namespace grxk {
 namespace {
 
-constexpr float kLog2e = 1.4426950408889634f, kLog2eLow = 1.925963033e-8f, kLn2 = 0.6931471805599453f;
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kLowest = -__FLT_MAX__;
 constexpr int kU = 4;         // chunks of a thread (backward, and a forward batch of a whole row)
 constexpr int kMaxTop = 64;
@@ -397,7 +400,7 @@ __global__ __launch_bounds__(64, AL ? 4 : 3) void logprob_pieces(LParams p) {
     Sums v;
     v.m = m;
     {
-      const float off = fmaf(-m, kLog2eLow, fmaf(-m, kLog2e, r));    // r - m log2 e
+      const float off = fmaf(-m, kLog2e, r);
       const float f = __builtin_amdgcn_exp2f(off);
       v.s = s * f;
       v.t = kLn2 * f * fmaf(s, off, t);
@@ -408,7 +411,8 @@ __global__ __launch_bounds__(64, AL ? 4 : 3) void logprob_pieces(LParams p) {
     v.t = wave_sum(v.t);
     // NaN and +inf (S is not finite then), or a maximum of over 64. (S may be 0 there: r does
     // not move for elements below -992 / log2 e, whose 2^(x log2 e - r) may all be too small.)
-    const bool odd = !(v.s < INFINITY) || (__ballot(m != -INFINITY) && !(fabsf(v.m) <= 64.0f));
+    const bool some = __ballot(m != -INFINITY);
+    const bool odd = !(v.s < INFINITY) || (some && !(fabsf(v.m) <= 64.0f));
     if (odd) {
       float s2 = 0.0f, t2 = 0.0f;
       for (int c = c0 + tid; c < c1 && rc.any(c); c += NT) {
@@ -424,6 +428,8 @@ __global__ __launch_bounds__(64, AL ? 4 : 3) void logprob_pieces(LParams p) {
       v.s = wave_sum(s2);
       v.t = wave_sum(t2);
     }
+    if (some && v.s < 1.0f) v.s = 1.0f;        // (NaN stays)
+    if (v.t > 0.0f) v.t = 0.0f;
     int found = 0;
     if constexpr (TOP) {
       if (!over && v.s < INFINITY) {

@@ -389,3 +389,30 @@ def test_rows_far_below_zero(dnn, dtype, vocab):
     spread = at + torch.randn((len(at), vocab), generator=gen)
     for x in (at.expand(-1, vocab), spread, one):
         check_forward(dnn, x.to(dtype).contiguous().cuda(), [r % vocab for r in range(len(at))], 3)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("vocab", [2, 700, 40000])
+@pytest.mark.parametrize("rest", [100, 30])
+def test_no_probability_above_one(dnn, dtype, vocab, rest):
+    """One logit m with all of the mass, m = -64 .. 64 and the others `rest` below it: its log
+    probability is never above 0 and the entropy never below, and both are right to 8 half
+    steps of 1. (Two powers of two, each within a unit in the last place, 4 half steps, and
+    their product, 1, make the sum; a log next to 1 moves by what the sum does. What the
+    others add is in the reference: 40000 e^-30 is 2^-28.)"""
+    m = torch.arange(-64.0, 65.0)
+    x = (m[:, None] - rest).expand(-1, vocab).clone()
+    at = torch.arange(len(m)) * 17 % vocab
+    x[torch.arange(len(m)), at] = m
+    x = x.to(dtype)
+    say(f"one logit, {dtype}, {vocab}, the others {rest} below")
+    logp, lse, H, best, index = (t.cpu() for t in forward(dnn, x.cuda(), ints(at.tolist()), 1))
+    ref = x.double().log_softmax(1)
+    want = ref.amax(1)
+    entropy = -(ref.exp() * ref).sum(1)
+    assert torch.equal(index[:, 0].long(), at)
+    assert (logp <= 0).all() and (best <= 0).all() and (H >= 0).all()
+    eight = 8 * HALF[F32]
+    assert ((logp.double() - want).abs() <= eight).all() and torch.equal(best[:, 0], logp)
+    assert ((H.double() - entropy).abs() <= eight + 2.0 ** -18 * entropy).all()
+    assert ((lse.double() - (m.double() - want)).abs() <= eight + HALF[F32] * m.abs()).all()
