@@ -542,12 +542,19 @@ __device__ __forceinline__ void add_parts(const float* ml, const float* po, int6
     vec v[4];
     float pm[4], pl[4];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {            // all loads first; a part too far counts as one of no slot
+    for (int u = 0; u < 4; ++u) {            // all loads first
       const int64_t at = min(y + u * by, count - 1) * each;
       v[u] = *(const vec*)(po + at * D);
-      pm[u] = y + u * by < count ? ml[2 * at] : -INFINITY;
+      pm[u] = ml[2 * at];
       pl[u] = ml[2 * at + 1];
     }
+#pragma unroll
+    for (int u = 1; u < 4; ++u)              // a part too far is one of no slot, in what it weighs too
+      if (y + u * by >= count) {
+        v[u] = vec(0.0f);
+        pm[u] = -INFINITY;
+        pl[u] = 0.0f;
+      }
     const float top = fmaxf(fmaxf(m, fmaxf(pm[0], pm[1])), fmaxf(pm[2], pm[3]));
     const float from = fmaxf(top, kLowest);  // -inf - from is -inf
     const float f = __builtin_amdgcn_exp2f(m - from);

@@ -427,3 +427,20 @@ def test_an_infinite_value_shows_whatever_it_weighs(dnn, dtype, room):
     q = query(gen, 4, 4, 64, dtype)
     q[..., 0] = 1.0
     check(dnn, c, q, 0.125)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("b,H,heads,d", [(1, 4, 2, 64), (40, 16, 2, 128), (40, 16, 2, 64), (3, 16, 16, 128)])
+def test_infinite_values_in_the_last_part(dnn, capfd, monkeypatch, dtype, b, H, heads, d):
+    """Sequences in every number of parts whose last slots hold infinite values: these show,
+    and nothing turns into NaN."""
+    gen = torch.Generator().manual_seed(24)
+    lengths = [1500 - 37 * (i % 23) for i in range(b)]
+    c = Cache(gen, dtype, lengths, heads, 16, d, False)
+    for v in c.V:
+        v[0, -1, 5], v[heads - 1, -20:, d - 1] = math.inf, -math.inf
+    c.store()
+    capfd.readouterr()
+    monkeypatch.setenv("GRXDNN_LOG", "1")
+    check(dnn, c, query(gen, b, H, d, dtype), 0.5 * d ** -0.5)
+    assert "kernel=split" in capfd.readouterr().err
