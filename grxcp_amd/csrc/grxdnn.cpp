@@ -102,20 +102,21 @@ bool same_shape(const grxdnnTensorStruct& a, const grxdnnTensorStruct& b) {
 }
 
 // Rows of a [..., hidden] tensor: all leading dimensions must collapse into
-// one row index with a single pitch. Returns false if they do not.
+// one row index with a single pitch. Returns false if they do not. What a
+// dimension of extent 1 has for a stride does not matter.
 bool row_layout(const grxdnnTensorStruct& t, int64_t* rows, int64_t* pitch) {
-  const int nb = t.nb;
-  const int hidden = t.dims[nb - 1];
-  if (nb == 1) { *rows = 1; *pitch = hidden; return true; }
-  int64_t r = 1;
-  for (int i = 0; i < nb - 1; ++i) r *= t.dims[i];
-  *rows = r;
-  *pitch = t.strides[nb - 2];
-  if (*pitch < hidden) return r <= 1;
-  for (int i = 0; i < nb - 2; ++i)
-    if (t.dims[i + 1] > 1 && (int64_t)t.strides[i] != (int64_t)t.strides[i + 1] * t.dims[i + 1])
-      return false;
-  return true;
+  const int hidden = t.dims[t.nb - 1];
+  *rows = 1;
+  *pitch = t.nb == 1 ? hidden : t.strides[t.nb - 2];
+  int64_t next = -1;               // what the next outer stride has to be, from the first extent above 1 on
+  for (int i = t.nb - 2; i >= 0; --i) {
+    *rows *= t.dims[i];
+    if (t.dims[i] == 1) continue;
+    if (next < 0) *pitch = t.strides[i];
+    else if (t.strides[i] != next) return false;
+    next = (int64_t)t.strides[i] * t.dims[i];
+  }
+  return *pitch >= hidden || *rows <= 1;
 }
 
 bool aligned16(const void* p) { return ((uintptr_t)p % 16) == 0; }

@@ -416,3 +416,54 @@ def test_no_probability_above_one(dnn, dtype, vocab, rest):
     assert ((logp.double() - want).abs() <= eight).all() and torch.equal(best[:, 0], logp)
     assert ((H.double() - entropy).abs() <= eight + 2.0 ** -18 * entropy).all()
     assert ((lse.double() - (m.double() - want)).abs() <= eight + HALF[F32] * m.abs()).all()
+
+
+def last_tokens(gen, dtype, rows, vocab, how):
+    """[rows, 1, vocab] views of a wider array whose other elements are NaN."""
+    shape = {"slice": (rows, 3, vocab), "transposed": (1, rows, vocab), "padded": (rows, 3, vocab + 5)}[how]
+    wide = torch.full(shape, math.nan, dtype=dtype, device="cuda")
+    x = {"slice": wide[:, -1:], "transposed": wide.transpose(0, 1), "padded": wide[:, 1:2, 5:]}[how]
+    assert x.shape == (rows, 1, vocab)
+    x.copy_(logits(gen, (rows, 1, vocab), dtype))
+    return wide, x
+
+
+@pytest.mark.parametrize("how", ["slice", "transposed", "padded"])
+@pytest.mark.parametrize("dtype,vocab", [(BF16, 1000), (F32, 777), (F16, 33000)])
+def test_a_dimension_of_one_before_the_vocabulary(dnn, dtype, vocab, how):
+    """The last tokens' logits of a batch, where the rows' pitch is not the stride next to
+    the vocabulary's."""
+    gen = torch.Generator().manual_seed(52)
+    wide, x = last_tokens(gen, dtype, 5, vocab, how)
+    tokens = [0, vocab - 1, -1, 3, 4]
+    check_forward(dnn, x, tokens, 4)
+    out, dx = last_tokens(gen, dtype, 5, vocab, how)
+    check_backward(dnn, x, tokens, True, gen, dx=dx)
+    dx.fill_(math.nan)
+    assert torch.isnan(out).all()                # nothing else was written
+
+
+@pytest.mark.parametrize("how", ["slice", "transposed", "padded"])
+def test_softmax_gelu_and_norms_of_a_dimension_of_one(dnn, how):
+    """The same views in the other calls that take rows, against 64 bits: a few half steps
+    of a sum of 1000 terms."""
+    gen = torch.Generator().manual_seed(53)
+    _, x = last_tokens(gen, F32, 6, 1000, how)
+    gamma, beta = (torch.randn(1000, generator=gen).cuda() for _ in range(2))
+    h, G, B = x.cpu().double()[:, 0], gamma.cpu().double(), beta.cpu().double()
+    rms = h * (h.square().mean(1, keepdim=True) + 1e-5).rsqrt() * G
+    layer = (h - h.mean(1, keepdim=True)) * (h.var(1, unbiased=False, keepdim=True) + 1e-5).rsqrt() * G + B
+    xd, wd = desc(x), desc(gamma)
+    for name, call, want in (
+            ("softmax", lambda yd, y: dnn.softmax(xd, x.data_ptr(), yd, y), h.softmax(1)),
+            ("gelu", lambda yd, y: dnn.gelu(0, xd, x.data_ptr(), yd, y), torch.nn.functional.gelu(h)),
+            ("rmsnorm", lambda yd, y: dnn.rmsnorm(xd, x.data_ptr(), wd, gamma.data_ptr(), 1e-5, yd, y), rms),
+            ("layernorm", lambda yd, y: dnn.layernorm(xd, x.data_ptr(), wd, gamma.data_ptr(), beta.data_ptr(), 1e-5,
+                                                      yd, y), layer)):
+        out, y = last_tokens(gen, F32, 6, 1000, how)
+        say(f"{name}, {how}")
+        g.check(call(desc(y), y.data_ptr()), name)
+        torch.cuda.synchronize()
+        assert torch.allclose(y.cpu().double()[:, 0], want, rtol=2.0 ** -16, atol=2.0 ** -18), name
+        y.fill_(math.nan)
+        assert torch.isnan(out).all(), name

@@ -310,3 +310,15 @@ def test_workspace_sizes(dnn):
     assert ask(dnn.h, T(BF16, [3, 6, 1, 64]).d, pool.d, table.d, None, ctypes.byref(out)) == INVALID
     assert L.grxdnnTokenLogProbGetWorkspaceSize(dnn.h, T(BF16, [6, 2]).d, 3, ctypes.byref(out)) == INVALID
     assert L.grxdnnTokenLogProbGetWorkspaceSize(dnn.h, None, 0, ctypes.byref(out)) == INVALID
+
+
+@needs_no_gpu
+def test_strides_of_a_dimension_of_one_do_not_matter(dnn):
+    """[B, 1, V] views of the last tokens' logits, of rows first and of transposed ones: the
+    pitch is the batch's, whatever the dimension of one has for a stride."""
+    for strides in ([7000, 1000, 1], [7000, 5, 1], [1000, 6000, 1], [1000, 0, 1]):
+        x = T(BF16, [6, 1, 1000], strides)
+        assert logprob(dnn, xd=x) == OK and gradient(dnn, xd=x, dxd=x) == OK, strides
+    assert logprob(dnn, xd=T(BF16, [6, 1, 1000], [500, 1000, 1])) == UNSUPPORTED       # rows that overlap
+    assert logprob(dnn, xd=T(BF16, [2, 1, 3, 1000], [5000, 9, 1100, 1])) == UNSUPPORTED
+    assert logprob(dnn, xd=T(BF16, [2, 1, 3, 1000], [3300, 9, 1100, 1])) == OK
