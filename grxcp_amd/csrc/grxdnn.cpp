@@ -720,7 +720,7 @@ grxdnnStatus_t grxdnnPagedAttentionForward(grxdnnHandle_t handle, grxdnnAttentio
   if (!half_rows(*qDesc) || !half_rows(*oDesc)) return GRXDNN_STATUS_NOT_SUPPORTED;
   if (!no_overlap(*oDesc) || (weights && !no_overlap(*weightsDesc))) return GRXDNN_STATUS_INVALID_VALUE;
   if (!q || !kCache || !vCache || !table || !lengths || !o) return GRXDNN_STATUS_INVALID_VALUE;
-  if (!grxk::paged_attention_fits(d.c, d.H)) return GRXDNN_STATUS_NOT_SUPPORTED;
+  if (!grxk::paged_attention_fits(d.c, d.H, weights != nullptr)) return GRXDNN_STATUS_NOT_SUPPORTED;
   const size_t need = grxk::paged_attention_workspace(d.c, d.H, weights != nullptr);
   if (workspaceBytes < need || (need && !workspace)) return GRXDNN_STATUS_INVALID_VALUE;
   if (may_alias(*oDesc, o, *qDesc, q) && !(o == q && same_strides(*oDesc, *qDesc)))

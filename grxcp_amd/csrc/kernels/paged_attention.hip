@@ -718,7 +718,7 @@ bool neighbours(int64_t head_stride, int64_t slot_stride) { return head_stride <
 struct Plan {
   int nt, hw, gtiles, rows, wgs;
   bool whole;
-  int64_t items, slots;
+  int64_t items, room, slots;
   size_t ml, po, scores;     // floats of the workspace, 16-byte multiples
 };
 
@@ -735,14 +735,15 @@ Plan plan_of(int B, int H, int heads, int D, int W, int page, bool neighbours, b
   x.nt = group > 16 ? 2 : 1;
   x.gtiles = (group + 16 * x.nt - 1) / (16 * x.nt);
   x.rows = std::min(group, 16 * x.nt);
-  x.slots = ((int64_t)W * page + 127) / 128 * 128;
   // A workgroup per (sequence, head) and no join where no sequence is long: up to 256
   // slots always, up to 512 where there are workgroups enough to read as fast as the
   // memory gives (a CU alone reads about 46 GB/s). us, split and joined / whole: 32 x 8
   // heads of 300 slots 20.0 / 11.4, of 500 21.1 / 15.9, 16 x 8 of 500 14.6 / 14.2, but
   // 4 x 8 of 500 10.9 / 12.4, 8 x 8 of 1000 14.4 / 23.0, 64 x 8 of 20 to 1000 35.8 / 38.2.
-  const int64_t room = (int64_t)W * page, each = (int64_t)B * heads * x.gtiles;
-  x.whole = (room <= 256 || (room <= 512 && each >= 128)) && each <= (1 << 20);
+  x.room = (int64_t)W * page;
+  x.slots = (x.room + 127) / 128 * 128;
+  const int64_t each = (int64_t)B * heads * x.gtiles;
+  x.whole = (x.room <= 256 || (x.room <= 512 && each >= 128)) && each <= (1 << 20);
   // Where the heads of a slot lie together, a workgroup takes up to four of them (a
   // wave each), so that what it reads at a time does: 16 sequences of 8192, 8 heads of
   // 128, 103 us with one head, 93 with four (90 where the slots of a head lie
@@ -759,6 +760,24 @@ Plan plan_of(int B, int H, int heads, int D, int W, int page, bool neighbours, b
   if (!x.whole) x.po = parts * x.hw * x.rows * D;
   if (weights) x.scores = (size_t)B * H * x.slots;
   return x;
+}
+
+// Workgroups of the join, for every sequence: `outs` for the outputs, then one per chunk
+// of 1024 slots of a key head's weights.
+struct JoinPlan {
+  int apiece;
+  int64_t outs, chunks, jobs;
+};
+JoinPlan join_plan(const Plan& x, int B, int H, int heads, bool weights) {
+  JoinPlan j{};
+  // A wave to a query head, or the workgroup: few heads have many parts each. us, wave /
+  // workgroup: 128 sequences of 800, 32 heads, 79.5 / 87.1; 16 of 8192 93.8 / 93.6; 2 of
+  // 131072 97.7 / 89.7; one of 8000 22.6 / 15.0.
+  j.apiece = (int64_t)B * H >= 512 ? 4 : 1;
+  j.outs = x.whole ? 0 : ((int64_t)H + j.apiece - 1) / j.apiece;
+  j.chunks = (x.room + 1023) / 1024;
+  j.jobs = j.outs + (weights ? heads * j.chunks : 0);
+  return j;
 }
 
 template <AttnType T, int D>
@@ -793,15 +812,9 @@ hipError_t run(const PagedAttnDesc& d, hipStream_t s) {
   else go(decode_split<T, D, 2, false>);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess || (x.whole && !d.weights)) return e;
-  // A wave to a query head, or the workgroup: few heads have many parts each. us, wave /
-  // workgroup: 128 sequences of 800, 32 heads, 79.5 / 87.1; 16 of 8192 93.8 / 93.6; 2 of
-  // 131072 97.7 / 89.7; one of 8000 22.6 / 15.0.
-  const int apiece = (int64_t)p.B * p.H >= 512 ? 4 : 1;
-  const int64_t outs = x.whole ? 0 : (p.H + apiece - 1) / apiece, chunks = ((int64_t)d.c.W * d.c.page + 1023) / 1024;
-  const int64_t jobs = outs + (d.weights ? p.heads * chunks : 0);
-  if (jobs > max_workgroups(256)) return hipErrorNotSupported;
-  hipLaunchKernelGGL((decode_join<T, D>), dim3((unsigned)jobs, (unsigned)std::min(p.B, 65535)), dim3(256), 0, s, p,
-                     (uint32_t)outs, apiece, (uint32_t)chunks);
+  const JoinPlan j = join_plan(x, p.B, p.H, p.heads, d.weights != nullptr);
+  hipLaunchKernelGGL((decode_join<T, D>), dim3((unsigned)j.jobs, (unsigned)std::min(p.B, 65535)), dim3(256), 0, s, p,
+                     (uint32_t)j.outs, j.apiece, (uint32_t)j.chunks);
   return hipGetLastError();
 }
 
@@ -812,9 +825,10 @@ size_t paged_attention_workspace(const PagedCache& c, int H, bool weights) {
   return (x.ml + x.po + x.scores) * sizeof(float);
 }
 
-bool paged_attention_fits(const PagedCache& c, int H) {
-  const Plan x = plan_of(c.B, H, c.heads, c.D, c.W, c.page, neighbours(c.k_sh, c.k_ss), false);
-  return (double)x.items * (x.slots / 32) < 0x1p31;
+bool paged_attention_fits(const PagedCache& c, int H, bool weights) {
+  const Plan x = plan_of(c.B, H, c.heads, c.D, c.W, c.page, neighbours(c.k_sh, c.k_ss), weights);
+  return (double)x.items * (x.slots / 32) < 0x1p31 &&
+         join_plan(x, c.B, H, c.heads, weights).jobs <= max_workgroups(256);
 }
 
 hipError_t launch_paged_attention(AttnType t, const PagedAttnDesc& d, hipStream_t s) {

@@ -183,8 +183,9 @@ hipError_t launch_paged_attention(AttnType t, const PagedAttnDesc& d, hipStream_
 // Workspace bytes of a call with H query heads (c's pointers are not looked at),
 // with or without the slots' weights.
 size_t paged_attention_workspace(const PagedCache& c, int H, bool weights);
-// Whether the kernels can count the slots that the table has room for.
-bool paged_attention_fits(const PagedCache& c, int H);
+// Whether the kernels can count the slots that the table has room for, and their
+// workgroups fit a launch.
+bool paged_attention_fits(const PagedCache& c, int H, bool weights);
 
 struct PagedEvictDesc {
   PagedCache c;

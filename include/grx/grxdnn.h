@@ -226,6 +226,10 @@ grxdnnStatus_t grxdnnPagedCacheAppend(grxdnnHandle_t handle,
  * with entries at or past lengths[b] left as they are. weightDecay: finite and
  * >= 0; with 0 the old weights are not read.
  *
+ * B * Hkv * ceil(G / 32) * W * P below 2^36, B * H below 2^29, and with weights
+ * Hkv * ceil(W * P / 1024) + H below 2^24 (else NOT_SUPPORTED, and nothing is
+ * launched).
+ *
  * workspace: device memory of at least the size that
  * grxdnnPagedAttentionGetWorkspaceSize gives for the same descriptors (a
  * smaller one is INVALID_VALUE; 16-byte aligned; its contents before the call

@@ -322,3 +322,17 @@ def test_strides_of_a_dimension_of_one_do_not_matter(dnn):
     assert logprob(dnn, xd=T(BF16, [6, 1, 1000], [500, 1000, 1])) == UNSUPPORTED       # rows that overlap
     assert logprob(dnn, xd=T(BF16, [2, 1, 3, 1000], [5000, 9, 1100, 1])) == UNSUPPORTED
     assert logprob(dnn, xd=T(BF16, [2, 1, 3, 1000], [3300, 9, 1100, 1])) == OK
+
+
+@needs_no_gpu
+def test_more_joining_workgroups_than_one_launch_takes(dnn):
+    """Refused before anything is launched: 17 heads of 2^30 slots have 2^24 + 2^20 chunks of
+    1024 weights. As many slots without weights, or fewer heads, pass."""
+    far = dict(kcd=T(BF16, [40, 17, 16, 64]), vcd=T(BF16, [40, 17, 16, 64]), td=T(I32, [1, 1 << 26]),
+               qd=T(BF16, [1, 17, 1, 64]), od=T(BF16, [1, 17, 1, 64]), table=1 << 43, ws=1 << 45, size=1 << 44)
+    w = dict(wd=T(F32, [1, 17, 1 << 30], [0, 1 << 30, 1]), w=1 << 44)
+    assert attend(dnn, **far, **w) == UNSUPPORTED
+    assert attend(dnn, **far, wd=None, w=None) == OK
+    few = dict(far, kcd=T(BF16, [40, 15, 16, 64]), vcd=T(BF16, [40, 15, 16, 64]), qd=T(BF16, [1, 15, 1, 64]),
+               od=T(BF16, [1, 15, 1, 64]))
+    assert attend(dnn, **few, wd=T(F32, [1, 15, 1 << 30], [0, 1 << 30, 1]), w=1 << 44) == OK
