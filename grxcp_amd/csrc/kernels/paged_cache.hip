@@ -79,6 +79,7 @@ struct EvictParams {
   int* kept;
   int* new_lengths;
   int B, heads, budget, recent;
+  int first;           // (sequence, head) of workgroup 0 of evict_select
 };
 
 constexpr int kWaves = 16;    // of a selecting workgroup
@@ -99,7 +100,7 @@ template <int N>
 __global__ __launch_bounds__(64 * kWaves) void evict_select(EvictParams p) {
   __shared__ int sums[2][3][kWaves], above_of[kWaves], ties_of[kWaves], few_n;
   __shared__ uint32_t few[64];
-  const int bh = blockIdx.x, b = bh / p.heads, h = bh - b * p.heads, tid = threadIdx.x;
+  const int bh = p.first + blockIdx.x, b = bh / p.heads, h = bh - b * p.heads, tid = threadIdx.x;
   const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int n = clamp_length(p.view.lengths[b], p.view.room), m = min(n, p.budget);
   const int old = n <= p.budget ? 0 : max(0, n - p.recent);   // slots that the weights decide on
@@ -297,14 +298,16 @@ hipError_t launch_paged_evict(const PagedEvictDesc& d, hipStream_t s) {
   p.new_lengths = d.new_lengths;
   p.B = d.c.B; p.heads = d.c.heads; p.budget = d.budget; p.recent = d.recent;
   const int64_t heads = (int64_t)p.B * p.heads;
-  if (heads > max_workgroups(64 * kWaves)) return hipErrorNotSupported;
-  const dim3 all((unsigned)heads), threads(64 * kWaves);
   const int each = (p.view.room + 64 * kWaves - 1) / (64 * kWaves);
-  if (each <= 8) hipLaunchKernelGGL(evict_select<8>, all, threads, 0, s, p);
-  else if (each <= 32) hipLaunchKernelGGL(evict_select<32>, all, threads, 0, s, p);
-  else hipLaunchKernelGGL(evict_select<0>, all, threads, 0, s, p);
-  const hipError_t e = hipGetLastError();
-  if (e != hipSuccess) return e;
+  for (int64_t first = 0; first < heads; first += max_workgroups(64 * kWaves)) {
+    p.first = (int)first;
+    const dim3 some((unsigned)std::min(heads - first, max_workgroups(64 * kWaves))), threads(64 * kWaves);
+    if (each <= 8) hipLaunchKernelGGL(evict_select<8>, some, threads, 0, s, p);
+    else if (each <= 32) hipLaunchKernelGGL(evict_select<32>, some, threads, 0, s, p);
+    else hipLaunchKernelGGL(evict_select<0>, some, threads, 0, s, p);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+  }
   const int chunks = d.c.D / 8, rows = 256 / chunks;
   const dim3 grid = tiles_by((p.budget + (int64_t)rows - 1) / rows, heads);
   if (chunks == 16) hipLaunchKernelGGL(evict_copy<16>, grid, dim3(256), 0, s, p);

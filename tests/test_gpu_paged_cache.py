@@ -317,3 +317,38 @@ def test_more_sequences_than_a_grid_has_rows(dnn):
         for pool, c in ((k, 0), (v, 1)):
             got = pool[new_table[here, i // page].long(), 0, i % page, c:c + 3]
             assert torch.equal(got, rows[who[here], want[here, i]].to(BF16)), (i, c)
+
+
+def test_evict_of_more_heads_than_one_launch_takes(dnn):
+    """2^22 + 24 (sequence, head) pairs of up to 2 slots, 1 of which stays: the heavier one,
+    the lower of equal ones."""
+    gen = torch.Generator(device="cuda").manual_seed(61)
+    b, heads, d, shared = 2 ** 19 + 3, 8, 64, 1000
+    def rand(hi, shape):
+        return torch.randint(0, hi, shape, generator=gen, device="cuda", dtype=torch.int32)
+    n, table = rand(3, (b,)), rand(shared, (b, 2))
+    k, v = (torch.zeros((shared + b, heads, 1, d), dtype=BF16, device="cuda") for _ in range(2))
+    k[:shared] = torch.randn((shared, heads, 1, d), generator=gen, device="cuda").to(BF16)
+    v[:shared] = torch.randn((shared, heads, 1, d), generator=gen, device="cuda").to(BF16)
+    w = rand(3, (b, heads, 2)).float()
+    new_table = torch.arange(shared, shared + b, device="cuda", dtype=torch.int32)[:, None]
+    kept = torch.full((b, heads, 1), -7, dtype=torch.int32, device="cuda")
+    new_n, new_w = torch.full_like(n, -9), torch.full((b, heads, 1), math.nan, device="cuda")
+    kd = desc(k)
+    say("eviction of 2^22 + 24 heads")
+    g.check(dnn.paged_evict(kd, k.data_ptr(), kd, v.data_ptr(), desc(table), table.data_ptr(), n.data_ptr(), desc(w),
+                            w.data_ptr(), 1, 0, kept.data_ptr(), desc(new_table), new_table.data_ptr(),
+                            new_n.data_ptr(), desc(new_w), new_w.data_ptr()), "evict")
+    torch.cuda.synchronize()
+    want = torch.where((n == 2)[:, None] & (w[..., 1] > w[..., 0]), 1, 0)
+    want = want.masked_fill((n == 0)[:, None], -1)
+    assert torch.equal(kept[..., 0].long(), want) and torch.equal(new_n, n.clamp(max=1))
+    slot = want.clamp(min=0)
+    assert torch.equal(new_w[..., 0], w.gather(2, slot[..., None])[..., 0].masked_fill(want < 0, 0.0))
+    page = table.long().gather(1, slot)
+    head = torch.arange(heads, device="cuda")
+    for pool in (k, v):
+        rows = pool[page, head, 0].masked_fill((want < 0)[..., None], 0.0)
+        assert torch.equal(pool[shared:, :, 0], rows)
+    del k, v, rows, w
+    torch.cuda.empty_cache()
