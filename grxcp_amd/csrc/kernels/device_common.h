@@ -90,7 +90,12 @@ __device__ __forceinline__ float wave_reduce(float v, Op op) {
 }
 
 __device__ __forceinline__ float wave_sum(float v) {
-  return wave_reduce(v, [](float a, float b) { return a + b; });
+  // Where v is a product, a first step contracted to an fma would round one lane's partial
+  // and not its partner's, and leave lanes with different sums.
+  return wave_reduce(v, [](float a, float b) {
+#pragma clang fp contract(off)
+    return a + b;
+  });
 }
 
 __device__ __forceinline__ float wave_max(float v) {

@@ -467,3 +467,19 @@ def test_softmax_gelu_and_norms_of_a_dimension_of_one(dnn, how):
         assert torch.allclose(y.cpu().double()[:, 0], want, rtol=2.0 ** -16, atol=2.0 ** -18), name
         y.fill_(math.nan)
         assert torch.isnan(out).all(), name
+
+
+@pytest.mark.parametrize("dtype,rows,vocab,top", [(F32, 32, 131072, 8), (F16, 300, 9000, 64), (BF16, 2500, 3000, 64)])
+def test_same_bits_every_time(dnn, dtype, rows, vocab, top):
+    """The alternatives are ranked in lists that fill in any order; whichever lane writes
+    one, its log probability is the same number, and the token's."""
+    gen = torch.Generator().manual_seed(55)
+    x = logits(gen, (rows, vocab), dtype)
+    tokens = x.float().argmax(1).int()
+    first = forward(dnn, x, tokens, top)
+    assert torch.equal(first[3][:, 0], first[0])
+    shift = x.float().gather(1, first[4].long()).double() - first[3].double()
+    assert (shift - shift[:, :1]).abs().max() <= 2.0 ** -19       # roundings of values below 16
+    for i in range(20):
+        for a, b in zip(first, forward(dnn, x, tokens, top)):
+            assert torch.equal(a, b), i
