@@ -444,7 +444,8 @@ __global__ __launch_bounds__(64, AL ? 4 : 3) void logprob_pieces(LParams p) {
 #pragma unroll
             for (int e = 0; e < V; ++e) {
               const uint64_t k = rank_key(y[e], rc.first(c) + e);
-              if (rc.has(c, e) && k < last && k > best) best = k;
+              // (NaN at place 0 is the largest key of all)
+              if (rc.has(c, e) && (i == 0 || k < last) && k > best) best = k;
             }
           }
 #pragma unroll

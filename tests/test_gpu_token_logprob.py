@@ -483,3 +483,17 @@ def test_same_bits_every_time(dnn, dtype, rows, vocab, top):
     for i in range(20):
         for a, b in zip(first, forward(dnn, x, tokens, top)):
             assert torch.equal(a, b), i
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("vocab,top", [(1, 1), (3, 3), (700, 4), (40000, 64)])
+def test_nan_in_the_first_place(dnn, dtype, vocab, top):
+    """NaN is the largest alternative at place 0 as elsewhere, alone and among others."""
+    gen = torch.Generator().manual_seed(54)
+    x = logits(gen, (4, vocab), dtype)
+    x[0, 0] = math.nan
+    x[1, [0, -1]] = math.nan
+    x[2, :] = math.nan
+    x[3, 1:] = math.inf
+    x[3, 0] = math.nan
+    check_forward(dnn, x, [0, vocab - 1, 0, 0], top)
