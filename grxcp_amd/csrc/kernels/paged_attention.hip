@@ -38,9 +38,9 @@
 // us for 32 query and 8 key heads of 128, bf16, pages of 16 slots: 48 sequences of 33 to
 // 4096 slots 76 (5.3 TB/s; 72 the split, 5 the join), 16 of 8192 93.6 (5.7), 2 of
 // 131072 with 4 key heads 90 (6.0), 64 of 500 26.9 (4.9), one of 201 6.7, one of 60 5.3.
-// 512 workgroups that fill a CU's registers start together, and each waits for lengths,
-// a table entry and its first tile in turn before the memory is busy; with the second
-// launch that is what a call has above its bytes.
+// The workgroups, as many as the CUs' registers hold (plan_of: two or three per CU), start
+// together, and each waits for lengths, a table entry and its first tile in turn before the
+// memory is busy; with the second launch that is what a call has above its bytes.
 
 #include "../launch.h"
 #include "device_common.h"

@@ -94,8 +94,10 @@ constexpr int kWaves = 16;    // of a selecting workgroup
 //    one that enough do, those go on in registers without a barrier.
 //  * Where every slot goes follows from the numbers of kept ones and of ties in the
 //    waves before and ballots within the wave: no loop over the slots with a barrier.
-// 128 heads of 6000 to 8192 slots to 2048: 19 us, bound by instruction issue on the 128
-// CUs that have one; a binary search over passes through memory, 256 threads, took 187.
+// 128 heads of 6000 to 8192 slots to 2048: 19 us on the 128 CUs that have one, bound by the
+// steps' latency: waves wait for loads, LDS and barriers in 59 % of their cycles, the VALU is
+// at work in 38 %. A binary search over passes through memory, 256 threads, took 187. Where
+// slots are read again (more than 32 a lane), 8 heads of 131072: 375 us.
 template <int N>
 __global__ __launch_bounds__(64 * kWaves) void evict_select(EvictParams p) {
   __shared__ int sums[2][3][kWaves], above_of[kWaves], ties_of[kWaves], few_n;

@@ -35,10 +35,11 @@
 //
 // Backward: one element-wise pass, bound by reading x and writing dx.
 //
-// us: 32 rows of 131072 bf16 with 8 alternatives 14.3 (8.4 MB: two launches, 11 and 4, of
-// which most is waiting), 256 rows 30.2 (2.2 TB/s), 2048 x 32000 without any 24.9 (5.3),
-// 4096 x 32001 fp32 86 (6.1); the gradient of 8192 x 65536 bf16 with entropy 345 (6.2), of
-// 500 x 50001 fp16 21.5 (4.7).
+// us: 32 rows of 131072 bf16 with 8 alternatives 14.3 (8.4 MB: two launches, 10 and 4; in
+// the first the VALU is at work half of the time, at five times the instructions that the
+// sums take), 256 rows 30.4 (2.2 TB/s; 17 of it VALU work), 2048 x 32000 without any 25.2
+// (5.2), 4096 x 32001 fp32 86 (6.1); the gradient of 8192 x 65536 bf16 with entropy 346
+// (6.2), of 500 x 50001 fp16 21.3 and of 500 x 50000 20.3 (4.7, 4.9).
 
 #include "../launch.h"
 #include "device_common.h"

@@ -178,7 +178,8 @@ int            grxdnnAttentionCycleSlotsNeeded(grxdnnHandle_t handle, int batch,
  * sequence has room for W * P slots (at most 2^31 - 4096). lengths: B ints, the
  * slots of each sequence that hold tokens; below 0 counts as 0, above W * P as
  * W * P. Tables, lengths and counts are device memory, read when the kernels
- * run: a captured call follows their contents on every replay.
+ * run: a captured call follows their contents on every replay, and they must not
+ * change while a call that reads them runs.
  *
  * Table entries of pages that a call does not reach are not read. An entry
  * outside [0, pages) that it does reach is never followed: a row written there
@@ -187,11 +188,11 @@ int            grxdnnAttentionCycleSlotsNeeded(grxdnnHandle_t handle, int batch,
  *
  * Types GRX_R_16BF or GRX_R_16F, one for all key, value, query and output
  * tensors; D is 64 or 128; innermost stride 1, the other strides multiples of 8
- * elements, pointers 16-byte aligned (else NOT_SUPPORTED). The two pools have
- * one shape and share no element; written tensors must not share elements of
- * their own or with what the call reads (INVALID_VALUE where the descriptors
- * show it; pages that two written table entries name are the caller's matter:
- * such rows hold one of the values written).
+ * elements, pointers 16-byte aligned, B * Hkv below 2^29 (else NOT_SUPPORTED).
+ * The two pools have one shape and share no element; written tensors must not
+ * share elements of their own or with what the call reads (INVALID_VALUE where
+ * the descriptors show it; pages that two written table entries name are the
+ * caller's matter: such rows hold one of the values written).
  * (New: planned by ref docs/designs/grxcp_roadmap.md:864-877, "attention".) */
 
 /* New rows behind the tokens that a cache holds: for every sequence b, head h
@@ -224,7 +225,9 @@ grxdnnStatus_t grxdnnPagedCacheAppend(grxdnnHandle_t handle,
  * [B, Hkv, S] GRX_R_32F, S >= W * P, innermost stride 1:
  *   weights[b,g,j] = weightDecay * weights[b,g,j] + sum_{h in group g} p[b,h,j],  j < lengths[b]
  * with entries at or past lengths[b] left as they are. weightDecay: finite and
- * >= 0; with 0 the old weights are not read.
+ * >= 0; with 0 the old weights are not read. Nothing else adds to them: what a
+ * prompt's tokens gave each other (grxdnnAttentionForward) is not in them, so the
+ * slots of a prompt are equal before the first call.
  *
  * B * Hkv * ceil(G / 32) * W * P below 2^36, B * H below 2^29, and with weights
  * Hkv * ceil(W * P / 1024) + H below 2^24 (else NOT_SUPPORTED, and nothing is
@@ -268,7 +271,9 @@ grxdnnStatus_t grxdnnPagedAttentionForward(grxdnnHandle_t handle,
  * The pages of table are the caller's again afterwards. kept: packed
  * [B, Hkv, budget] ints. weights, newWeights: [B, Hkv, S], S >= W * P and
  * [B, Hkv, S2], S2 >= budget, GRX_R_32F, innermost stride 1. newLengths may be
- * lengths itself. budget >= 1. */
+ * lengths itself. budget >= 1. A slot on a page that does not exist is kept or not
+ * by its weight like the others; its row of newTable is left as it was, and counts
+ * as a slot from then on. */
 grxdnnStatus_t grxdnnPagedCacheEvict(grxdnnHandle_t handle,
                                      grxdnnTensorDescriptor_t kCacheDesc, void* kCache,
                                      grxdnnTensorDescriptor_t vCacheDesc, void* vCache,
