@@ -32,6 +32,7 @@ STATUS = {
 }
 SUCCESS, NOT_INITIALIZED, ALLOC_FAILED, INVALID_VALUE = 0, 1, 2, 3
 GELU_ERF, GELU_TANH = 0, 1
+ROPE_HALVES, ROPE_PAIRS = 0, 1
 ARCH_MISMATCH, EXECUTION_FAILED, NOT_SUPPORTED, INTERNAL_ERROR = 4, 5, 6, 7
 TENSOR_FP16, TENSOR_TF32, TENSOR_FP8, TENSOR_FP4 = 0x01, 0x02, 0x04, 0x08
 TENSOR_INT8, TENSOR_INT4, TENSOR_BF16 = 0x10, 0x20, 0x40
@@ -145,6 +146,9 @@ _DNN = {
                                        c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]),
     "grxdnnSetCycleProbe": (c_int, [c_void_p, c_void_p, c_int]),
     "grxdnnAttentionCycleSlotsNeeded": (c_int, [c_void_p, c_int, c_int, c_int]),
+    "grxdnnQkNormRopeForward": (c_int, [c_void_p] * 8 + [c_float, c_int, c_int] + [c_void_p] * 6),
+    "grxdnnQkNormRopeGetWorkspaceSize": (c_int, [c_void_p] * 4 + [POINTER(c_size_t)]),
+    "grxdnnQkNormRopeBackward": (c_int, [c_void_p] * 8 + [c_float, c_int, c_int] + [c_void_p] * 13 + [c_size_t]),
     "grxdnnPagedCacheAppend": (c_int, [c_void_p] * 13),
     "grxdnnPagedAttentionGetWorkspaceSize": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
                                                      POINTER(c_size_t)]),
@@ -392,6 +396,26 @@ class Dnn:
 
     def gelu(self, mode: int, xd, x, yd, y) -> int:
         return self.L.grxdnnGeluForward(self.h, mode, xd.d, x, yd.d, y)
+
+    def qk_norm_rope(self, qd, q, kd, k, wd, q_gamma, k_gamma, eps, mode, rotary, positions, inv_freq, yqd, yq, ykd,
+                     yk) -> int:
+        """kd, k, k_gamma, ykd, yk: None where there are only queries; wd and the gammas: None for no norm."""
+        return self.L.grxdnnQkNormRopeForward(self.h, qd.d, q, kd.d if kd else None, k, wd.d if wd else None, q_gamma,
+                                              k_gamma, eps, mode, rotary, positions, inv_freq, yqd.d, yq,
+                                              ykd.d if ykd else None, yk)
+
+    def qk_norm_rope_workspace(self, qd, kd, wd) -> int:
+        n = c_size_t(0)
+        check(self.L.grxdnnQkNormRopeGetWorkspaceSize(self.h, qd.d, kd.d if kd else None, wd.d if wd else None,
+                                                      ctypes.byref(n)), "qk norm rope workspace")
+        return n.value
+
+    def qk_norm_rope_backward(self, qd, q, kd, k, wd, q_gamma, k_gamma, eps, mode, rotary, positions, inv_freq, dyqd,
+                              dyq, dykd, dyk, dqd, dq, dkd, dk, dq_gamma, dk_gamma, ws, ws_bytes) -> int:
+        return self.L.grxdnnQkNormRopeBackward(self.h, qd.d, q, kd.d if kd else None, k, wd.d if wd else None, q_gamma,
+                                               k_gamma, eps, mode, rotary, positions, inv_freq, dyqd.d, dyq,
+                                               dykd.d if dykd else None, dyk, dqd.d, dq, dkd.d if dkd else None, dk,
+                                               dq_gamma, dk_gamma, ws, ws_bytes)
 
     def paged_append(self, kd, k, vd, v, kcd, kc, vcd, vc, td, table, lengths, counts=None) -> int:
         return self.L.grxdnnPagedCacheAppend(self.h, kd.d, k, vd.d, v, kcd.d, kc, vcd.d, vc, td.d, table,

@@ -162,62 +162,75 @@ bool same_strides(const grxdnnTensorStruct& a, const grxdnnTensorStruct& b) {
   return true;
 }
 
-// Whether delta = sum_i strides[i] * d_i has a solution with |d_i| <
-// extents[i], for dimensions taken in decreasing stride order from `from`;
-// reach[i] is the largest |sum| the dimensions after i can make. Returns
-// true ("may share an element") when the search would take too many steps.
-bool offset_reachable(const int64_t* strides, const int64_t* extents, const int64_t* reach,
-                      int n, int from, int64_t delta, int* budget) {
-  if (from == n) return delta == 0;
-  const int64_t s = strides[from], r = reach[from], e = extents[from] - 1;
-  // d with |delta - s*d| <= r: d in [ceil((delta-r)/s), floor((delta+r)/s)]
+// Whether delta = sum_i strides[i] * d_i has a solution with lo[i] <= d_i <= hi[i]
+// (lo <= 0 <= hi), for dimensions taken in decreasing stride order from `from`;
+// below[i] and above[i] are the least and the largest sum the dimensions after i can
+// make. Returns true ("may share an element") when the search would take too many steps.
+struct Offsets {
+  int n = 0;
+  int64_t strides[GRXDNN_DIM_MAX], lo[GRXDNN_DIM_MAX], hi[GRXDNN_DIM_MAX];
+  int64_t below[GRXDNN_DIM_MAX], above[GRXDNN_DIM_MAX];
+};
+bool offset_reachable(const Offsets& o, int from, int64_t delta, int* budget) {
+  if (from == o.n) return delta == 0;
+  const int64_t s = o.strides[from];
+  // d with below <= delta - s*d <= above: d in [ceil((delta-above)/s), floor((delta-below)/s)]
   auto floor_div = [](int64_t a, int64_t b) { return a >= 0 ? a / b : -((-a + b - 1) / b); };
-  int64_t lo = -floor_div(-(delta - r), s), hi = floor_div(delta + r, s);
-  if (lo < -e) lo = -e;
-  if (hi > e) hi = e;
+  int64_t lo = -floor_div(-(delta - o.above[from]), s), hi = floor_div(delta - o.below[from], s);
+  if (lo < o.lo[from]) lo = o.lo[from];
+  if (hi > o.hi[from]) hi = o.hi[from];
   for (int64_t d = lo; d <= hi; ++d) {
     if (--*budget < 0) return true;
-    if (offset_reachable(strides, extents, reach, n, from + 1, delta - s * d, budget)) return true;
+    if (offset_reachable(o, from + 1, delta - s * d, budget)) return true;
   }
   return false;
 }
 
-// Two views of one shape and the same strides (bases a and b, elements of
-// `elem` bytes) share an element's address. An exact test of the element
-// offsets, so that e.g. O written over the Q slot of a packed [B,S,3,H,D]
-// QKV buffer is told apart from O overlapping K or V. Views whose bases do
-// not differ by whole elements are taken to overlap when their spans do.
-bool views_share_element(const grxdnnTensorStruct& t, const void* a, const void* b, size_t elem) {
+// Two views (bases a and b, elements of `elem` bytes) share an element's address. An
+// exact test of the element offsets where they have the same strides, whatever their
+// extents (the stride of an extent of 1 aside), so that e.g. O written over the Q slot of
+// a packed [B,S,3,H,D] QKV buffer is told apart from O overlapping K or V. Views of
+// other strides, or whose bases do not differ by whole elements, are taken to overlap
+// when their spans do.
+bool views_share_element(const grxdnnTensorStruct& ta, const void* a, const grxdnnTensorStruct& tb, const void* b,
+                         size_t elem) {
   const int64_t diff = (int64_t)((intptr_t)b - (intptr_t)a);
-  if (diff % (int64_t)elem != 0) return intersect(span_of(t, a, elem), span_of(t, b, elem));
-  int64_t strides[GRXDNN_DIM_MAX], extents[GRXDNN_DIM_MAX], reach[GRXDNN_DIM_MAX];
-  int n = 0;
-  for (int i = 0; i < t.nb; ++i) {
-    if (t.dims[i] <= 0) return false;                      // an empty view
-    if (t.dims[i] == 1 || t.strides[i] == 0) continue;     // contributes no offset
-    strides[n] = t.strides[i];
-    extents[n] = t.dims[i];
-    ++n;
+  bool exact = ta.nb == tb.nb && diff % (int64_t)elem == 0;
+  Offsets o;
+  for (int i = 0; exact && i < ta.nb; ++i) {
+    const int ea = ta.dims[i], eb = tb.dims[i];
+    if (ea <= 0 || eb <= 0) return false;                  // an empty view
+    if (ea > 1 && eb > 1 && ta.strides[i] != tb.strides[i]) exact = false;
+    const int stride = ea > 1 ? ta.strides[i] : tb.strides[i];
+    if ((ea == 1 && eb == 1) || stride == 0) continue;     // contributes no offset
+    o.strides[o.n] = stride;
+    o.lo[o.n] = 1 - (int64_t)eb;
+    o.hi[o.n] = (int64_t)ea - 1;
+    ++o.n;
   }
-  for (int x = 1; x < n; ++x)                              // decreasing stride
-    for (int y = x; y > 0 && strides[y] > strides[y - 1]; --y) {
-      std::swap(strides[y], strides[y - 1]);
-      std::swap(extents[y], extents[y - 1]);
+  if (!exact) return intersect(span_of(ta, a, elem), span_of(tb, b, elem));
+  for (int x = 1; x < o.n; ++x)                            // decreasing stride
+    for (int y = x; y > 0 && o.strides[y] > o.strides[y - 1]; --y) {
+      std::swap(o.strides[y], o.strides[y - 1]);
+      std::swap(o.lo[y], o.lo[y - 1]);
+      std::swap(o.hi[y], o.hi[y - 1]);
     }
-  int64_t acc = 0;
-  for (int i = n - 1; i >= 0; --i) {
-    reach[i] = acc;
-    acc += strides[i] * (extents[i] - 1);
+  int64_t below = 0, above = 0;
+  for (int i = o.n - 1; i >= 0; --i) {
+    o.below[i] = below;
+    o.above[i] = above;
+    below += o.strides[i] * o.lo[i];
+    above += o.strides[i] * o.hi[i];
   }
   int budget = 4096;
-  return offset_reachable(strides, extents, reach, n, 0, diff / (int64_t)elem, &budget);
+  return offset_reachable(o, 0, diff / (int64_t)elem, &budget);
 }
 
 // O may share no element with x: the exact test where the two views have the
 // same strides, the span test otherwise.
 bool may_alias(const grxdnnTensorStruct& od, const void* o, const grxdnnTensorStruct& xd,
                const void* x) {
-  if (same_strides(od, xd)) return views_share_element(od, o, x, 2);
+  if (same_strides(od, xd)) return views_share_element(od, o, xd, x, 2);
   return intersect(span_of(od, o, 2), span_of(xd, x, 2));
 }
 
@@ -382,6 +395,167 @@ grxdnnStatus_t logit_rows(const grxdnnTensorStruct& x, grxk::NormType* nt, int64
 }
 
 size_t element_size(grxk::NormType t) { return t == grxk::NormType::F32 ? 4 : 2; }
+
+// 16-byte vector access along the last dimension, of elements of `elem` bytes.
+bool vector_rows(const grxdnnTensorStruct& t, int elem) {
+  if (t.strides[t.nb - 1] != 1) return false;
+  for (int i = 0; i < t.nb - 1; ++i)
+    if (t.dims[i] > 1 && (int64_t)t.strides[i] * elem % 16 != 0) return false;
+  return true;
+}
+
+// An array of a call: a tensor, or `bytes` packed ones.
+struct Operand {
+  const grxdnnTensorStruct* d;
+  const void* p;
+  int64_t bytes;
+};
+bool share(const Operand& a, const Operand& b, size_t elem) {
+  if (!a.p || !b.p) return false;
+  if (a.d && b.d) return views_share_element(*a.d, a.p, *b.d, b.p, elem);
+  return intersect(a.d ? span_of(*a.d, a.p, elem) : bytes_at(a.p, a.bytes),
+                   b.d ? span_of(*b.d, b.p, elem) : bytes_at(b.p, b.bytes));
+}
+bool in_place(const Operand& a, const Operand& b) { return a.d && b.d && a.p == b.p && same_strides(*a.d, *b.d); }
+
+// Queries or keys of a call: what they are read from, the gradient of what came out, and
+// what is written (backward: dx). All of them null without keys.
+struct QkSide {
+  grxdnnTensorDescriptor_t xd; const void* x;
+  const void* gamma;
+  grxdnnTensorDescriptor_t dyd; const void* dy;
+  grxdnnTensorDescriptor_t yd; void* y;
+  float* dgamma;
+};
+
+grxdnnStatus_t qk_type(grxDataType_t type, grxk::NormType* nt) {
+  switch (type) {
+    case GRX_R_16BF: *nt = grxk::NormType::BF16; return GRXDNN_STATUS_SUCCESS;
+    case GRX_R_16F:  *nt = grxk::NormType::F16; return GRXDNN_STATUS_SUCCESS;
+    case GRX_R_32F:  *nt = grxk::NormType::F32; return GRXDNN_STATUS_SUCCESS;
+    default: return GRXDNN_STATUS_NOT_SUPPORTED;
+  }
+}
+
+constexpr int64_t kMaxTokens = INT_MAX - 4095;   // of a call, counted in 32 bits past the last
+constexpr int kMaxHeads = 1 << 20;
+
+grxdnnStatus_t qk_shape(grxdnnTensorDescriptor_t qDesc, grxdnnTensorDescriptor_t kDesc,
+                        grxdnnTensorDescriptor_t wDesc, grxk::NormType* nt, grxk::QkRopeDesc* d) {
+  if (!qDesc || !qDesc->set || (kDesc && !kDesc->set) || (wDesc && !wDesc->set)) return GRXDNN_STATUS_INVALID_VALUE;
+  if (qDesc->nb != 4 || (kDesc && kDesc->nb != 4)) return GRXDNN_STATUS_INVALID_VALUE;
+  for (int i : {0, 2, 3})
+    if (kDesc && kDesc->dims[i] != qDesc->dims[i]) return GRXDNN_STATUS_INVALID_VALUE;
+  d->D = qDesc->dims[3];
+  if (wDesc && (wDesc->nb != 1 || wDesc->dims[0] != d->D)) return GRXDNN_STATUS_INVALID_VALUE;
+  const grxdnnStatus_t s = qk_type(qDesc->type, nt);
+  if (s != GRXDNN_STATUS_SUCCESS) return s;
+  if ((kDesc && kDesc->type != qDesc->type) || (wDesc && wDesc->type != qDesc->type))
+    return GRXDNN_STATUS_NOT_SUPPORTED;
+  if (d->D != 64 && d->D != 128 && d->D != 256) return GRXDNN_STATUS_NOT_SUPPORTED;
+  if (wDesc && wDesc->strides[0] != 1) return GRXDNN_STATUS_NOT_SUPPORTED;
+  d->B = qDesc->dims[0];
+  d->S = qDesc->dims[2];
+  d->heads[0] = qDesc->dims[1];
+  d->heads[1] = kDesc ? kDesc->dims[1] : 0;
+  if ((int64_t)d->B * d->S > kMaxTokens || (int64_t)d->heads[0] + d->heads[1] > kMaxHeads)
+    return GRXDNN_STATUS_NOT_SUPPORTED;
+  return GRXDNN_STATUS_SUCCESS;
+}
+
+grxdnnStatus_t qk_norm_rope(grxdnnHandle_t handle, const QkSide (&side)[2], grxdnnTensorDescriptor_t wDesc, float eps,
+                            grxdnnRopeMode_t mode, int rotaryDim, const int* positions, const float* frequencies,
+                            bool backward, void* workspace, size_t workspaceBytes) {
+  if (!handle) return GRXDNN_STATUS_NOT_INITIALIZED;
+  const bool keys = side[1].xd != nullptr;
+  const QkSide& k = side[1];
+  if (!keys && (k.x || k.gamma || k.dyd || k.dy || k.yd || k.y || k.dgamma)) return GRXDNN_STATUS_INVALID_VALUE;
+  grxk::QkRopeDesc d{};
+  grxk::NormType nt{};
+  grxdnnStatus_t s = qk_shape(side[0].xd, keys ? k.xd : nullptr, wDesc, &nt, &d);
+  if (s != GRXDNN_STATUS_SUCCESS) return s;
+  if (mode != GRXDNN_ROPE_HALVES && mode != GRXDNN_ROPE_PAIRS) return GRXDNN_STATUS_INVALID_VALUE;
+  if (rotaryDim < 0 || rotaryDim > d.D) return GRXDNN_STATUS_INVALID_VALUE;
+  if (rotaryDim % 16 != 0) return GRXDNN_STATUS_NOT_SUPPORTED;
+  if (wDesc ? !std::isfinite(eps) || eps < 0.0f : rotaryDim == 0) return GRXDNN_STATUS_INVALID_VALUE;
+  const int elem = (int)element_size(nt);
+  for (int i = 0; i < 1 + keys; ++i) {
+    const QkSide& x = side[i];
+    for (auto t : {x.yd, backward ? x.dyd : x.yd}) {
+      if (!t || !t->set || !same_shape(*t, *x.xd)) return GRXDNN_STATUS_INVALID_VALUE;
+      if (t->type != x.xd->type) return GRXDNN_STATUS_NOT_SUPPORTED;
+    }
+    if (!wDesc && (x.gamma || x.dgamma)) return GRXDNN_STATUS_INVALID_VALUE;
+  }
+  const bool gains = side[0].dgamma || k.dgamma;
+  const int64_t tokens = (int64_t)d.B * d.S;
+  const bool empty = tokens == 0 || d.heads[0] + d.heads[1] == 0;
+  if (empty && !gains) return GRXDNN_STATUS_SUCCESS;
+  const bool reads_x = !backward || wDesc;
+  for (int i = 0; i < 1 + keys; ++i) {
+    const QkSide& x = side[i];
+    if (d.heads[i] == 0 || empty) continue;
+    for (auto t : {x.yd, reads_x ? x.xd : x.yd, backward ? x.dyd : x.yd})
+      if (!vector_rows(*t, elem)) return GRXDNN_STATUS_NOT_SUPPORTED;
+    if (!no_overlap(*x.yd)) return GRXDNN_STATUS_INVALID_VALUE;
+    if ((reads_x && !x.x) || (wDesc && !x.gamma) || (backward && !x.dy) || !x.y) return GRXDNN_STATUS_INVALID_VALUE;
+  }
+  if (rotaryDim && !empty && (!positions || !frequencies)) return GRXDNN_STATUS_INVALID_VALUE;
+  const size_t need = gains && !empty ? grxk::qk_norm_rope_workspace(tokens, d.heads[0], d.heads[1], d.D) : 0;
+  if (need && (!workspace || workspaceBytes < need)) return GRXDNN_STATUS_INVALID_VALUE;
+  // What is written, against everything else that the call reads or writes.
+  const int64_t row = 4ll * d.D;
+  Operand all[13];
+  int n = 0, written = 0;
+  auto add = [&](const grxdnnTensorStruct* t, const void* p, int64_t bytes) { all[n++] = {t, p, bytes}; };
+  for (const QkSide& x : side)
+    if (!empty) add(x.yd, x.y, 0);
+  for (const QkSide& x : side) add(nullptr, x.dgamma, row);
+  add(nullptr, need ? workspace : nullptr, (int64_t)need);
+  written = n;
+  for (const QkSide& x : side)
+    if (!empty) {
+      add(x.xd, reads_x ? x.x : nullptr, 0);
+      add(x.dyd, x.dy, 0);
+      add(nullptr, x.gamma, (int64_t)elem * d.D);
+    }
+  if (rotaryDim && !empty) {
+    add(nullptr, positions, 4 * tokens);
+    add(nullptr, frequencies, 2ll * rotaryDim);
+  }
+  for (int i = 0; i < written; ++i)
+    for (int j = i + 1; j < n; ++j) {
+      if (!share(all[i], all[j], elem)) continue;
+      // a row is read by the lanes that write it: in place, over x or over dy of its side
+      const int at = i < 2 && j >= written ? (j - written) / 3 : -1;
+      if (at == i && in_place(all[i], all[j])) continue;
+      return GRXDNN_STATUS_INVALID_VALUE;
+    }
+  for (int i = 0; i < 1 + keys; ++i)
+    for (const void* p : {reads_x ? side[i].x : nullptr, side[i].gamma, side[i].dy, (const void*)side[i].y})
+      if (!aligned16(p)) return GRXDNN_STATUS_NOT_SUPPORTED;
+  if (need && !aligned16(workspace)) return GRXDNN_STATUS_NOT_SUPPORTED;
+  s = ensure_device(*handle);
+  if (s != GRXDNN_STATUS_SUCCESS) return s;
+  auto rows = [](grxdnnTensorDescriptor_t t, const void* p) {
+    return t ? grxk::QkRows{p, t->strides[0], t->strides[1], t->strides[2]} : grxk::QkRows{};
+  };
+  for (int i = 0; i < 1 + keys; ++i) {
+    const QkSide& x = side[i];
+    d.x[i] = rows(x.xd, x.x);
+    d.dy[i] = rows(x.dyd, x.dy);
+    d.y[i] = rows(x.yd, x.y);
+    d.gamma[i] = x.gamma;
+    d.dgamma[i] = x.dgamma;
+  }
+  d.eps = eps;
+  d.pairs = mode == GRXDNN_ROPE_PAIRS;
+  d.rotary = rotaryDim;
+  d.positions = positions;
+  d.inv_freq = frequencies;
+  d.ws = workspace;
+  return from_hip(grxk::launch_qk_norm_rope(nt, d, backward, handle->stream));
+}
 
 }  // namespace
 
@@ -629,6 +803,47 @@ int grxdnnAttentionCycleSlotsNeeded(grxdnnHandle_t handle, int batch, int heads,
   if (batch <= 0 || heads <= 0 || seqLen <= 0) return 0;
   const int64_t s = grxk::attention_probe_slots(batch, heads, seqLen);
   return s > INT_MAX ? INT_MAX : (int)s;
+}
+
+grxdnnStatus_t grxdnnQkNormRopeForward(grxdnnHandle_t handle, grxdnnTensorDescriptor_t qDesc, const void* q,
+                                       grxdnnTensorDescriptor_t kDesc, const void* k,
+                                       grxdnnTensorDescriptor_t wDesc, const void* qGamma, const void* kGamma,
+                                       float eps, grxdnnRopeMode_t mode, int rotaryDim, const int* positions,
+                                       const float* inverseFrequencies, grxdnnTensorDescriptor_t yqDesc, void* yq,
+                                       grxdnnTensorDescriptor_t ykDesc, void* yk) {
+  const QkSide side[2] = {{qDesc, q, qGamma, nullptr, nullptr, yqDesc, yq, nullptr},
+                          {kDesc, k, kGamma, nullptr, nullptr, ykDesc, yk, nullptr}};
+  return qk_norm_rope(handle, side, wDesc, eps, mode, rotaryDim, positions, inverseFrequencies, false, nullptr, 0);
+}
+
+grxdnnStatus_t grxdnnQkNormRopeGetWorkspaceSize(grxdnnHandle_t handle, grxdnnTensorDescriptor_t qDesc,
+                                                grxdnnTensorDescriptor_t kDesc, grxdnnTensorDescriptor_t wDesc,
+                                                size_t* bytes) {
+  if (!handle) return GRXDNN_STATUS_NOT_INITIALIZED;
+  if (!bytes) return GRXDNN_STATUS_INVALID_VALUE;
+  grxk::QkRopeDesc d{};
+  grxk::NormType nt{};
+  const grxdnnStatus_t s = qk_shape(qDesc, kDesc, wDesc, &nt, &d);
+  if (s != GRXDNN_STATUS_SUCCESS) return s;
+  const int64_t tokens = (int64_t)d.B * d.S;
+  *bytes = wDesc && tokens && d.heads[0] + d.heads[1]
+               ? grxk::qk_norm_rope_workspace(tokens, d.heads[0], d.heads[1], d.D) : 0;
+  return GRXDNN_STATUS_SUCCESS;
+}
+
+grxdnnStatus_t grxdnnQkNormRopeBackward(grxdnnHandle_t handle, grxdnnTensorDescriptor_t qDesc, const void* q,
+                                        grxdnnTensorDescriptor_t kDesc, const void* k,
+                                        grxdnnTensorDescriptor_t wDesc, const void* qGamma, const void* kGamma,
+                                        float eps, grxdnnRopeMode_t mode, int rotaryDim, const int* positions,
+                                        const float* inverseFrequencies, grxdnnTensorDescriptor_t dyqDesc,
+                                        const void* dyq, grxdnnTensorDescriptor_t dykDesc, const void* dyk,
+                                        grxdnnTensorDescriptor_t dqDesc, void* dq, grxdnnTensorDescriptor_t dkDesc,
+                                        void* dk, float* dqGamma, float* dkGamma, void* workspace,
+                                        size_t workspaceBytes) {
+  const QkSide side[2] = {{qDesc, q, qGamma, dyqDesc, dyq, dqDesc, dq, dqGamma},
+                          {kDesc, k, kGamma, dykDesc, dyk, dkDesc, dk, dkGamma}};
+  return qk_norm_rope(handle, side, wDesc, eps, mode, rotaryDim, positions, inverseFrequencies, true, workspace,
+                      workspaceBytes);
 }
 
 grxdnnStatus_t grxdnnPagedCacheAppend(grxdnnHandle_t handle, grxdnnTensorDescriptor_t kDesc, const void* k,

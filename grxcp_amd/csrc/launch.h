@@ -134,6 +134,26 @@ struct RowDesc {
 hipError_t launch_softmax(NormType t, const RowDesc& d, hipStream_t s);
 hipError_t launch_gelu(NormType t, bool tanh_form, const RowDesc& d, hipStream_t s);
 
+// Norm and rotation of queries (0) and keys (1), [B, heads, S, D]; the gradient where
+// `backward` is asked for.
+struct QkRows { const void* p; int64_t sb, sh, ss; };   // strides (elements) of b, h, s
+struct QkRopeDesc {
+  int B, S, D;
+  int heads[2];                        // 0: not there
+  QkRows x[2], dy[2], y[2];            // y: dx of a backward call
+  const void* gamma[2];                // null: no norm
+  float eps;
+  bool pairs;
+  int rotary;
+  const int* positions;
+  const float* inv_freq;
+  float* dgamma[2];                    // null: not asked for
+  void* ws;
+};
+hipError_t launch_qk_norm_rope(NormType t, const QkRopeDesc& d, bool backward, hipStream_t s);
+// Workspace bytes of a backward call with gradients of the gains.
+size_t qk_norm_rope_workspace(int64_t tokens, int hq, int hk, int D);
+
 enum class AttnType { BF16, F16 };
 struct AttnDesc {
   int B, H, S, D;

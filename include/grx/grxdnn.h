@@ -168,6 +168,83 @@ grxdnnStatus_t grxdnnSetCycleProbe(grxdnnHandle_t handle, grxCycleSlot* slots,
 int            grxdnnAttentionCycleSlotsNeeded(grxdnnHandle_t handle, int batch,
                                                int heads, int seqLen);
 
+/* ---- norm and rotation of queries and keys ----------------------------------
+ *
+ * What comes between a projection and attention, in one pass: every head's row of
+ * D values normalised by itself, and turned by its token's position.
+ *   n = x / sqrt(mean(x^2) + eps),  u = n * gamma     (without gains: u = x)
+ *   y[j] = u[j] cos - u[j'] sin,  y[j'] = u[j'] cos + u[j] sin
+ *                                 of positions[b,s] * inverseFrequencies[i]
+ * for the i-th of rotaryDim / 2 pairs (j, j'): (i, i + rotaryDim / 2) for
+ * GRXDNN_ROPE_HALVES, (2i, 2i + 1) for GRXDNN_ROPE_PAIRS. Values from rotaryDim on
+ * are not turned.
+ *
+ * q, yq: [B, H, S, D] and k, yk: [B, Hkv, S, D] of one type (GRX_R_16BF, GRX_R_16F
+ * or GRX_R_32F), any strides that are multiples of 16 bytes (views of a packed
+ * projection, of [B, S, H, D] memory), innermost stride 1, pointers 16-byte
+ * aligned; D is 64, 128 or 256, B * S at most 2^31 - 4096 and H + Hkv at most 2^20
+ * (else NOT_SUPPORTED). qGamma, kGamma: [D] of that type, contiguous, described
+ * by wDesc; wDesc and both NULL: no norm, and eps is not looked at. All key
+ * arguments NULL together: queries alone. rotaryDim: 0 .. D in steps of 16;
+ * 0: no rotation, positions and inverseFrequencies are not read and may be NULL
+ * (norm or rotation: INVALID_VALUE for neither). positions: B * S ints, packed
+ * (a decoding step's are the sequences' lengths before the token), negative ones
+ * turn back; inverseFrequencies: rotaryDim / 2 fp32. Both are device memory, read
+ * when the kernels run.
+ *
+ * Sums and products are fp32 and y is rounded once; angles are reduced from the
+ * whole product (64 bits and its remainder), for |angle| < 2^40. A row whose sum
+ * of squares exceeds fp32's range is scaled by 0. Outputs must not share elements
+ * of their own or with each other or with what the call reads, but yq may be q
+ * and yk k (same pointer and strides); else INVALID_VALUE.
+ * (New: planned by ref docs/designs/grxcp_roadmap.md:864-877.) */
+typedef enum {
+  GRXDNN_ROPE_HALVES = 0,
+  GRXDNN_ROPE_PAIRS  = 1
+} grxdnnRopeMode_t;
+
+grxdnnStatus_t grxdnnQkNormRopeForward(grxdnnHandle_t handle,
+                                       grxdnnTensorDescriptor_t qDesc, const void* q,
+                                       grxdnnTensorDescriptor_t kDesc, const void* k,
+                                       grxdnnTensorDescriptor_t wDesc, const void* qGamma,
+                                       const void* kGamma, float eps,
+                                       grxdnnRopeMode_t mode, int rotaryDim,
+                                       const int* positions, const float* inverseFrequencies,
+                                       grxdnnTensorDescriptor_t yqDesc, void* yq,
+                                       grxdnnTensorDescriptor_t ykDesc, void* yk);
+
+/* The gradient of that, from the forward call's inputs and the gradients dyq, dyk of
+ * its outputs. With g the row of dy turned back:
+ *   dx = r (g gamma - n mean(g gamma n)),  r = 1 / sqrt(mean(x^2) + eps)     (without gains: dx = g)
+ *   dqGamma[j] = sum over b, h, s of g[j] n[j],  and dkGamma over the keys' rows
+ * dyq, dq: [B, H, S, D], dyk, dk: [B, Hkv, S, D], of the inputs' type and rules; dq may
+ * be dyq and dk dyk (same pointer and strides), or q and k. dqGamma, dkGamma: D fp32
+ * each, overwritten, packed; NULL for what is not asked for, and without gains. Without
+ * gains q and k are not read and may be NULL (their descriptors are needed). Sums are
+ * fp32, in an order that does not change from call to call.
+ * workspace: device memory of at least the size that
+ * grxdnnQkNormRopeGetWorkspaceSize gives for the same descriptors (kDesc NULL
+ * without keys; 0 bytes without wDesc), 16-byte aligned; needed where dqGamma or
+ * dkGamma is asked for. Calls that may run at the same time, captured graphs
+ * included, need workspaces of their own. */
+grxdnnStatus_t grxdnnQkNormRopeGetWorkspaceSize(grxdnnHandle_t handle,
+                                                grxdnnTensorDescriptor_t qDesc,
+                                                grxdnnTensorDescriptor_t kDesc,
+                                                grxdnnTensorDescriptor_t wDesc, size_t* bytes);
+grxdnnStatus_t grxdnnQkNormRopeBackward(grxdnnHandle_t handle,
+                                        grxdnnTensorDescriptor_t qDesc, const void* q,
+                                        grxdnnTensorDescriptor_t kDesc, const void* k,
+                                        grxdnnTensorDescriptor_t wDesc, const void* qGamma,
+                                        const void* kGamma, float eps,
+                                        grxdnnRopeMode_t mode, int rotaryDim,
+                                        const int* positions, const float* inverseFrequencies,
+                                        grxdnnTensorDescriptor_t dyqDesc, const void* dyq,
+                                        grxdnnTensorDescriptor_t dykDesc, const void* dyk,
+                                        grxdnnTensorDescriptor_t dqDesc, void* dq,
+                                        grxdnnTensorDescriptor_t dkDesc, void* dk,
+                                        float* dqGamma, float* dkGamma,
+                                        void* workspace, size_t workspaceBytes);
+
 /* ---- paged key-value cache --------------------------------------------------
  *
  * Keys and values of running sequences lie in two pools, each described by a
