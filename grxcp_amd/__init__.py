@@ -154,6 +154,8 @@ _DNN = {
                                                      POINTER(c_size_t)]),
     "grxdnnPagedAttentionForward": (c_int, [c_void_p] * 11 + [c_float] + [c_void_p] * 5 + [c_size_t]),
     "grxdnnPagedCacheEvict": (c_int, [c_void_p] * 10 + [c_int, c_int] + [c_void_p] * 6),
+    "grxdnnPagedCacheAppendQuantized": (c_int, [c_void_p] * 16),
+    "grxdnnPagedCacheReadQuantized": (c_int, [c_void_p] * 16),
     "grxdnnTokenLogProbGetWorkspaceSize": (c_int, [c_void_p, c_void_p, c_int, POINTER(c_size_t)]),
     "grxdnnTokenLogProbForward": (c_int, [c_void_p] * 7 + [c_int, c_void_p, c_void_p, c_void_p, c_size_t]),
     "grxdnnTokenLogProbBackward": (c_int, [c_void_p] * 10),
@@ -437,6 +439,16 @@ class Dnn:
                     new_lengths, nwd, new_w) -> int:
         return self.L.grxdnnPagedCacheEvict(self.h, kcd.d, kc, vcd.d, vc, td.d, table, lengths, wd.d, w, budget,
                                             recent, kept, ntd.d, new_table, new_lengths, nwd.d, new_w)
+
+    def paged_append_quantized(self, kd, k, vd, v, kcd, kc, vcd, vc, sd, ks, vs, td, table, lengths,
+                               counts=None) -> int:
+        return self.L.grxdnnPagedCacheAppendQuantized(self.h, kd.d, k, vd.d, v, kcd.d, kc, vcd.d, vc, sd.d, ks, vs,
+                                                      td.d, table, lengths, counts)
+
+    def paged_read_quantized(self, kcd, kc, vcd, vc, sd, ks, vs, td, table, lengths, first, kd, k, vd, v) -> int:
+        """first: each sequence's first slot to read, or None for 0."""
+        return self.L.grxdnnPagedCacheReadQuantized(self.h, kcd.d, kc, vcd.d, vc, sd.d, ks, vs, td.d, table, lengths,
+                                                    first, kd.d, k, vd.d, v)
 
     def token_logprob_workspace(self, xd, top: int) -> int:
         n = c_size_t(0)

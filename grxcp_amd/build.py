@@ -50,6 +50,7 @@ LIBS = {
                        "kernels/noalloc_scratch.hip"], ["grxrt"]),
     "libgrxdnn.so": (["grxdnn.cpp", "kernels/norms.hip", "kernels/softmax_gelu.hip",
                       "kernels/attention.hip", "kernels/paged_cache.hip",
+                      "kernels/paged_cache_i8.hip",
                       "kernels/paged_attention.hip", "kernels/token_logprob.hip",
                       "kernels/qk_norm_rope.hip"], ["grxrt"]),
 }

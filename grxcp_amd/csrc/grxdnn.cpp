@@ -322,17 +322,11 @@ grxdnnStatus_t row_common(grxdnnHandle_t handle, grxdnnTensorDescriptor_t xDesc,
 
 bool half_type(grxDataType_t t) { return t == GRX_R_16BF || t == GRX_R_16F; }
 
-// 16-byte vector access along the last dimension: contiguous, rows on 16 bytes.
-bool half_rows(const grxdnnTensorStruct& t) {
-  if (t.strides[t.nb - 1] != 1) return false;
-  for (int i = 0; i < t.nb - 1; ++i)
-    if (t.dims[i] > 1 && t.strides[i] % 8 != 0) return false;
-  return true;
-}
-
 // Slots that a sequence may have room for: the kernels count them in 32 bits, up to a
 // tile's or a workgroup's worth past the last.
 constexpr int kMaxRoom = INT_MAX - 4095;
+// Slots that may share a scale: a workgroup holds their values in registers.
+constexpr int kMaxBlock = 256;
 
 // A table of pages: [B, W] ints, rows of any pitch.
 bool table_shape(const grxdnnTensorStruct& t) {
@@ -345,16 +339,28 @@ bool weights_shape(const grxdnnTensorStruct& t, int B, int heads, int64_t slots)
          (t.dims[2] <= 1 || t.strides[2] == 1);
 }
 
-// The pools and the table of a paged call, but for their pointers.
+// 16-byte vector access along the last dimension, of elements of `elem` bytes.
+bool vector_rows(const grxdnnTensorStruct& t, int elem) {
+  if (t.strides[t.nb - 1] != 1) return false;
+  for (int i = 0; i < t.nb - 1; ++i)
+    if (t.dims[i] > 1 && (int64_t)t.strides[i] * elem % 16 != 0) return false;
+  return true;
+}
+
+bool half_rows(const grxdnnTensorStruct& t) { return vector_rows(t, 2); }
+
+// The pools and the table of a paged call, but for their pointers. codes: pools of 8 bits.
 grxdnnStatus_t paged_cache(grxdnnTensorDescriptor_t kDesc, grxdnnTensorDescriptor_t vDesc,
-                           grxdnnTensorDescriptor_t tableDesc, bool written, grxk::PagedCache* c) {
+                           grxdnnTensorDescriptor_t tableDesc, bool written, grxk::PagedCache* c,
+                           bool codes = false) {
   if (!kDesc || !vDesc || !tableDesc || !kDesc->set || !vDesc->set || !tableDesc->set)
     return GRXDNN_STATUS_INVALID_VALUE;
   if (kDesc->nb != 4 || !same_shape(*kDesc, *vDesc) || !table_shape(*tableDesc))
     return GRXDNN_STATUS_INVALID_VALUE;
   for (int i = 0; i < 4; ++i)
     if (kDesc->dims[i] < 1) return GRXDNN_STATUS_INVALID_VALUE;
-  if (!half_type(kDesc->type) || vDesc->type != kDesc->type) return GRXDNN_STATUS_NOT_SUPPORTED;
+  if (codes ? kDesc->type != GRX_R_8I : !half_type(kDesc->type)) return GRXDNN_STATUS_NOT_SUPPORTED;
+  if (vDesc->type != kDesc->type) return GRXDNN_STATUS_NOT_SUPPORTED;
   c->pages = kDesc->dims[0];
   c->heads = kDesc->dims[1];
   c->page = kDesc->dims[2];
@@ -366,10 +372,26 @@ grxdnnStatus_t paged_cache(grxdnnTensorDescriptor_t kDesc, grxdnnTensorDescripto
   if ((int64_t)c->W * c->page > kMaxRoom) return GRXDNN_STATUS_NOT_SUPPORTED;
   // (sequence, head) pairs are counted in 32 bits
   if ((int64_t)c->B * c->heads > INT_MAX / 4) return GRXDNN_STATUS_NOT_SUPPORTED;
-  if (!half_rows(*kDesc) || !half_rows(*vDesc)) return GRXDNN_STATUS_NOT_SUPPORTED;
+  const int elem = codes ? 1 : 2;
+  if (!vector_rows(*kDesc, elem) || !vector_rows(*vDesc, elem)) return GRXDNN_STATUS_NOT_SUPPORTED;
   if (written && (!no_overlap(*kDesc) || !no_overlap(*vDesc))) return GRXDNN_STATUS_INVALID_VALUE;
   c->k_sp = kDesc->strides[0]; c->k_sh = kDesc->strides[1]; c->k_ss = kDesc->strides[2];
   c->v_sp = vDesc->strides[0]; c->v_sh = vDesc->strides[1]; c->v_ss = vDesc->strides[2];
+  return GRXDNN_STATUS_SUCCESS;
+}
+
+// The scales of a cache in 8 bits, [pages, heads, page / block], but for their pointers.
+grxdnnStatus_t quant_scales(grxdnnTensorDescriptor_t scaleDesc, const grxk::PagedCache& c, bool written,
+                            grxk::QuantScales* q) {
+  if (!scaleDesc || !scaleDesc->set || scaleDesc->nb != 3) return GRXDNN_STATUS_INVALID_VALUE;
+  const int blocks = scaleDesc->dims[2];
+  if (scaleDesc->dims[0] != c.pages || scaleDesc->dims[1] != c.heads || blocks < 1 || c.page % blocks != 0)
+    return GRXDNN_STATUS_INVALID_VALUE;
+  if (scaleDesc->type != GRX_R_32F) return GRXDNN_STATUS_NOT_SUPPORTED;
+  q->block = c.page / blocks;
+  if (q->block > kMaxBlock) return GRXDNN_STATUS_NOT_SUPPORTED;
+  if (written && !no_overlap(*scaleDesc)) return GRXDNN_STATUS_INVALID_VALUE;
+  q->sp = scaleDesc->strides[0]; q->sh = scaleDesc->strides[1]; q->sb = scaleDesc->strides[2];
   return GRXDNN_STATUS_SUCCESS;
 }
 
@@ -396,25 +418,27 @@ grxdnnStatus_t logit_rows(const grxdnnTensorStruct& x, grxk::NormType* nt, int64
 
 size_t element_size(grxk::NormType t) { return t == grxk::NormType::F32 ? 4 : 2; }
 
-// 16-byte vector access along the last dimension, of elements of `elem` bytes.
-bool vector_rows(const grxdnnTensorStruct& t, int elem) {
-  if (t.strides[t.nb - 1] != 1) return false;
-  for (int i = 0; i < t.nb - 1; ++i)
-    if (t.dims[i] > 1 && (int64_t)t.strides[i] * elem % 16 != 0) return false;
-  return true;
-}
-
-// An array of a call: a tensor, or `bytes` packed ones.
+// An array of a call: a tensor, or `bytes` packed ones. A null pointer: not there.
 struct Operand {
   const grxdnnTensorStruct* d;
   const void* p;
   int64_t bytes;
 };
-bool share(const Operand& a, const Operand& b, size_t elem) {
+size_t type_size(grxDataType_t t) { return t == GRX_R_8I ? 1 : half_type(t) ? 2 : 4; }
+Span span_of(const Operand& a) { return a.d ? span_of(*a.d, a.p, type_size(a.d->type)) : bytes_at(a.p, a.bytes); }
+// Element by element where the two have one type and the same strides, else by their spans.
+bool share(const Operand& a, const Operand& b) {
   if (!a.p || !b.p) return false;
-  if (a.d && b.d) return views_share_element(*a.d, a.p, *b.d, b.p, elem);
-  return intersect(a.d ? span_of(*a.d, a.p, elem) : bytes_at(a.p, a.bytes),
-                   b.d ? span_of(*b.d, b.p, elem) : bytes_at(b.p, b.bytes));
+  if (a.d && b.d && a.d->type == b.d->type)
+    return views_share_element(*a.d, a.p, *b.d, b.p, type_size(a.d->type));
+  return intersect(span_of(a), span_of(b));
+}
+// Whether one of the first `written` of n arrays shares an element with another one.
+bool shared_by_written(const Operand* all, int n, int written) {
+  for (int i = 0; i < written; ++i)
+    for (int j = i + 1; j < n; ++j)
+      if (share(all[i], all[j])) return true;
+  return false;
 }
 bool in_place(const Operand& a, const Operand& b) { return a.d && b.d && a.p == b.p && same_strides(*a.d, *b.d); }
 
@@ -525,7 +549,7 @@ grxdnnStatus_t qk_norm_rope(grxdnnHandle_t handle, const QkSide (&side)[2], grxd
   }
   for (int i = 0; i < written; ++i)
     for (int j = i + 1; j < n; ++j) {
-      if (!share(all[i], all[j], elem)) continue;
+      if (!share(all[i], all[j])) continue;
       // a row is read by the lanes that write it: in place, over x or over dy of its side
       const int at = i < 2 && j >= written ? (j - written) / 3 : -1;
       if (at == i && in_place(all[i], all[j])) continue;
@@ -1024,6 +1048,98 @@ grxdnnStatus_t grxdnnPagedCacheEvict(grxdnnHandle_t handle, grxdnnTensorDescript
   d.new_weights = newWeights; d.nw_sb = newWeightsDesc->strides[0]; d.nw_sh = newWeightsDesc->strides[1];
   d.nw_slots = newWeightsDesc->dims[2];
   return from_hip(grxk::launch_paged_evict(d, handle->stream));
+}
+
+grxdnnStatus_t grxdnnPagedCacheAppendQuantized(grxdnnHandle_t handle, grxdnnTensorDescriptor_t kDesc, const void* k,
+                                               grxdnnTensorDescriptor_t vDesc, const void* v,
+                                               grxdnnTensorDescriptor_t kCacheDesc, void* kCache,
+                                               grxdnnTensorDescriptor_t vCacheDesc, void* vCache,
+                                               grxdnnTensorDescriptor_t scaleDesc, float* kScale, float* vScale,
+                                               grxdnnTensorDescriptor_t tableDesc, const int* table,
+                                               const int* lengths, const int* counts) {
+  if (!handle) return GRXDNN_STATUS_NOT_INITIALIZED;
+  if (!kDesc || !vDesc || !kDesc->set || !vDesc->set) return GRXDNN_STATUS_INVALID_VALUE;
+  grxk::PagedAppendDesc d{};
+  grxk::QuantScales q{};
+  grxdnnStatus_t s = paged_cache(kCacheDesc, vCacheDesc, tableDesc, true, &d.c, true);
+  if (s != GRXDNN_STATUS_SUCCESS) return s;
+  s = quant_scales(scaleDesc, d.c, true, &q);
+  if (s != GRXDNN_STATUS_SUCCESS) return s;
+  if (kDesc->nb != 4 || !same_shape(*kDesc, *vDesc) || kDesc->dims[0] != d.c.B ||
+      kDesc->dims[1] != d.c.heads || kDesc->dims[3] != d.c.D)
+    return GRXDNN_STATUS_INVALID_VALUE;
+  if (!half_type(kDesc->type) || vDesc->type != kDesc->type) return GRXDNN_STATUS_NOT_SUPPORTED;
+  d.T = kDesc->dims[2];
+  // (block, head) pairs of a sequence are counted in 32 bits
+  if (((int64_t)d.T + 2 * kMaxBlock) * d.c.heads > INT_MAX) return GRXDNN_STATUS_NOT_SUPPORTED;
+  if (d.c.B == 0 || d.T == 0) return GRXDNN_STATUS_SUCCESS;
+  if (!half_rows(*kDesc) || !half_rows(*vDesc)) return GRXDNN_STATUS_NOT_SUPPORTED;
+  if (!k || !v || !kCache || !vCache || !kScale || !vScale || !table || !lengths) return GRXDNN_STATUS_INVALID_VALUE;
+  const Operand all[] = {{kCacheDesc, kCache, 0}, {vCacheDesc, vCache, 0}, {scaleDesc, kScale, 0},
+                         {scaleDesc, vScale, 0},
+                         // only read from here on
+                         {kDesc, k, 0}, {vDesc, v, 0}, {tableDesc, table, 0}, {nullptr, lengths, 4ll * d.c.B},
+                         {nullptr, counts, 4ll * d.c.B}};
+  if (shared_by_written(all, 9, 4)) return GRXDNN_STATUS_INVALID_VALUE;
+  if (!aligned16(k) || !aligned16(v) || !aligned16(kCache) || !aligned16(vCache))
+    return GRXDNN_STATUS_NOT_SUPPORTED;
+  s = ensure_device(*handle);
+  if (s != GRXDNN_STATUS_SUCCESS) return s;
+  d.c.k = kCache; d.c.v = vCache; d.c.table = table; d.c.lengths = lengths;
+  q.k = kScale; q.v = vScale;
+  d.k = k; d.k_sb = kDesc->strides[0]; d.k_sh = kDesc->strides[1]; d.k_st = kDesc->strides[2];
+  d.v = v; d.v_sb = vDesc->strides[0]; d.v_sh = vDesc->strides[1]; d.v_st = vDesc->strides[2];
+  d.counts = counts;
+  return from_hip(grxk::launch_paged_append_i8(
+      kDesc->type == GRX_R_16BF ? grxk::AttnType::BF16 : grxk::AttnType::F16, d, q, handle->stream));
+}
+
+grxdnnStatus_t grxdnnPagedCacheReadQuantized(grxdnnHandle_t handle, grxdnnTensorDescriptor_t kCacheDesc,
+                                             const void* kCache, grxdnnTensorDescriptor_t vCacheDesc,
+                                             const void* vCache, grxdnnTensorDescriptor_t scaleDesc,
+                                             const float* kScale, const float* vScale,
+                                             grxdnnTensorDescriptor_t tableDesc, const int* table,
+                                             const int* lengths, const int* first, grxdnnTensorDescriptor_t kDesc,
+                                             void* k, grxdnnTensorDescriptor_t vDesc, void* v) {
+  if (!handle) return GRXDNN_STATUS_NOT_INITIALIZED;
+  if (!kDesc || !vDesc || !kDesc->set || !vDesc->set) return GRXDNN_STATUS_INVALID_VALUE;
+  grxk::PagedReadDesc d{};
+  grxk::QuantScales q{};
+  grxdnnStatus_t s = paged_cache(kCacheDesc, vCacheDesc, tableDesc, false, &d.c, true);
+  if (s != GRXDNN_STATUS_SUCCESS) return s;
+  s = quant_scales(scaleDesc, d.c, false, &q);
+  if (s != GRXDNN_STATUS_SUCCESS) return s;
+  if (kDesc->nb != 4 || !same_shape(*kDesc, *vDesc) || kDesc->dims[0] != d.c.B ||
+      kDesc->dims[1] != d.c.heads || kDesc->dims[3] != d.c.D)
+    return GRXDNN_STATUS_INVALID_VALUE;
+  grxk::NormType nt{};
+  s = qk_type(kDesc->type, &nt);
+  if (s != GRXDNN_STATUS_SUCCESS) return s;
+  if (vDesc->type != kDesc->type) return GRXDNN_STATUS_NOT_SUPPORTED;
+  d.T = kDesc->dims[2];
+  if ((int64_t)d.T * d.c.heads > kMaxRoom) return GRXDNN_STATUS_NOT_SUPPORTED;   // counted in 32 bits
+  if (d.c.B == 0 || d.T == 0) return GRXDNN_STATUS_SUCCESS;
+  const size_t elem = element_size(nt);
+  if (!vector_rows(*kDesc, (int)elem) || !vector_rows(*vDesc, (int)elem)) return GRXDNN_STATUS_NOT_SUPPORTED;
+  if (!no_overlap(*kDesc) || !no_overlap(*vDesc)) return GRXDNN_STATUS_INVALID_VALUE;
+  if (!k || !v || !kCache || !vCache || !kScale || !vScale || !table || !lengths) return GRXDNN_STATUS_INVALID_VALUE;
+  const Operand all[] = {{kDesc, k, 0}, {vDesc, v, 0},
+                         // only read from here on
+                         {kCacheDesc, kCache, 0}, {vCacheDesc, vCache, 0}, {scaleDesc, kScale, 0},
+                         {scaleDesc, vScale, 0}, {tableDesc, table, 0}, {nullptr, lengths, 4ll * d.c.B},
+                         {nullptr, first, 4ll * d.c.B}};
+  if (shared_by_written(all, 9, 2)) return GRXDNN_STATUS_INVALID_VALUE;
+  if (!aligned16(k) || !aligned16(v) || !aligned16(kCache) || !aligned16(vCache))
+    return GRXDNN_STATUS_NOT_SUPPORTED;
+  s = ensure_device(*handle);
+  if (s != GRXDNN_STATUS_SUCCESS) return s;
+  d.c.k = const_cast<void*>(kCache); d.c.v = const_cast<void*>(vCache);
+  d.c.table = table; d.c.lengths = lengths;
+  q.k = const_cast<float*>(kScale); q.v = const_cast<float*>(vScale);
+  d.k = k; d.k_sb = kDesc->strides[0]; d.k_sh = kDesc->strides[1]; d.k_st = kDesc->strides[2];
+  d.v = v; d.v_sb = vDesc->strides[0]; d.v_sh = vDesc->strides[1]; d.v_st = vDesc->strides[2];
+  d.first = first;
+  return from_hip(grxk::launch_paged_read_i8(nt, d, q, handle->stream));
 }
 
 grxdnnStatus_t grxdnnTokenLogProbGetWorkspaceSize(grxdnnHandle_t handle, grxdnnTensorDescriptor_t xDesc,

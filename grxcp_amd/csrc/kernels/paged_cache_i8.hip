@@ -1,0 +1,333 @@
+// grxDNN paged key-value cache in 8 bits on gfx950: rows quantised as they are written,
+// and read back.
+//
+// New: the reference plans attention for grxDNN (ref
+// docs/designs/grxcp_roadmap.md:864-877) and ships neither it nor a cache.
+//
+// A block of `block` slots of one head has one scale, the largest magnitude / 127
+// rounded up to 8 significant bits. With that a quotient x / scale of a 16-bit value is
+// either half way between two codes or further from there than 2^-17 of it: |x / s - (k + 1/2)|
+// = |2x - (2k + 1) s| / 2s is a whole number of the smaller last bit of 2x and s, and that
+// is at least 1 / 2S (S < 2^8 the significand of s) or 1 / X of the quotient (X < 2^11 that
+// of x; 2^15 for a code times an older scale). So codes are the same in every arithmetic
+// that keeps 2^-17, and ties go to the even code once the quotient is rounded correctly.
+
+#include "../launch.h"
+#include "device_common.h"
+#include "paged_common.h"
+#include "row_io.h"
+
+#include <algorithm>
+
+namespace grxk {
+namespace {
+
+constexpr int kThreads = 256;
+
+// A pool of codes as the kernels address it, strides in bytes, and its scales.
+struct Pool8 {
+  uint8_t* p;
+  int64_t sp, sh, ss;
+  float* scale;
+  int64_t cp, ch, cb;
+  __device__ __forceinline__ uint8_t* row(int page, int h, int slot) const { return p + page * sp + h * sh + slot * ss; }
+  __device__ __forceinline__ float* scale_of(int page, int h, int block) const {
+    return scale + page * cp + h * ch + block * cb;
+  }
+};
+Pool8 pool_of(const PagedCache& c, const QuantScales& q, bool values) {
+  return values ? Pool8{(uint8_t*)c.v, c.v_sp, c.v_sh, c.v_ss, q.v, q.sp, q.sh, q.sb}
+                : Pool8{(uint8_t*)c.k, c.k_sp, c.k_sh, c.k_ss, q.k, q.sp, q.sh, q.sb};
+}
+PagedView view_of(const PagedCache& c) {
+  return {c.table, c.table_rs, c.lengths, c.pages, c.page, c.W * c.page, page_div(c.page)};
+}
+
+// ---- append ------------------------------------------------------------------
+
+struct NewRows {
+  const uint8_t* p;
+  int64_t sb, sh, st;    // bytes
+};
+struct AppendParams {
+  PagedView view;
+  Pool8 pool[2];
+  NewRows rows[2];
+  const int* counts;
+  PageDiv by_heads, by_block;
+  int B, T, heads, block;
+};
+
+template <NormType T> __device__ __forceinline__ float half_value(uint32_t bits) {
+  return T == NormType::BF16 ? bf16_to_f32((uint16_t)bits) : f16_to_f32((uint16_t)bits);
+}
+
+// The scale of values of which `bits` (of the 16-bit type, no sign) is the largest
+// magnitude: NaN if that is an infinity or NaN.
+template <NormType T> __device__ __forceinline__ float scale_for(uint32_t bits) {
+  const float most = half_value<T>(bits);
+  if (!(most <= __FLT_MAX__)) return __uint_as_float(0x7fc00000u);
+  if (most == 0.0f) return 0.0f;
+  const uint32_t up = (__float_as_uint(most / 127.0f) + 0xffffu) & 0xffff0000u;
+  return fmaxf(__uint_as_float(up), 0x1p-126f);
+}
+
+// The codes of 4 values: x / s rounded to the nearest whole number, ties to the even one.
+// r = 1 / s correctly rounded; the remainder x - y s is exact where the quotient has few
+// bits, so that a tie is one. Adding 1.5 * 2^23 rounds and leaves the code in the low byte.
+__device__ __forceinline__ uint32_t codes4(const float* x, float s, float r) {
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float y = x[i] * r;
+    const float z = fmaf(fmaf(-y, s, x[i]), r, y);
+    w[i] = __float_as_uint(z + 12582912.0f);
+  }
+  const uint32_t lo = __builtin_amdgcn_perm(w[1], w[0], 0x0c0c0400u), hi = __builtin_amdgcn_perm(w[3], w[2], 0x0c0c0400u);
+  return lo | hi << 16;
+}
+
+template <int CTRL> __device__ __forceinline__ uint32_t dpp_max(uint32_t v) {
+  return max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, CTRL, 0xf, 0xf, false));
+}
+// The largest over L neighbouring lanes (8, 16 or 64), in each.
+template <int L> __device__ __forceinline__ uint32_t lanes_max(uint32_t v) {
+  v = dpp_max<0xb1>(v);
+  v = dpp_max<0x4e>(v);
+  v = dpp_max<0x141>(v);
+  if constexpr (L >= 16) v = dpp_max<0x140>(v);
+  if constexpr (L == 64) {
+    const auto a = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    v = max(a[0], a[1]);
+    const auto b = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    v = max(b[0], b[1]);
+  }
+  return v;
+}
+
+// One task: the block of one head's keys or values (blockIdx.z) that gets new rows, by L
+// threads with N chunks of 8 values each, held in registers between the maximum and the
+// codes: read once. Rows that the block already holds are rounded again, to the new scale,
+// where that is larger.
+template <NormType T, int C, int L, int N>   // C: chunks of a row
+__global__ __launch_bounds__(kThreads) void append_i8(AppendParams p) {
+  __shared__ uint32_t most_of[kThreads / 64];
+  const int tid = threadIdx.x, l = tid % L;
+  const Pool8& pool = p.pool[blockIdx.z];
+  const NewRows& in = p.rows[blockIdx.z];
+  for (int b = blockIdx.y; b < p.B; b += gridDim.y) {
+    const int n = clamp_length(p.view.lengths[b], p.view.room);
+    const int count = min(p.counts ? min(p.counts[b], p.T) : p.T, p.view.room - n);   // the others have no place
+    if (count <= 0) continue;
+    const int b0 = div_page(p.by_block, n), blocks = div_page(p.by_block, n + count - 1) - b0 + 1;
+    const int64_t tasks = (int64_t)blocks * p.heads;
+    for (int64_t t0 = (int64_t)blockIdx.x * (kThreads / L); t0 < tasks; t0 += (int64_t)gridDim.x * (kThreads / L)) {
+      const int64_t task = t0 + tid / L;
+      const bool mine = task < tasks;
+      const int at = mine ? (int)task : 0;
+      const int j = div_page(p.by_heads, at), h = at - j * p.heads;
+      const int lo = (b0 + j) * p.block;                      // its first slot
+      const int old = max(0, n - lo), end = min(p.block, n + count - lo);
+      int page, row;
+      const bool there = find_slot(p.view, b, lo, &page, &row) & mine;
+      float* scale = pool.scale_of(page, h, div_page(p.by_block, row));
+      const float before = there && old > 0 ? *scale : 0.0f;
+      const uint8_t* src = in.p + b * in.sb + h * in.sh;
+      u32x4 x[N];
+      uint32_t most = 0;
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const int c = i * L + l, r = c / C;
+        x[i] = u32x4{0, 0, 0, 0};
+        if (there && r >= old && r < end)
+          x[i] = __builtin_nontemporal_load((const u32x4*)(src + (int64_t)(lo + r - n) * in.st) + c % C);
+      }
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) most = max(max(most, x[i][e] & 0x7fffu), x[i][e] >> 16 & 0x7fffu);
+      if constexpr (L <= 64) {
+        most = lanes_max<L>(most);
+      } else {
+        most = lanes_max<64>(most);
+        __syncthreads();                                      // the task before has read
+        if ((tid & 63) == 0) most_of[tid >> 6] = most;
+        __syncthreads();
+        most = max(max(most_of[0], most_of[1]), max(most_of[2], most_of[3]));
+      }
+      if (!there) continue;                                   // (L = 256: of the whole workgroup)
+      const float need = scale_for<T>(most);
+      float s = fmaxf(need, before);
+      if (s > 0.0f) s = fmaxf(s, 0x1p-126f);
+      if (need != need || before != before) s = __uint_as_float(0x7fc00000u);
+      const bool fine = s > 0.0f && s <= __FLT_MAX__;
+      const float r1 = fine ? 1.0f / s : 0.0f;
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const int c = i * L + l, r = c / C;
+        if (r < old || r >= end) continue;
+        float f[8];
+        Io<T>::unpack(x[i], f);
+        u32x2 w = {codes4(f, s, r1), codes4(f + 4, s, r1)};
+        if (!fine) w = u32x2{0, 0};
+        *(u32x2*)(pool.row(page, h, row + r) + 8 * (c % C)) = w;
+      }
+      if (old > 0 && s > before && fine) {
+        for (int i = 0; i < N; ++i) {
+          const int c = i * L + l, r = c / C;
+          if (r >= old) continue;
+          u32x2* to = (u32x2*)(pool.row(page, h, row + r) + 8 * (c % C));
+          u32x2 w = *to;
+          float f[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) f[e] = (float)(int8_t)(w[e / 4] >> 8 * (e % 4)) * before;
+          *to = u32x2{codes4(f, s, r1), codes4(f + 4, s, r1)};
+        }
+      }
+      if (l == 0) *scale = s;
+    }
+  }
+}
+
+template <NormType T, int C> hipError_t run_append(const AppendParams& p, hipStream_t s) {
+  const int64_t blocks = ((int64_t)p.T + 2 * p.block - 2) / p.block;   // of a sequence, at most
+  auto go = [&](auto kern, int lanes) {
+    const int64_t tasks = blocks * p.heads, per = kThreads / lanes;
+    const dim3 grid((unsigned)std::min<int64_t>((tasks + per - 1) / per, 1 << 20), (unsigned)std::min(p.B, 65535), 2);
+    hipLaunchKernelGGL(kern, grid, dim3(kThreads), 0, s, p);
+    return hipGetLastError();
+  };
+  const int chunks = p.block * C;
+  if (p.block == 1) return go(append_i8<T, C, C, 1>, C);
+  if (chunks <= 64) return go(append_i8<T, C, 64, 1>, 64);
+  if (chunks <= 128) return go(append_i8<T, C, 64, 2>, 64);
+  if (chunks <= 256) return go(append_i8<T, C, 64, 4>, 64);
+  if (chunks <= 512) return go(append_i8<T, C, 64, 8>, 64);
+  if (chunks <= 1024) return go(append_i8<T, C, 256, 4>, 256);
+  if (chunks <= 2048) return go(append_i8<T, C, 256, 8>, 256);
+  if (chunks <= 4096) return go(append_i8<T, C, 256, 16>, 256);
+  return hipErrorNotSupported;
+}
+
+// ---- read --------------------------------------------------------------------
+
+struct ReadParams {
+  PagedView view;
+  Pool8 pool[2];
+  uint8_t* out[2];
+  int64_t sb[2], sh[2], st[2];   // bytes
+  const int* first;
+  PageDiv by_heads, by_block;
+  int B, T, heads;
+};
+
+// 8 codes times their scale; what is past the type's range is its largest value. zero: 0,
+// or NaN for a scale that is none.
+template <NormType T> __device__ __forceinline__ void put8(uint8_t* to, u32x2 w, float s, float zero) {
+  constexpr float kMost = T == NormType::F16 ? 65504.0f : T == NormType::BF16 ? 0x1.fep127f : __FLT_MAX__;
+  float f[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e)
+    f[e] = fminf(fmaxf((float)(int8_t)(w[e / 4] >> 8 * (e % 4)) * s, -kMost), kMost) + zero;
+#pragma unroll
+  for (int i = 0; i < 8 / Io<T>::kVec; ++i) ((u32x4*)to)[i] = Io<T>::pack(f + i * Io<T>::kVec);
+}
+
+// U rows of a key and a value to a thread's chunk, all loaded before the first is stored.
+template <NormType T, int C>
+__global__ __launch_bounds__(kThreads) void read_i8(ReadParams p) {
+  constexpr int R = kThreads / C, U = 4;
+  constexpr int E = T == NormType::F32 ? 4 : 2;
+  const int c = threadIdx.x % C, first = threadIdx.x / C;
+  const int rows = p.T * p.heads;
+  for (int b = blockIdx.y; b < p.B; b += gridDim.y) {
+    const int len = clamp_length(p.view.lengths[b], p.view.room);
+    const int64_t from = p.first ? max(0, p.first[b]) : 0;
+    for (int64_t r0 = (int64_t)blockIdx.x * R * U; r0 < rows; r0 += (int64_t)gridDim.x * R * U) {
+      u32x2 w[2][U];
+      float s[2][U];
+      int t[U], h[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int r = (int)min<int64_t>(r0 + u * R + first, rows - 1);
+        t[u] = div_page(p.by_heads, r);
+        h[u] = r - t[u] * p.heads;
+        const int64_t slot = from + t[u];
+        int page, row;
+        const bool there = find_slot(p.view, b, (int)min<int64_t>(slot, max(len - 1, 0)), &page, &row) & (slot < len);
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          w[x][u] = u32x2{0, 0};
+          s[x][u] = 0.0f;
+          if (there) {
+            w[x][u] = __builtin_nontemporal_load((const u32x2*)(p.pool[x].row(page, h[u], row) + 8 * c));
+            s[x][u] = *p.pool[x].scale_of(page, h[u], div_page(p.by_block, row));
+          }
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (r0 + u * R + first >= rows) break;
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          uint8_t* to = p.out[x] + b * p.sb[x] + h[u] * p.sh[x] + t[u] * p.st[x];
+          put8<T>(to + 8 * E * c, w[x][u], s[x][u], s[x][u] * 0.0f);
+        }
+      }
+    }
+  }
+}
+
+template <NormType T, int C> hipError_t run_read(const ReadParams& p, hipStream_t s) {
+  const int64_t rows = (int64_t)p.T * p.heads, per = kThreads / C * 4;
+  const dim3 grid((unsigned)std::min<int64_t>((rows + per - 1) / per, 1 << 20), (unsigned)std::min(p.B, 65535));
+  hipLaunchKernelGGL((read_i8<T, C>), grid, dim3(kThreads), 0, s, p);
+  return hipGetLastError();
+}
+
+}  // namespace
+
+hipError_t launch_paged_append_i8(AttnType t, const PagedAppendDesc& d, const QuantScales& q, hipStream_t s) {
+  AppendParams p{};
+  p.view = view_of(d.c);
+  p.pool[0] = pool_of(d.c, q, false);
+  p.pool[1] = pool_of(d.c, q, true);
+  p.rows[0] = {(const uint8_t*)d.k, 2 * d.k_sb, 2 * d.k_sh, 2 * d.k_st};
+  p.rows[1] = {(const uint8_t*)d.v, 2 * d.v_sb, 2 * d.v_sh, 2 * d.v_st};
+  p.counts = d.counts;
+  p.by_heads = page_div(d.c.heads);
+  p.by_block = page_div(q.block);
+  p.B = d.c.B; p.T = d.T; p.heads = d.c.heads; p.block = q.block;
+  if (t == AttnType::BF16) {
+    if (d.c.D == 128) return run_append<NormType::BF16, 16>(p, s);
+    if (d.c.D == 64) return run_append<NormType::BF16, 8>(p, s);
+  } else {
+    if (d.c.D == 128) return run_append<NormType::F16, 16>(p, s);
+    if (d.c.D == 64) return run_append<NormType::F16, 8>(p, s);
+  }
+  return hipErrorNotSupported;
+}
+
+hipError_t launch_paged_read_i8(NormType t, const PagedReadDesc& d, const QuantScales& q, hipStream_t s) {
+  ReadParams p{};
+  const int size = t == NormType::F32 ? 4 : 2;
+  p.view = view_of(d.c);
+  p.pool[0] = pool_of(d.c, q, false);
+  p.pool[1] = pool_of(d.c, q, true);
+  p.out[0] = (uint8_t*)d.k; p.sb[0] = size * d.k_sb; p.sh[0] = size * d.k_sh; p.st[0] = size * d.k_st;
+  p.out[1] = (uint8_t*)d.v; p.sb[1] = size * d.v_sb; p.sh[1] = size * d.v_sh; p.st[1] = size * d.v_st;
+  p.first = d.first;
+  p.by_heads = page_div(d.c.heads);
+  p.by_block = page_div(q.block);
+  p.B = d.c.B; p.T = d.T; p.heads = d.c.heads;
+  if (d.c.D != 64 && d.c.D != 128) return hipErrorNotSupported;
+  const bool wide = d.c.D == 128;
+  switch (t) {
+    case NormType::BF16: return wide ? run_read<NormType::BF16, 16>(p, s) : run_read<NormType::BF16, 8>(p, s);
+    case NormType::F16:  return wide ? run_read<NormType::F16, 16>(p, s) : run_read<NormType::F16, 8>(p, s);
+    case NormType::F32:  return wide ? run_read<NormType::F32, 16>(p, s) : run_read<NormType::F32, 8>(p, s);
+  }
+  return hipErrorNotSupported;
+}
+
+}  // namespace grxk

@@ -189,6 +189,23 @@ struct PagedAppendDesc {
 };
 hipError_t launch_paged_append(const PagedAppendDesc& d, hipStream_t s);
 
+// The scales of a cache in 8 bits: one for each `block` slots of a head's keys and values.
+struct QuantScales {
+  float* k;
+  float* v;
+  int64_t sp, sh, sb;                        // strides (elements) of page, head, block
+  int block;
+};
+hipError_t launch_paged_append_i8(AttnType t, const PagedAppendDesc& d, const QuantScales& q, hipStream_t s);
+struct PagedReadDesc {
+  PagedCache c;
+  void* k; int64_t k_sb, k_sh, k_st;         // rows [B, heads, T, D]
+  void* v; int64_t v_sb, v_sh, v_st;
+  int T;
+  const int* first;                          // may be null: 0
+};
+hipError_t launch_paged_read_i8(NormType t, const PagedReadDesc& d, const QuantScales& q, hipStream_t s);
+
 struct PagedAttnDesc {
   PagedCache c;
   int H;                                     // query heads, a multiple of c.heads

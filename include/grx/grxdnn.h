@@ -362,6 +362,61 @@ grxdnnStatus_t grxdnnPagedCacheEvict(grxdnnHandle_t handle,
                                      int* newLengths,
                                      grxdnnTensorDescriptor_t newWeightsDesc, float* newWeights);
 
+/* ---- paged key-value cache in 8 bits ----------------------------------------
+ *
+ * The cache above with pools of GRX_R_8I codes: half the memory and half of what
+ * attention reads. A code c of a block of slots stands for c * scale of the block:
+ * scales are GRX_R_32F [pages, Hkv, N], any strides, N a divisor of P, so that row r of
+ * a page belongs to block r / (P / N) (N = P: a scale for each slot; 1: one for the
+ * page's). kScale and vScale are of one descriptor. Blocks have 1 .. 256 slots (else
+ * NOT_SUPPORTED). The pools' strides but the last are multiples of 16 elements; what
+ * is said above of tables, lengths, entries and overlaps holds, and D is 64 or 128.
+ * (New: planned by ref docs/designs/grxcp_roadmap.md:864-877, "attention".) */
+
+/* New rows behind the tokens that the cache holds, as grxdnnPagedCacheAppend puts
+ * them, in 8 bits. For every block of every head that gets rows, keys and values each:
+ *   need   = the least number of 8 significant bits (and at least 2^-126) that is not
+ *            below max |x| / 127 over the block's new rows; 0 where all are 0, NaN where
+ *            one is infinite or NaN
+ *   scale' = max(scale, need) where the block holds rows of the sequence already
+ *            (NaN if one of the two is), else need: what scale held before is not looked at
+ *   code   = x / scale' to the nearest whole number, ties to the even one
+ * and, where scale' > scale, the codes of rows that it holds already become code *
+ * scale / scale', rounded so. Where scale' is 0 or not finite the new rows' codes are 0 and
+ * the others stay: with NaN the whole block reads as NaN until it is begun anew. Rows
+ * behind the new ones are left as they are.
+ * Slots of a block that another sequence shares must not be followed by rows of this
+ * call (they would be rounded again): share whole blocks.
+ * k, v: [B, Hkv, T, D], GRX_R_16BF or GRX_R_16F, counts as in grxdnnPagedCacheAppend;
+ * (T + 512) * Hkv below 2^31. Scales that the caller sets are finite and >= 0. */
+grxdnnStatus_t grxdnnPagedCacheAppendQuantized(grxdnnHandle_t handle,
+                                               grxdnnTensorDescriptor_t kDesc, const void* k,
+                                               grxdnnTensorDescriptor_t vDesc, const void* v,
+                                               grxdnnTensorDescriptor_t kCacheDesc, void* kCache,
+                                               grxdnnTensorDescriptor_t vCacheDesc, void* vCache,
+                                               grxdnnTensorDescriptor_t scaleDesc, float* kScale,
+                                               float* vScale,
+                                               grxdnnTensorDescriptor_t tableDesc, const int* table,
+                                               const int* lengths, const int* counts);
+
+/* Rows of such a cache: for every sequence b, head h and t < T,
+ *   k[b, h, t, :] = scale * code of slot first[b] + t      (and v)
+ * and 0 where that slot is at or past lengths[b] or on a page that does not exist.
+ * first: B ints (below 0 counts as 0), or NULL for 0 each. k, v: [B, Hkv, T, D] of
+ * GRX_R_16BF, GRX_R_16F or GRX_R_32F, strides multiples of 16 bytes, T * Hkv at most
+ * 2^31 - 4096; rounded once; what is past the type's range comes back as its largest
+ * value. A prompt's next chunk attends to them (grxdnnAttentionForward), or they go into
+ * a cache of 16 bits. */
+grxdnnStatus_t grxdnnPagedCacheReadQuantized(grxdnnHandle_t handle,
+                                             grxdnnTensorDescriptor_t kCacheDesc, const void* kCache,
+                                             grxdnnTensorDescriptor_t vCacheDesc, const void* vCache,
+                                             grxdnnTensorDescriptor_t scaleDesc, const float* kScale,
+                                             const float* vScale,
+                                             grxdnnTensorDescriptor_t tableDesc, const int* table,
+                                             const int* lengths, const int* first,
+                                             grxdnnTensorDescriptor_t kDesc, void* k,
+                                             grxdnnTensorDescriptor_t vDesc, void* v);
+
 /* ---- log probabilities of tokens ---------------------------------------------
  * x: logits [..., V] under softmax's layout rules and types (rows flatten to one
  * row stride; GRX_R_16BF, GRX_R_16F, GRX_R_32F; V = 1 .. 2^24). For row r of the R:
