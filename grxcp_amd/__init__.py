@@ -156,6 +156,8 @@ _DNN = {
     "grxdnnPagedCacheEvict": (c_int, [c_void_p] * 10 + [c_int, c_int] + [c_void_p] * 6),
     "grxdnnPagedCacheAppendQuantized": (c_int, [c_void_p] * 16),
     "grxdnnPagedCacheReadQuantized": (c_int, [c_void_p] * 16),
+    "grxdnnPagedAttentionQuantizedGetWorkspaceSize": (c_int, [c_void_p] * 4 + [POINTER(c_size_t)]),
+    "grxdnnPagedAttentionQuantizedForward": (c_int, [c_void_p] * 17 + [c_size_t]),
     "grxdnnTokenLogProbGetWorkspaceSize": (c_int, [c_void_p, c_void_p, c_int, POINTER(c_size_t)]),
     "grxdnnTokenLogProbForward": (c_int, [c_void_p] * 7 + [c_int, c_void_p, c_void_p, c_void_p, c_size_t]),
     "grxdnnTokenLogProbBackward": (c_int, [c_void_p] * 10),
@@ -449,6 +451,17 @@ class Dnn:
         """first: each sequence's first slot to read, or None for 0."""
         return self.L.grxdnnPagedCacheReadQuantized(self.h, kcd.d, kc, vcd.d, vc, sd.d, ks, vs, td.d, table, lengths,
                                                     first, kd.d, k, vd.d, v)
+
+    def paged_attention_quantized_workspace(self, qd, kcd, td) -> int:
+        n = c_size_t(0)
+        check(self.L.grxdnnPagedAttentionQuantizedGetWorkspaceSize(self.h, qd.d, kcd.d, td.d, ctypes.byref(n)),
+              "paged attention workspace")
+        return n.value
+
+    def paged_attention_quantized(self, ad, qd, q, kcd, kc, vcd, vc, sd, ks, vs, td, table, lengths, od, o, ws,
+                                  ws_bytes) -> int:
+        return self.L.grxdnnPagedAttentionQuantizedForward(self.h, ad.d, qd.d, q, kcd.d, kc, vcd.d, vc, sd.d, ks, vs,
+                                                           td.d, table, lengths, od.d, o, ws, ws_bytes)
 
     def token_logprob_workspace(self, xd, top: int) -> int:
         n = c_size_t(0)

@@ -42,6 +42,7 @@ HOST_FLAGS = ["-O2", "-std=c++17", "-fPIC", "-fvisibility=hidden", "-Wall", "-We
 EXTRA = {
     "kernels/attention.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
     "kernels/paged_attention.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
+    "kernels/paged_attention_i8.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
 }
 
 LIBS = {
@@ -51,7 +52,7 @@ LIBS = {
     "libgrxdnn.so": (["grxdnn.cpp", "kernels/norms.hip", "kernels/softmax_gelu.hip",
                       "kernels/attention.hip", "kernels/paged_cache.hip",
                       "kernels/paged_cache_i8.hip",
-                      "kernels/paged_attention.hip", "kernels/token_logprob.hip",
+                      "kernels/paged_attention.hip", "kernels/paged_attention_i8.hip", "kernels/token_logprob.hip",
                       "kernels/qk_norm_rope.hip"], ["grxrt"]),
 }
 

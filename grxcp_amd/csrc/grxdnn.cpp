@@ -1142,6 +1142,77 @@ grxdnnStatus_t grxdnnPagedCacheReadQuantized(grxdnnHandle_t handle, grxdnnTensor
   return from_hip(grxk::launch_paged_read_i8(nt, d, q, handle->stream));
 }
 
+grxdnnStatus_t grxdnnPagedAttentionQuantizedGetWorkspaceSize(grxdnnHandle_t handle, grxdnnTensorDescriptor_t qDesc,
+                                                             grxdnnTensorDescriptor_t kCacheDesc,
+                                                             grxdnnTensorDescriptor_t tableDesc, size_t* bytes) {
+  if (!handle) return GRXDNN_STATUS_NOT_INITIALIZED;
+  if (!qDesc || !qDesc->set || !bytes) return GRXDNN_STATUS_INVALID_VALUE;
+  grxk::PagedCache c{};
+  const grxdnnStatus_t s = paged_cache(kCacheDesc, kCacheDesc, tableDesc, false, &c, true);
+  if (s != GRXDNN_STATUS_SUCCESS) return s;
+  if (qDesc->nb != 4 || qDesc->dims[0] != c.B || qDesc->dims[1] < 1 || qDesc->dims[1] % c.heads != 0 ||
+      qDesc->dims[3] != c.D)
+    return GRXDNN_STATUS_INVALID_VALUE;
+  *bytes = c.B == 0 ? 0 : grxk::paged_attention_i8_workspace(c, qDesc->dims[1]);
+  return GRXDNN_STATUS_SUCCESS;
+}
+
+grxdnnStatus_t grxdnnPagedAttentionQuantizedForward(grxdnnHandle_t handle, grxdnnAttentionDescriptor_t attnDesc,
+                                                    grxdnnTensorDescriptor_t qDesc, const void* q,
+                                                    grxdnnTensorDescriptor_t kCacheDesc, const void* kCache,
+                                                    grxdnnTensorDescriptor_t vCacheDesc, const void* vCache,
+                                                    grxdnnTensorDescriptor_t scaleDesc, const float* kScale,
+                                                    const float* vScale, grxdnnTensorDescriptor_t tableDesc,
+                                                    const int* table, const int* lengths,
+                                                    grxdnnTensorDescriptor_t oDesc, void* o, void* workspace,
+                                                    size_t workspaceBytes) {
+  if (!handle) return GRXDNN_STATUS_NOT_INITIALIZED;
+  if (!attnDesc || !qDesc || !oDesc || !attnDesc->set || !qDesc->set || !oDesc->set)
+    return GRXDNN_STATUS_INVALID_VALUE;
+  grxk::PagedAttnDesc d{};
+  grxk::QuantScales scales{};
+  grxdnnStatus_t s = paged_cache(kCacheDesc, vCacheDesc, tableDesc, false, &d.c, true);
+  if (s != GRXDNN_STATUS_SUCCESS) return s;
+  s = quant_scales(scaleDesc, d.c, false, &scales);
+  if (s != GRXDNN_STATUS_SUCCESS) return s;
+  if (qDesc->nb != 4 || !same_shape(*qDesc, *oDesc) || qDesc->dims[0] != d.c.B || qDesc->dims[1] < 1 ||
+      qDesc->dims[1] % d.c.heads != 0 || qDesc->dims[3] != d.c.D)
+    return GRXDNN_STATUS_INVALID_VALUE;
+  if (!half_type(qDesc->type) || oDesc->type != qDesc->type) return GRXDNN_STATUS_NOT_SUPPORTED;
+  d.H = qDesc->dims[1];
+  // one query per sequence; (sequence, query head) pairs are counted in 32 bits
+  if (qDesc->dims[2] != 1 || d.H / d.c.heads > 1024 || (int64_t)d.c.B * d.H > INT_MAX / 4)
+    return GRXDNN_STATUS_NOT_SUPPORTED;
+  if (d.c.B == 0) return GRXDNN_STATUS_SUCCESS;
+  if (!half_rows(*qDesc) || !half_rows(*oDesc)) return GRXDNN_STATUS_NOT_SUPPORTED;
+  if (!no_overlap(*oDesc)) return GRXDNN_STATUS_INVALID_VALUE;
+  if (!q || !kCache || !vCache || !kScale || !vScale || !table || !lengths || !o) return GRXDNN_STATUS_INVALID_VALUE;
+  if (!grxk::paged_attention_i8_fits(d.c, d.H)) return GRXDNN_STATUS_NOT_SUPPORTED;
+  const size_t need = grxk::paged_attention_i8_workspace(d.c, d.H);
+  if (workspaceBytes < need || (need && !workspace)) return GRXDNN_STATUS_INVALID_VALUE;
+  const Operand out{oDesc, o, 0}, room{nullptr, need ? workspace : nullptr, (int64_t)need}, query{qDesc, q, 0};
+  const Operand all[] = {out, room,
+                         // only read from here on
+                         {kCacheDesc, kCache, 0}, {vCacheDesc, vCache, 0}, {scaleDesc, kScale, 0},
+                         {scaleDesc, vScale, 0}, {tableDesc, table, 0}, {nullptr, lengths, 4ll * d.c.B}};
+  if (shared_by_written(all, 8, 2) || share(room, query) || (share(out, query) && !in_place(out, query)))
+    return GRXDNN_STATUS_INVALID_VALUE;
+  if (!aligned16(q) || !aligned16(kCache) || !aligned16(vCache) || !aligned16(o) ||
+      (need && !aligned16(workspace)))
+    return GRXDNN_STATUS_NOT_SUPPORTED;
+  s = ensure_device(*handle);
+  if (s != GRXDNN_STATUS_SUCCESS) return s;
+  d.c.k = const_cast<void*>(kCache); d.c.v = const_cast<void*>(vCache);
+  d.c.table = table; d.c.lengths = lengths;
+  scales.k = const_cast<float*>(kScale); scales.v = const_cast<float*>(vScale);
+  d.scale = attnDesc->scale;
+  d.q = q; d.q_sb = qDesc->strides[0]; d.q_sh = qDesc->strides[1];
+  d.o = o; d.o_sb = oDesc->strides[0]; d.o_sh = oDesc->strides[1];
+  d.ws = workspace;
+  return from_hip(grxk::launch_paged_attention_i8(
+      qDesc->type == GRX_R_16BF ? grxk::AttnType::BF16 : grxk::AttnType::F16, d, scales, handle->stream));
+}
+
 grxdnnStatus_t grxdnnTokenLogProbGetWorkspaceSize(grxdnnHandle_t handle, grxdnnTensorDescriptor_t xDesc,
                                                   int topCount, size_t* bytes) {
   if (!handle) return GRXDNN_STATUS_NOT_INITIALIZED;

@@ -82,46 +82,9 @@ __global__ __launch_bounds__(64 * kWaves, (wgs_per_cu<D, NT>())) void decode_spl
   const int tid = threadIdx.x, lane = tid & 63, l16 = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
 
-  // The share: sequence b, item `it` of it, from unit `i` on, `left` units.
-  uint32_t b = 0, it = 0, i = 0, share = blockIdx.x, left;
-  // Lengths of the first 64 sequences stay in the lanes; the others' are read again.
-  const int len64 = lane < p.B ? clamp_length(p.view.lengths[lane], p.view.room) : 0;
-  if (p.whole) {
-    b = blockIdx.x / p.items;
-    it = blockIdx.x - b * p.items;
-    left = 1;
-  } else {
-    const uint32_t first64 = lane < p.B ? units_of(p, len64) : 0;
-    uint32_t total = first64;
-    for (int x = lane + 64; x < p.B; x += 64) total += units_of(p, clamp_length(p.view.lengths[x], p.view.room));
-    const Shares sh = shares(p, wave_total(total) * p.items);
-    if (blockIdx.x >= sh.n) return;
-    // Neighbouring shares go to one XCD (workgroups are dealt over the eight in turn).
-    if (sh.n == p.wgs) share = (blockIdx.x & 7) * (p.wgs >> 3) + (blockIdx.x >> 3);
-    const uint32_t u0 = sh.begin(share);
-    left = sh.begin(share + 1) - u0;
-    uint32_t base = 0;               // units of the sequences before this 64
-    for (int b0 = 0;; b0 += 64) {
-      const uint32_t mine = b0 == 0 ? first64
-                            : b0 + lane < p.B ? units_of(p, clamp_length(p.view.lengths[b0 + lane], p.view.room)) : 0;
-      const uint32_t upto = wave_upto(mine);
-      const uint64_t past = __ballot((base + upto) * p.items > u0);
-      if (past) {                    // u0 < total: some sequence ends past it
-        const int at = __ffsll((unsigned long long)past) - 1;
-        b = b0 + at;
-        const uint32_t n = (uint32_t)__builtin_amdgcn_readlane((int)mine, at);
-        const uint32_t first = (base + (uint32_t)__builtin_amdgcn_readlane((int)upto, at) - n) * p.items;
-        it = (u0 - first) / n;
-        i = (u0 - first) - it * n;
-        break;
-      }
-      base += (uint32_t)__builtin_amdgcn_readlane((int)upto, 63);
-    }
-  }
-  b = __builtin_amdgcn_readfirstlane(b);
-  it = __builtin_amdgcn_readfirstlane(it);
-  i = __builtin_amdgcn_readfirstlane(i);
-  left = __builtin_amdgcn_readfirstlane(left);
+  uint32_t b, it, i, share, left;
+  int len64;
+  if (!find_share(p, lane, b, it, i, share, left, len64)) return;
 
   uint8_t* vt = smem + wave * 2 * kStage * 16;
   const int kk = lane & 31;
@@ -332,40 +295,7 @@ __global__ __launch_bounds__(64 * kWaves, (wgs_per_cu<D, NT>())) void decode_spl
         ml[wave][1][l16] = sum;
       }
       __syncthreads();
-      constexpr int E = D / 16;      // values of a thread, of 16 to a row
-      const int r = tid >> 4, d0 = (tid & 15) * E;
-      const int row = 16 * t + r;    // in the tile
-      if (q0 + row >= p.group) continue;
-      for (int y = 0; y < p.hw; ++y) {
-        float top = -INFINITY;
-        for (int x = y * of; x < (y + 1) * of; ++x) top = fmaxf(top, ml[x][0][r]);
-        float lsum = 0.0f, acc[E];
-#pragma unroll
-        for (int e = 0; e < E; ++e) acc[e] = 0.0f;
-        for (int x = y * of; x < (y + 1) * of; ++x) {
-          const float f = __builtin_amdgcn_exp2f(ml[x][0][r] - fmaxf(top, kLowest));
-          lsum = fmaf(f, ml[x][1][r], lsum);
-#pragma unroll
-          for (int e = 0; e < E; ++e) acc[e] = fmaf(f, mo[(x * 16 + r) * kPitch + d0 + e], acc[e]);
-        }
-        const int64_t at = (part * p.hw + y) * p.rows + row;
-        if (whole) {
-          const float inv = top == -INFINITY ? 0.0f : 1.0f / lsum;   // no slot: 0; only -inf scores: 0 * inf
-          uint32_t out[E / 2];
-#pragma unroll
-          for (int e = 0; e < E / 2; ++e) out[e] = IO::pack2(acc[2 * e] * inv, acc[2 * e + 1] * inv);
-          uint8_t* to = p.o + (int64_t)b * p.o_sb + ((hg * p.hw + y) * p.group + q0 + row) * p.o_sh + 2 * d0;
-          if constexpr (E == 8) *(u32x4*)to = u32x4{out[0], out[1], out[2], out[3]};
-          else *(u32x2*)to = u32x2{out[0], out[1]};
-        } else {
-#pragma unroll
-          for (int e = 0; e < E; e += 4) *(f32x4*)(p.po + at * D + d0 + e) = f32x4{acc[e], acc[e + 1], acc[e + 2], acc[e + 3]};
-        }
-        if (d0 == 0 && (!whole || p.scores)) {
-          p.ml[2 * at] = top;
-          p.ml[2 * at + 1] = lsum;
-        }
-      }
+      meet<T, D>(p, tid, of, hg, q0, 16 * t, b, part, whole, mo, ml);
     }
     wait_all();
     __syncthreads();                 // the tiles' LDS is free again

@@ -1,0 +1,481 @@
+// grxDNN attention of one new token per sequence over a paged key-value cache in 8 bits,
+// on gfx950.
+//
+// New: the reference plans attention for grxDNN (ref
+// docs/designs/grxcp_roadmap.md:864-877) and ships no code.
+//
+// The work is divided as over a cache of 16 bits (paged_attention.hip): units of a tile for
+// each of a workgroup's four waves, shares of equal size, parts joined in the order of the
+// slots. Half the bytes, so a wave's tile has 64 slots, 16 KB of codes again. What differs:
+//
+//  * scores are S^T = K Q^T on the 8-bit matrix cores (v_mfma_i32_16x16x64_i8): the codes of
+//    K go in as they lie, with no conversion. A query's row is held as whole numbers of 23
+//    bits of its largest value in three digits of base 256 (-128 .. 127), so a product
+//    takes three instructions and is exact: what is lost is the rounding of q to 2^-22 of
+//    the row's largest value. The slot's scale multiplies the sum;
+//  * O^T += V^T P^T on the fp16 matrix cores: the transposing LDS read of bytes brings 8
+//    slots of a value's dimension, and a code c becomes fp16 exactly, as the last bits of
+//    1024 + (c + 128) less 1152. The weights carry the slots' scales, relative to a power of
+//    two R not below any the wave has seen, and are split in two fp16 numbers;
+//  * a lane finds page, row and both scales of one slot of the tile, and hands them to the
+//    others through LDS.
+
+#include "paged_split.h"
+
+#include <cstdio>
+
+namespace grxk {
+namespace {
+
+// Slots of a wave's tile: with two tiles of query heads half as many, for the registers.
+template <int NT> constexpr int tile() { return NT == 1 ? 64 : 32; }
+
+struct QParams {
+  DParams d;                              // pools' strides in 16-byte chunks of codes
+  const float* ks; const float* vs;
+  int64_t cp, ch, cb;                     // the scales' strides
+  PageDiv by_block;
+};
+
+template <int D, int NT> constexpr int wgs_per_cu() { return 2; }
+
+// 16-byte chunk of a V row in LDS: chunk ^ vswz(row). The 8 rows of a transposing read (4g ..
+// 4g + 3 and 16 + 4g .. 16 + 4g + 3) touch every bank of 128 bytes once.
+template <int D> __device__ __forceinline__ int vswz(int row) {
+  if constexpr (D == 128) return (row & 3) | (row >> 2 & 4);
+  else return (row >> 1 & 1) | (row >> 3 & 2);
+}
+
+typedef int i32x2 __attribute__((ext_vector_type(2)));
+typedef __attribute__((address_space(3))) i32x2* lds_i32x2_t;
+
+// 8 codes as fp16.
+__device__ __forceinline__ i32x4 to_half(i32x2 w) {
+  typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+  i32x4 r;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t u = (uint32_t)w[i / 2] ^ 0x80808080u;
+    const uint32_t h = __builtin_amdgcn_perm(0x64646464u, u, i % 2 ? 0x04030402u : 0x04010400u);
+    r[i] = __builtin_bit_cast(int, __builtin_bit_cast(f16x2, h) - f16x2{1152.0f, 1152.0f});
+  }
+  return r;
+}
+
+// 4 values x, |x| scale < 2^22, as whole numbers in digits of base 256: the digits' bytes.
+struct Digits { int d[3]; };            // the first is the highest
+__device__ __forceinline__ Digits digits4(const float* x, float scale) {
+  uint32_t m[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)            // + 1.5 * 2^23 rounds; + 0x8080 makes the lower two unsigned
+    m[i] = __float_as_uint(fmaf(x[i], scale, 12582912.0f)) + (0x8080u - 0x400000u);
+  const uint32_t a = __builtin_amdgcn_perm(m[1], m[0], 0x05010400u), b = __builtin_amdgcn_perm(m[3], m[2], 0x05010400u);
+  const uint32_t c = __builtin_amdgcn_perm(m[1], m[0], 0x0c0c0602u), d = __builtin_amdgcn_perm(m[3], m[2], 0x0c0c0602u);
+  return {(int)__builtin_amdgcn_perm(d, c, 0x05040100u), (int)(__builtin_amdgcn_perm(b, a, 0x07060302u) ^ 0x80808080u),
+          (int)(__builtin_amdgcn_perm(b, a, 0x05040100u) ^ 0x80808080u)};
+}
+
+// 1 / x of a power of two, 2^-126 .. 2^126.
+__device__ __forceinline__ float inverse(float x) { return __uint_as_float((254u << 23) - __float_as_uint(x)); }
+
+template <AttnType T> __device__ __forceinline__ void unpack8(u32x4 w, float* f) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (T == AttnType::BF16) {
+      f[2 * i] = __uint_as_float(w[i] << 16);
+      f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    } else {
+      f[2 * i] = f16_to_f32((uint16_t)w[i]);
+      f[2 * i + 1] = f16_to_f32((uint16_t)(w[i] >> 16));
+    }
+  }
+}
+
+template <AttnType T, int D, int NT, bool ONCE>
+__global__ __launch_bounds__(64 * kWaves, (wgs_per_cu<D, NT>())) void decode_split_i8(QParams qp) {
+  using W = PIo<AttnType::F16>;      // the weights' type
+  constexpr float kUnscale = 0x1p-11f;
+  static_assert(W::kTop == 11.0f);
+  const DParams& p = qp.d;
+  constexpr int kTile = tile<NT>();
+  constexpr int F = D / 64;          // contraction steps of a score
+  constexpr int DT = D / 16;         // tiles of the head dimension
+  constexpr int CH = D / 16;         // chunks of a row
+  constexpr int RPI = 64 / CH;       // V rows per load
+  constexpr int KT = kTile / 16;     // tiles of 16 slots
+  constexpr int kStage = kTile * CH; // chunks of a V tile
+  constexpr int kPitch = D + 4;
+  constexpr int kV = kWaves * 2 * kStage * 16, kMerge = kWaves * 16 * kPitch * 4;
+  __shared__ __attribute__((aligned(1024))) uint8_t smem[kV > kMerge ? kV : kMerge];
+  __shared__ uint64_t rows[kWaves][2][kTile];
+  __shared__ __attribute__((aligned(16))) float scales[kWaves][2][kTile];
+  __shared__ float ml[kWaves][2][16];
+
+  const int tid = threadIdx.x, lane = tid & 63, l16 = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+
+  uint32_t b, it, i, share, left;
+  int len64;
+  if (!find_share(p, lane, b, it, i, share, left, len64)) return;
+
+  uint8_t* vt = smem + wave * 2 * kStage * 16;
+  const int of = kWaves / p.hw;      // waves of a key head
+  const int hd = wave / of, sub = wave - hd * of;
+
+  while (left > 0) {
+    const int len = b < 64 ? __builtin_amdgcn_readlane(len64, b)
+                           : __builtin_amdgcn_readfirstlane(clamp_length(p.view.lengths[b], p.view.room));
+    const uint32_t n = units_of(p, len);
+    if (p.whole) left = n;
+    const uint32_t take = min(left, n - i);
+    const int hg = (int)it / p.gtiles, q0 = ((int)it - hg * p.gtiles) * 16 * NT;   // first query head of the group
+    const int h = hg * p.hw + hd;                                       // the wave's key head
+    const int* table = p.view.table + (int64_t)b * p.view.table_rs;
+    const uint8_t* kbase = p.k + 16ull * h * p.k_sh;
+    const uint8_t* vbase = p.v + 16ull * h * p.v_sh;
+
+    f32x4 o[NT][DT];
+    float m[NT], l[NT];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      m[t] = -INFINITY;              // no slot yet
+      l[t] = 0.0f;
+#pragma unroll
+      for (int d = 0; d < DT; ++d) o[t][d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+    float R = 0x1p-126f;             // o is in units of it
+
+    i32x4 kf[2][KT][F];
+    float ksr[2], vsr[2];            // the scales of the lane's slot
+    uint64_t live[2];
+    const int step = 1 << p.shift;
+    int key = (int)(i << p.shift) + sub * kTile;                        // the wave's first slot
+    const int end = (int)min((uint32_t)len, (i + take) << p.shift);
+    auto entry = [&](int key0) __attribute__((always_inline)) {
+      const int j = key0 + lane;
+      return lane < kTile && j < end ? table[div_page(p.view.div, j)] : -1;
+    };
+    // Loads of the tile at key0, whose table entries are e, into buffer BUF.
+    auto issue = [&](auto buf, int key0, int e) __attribute__((always_inline)) {
+      constexpr int BUF = decltype(buf)::value;
+      const int j = key0 + lane;
+      const int page = lane < kTile && j < end ? checked_page(e, p.view.pages) : -1;
+      const int row = j - div_page(p.view.div, j) * p.view.page;
+      const bool there = page >= 0;
+      const uint64_t pg = (uint32_t)page, r64 = (uint32_t)row;
+      if (lane < kTile) {
+        rows[wave][0][lane] = (uint64_t)(there ? kbase + 16 * (pg * p.k_sp + r64 * p.k_ss) : (const uint8_t*)zero_row);
+        rows[wave][1][lane] = (uint64_t)(there ? vbase + 16 * (pg * p.v_sp + r64 * p.v_ss) : (const uint8_t*)zero_row);
+      }
+      live[BUF] = __ballot(there);
+      ksr[BUF] = vsr[BUF] = 0.0f;
+      if (there) {
+        const int64_t at = page * qp.cp + h * qp.ch + div_page(qp.by_block, row) * qp.cb;
+        ksr[BUF] = qp.ks[at];
+        vsr[BUF] = qp.vs[at];
+      }
+      __builtin_amdgcn_wave_barrier();
+#pragma unroll
+      for (int kt = 0; kt < KT; ++kt) {
+        const uint8_t* src = (const uint8_t*)rows[wave][0][16 * kt + l16] + 16 * g;
+#pragma unroll
+        for (int f = 0; f < F; ++f) {
+          if constexpr (ONCE) kf[BUF][kt][f] = __builtin_nontemporal_load((const i32x4*)(src + 64 * f));
+          else kf[BUF][kt][f] = *(const i32x4*)(src + 64 * f);
+        }
+      }
+#pragma unroll
+      for (int x = 0; x < kTile / RPI; ++x) {
+        const int r = RPI * x + lane / CH;
+        const uint8_t* src = (const uint8_t*)rows[wave][1][r] + 16 * ((lane % CH) ^ vswz<D>(r));
+        dma16<ONCE>(src, lds_addr(vt + (BUF * kStage + 64 * x) * 16));
+      }
+    };
+    int e = entry(key);
+    int next = entry(key + step);
+
+    u32x4 raw[NT][F][2];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      const int r = q0 + 16 * t + l16;
+      const uint8_t* src = r < p.group ? p.q + (int64_t)b * p.q_sb + (h * p.group + r) * p.q_sh : (const uint8_t*)zero_row;
+#pragma unroll
+      for (int f = 0; f < F; ++f)
+#pragma unroll
+        for (int x = 0; x < 2; ++x) raw[t][f][x] = *(const u32x4*)(src + 2 * (64 * f + 16 * g + 8 * x));
+    }
+    if (key < end) issue(Buf<0>{}, key, e);
+    // The queries' digits, and what a sum of them stands for.
+    i32x4 qd[NT][3][F];
+    float unit[NT];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      float top = 0.0f, odd = 0.0f;
+#pragma unroll
+      for (int f = 0; f < F; ++f)
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          float v[8];
+          unpack8<T>(raw[t][f][x], v);
+#pragma unroll
+          for (int u = 0; u < 8; ++u) {
+            top = fmaxf(top, fabsf(v[u]));
+            odd = fmaf(v[u], 0.0f, odd);         // NaN where a value is not finite
+          }
+        }
+      top = over_query(top, [](float a, float x) { return fmaxf(a, x); });
+      odd = over_query(odd, [](float a, float x) { return a + x; });
+      // 2^e <= top < 2^(e+1): top * 2^(21-e) is below 2^22
+      const int e = min(max((int)(__float_as_uint(top) >> 23), 127 - 105), 254) - 127;
+      const float scale = __uint_as_float((uint32_t)(127 + 21 - e) << 23);
+      unit[t] = __uint_as_float((uint32_t)(127 - 21 + e) << 23) * p.c + odd;
+#pragma unroll
+      for (int f = 0; f < F; ++f)
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          float v[8];
+          unpack8<T>(raw[t][f][x / 2], v);
+          const Digits q = digits4(v + x % 2 * 4, scale);
+#pragma unroll
+          for (int y = 0; y < 3; ++y) qd[t][y][f][x] = q.d[y];
+        }
+    }
+
+    auto compute = [&](auto buf) __attribute__((always_inline)) {
+      constexpr int BUF = decltype(buf)::value;
+      const uint64_t mask = live[BUF];
+      if (!mask) return;                         // nothing to add
+      if (__ballot(!(vsr[BUF] <= R))) {
+        const uint32_t top = __float_as_uint(fmaxf(wave_max(vsr[BUF]), 0.0f));
+        const float up = __uint_as_float(min((top + 0x7fffffu) & 0x7f800000u, 0x7e800000u));
+        if (up > R) {
+          const float f = R * inverse(up);
+          R = up;
+#pragma unroll
+          for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int d = 0; d < DT; ++d) o[t][d] *= f;
+        }
+      }
+      if (lane < kTile) {
+        scales[wave][0][lane] = ksr[BUF];
+        scales[wave][1][lane] = vsr[BUF] * inverse(R);
+      }
+      __builtin_amdgcn_wave_barrier();
+      i32x4 pf[NT][KT / 2], pr[NT][KT / 2];      // the weights: leading bits, rest
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        f32x4 s[KT];
+#pragma unroll
+        for (int kt = 0; kt < KT; ++kt) {
+          i32x4 a[3];
+#pragma unroll
+          for (int x = 0; x < 3; ++x) {
+            a[x] = i32x4{0, 0, 0, 0};
+#pragma unroll
+            for (int f = 0; f < F; ++f)
+              a[x] = __builtin_amdgcn_mfma_i32_16x16x64_i8(kf[BUF][kt][f], qd[t][x][f], a[x], 0, 0, 0);
+          }
+          const f32x4 by = *(const f32x4*)&scales[wave][0][16 * kt + 4 * g];
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            s[kt][r] = fmaf(fmaf((float)a[0][r], 256.0f, (float)a[1][r]), 256.0f, (float)a[2][r]) * (by[r] * unit[t]);
+        }
+        if (mask != (kTile == 64 ? ~0ull : 0xffffffffull)) {
+#pragma unroll
+          for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+              if (!(mask >> (16 * kt + 4 * g + r) & 1)) s[kt][r] = -INFINITY;
+        }
+        float mx = s[0][0];
+#pragma unroll
+        for (int x = 1; x < 4 * KT; ++x) mx = fmaxf(mx, s[x / 4][x % 4]);
+        mx = over_query(mx, [](float a, float x) { return fmaxf(a, x); });
+        mx = fmaxf(mx, kLowest);     // -inf scores weigh 0; a row of only such has l = 0 and is NaN
+        const bool raise = mx - m[t] > kLazy;
+        if (__ballot(raise)) {
+          const float top = raise ? mx : m[t];
+          const float alpha = raise ? __builtin_amdgcn_exp2f(m[t] - top) : 1.0f;
+          m[t] = top;
+          l[t] *= alpha;
+#pragma unroll
+          for (int d = 0; d < DT; ++d) o[t][d] *= alpha;
+        }
+#pragma unroll
+        for (int kt = 0; kt < KT; ++kt) {
+          const f32x4 by = *(const f32x4*)&scales[wave][1][16 * kt + 4 * g];
+          float w[4];
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            w[r] = __builtin_amdgcn_exp2f((s[kt][r] - m[t]) + W::kTop);
+            l[t] += w[r];
+            w[r] *= by[r];
+          }
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            int a, b;
+            W::split2(w[2 * x], w[2 * x + 1], a, b);
+            pf[t][kt / 2][kt % 2 * 2 + x] = a;
+            pr[t][kt / 2][kt % 2 * 2 + x] = b;
+          }
+        }
+      }
+      const uint8_t* v0 = vt + BUF * kStage * 16;
+      const int in = l16 >> 1;                   // the lane's row of a transposing read
+      const int r0 = in < 4 ? 4 * g + in : 12 + 4 * g + in;
+#pragma unroll
+      for (int d = 0; d < DT; ++d) {
+        i32x4 vf[KT / 2];
+#pragma unroll
+        for (int x = 0; x < KT / 2; ++x) {
+          const int r = 32 * x + r0;
+          vf[x] = to_half(__builtin_amdgcn_ds_read_tr8_b64_v2i32(
+              (lds_i32x2_t)(v0 + r * D + 16 * (d ^ vswz<D>(r)) + 8 * (lane & 1))));
+        }
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+          for (int x = 0; x < KT / 2; ++x) o[t][d] = W::mma(vf[x], pf[t][x], o[t][d]);
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+          for (int x = 0; x < KT / 2; ++x) o[t][d] = W::mma(vf[x], pr[t][x], o[t][d]);
+      }
+    };
+    while (key < end) {
+      wait_all();
+      if (key + step < end) {
+        issue(Buf<1>{}, key + step, next);
+        next = entry(key + 2 * step);
+      }
+      compute(Buf<0>{});
+      key += step;
+      if (key >= end) break;
+      wait_all();
+      if (key + step < end) {
+        issue(Buf<0>{}, key + step, next);
+        next = entry(key + 2 * step);
+      }
+      compute(Buf<1>{});
+      key += step;
+    }
+
+    // The results of a key head's waves meet: 16 query heads at a time.
+    const bool whole = take == n;
+    const int64_t part = p.whole ? share : (int64_t)b * p.items + it + share;
+    float* mo = (float*)smem;
+    const float back = R * kUnscale;
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      wait_all();
+      __syncthreads();               // every wave is done with its tiles, or with the rows before
+#pragma unroll
+      for (int d = 0; d < DT; ++d) *(f32x4*)&mo[(wave * 16 + l16) * kPitch + 16 * d + 4 * g] = o[t][d] * back;
+      const float sum = over_query(l[t], [](float a, float x) { return a + x; }) * kUnscale;
+      if (g == 0) {
+        ml[wave][0][l16] = m[t];
+        ml[wave][1][l16] = sum;
+      }
+      __syncthreads();
+      meet<T, D>(p, tid, of, hg, q0, 16 * t, b, part, whole, mo, ml);
+    }
+    wait_all();
+    __syncthreads();                 // the tiles' LDS is free again
+
+    left -= take;
+    i = 0;
+    if (++it == p.items) {
+      it = 0;
+      ++b;
+    }
+  }
+}
+
+// ---- launch --------------------------------------------------------------------
+
+Plan plan_of(int B, int H, int heads, int D, int W, int page, bool neighbours) {
+  Plan x{};
+  const int group = H / heads;
+  x.nt = group > 16 ? 2 : 1;
+  x.gtiles = (group + 16 * x.nt - 1) / (16 * x.nt);
+  x.rows = std::min(group, 16 * x.nt);
+  x.room = (int64_t)W * page;
+  x.slots = (x.room + 255) / 256 * 256;
+  const int64_t each = (int64_t)B * heads * x.gtiles;
+  x.whole = (x.room <= 256 || (x.room <= 512 && each >= 128)) && each <= (1 << 20);
+  x.hw = 1;
+  if (!x.whole && neighbours)
+    for (int hw = 4; hw > 1 && x.hw == 1; hw /= 2)
+      if (heads % hw == 0 && (int64_t)B * (heads / hw) * x.gtiles >= 64) x.hw = hw;
+  x.items = (int64_t)B * (heads / x.hw) * x.gtiles;
+  x.wgs = x.whole ? (int)x.items : 2 * compute_units();
+  const size_t parts = x.whole ? (size_t)x.items : (size_t)x.items + x.wgs;
+  if (!x.whole) x.ml = (parts * x.hw * x.rows * 2 + 3) / 4 * 4;
+  if (!x.whole) x.po = parts * x.hw * x.rows * D;
+  return x;
+}
+
+template <AttnType T, int D>
+hipError_t run(const PagedAttnDesc& d, const QuantScales& q, hipStream_t s) {
+  const Plan x = plan_of(d.c.B, d.H, d.c.heads, D, d.c.W, d.c.page, neighbours(d.c.k_sh, d.c.k_ss));
+  QParams qp{};
+  DParams& p = qp.d;
+  p.view = {d.c.table, d.c.table_rs, d.c.lengths, d.c.pages, d.c.page, d.c.W * d.c.page, page_div(d.c.page)};
+  p.k = (const uint8_t*)d.c.k; p.k_sp = d.c.k_sp / 16; p.k_sh = d.c.k_sh / 16; p.k_ss = d.c.k_ss / 16;
+  p.v = (const uint8_t*)d.c.v; p.v_sp = d.c.v_sp / 16; p.v_sh = d.c.v_sh / 16; p.v_ss = d.c.v_ss / 16;
+  p.q = (const uint8_t*)d.q; p.q_sb = 2 * d.q_sb; p.q_sh = 2 * d.q_sh;
+  p.o = (uint8_t*)d.o; p.o_sb = 2 * d.o_sb; p.o_sh = 2 * d.o_sh;
+  float* ws = (float*)d.ws;
+  p.ml = ws;
+  p.po = ws + x.ml;
+  p.slots = x.slots;
+  p.B = d.c.B; p.H = d.H; p.heads = d.c.heads; p.group = d.H / d.c.heads;
+  p.hw = x.hw; p.shift = (x.nt == 1 ? 6 : 5) + (x.hw == 4 ? 0 : x.hw == 2 ? 1 : 2);
+  p.gtiles = x.gtiles; p.items = d.c.heads / x.hw * x.gtiles; p.rows = x.rows; p.wgs = x.wgs; p.whole = x.whole;
+  p.c = d.scale * 1.4426950408889634f;
+  qp.ks = q.k; qp.vs = q.v;
+  qp.cp = q.sp; qp.ch = q.sh; qp.cb = q.sb;
+  qp.by_block = page_div(q.block);
+  if (log_dnn_launches())
+    std::fprintf(stderr, "grxdnn: paged attention i8 %s b=%d h=%d hkv=%d d=%d page=%d block=%d room=%d kernel=%s%d\n",
+                 T == AttnType::BF16 ? "bf16" : "f16", p.B, p.H, p.heads, D, p.view.page, q.block, p.view.room,
+                 x.whole ? "whole" : "split", x.hw);
+  const dim3 grid(x.wgs), threads(64 * kWaves);
+  auto go = [&](auto kern) { hipLaunchKernelGGL(kern, grid, threads, 0, s, qp); };
+  if (x.nt == 1) go(decode_split_i8<T, D, 1, true>);
+  else if (x.gtiles == 1) go(decode_split_i8<T, D, 2, true>);
+  else go(decode_split_i8<T, D, 2, false>);
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess || x.whole) return e;
+  const JoinPlan j = join_plan(x, p.B, p.H, p.heads, false);
+  hipLaunchKernelGGL((decode_join<T, D>), dim3((unsigned)j.jobs, (unsigned)std::min(p.B, 65535)), dim3(256), 0, s, p,
+                     (uint32_t)j.outs, j.apiece, (uint32_t)j.chunks);
+  return hipGetLastError();
+}
+
+}  // namespace
+
+size_t paged_attention_i8_workspace(const PagedCache& c, int H) {
+  const Plan x = plan_of(c.B, H, c.heads, c.D, c.W, c.page, neighbours(c.k_sh, c.k_ss));
+  return (x.ml + x.po) * sizeof(float);
+}
+
+bool paged_attention_i8_fits(const PagedCache& c, int H) {
+  const Plan x = plan_of(c.B, H, c.heads, c.D, c.W, c.page, neighbours(c.k_sh, c.k_ss));
+  return (double)x.items * (x.slots / 32) < 0x1p31 &&
+         join_plan(x, c.B, H, c.heads, false).jobs <= max_workgroups(256);
+}
+
+hipError_t launch_paged_attention_i8(AttnType t, const PagedAttnDesc& d, const QuantScales& q, hipStream_t s) {
+  if (t == AttnType::BF16) {
+    if (d.c.D == 128) return run<AttnType::BF16, 128>(d, q, s);
+    if (d.c.D == 64) return run<AttnType::BF16, 64>(d, q, s);
+  } else {
+    if (d.c.D == 128) return run<AttnType::F16, 128>(d, q, s);
+    if (d.c.D == 64) return run<AttnType::F16, 64>(d, q, s);
+  }
+  return hipErrorNotSupported;
+}
+
+}  // namespace grxk

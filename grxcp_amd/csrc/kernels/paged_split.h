@@ -121,6 +121,53 @@ __device__ __forceinline__ Shares shares(const DParams& p, uint32_t total) {
   return s;
 }
 
+// The workgroup's share: sequence b, item `it` of it, from unit `i` on, `left` units. False:
+// it has none. Lengths of the first 64 sequences stay in the lanes (len64); the others' are
+// read again.
+__device__ __forceinline__ bool find_share(const DParams& p, int lane, uint32_t& b, uint32_t& it, uint32_t& i,
+                                           uint32_t& share, uint32_t& left, int& len64) {
+  b = it = i = 0;
+  share = blockIdx.x;
+  len64 = lane < p.B ? clamp_length(p.view.lengths[lane], p.view.room) : 0;
+  if (p.whole) {
+    b = blockIdx.x / p.items;
+    it = blockIdx.x - b * p.items;
+    left = 1;
+  } else {
+    const uint32_t first64 = lane < p.B ? units_of(p, len64) : 0;
+    uint32_t total = first64;
+    for (int x = lane + 64; x < p.B; x += 64) total += units_of(p, clamp_length(p.view.lengths[x], p.view.room));
+    const Shares sh = shares(p, wave_total(total) * p.items);
+    if (blockIdx.x >= sh.n) return false;
+    // Neighbouring shares go to one XCD (workgroups are dealt over the eight in turn).
+    if (sh.n == p.wgs) share = (blockIdx.x & 7) * (p.wgs >> 3) + (blockIdx.x >> 3);
+    const uint32_t u0 = sh.begin(share);
+    left = sh.begin(share + 1) - u0;
+    uint32_t base = 0;               // units of the sequences before this 64
+    for (int b0 = 0;; b0 += 64) {
+      const uint32_t mine = b0 == 0 ? first64
+                            : b0 + lane < p.B ? units_of(p, clamp_length(p.view.lengths[b0 + lane], p.view.room)) : 0;
+      const uint32_t upto = wave_upto(mine);
+      const uint64_t past = __ballot((base + upto) * p.items > u0);
+      if (past) {                    // u0 < total: some sequence ends past it
+        const int at = __ffsll((unsigned long long)past) - 1;
+        b = b0 + at;
+        const uint32_t n = (uint32_t)__builtin_amdgcn_readlane((int)mine, at);
+        const uint32_t first = (base + (uint32_t)__builtin_amdgcn_readlane((int)upto, at) - n) * p.items;
+        it = (u0 - first) / n;
+        i = (u0 - first) - it * n;
+        break;
+      }
+      base += (uint32_t)__builtin_amdgcn_readlane((int)upto, 63);
+    }
+  }
+  b = __builtin_amdgcn_readfirstlane(b);
+  it = __builtin_amdgcn_readfirstlane(it);
+  i = __builtin_amdgcn_readfirstlane(i);
+  left = __builtin_amdgcn_readfirstlane(left);
+  return true;
+}
+
 // ---- loads and lanes -----------------------------------------------------------
 
 __device__ __forceinline__ void wait_all() {
@@ -145,6 +192,49 @@ template <class Op> __device__ __forceinline__ float over_query(float v, Op op) 
   v = op(__uint_as_float(a[0]), __uint_as_float(a[1]));
   const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
   return op(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+
+// The results of a workgroup's waves, of which `of` share a key head, for 16 query heads:
+// O rows [wave][16][D + 4] in mo, maxima and sums in ml. To o where `whole`, else to `part`.
+template <AttnType T, int D>
+__device__ __forceinline__ void meet(const DParams& p, int tid, int of, int hg, int q0, int row0, uint32_t b,
+                                     int64_t part, bool whole, const float* mo, const float (*ml)[2][16]) {
+  using IO = PIo<T>;
+  constexpr int kPitch = D + 4;
+        constexpr int E = D / 16;      // values of a thread, of 16 to a row
+        const int r = tid >> 4, d0 = (tid & 15) * E;
+        const int row = row0 + r;      // in the tile
+        if (q0 + row >= p.group) return;
+        for (int y = 0; y < p.hw; ++y) {
+          float top = -INFINITY;
+          for (int x = y * of; x < (y + 1) * of; ++x) top = fmaxf(top, ml[x][0][r]);
+          float lsum = 0.0f, acc[E];
+  #pragma unroll
+          for (int e = 0; e < E; ++e) acc[e] = 0.0f;
+          for (int x = y * of; x < (y + 1) * of; ++x) {
+            const float f = __builtin_amdgcn_exp2f(ml[x][0][r] - fmaxf(top, kLowest));
+            lsum = fmaf(f, ml[x][1][r], lsum);
+  #pragma unroll
+            for (int e = 0; e < E; ++e) acc[e] = fmaf(f, mo[(x * 16 + r) * kPitch + d0 + e], acc[e]);
+          }
+          const int64_t at = (part * p.hw + y) * p.rows + row;
+          if (whole) {
+            const float inv = top == -INFINITY ? 0.0f : 1.0f / lsum;   // no slot: 0; only -inf scores: 0 * inf
+            uint32_t out[E / 2];
+  #pragma unroll
+            for (int e = 0; e < E / 2; ++e) out[e] = IO::pack2(acc[2 * e] * inv, acc[2 * e + 1] * inv);
+            uint8_t* to = p.o + (int64_t)b * p.o_sb + ((hg * p.hw + y) * p.group + q0 + row) * p.o_sh + 2 * d0;
+            if constexpr (E == 8) *(u32x4*)to = u32x4{out[0], out[1], out[2], out[3]};
+            else *(u32x2*)to = u32x2{out[0], out[1]};
+          } else {
+  #pragma unroll
+            for (int e = 0; e < E; e += 4) *(f32x4*)(p.po + at * D + d0 + e) = f32x4{acc[e], acc[e + 1], acc[e + 2], acc[e + 3]};
+          }
+          if (d0 == 0 && (!whole || p.scores)) {
+            p.ml[2 * at] = top;
+            p.ml[2 * at + 1] = lsum;
+          }
+        }
 }
 
 // ---- the join ------------------------------------------------------------------

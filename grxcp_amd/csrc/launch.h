@@ -224,6 +224,11 @@ size_t paged_attention_workspace(const PagedCache& c, int H, bool weights);
 // workgroups fit a launch.
 bool paged_attention_fits(const PagedCache& c, int H, bool weights);
 
+// The same over a cache in 8 bits, without the slots' weights.
+hipError_t launch_paged_attention_i8(AttnType t, const PagedAttnDesc& d, const QuantScales& q, hipStream_t s);
+size_t paged_attention_i8_workspace(const PagedCache& c, int H);
+bool paged_attention_i8_fits(const PagedCache& c, int H);
+
 struct PagedEvictDesc {
   PagedCache c;
   const float* weights; int64_t w_sb, w_sh;

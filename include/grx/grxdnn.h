@@ -417,6 +417,31 @@ grxdnnStatus_t grxdnnPagedCacheReadQuantized(grxdnnHandle_t handle,
                                              grxdnnTensorDescriptor_t kDesc, void* k,
                                              grxdnnTensorDescriptor_t vDesc, void* v);
 
+/* Attention of one new token per sequence over such a cache: grxdnnPagedAttentionForward
+ * without weights, with the slots' codes times their scales for keys and values.
+ * q, o: [B, H, 1, D], GRX_R_16BF or GRX_R_16F; its rules and limits hold. A query's row is
+ * taken to 2^-22 of its largest value (or to 2^-127), products with the codes are
+ * exact, scores, softmax and sums fp32, the weights of the values keep 21 bits, and o is
+ * rounded once. A row of q with NaN or infinities in it gives NaN, and so does a head
+ * of a sequence with a scale of NaN among its slots' blocks. Values' scales up to 2^95.
+ * workspace: as there, of grxdnnPagedAttentionQuantizedGetWorkspaceSize. */
+grxdnnStatus_t grxdnnPagedAttentionQuantizedGetWorkspaceSize(grxdnnHandle_t handle,
+                                                             grxdnnTensorDescriptor_t qDesc,
+                                                             grxdnnTensorDescriptor_t kCacheDesc,
+                                                             grxdnnTensorDescriptor_t tableDesc,
+                                                             size_t* bytes);
+grxdnnStatus_t grxdnnPagedAttentionQuantizedForward(grxdnnHandle_t handle,
+                                                    grxdnnAttentionDescriptor_t attnDesc,
+                                                    grxdnnTensorDescriptor_t qDesc, const void* q,
+                                                    grxdnnTensorDescriptor_t kCacheDesc, const void* kCache,
+                                                    grxdnnTensorDescriptor_t vCacheDesc, const void* vCache,
+                                                    grxdnnTensorDescriptor_t scaleDesc, const float* kScale,
+                                                    const float* vScale,
+                                                    grxdnnTensorDescriptor_t tableDesc, const int* table,
+                                                    const int* lengths,
+                                                    grxdnnTensorDescriptor_t oDesc, void* o,
+                                                    void* workspace, size_t workspaceBytes);
+
 /* ---- log probabilities of tokens ---------------------------------------------
  * x: logits [..., V] under softmax's layout rules and types (rows flatten to one
  * row stride; GRX_R_16BF, GRX_R_16F, GRX_R_32F; V = 1 .. 2^24). For row r of the R:

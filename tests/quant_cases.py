@@ -34,10 +34,11 @@ def over(x, s):
 class QuantCache:
     """Pools of codes and scales. Every slot that holds no token has code 77, every block that
     holds none the scale `unset` (NaN: what no call may look at). One page more on either
-    side. Sequences begin with lengths[b] rows of normal values, appended by `append_ref`."""
+    side. Sequences begin with lengths[b] rows of normal values, appended by `append_ref`, or
+    (quick) of any codes and scales."""
 
     def __init__(self, gen, lengths, heads, page, block, d, tokmajor=False, room=None, spare=3, unset=math.nan,
-                 dtype=torch.bfloat16, scale=1.0):
+                 dtype=torch.bfloat16, scale=1.0, quick=False):
         b = len(lengths)
         self.heads, self.page, self.block, self.d = heads, page, block, d
         self.width = max(1, -(-max([room or 0, *lengths]) // page))
@@ -49,8 +50,13 @@ class QuantCache:
         self.pools = [torch.full(shape, 77, dtype=I8) for _ in range(2)]
         self.scales = [torch.full((total + 2, heads, page // block), unset) for _ in range(2)]
         self.n = [0] * b
-        new = [torch.randn((b, heads, max([*lengths, 1]), d), generator=gen).mul(scale).to(dtype) for _ in range(2)]
         self.cuda(tokmajor)
+        if quick:
+            self.n = list(lengths)
+            self.fill(gen, scale)
+            self.lengths = ints(self.n)
+            return
+        new = [torch.randn((b, heads, max([*lengths, 1]), d), generator=gen).mul(scale).to(dtype) for _ in range(2)]
         self.lengths = ints(self.n)
         want = self.append_ref(*new, lengths)
         self.store(*want)
@@ -65,6 +71,20 @@ class QuantCache:
         self.k, self.v = (p[1:-1] for p in self.guarded)
         self.ks, self.vs = (s[1:-1] for s in self.guarded_scales)
         del self.pools, self.scales
+
+    def fill(self, gen, scale):
+        """Codes of normal values and scales around them for every slot that holds a token."""
+        k, v, ks, vs = self.state()
+        table = self.table.cpu()
+        for i, n in enumerate(self.n):
+            at = torch.arange(n)
+            page, row = table[i, at // self.page].long(), at % self.page
+            for pool, scales in ((k, ks), (v, vs)):
+                rows = torch.randn((n, self.heads, self.d), generator=gen).mul(36).round().clamp(-127, 127)
+                pool[page, :, row] = rows.to(I8)
+                by = torch.randn((n, self.heads), generator=gen).mul(0.3).exp().mul(3 * scale / 127)
+                scales[page, :, row // self.block] = by
+        self.store(k, v, ks, vs)
 
     def store(self, k, v, ks, vs):
         for to, x in ((self.k, k), (self.v, v), (self.ks, ks), (self.vs, vs)):
@@ -141,3 +161,45 @@ def read(dnn, c, k, v, first=None):
     g.check(dnn.paged_read_quantized(*c.args(), None if first is None else first.data_ptr(), desc(k), k.data_ptr(),
                                      desc(v), v.data_ptr()), "read")
     torch.cuda.synchronize()
+
+
+def attend(dnn, c, q, o, scale, expect=g.SUCCESS):
+    from paged_cases import Workspace
+    args = c.args()
+    qd, od = desc(q), desc(o)
+    ws = Workspace(dnn.paged_attention_quantized_workspace(qd, args[0], args[7]))
+    st = dnn.paged_attention_quantized(g.AttnDesc(True, scale), qd, q.data_ptr(), *args, od, o.data_ptr(), ws.p, ws.size)
+    assert st == expect, g.STATUS[st]
+    torch.cuda.synchronize()
+
+
+def attention_ref(q, K, V, scale, there=None):
+    """o of one sequence and the bound on its error: q [H, d], K and V [heads, n, d] in 64 bits
+    (host), there: which slots are.
+
+    A query's value is off by at most 2^-22 of its row's largest one, a product with a code is
+    exact, three fp32 roundings join the digits, three more the scales (softmaxScale * log2 e, the
+    slot's, their product): a score is off by 2^-22 max|q| sum|k| and 8 half steps of sum |q k|, and
+    e^x moves by that much, relatively. 2^-18 covers exp2, the fp32 sums and rescalings and the
+    division. The weights keep 21 bits, but at least 2^-24 of 2^-11 of the largest scale of a
+    value (and a power of two above); o is rounded once."""
+    H, d = q.shape
+    heads, n, _ = K.shape
+    group = H // heads
+    live = torch.ones(n, dtype=torch.bool) if there is None else there
+    k, v = (x.repeat_interleave(group, 0)[:, live] for x in (K, V))
+    if not k.shape[1]:
+        zero = torch.zeros(H, d, dtype=torch.float64)
+        return zero, zero
+    q64 = q.double()
+    s = torch.matmul(k, q64[:, :, None])[..., 0] * scale
+    p = torch.softmax(s, 1)
+    o = torch.matmul(p[:, None], v)[:, 0]
+    size = torch.matmul(k.abs(), q64.abs()[:, :, None])[..., 0]
+    off = 2.0 ** -22 * q64.abs().amax(1, keepdim=True) * k.abs().sum(2)
+    delta = (off + 8 * 2.0 ** -24 * size).amax(1, keepdim=True) * scale
+    rel = 2 * delta + 2.0 ** -18 + 2.0 ** -20
+    u = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}[q.dtype]
+    mass = torch.matmul(p[:, None], v.abs())[:, 0]
+    floor = k.shape[1] * 2.0 ** -34 * 2 * v.abs().amax((1, 2))[:, None]
+    return o, u * o.abs() + (1 + u) * (rel * mass + floor) + (2.0 ** -25 if q.dtype == torch.float16 else 0.0)

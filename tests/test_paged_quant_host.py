@@ -1,4 +1,6 @@
 """The 8-bit paged cache's entry points without a GPU: argument checks."""
+import ctypes
+
 import pytest
 
 import grxcp_amd as g
@@ -36,6 +38,14 @@ def read(dnn, **kw):
     assert set(kw) <= set(a)
     a.update(kw)
     return dnn.paged_read_quantized(*a.values())
+
+
+def attend(dnn, size=1 << 24, **kw):
+    a = dict(ad=g.AttnDesc(True, 0.125), qd=T(BF16, [3, 8, 1, 64]), q=at(1), **cache(), od=T(BF16, [3, 8, 1, 64]),
+             o=at(2), ws=at(10))
+    assert set(kw) <= set(a)
+    a.update(kw)
+    return dnn.paged_attention_quantized(*a.values(), size)
 
 
 BOTH = (append, read)
@@ -134,3 +144,68 @@ def test_overlaps_are_refused(dnn):
         for p in (1, 2, 3, 4, 5, 6, 7, 8, 9):
             if (n, p) not in (("k", 1), ("v", 2)):
                 assert read(dnn, **{n: at(p)}) == INVALID, (n, p)
+
+
+# ---- attention -----------------------------------------------------------------
+
+@needs_no_gpu
+def test_valid_attention_calls_reach_the_device_check(dnn):
+    assert attend(dnn) == OK and attend(dnn, ad=g.AttnDesc(False, 0.125)) == OK
+    half = T(F16, [3, 8, 1, 64])
+    assert attend(dnn, qd=half, od=half) == OK
+    tok = T(I8, POOL, [4096, 64, 256, 1])
+    assert attend(dnn, kcd=tok, vcd=tok) == OK
+    row = T(BF16, [3, 8, 1, 64], [1536, 64, 1536, 1])
+    assert attend(dnn, qd=row, od=row) == OK and attend(dnn, qd=row, od=row, o=at(1)) == OK
+    many = T(BF16, [3, 4096, 1, 64])
+    assert attend(dnn, qd=many, od=many, size=1 << 40) == OK
+    assert attend(dnn, td=T(I32, TABLE, [0, 1])) == OK and attend(dnn, vc=at(3), vs=at(5)) == OK
+
+
+def test_refused_attention_calls(dnn):
+    d = g.Dnn()
+    h, d.h = d.h, None
+    assert attend(d) == g.NOT_INITIALIZED
+    d.h = h
+    d.close()
+    for n in ("ad", "qd", "kcd", "vcd", "sd", "td", "od"):
+        if n != "ad":
+            assert attend(dnn, **{n: Unset()}) == INVALID, n
+        assert attend(dnn, **{n: Null()}) == INVALID, n
+    for n in ("q", "kc", "vc", "ks", "vs", "table", "lengths", "o"):
+        assert attend(dnn, **{n: None}) == INVALID, n
+    for h in (0, 6):
+        assert attend(dnn, qd=T(BF16, [3, h, 1, 64]), od=T(BF16, [3, h, 1, 64])) == INVALID
+    assert attend(dnn, od=T(BF16, [3, 4, 1, 64])) == INVALID
+    assert attend(dnn, qd=T(BF16, [2, 8, 1, 64]), od=T(BF16, [2, 8, 1, 64])) == INVALID
+    assert attend(dnn, sd=T(F32, [40, 4, 3])) == INVALID and attend(dnn, vcd=T(I8, [41, 4, 16, 64])) == INVALID
+    assert attend(dnn, od=T(F16, [3, 8, 1, 64])) == UNSUPPORTED
+    assert attend(dnn, qd=T(F32, [3, 8, 1, 64]), od=T(F32, [3, 8, 1, 64])) == UNSUPPORTED
+    assert attend(dnn, kcd=T(BF16, POOL), vcd=T(BF16, POOL)) == UNSUPPORTED
+    assert attend(dnn, qd=T(BF16, [3, 8, 2, 64]), od=T(BF16, [3, 8, 2, 64])) == UNSUPPORTED
+    wide = T(BF16, [3, 4100, 1, 64])
+    assert attend(dnn, qd=wide, od=wide, size=1 << 40) == UNSUPPORTED
+    for n in ("q", "kc", "vc", "o", "ws"):
+        assert attend(dnn, **{n: at(20) + 8}) == UNSUPPORTED or dnn.paged_attention_quantized_workspace(
+            T(BF16, [3, 8, 1, 64]), T(I8, POOL), T(I32, TABLE)) == 0, n
+    assert attend(dnn, od=T(BF16, [3, 8, 1, 64], [0, 64, 64, 1])) == INVALID
+    none = T(BF16, [0, 8, 1, 64])
+    assert attend(dnn, qd=none, od=none, td=T(I32, [0, 8]), q=None) == g.SUCCESS
+    for p in (3, 4, 5, 6, 7, 8):
+        assert attend(dnn, o=at(p)) == INVALID, p
+    assert attend(dnn, o=at(1) + 128) == INVALID
+    # a table long enough for shares
+    far = dict(td=T(I32, [3, 400]))
+    need = dnn.paged_attention_quantized_workspace(T(BF16, [3, 8, 1, 64]), T(I8, POOL), far["td"])
+    assert need > 0 and attend(dnn, **far, size=need - 1) == INVALID and attend(dnn, **far, ws=None) == INVALID
+    assert attend(dnn, **far, ws=at(10) + 4) == UNSUPPORTED
+    for p in range(1, 9):
+        assert attend(dnn, **far, ws=at(p)) == INVALID, p
+    L, out = g.load().dnn, ctypes.c_size_t()
+    ask = L.grxdnnPagedAttentionQuantizedGetWorkspaceSize
+    q, pool, table = T(BF16, [3, 8, 1, 64]), T(I8, POOL), T(I32, TABLE)
+    assert ask(None, q.d, pool.d, table.d, ctypes.byref(out)) == g.NOT_INITIALIZED
+    assert ask(dnn.h, q.d, pool.d, table.d, None) == INVALID
+    assert ask(dnn.h, None, pool.d, table.d, ctypes.byref(out)) == INVALID
+    assert ask(dnn.h, T(BF16, [3, 6, 1, 64]).d, pool.d, table.d, ctypes.byref(out)) == INVALID
+    assert ask(dnn.h, q.d, T(BF16, POOL).d, table.d, ctypes.byref(out)) == UNSUPPORTED
