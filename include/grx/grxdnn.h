@@ -194,7 +194,8 @@ int            grxdnnAttentionCycleSlotsNeeded(grxdnnHandle_t handle, int batch,
  *
  * Sums and products are fp32 and y is rounded once; angles are reduced from the
  * whole product (64 bits and its remainder), for |angle| < 2^40. A row whose sum
- * of squares exceeds fp32's range is scaled by 0. Outputs must not share elements
+ * of squares exceeds fp32's range is scaled by 0; mean(x^2) + eps is to be 2^-126 or
+ * more (a row of zeros with eps 0 is NaN, as in the formula). Outputs must not share elements
  * of their own or with each other or with what the call reads, but yq may be q
  * and yk k (same pointer and strides); else INVALID_VALUE.
  * (New: planned by ref docs/designs/grxcp_roadmap.md:864-877.) */
