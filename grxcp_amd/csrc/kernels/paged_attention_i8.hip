@@ -17,8 +17,22 @@
 //    slots of a value's dimension, and a code c becomes fp16 exactly, as the last bits of
 //    1024 + (c + 128) less 1152. The weights carry the slots' scales, relative to a power of
 //    two R not below any the wave has seen, and are split in two fp16 numbers;
+//  * a group of up to 4 (8) query heads leaves 12 (8) of a product's 16 columns empty. They
+//    get the same queries again, and each set of columns goes on with a quarter (half) of
+//    the tile's slots: the softmax is done once for every score. In the product with V a
+//    set's weights of the others' slots are 0, and the sets' results are added at the end;
 //  * a lane finds page, row and both scales of one slot of the tile, and hands them to the
 //    others through LDS.
+//
+// us, 32 query and 8 key heads of 128, bf16, a scale for 16 slots: 48 sequences of 33 to 4096
+// slots 51.9 (3.9 TB/s; the join 5), 48 of 8000 142 (5.5), 64 of 800 28.8, one of 201 7.5; 2 of
+// 131072 with 4 key heads, a scale each, 54 (5.1). What a call has above its bytes (6.3 TB/s
+// from one length to the next) are 11 us: launch, lengths, table, queries and the first tile
+// one after the other, and the join. Loads alone, without scales and products, take 48 of the
+// 52 that the batch took; 2 of them the sets of columns saved, 0.5 the digits made while the
+// first tile comes. Rows of K loaded by 8 neighbours together (128 bytes), each row as two of
+// the product's, were faster in few tiles (48 of 500 17.4 for 18.8) and slower in many (55.5
+// for 54.0 in the long ones).
 
 #include "paged_split.h"
 
@@ -37,8 +51,6 @@ struct QParams {
   PageDiv by_block;
 };
 
-template <int D, int NT> constexpr int wgs_per_cu() { return 2; }
-
 // 16-byte chunk of a V row in LDS: chunk ^ vswz(row). The 8 rows of a transposing read (4g ..
 // 4g + 3 and 16 + 4g .. 16 + 4g + 3) touch every bank of 128 bytes once.
 template <int D> __device__ __forceinline__ int vswz(int row) {
@@ -46,6 +58,9 @@ template <int D> __device__ __forceinline__ int vswz(int row) {
   else return (row >> 1 & 1) | (row >> 3 & 2);
 }
 
+// Addresses come out of LDS, and the compiler takes a pointer that does for one of any memory:
+// such a load would hold up every later LDS access until it is back.
+typedef const __attribute__((address_space(1))) i32x4* global_i32x4_t;
 typedef int i32x2 __attribute__((ext_vector_type(2)));
 typedef __attribute__((address_space(3))) i32x2* lds_i32x2_t;
 
@@ -78,6 +93,13 @@ __device__ __forceinline__ Digits digits4(const float* x, float scale) {
 // 1 / x of a power of two, 2^-126 .. 2^126.
 __device__ __forceinline__ float inverse(float x) { return __uint_as_float((254u << 23) - __float_as_uint(x)); }
 
+// op over the sets of a group of 16 lanes, in each.
+template <int SETS, class Op> __device__ __forceinline__ float over_sets(float v, Op op) {
+  if constexpr (SETS >= 2) v = op(v, dpp_f<0x128>(v));   // row_ror 8
+  if constexpr (SETS >= 4) v = op(v, dpp_f<0x124>(v));   // row_ror 4
+  return v;
+}
+
 template <AttnType T> __device__ __forceinline__ void unpack8(u32x4 w, float* f) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -91,8 +113,8 @@ template <AttnType T> __device__ __forceinline__ void unpack8(u32x4 w, float* f)
   }
 }
 
-template <AttnType T, int D, int NT, bool ONCE>
-__global__ __launch_bounds__(64 * kWaves, (wgs_per_cu<D, NT>())) void decode_split_i8(QParams qp) {
+template <AttnType T, int D, int NT, int SETS, bool ONCE>
+__global__ __launch_bounds__(64 * kWaves, 2) void decode_split_i8(QParams qp) {
   using W = PIo<AttnType::F16>;      // the weights' type
   constexpr float kUnscale = 0x1p-11f;
   static_assert(W::kTop == 11.0f);
@@ -103,6 +125,9 @@ __global__ __launch_bounds__(64 * kWaves, (wgs_per_cu<D, NT>())) void decode_spl
   constexpr int CH = D / 16;         // chunks of a row
   constexpr int RPI = 64 / CH;       // V rows per load
   constexpr int KT = kTile / 16;     // tiles of 16 slots
+  constexpr int HC = 16 / SETS;      // columns of a set: query heads
+  constexpr int MT = KT / SETS;      // tiles of 16 slots that a lane looks after
+  static_assert(NT == 1 || SETS == 1, "sets are for groups that leave columns empty");
   constexpr int kStage = kTile * CH; // chunks of a V tile
   constexpr int kPitch = D + 4;
   constexpr int kV = kWaves * 2 * kStage * 16, kMerge = kWaves * 16 * kPitch * 4;
@@ -113,6 +138,7 @@ __global__ __launch_bounds__(64 * kWaves, (wgs_per_cu<D, NT>())) void decode_spl
 
   const int tid = threadIdx.x, lane = tid & 63, l16 = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int set = l16 / HC;
 
   uint32_t b, it, i, share, left;
   int len64;
@@ -177,11 +203,11 @@ __global__ __launch_bounds__(64 * kWaves, (wgs_per_cu<D, NT>())) void decode_spl
       __builtin_amdgcn_wave_barrier();
 #pragma unroll
       for (int kt = 0; kt < KT; ++kt) {
-        const uint8_t* src = (const uint8_t*)rows[wave][0][16 * kt + l16] + 16 * g;
+        const uint64_t src = rows[wave][0][16 * kt + l16] + 16 * g;
 #pragma unroll
         for (int f = 0; f < F; ++f) {
-          if constexpr (ONCE) kf[BUF][kt][f] = __builtin_nontemporal_load((const i32x4*)(src + 64 * f));
-          else kf[BUF][kt][f] = *(const i32x4*)(src + 64 * f);
+          if constexpr (ONCE) kf[BUF][kt][f] = __builtin_nontemporal_load((global_i32x4_t)(src + 64 * f));
+          else kf[BUF][kt][f] = *(global_i32x4_t)(src + 64 * f);
         }
       }
 #pragma unroll
@@ -197,14 +223,14 @@ __global__ __launch_bounds__(64 * kWaves, (wgs_per_cu<D, NT>())) void decode_spl
     u32x4 raw[NT][F][2];
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-      const int r = q0 + 16 * t + l16;
+      const int r = q0 + 16 * t + (l16 & (HC - 1));
       const uint8_t* src = r < p.group ? p.q + (int64_t)b * p.q_sb + (h * p.group + r) * p.q_sh : (const uint8_t*)zero_row;
 #pragma unroll
       for (int f = 0; f < F; ++f)
 #pragma unroll
         for (int x = 0; x < 2; ++x) raw[t][f][x] = *(const u32x4*)(src + 2 * (64 * f + 16 * g + 8 * x));
     }
-    if (key < end) issue(Buf<0>{}, key, e);
+    issue(Buf<0>{}, key, e);         // (zeros where the wave has no slot)
     // The queries' digits, and what a sum of them stands for.
     i32x4 qd[NT][3][F];
     float unit[NT];
@@ -265,32 +291,41 @@ __global__ __launch_bounds__(64 * kWaves, (wgs_per_cu<D, NT>())) void decode_spl
       i32x4 pf[NT][KT / 2], pr[NT][KT / 2];      // the weights: leading bits, rest
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
-        f32x4 s[KT];
+        f32x4 s[MT];                             // of the lane's tiles, set * MT ..
 #pragma unroll
-        for (int kt = 0; kt < KT; ++kt) {
+        for (int k = 0; k < MT; ++k) {
           i32x4 a[3];
 #pragma unroll
           for (int x = 0; x < 3; ++x) {
-            a[x] = i32x4{0, 0, 0, 0};
 #pragma unroll
-            for (int f = 0; f < F; ++f)
-              a[x] = __builtin_amdgcn_mfma_i32_16x16x64_i8(kf[BUF][kt][f], qd[t][x][f], a[x], 0, 0, 0);
+            for (int c = 0; c < SETS; ++c) {
+              i32x4 sum = {0, 0, 0, 0};
+#pragma unroll
+              for (int f = 0; f < F; ++f)
+                sum = __builtin_amdgcn_mfma_i32_16x16x64_i8(kf[BUF][c * MT + k][f], qd[t][x][f], sum, 0, 0, 0);
+              if (c == 0) a[x] = sum;
+              else
+#pragma unroll
+                for (int r = 0; r < 4; ++r) a[x][r] = set == c ? sum[r] : a[x][r];
+            }
           }
-          const f32x4 by = *(const f32x4*)&scales[wave][0][16 * kt + 4 * g];
+          const f32x4 by = *(const f32x4*)&scales[wave][0][16 * (set * MT + k) + 4 * g];
 #pragma unroll
           for (int r = 0; r < 4; ++r)
-            s[kt][r] = fmaf(fmaf((float)a[0][r], 256.0f, (float)a[1][r]), 256.0f, (float)a[2][r]) * (by[r] * unit[t]);
+            s[k][r] = fmaf(fmaf((float)a[0][r], 256.0f, (float)a[1][r]), 256.0f, (float)a[2][r]) * (by[r] * unit[t]);
         }
         if (mask != (kTile == 64 ? ~0ull : 0xffffffffull)) {
+          const uint64_t mine = mask >> (16 * set * MT + 4 * g);
 #pragma unroll
-          for (int kt = 0; kt < KT; ++kt)
+          for (int k = 0; k < MT; ++k)
 #pragma unroll
             for (int r = 0; r < 4; ++r)
-              if (!(mask >> (16 * kt + 4 * g + r) & 1)) s[kt][r] = -INFINITY;
+              if (!(mine >> (16 * k + r) & 1)) s[k][r] = -INFINITY;
         }
         float mx = s[0][0];
 #pragma unroll
-        for (int x = 1; x < 4 * KT; ++x) mx = fmaxf(mx, s[x / 4][x % 4]);
+        for (int x = 1; x < 4 * MT; ++x) mx = fmaxf(mx, s[x / 4][x % 4]);
+        mx = over_sets<SETS>(mx, [](float a, float x) { return fmaxf(a, x); });
         mx = over_query(mx, [](float a, float x) { return fmaxf(a, x); });
         mx = fmaxf(mx, kLowest);     // -inf scores weigh 0; a row of only such has l = 0 and is NaN
         const bool raise = mx - m[t] > kLazy;
@@ -302,24 +337,28 @@ __global__ __launch_bounds__(64 * kWaves, (wgs_per_cu<D, NT>())) void decode_spl
 #pragma unroll
           for (int d = 0; d < DT; ++d) o[t][d] *= alpha;
         }
+        int hi[MT][2], lo[MT][2];
 #pragma unroll
-        for (int kt = 0; kt < KT; ++kt) {
-          const f32x4 by = *(const f32x4*)&scales[wave][1][16 * kt + 4 * g];
+        for (int k = 0; k < MT; ++k) {
+          const f32x4 by = *(const f32x4*)&scales[wave][1][16 * (set * MT + k) + 4 * g];
           float w[4];
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            w[r] = __builtin_amdgcn_exp2f((s[kt][r] - m[t]) + W::kTop);
+            w[r] = __builtin_amdgcn_exp2f((s[k][r] - m[t]) + W::kTop);
             l[t] += w[r];
             w[r] *= by[r];
           }
 #pragma unroll
-          for (int x = 0; x < 2; ++x) {
-            int a, b;
-            W::split2(w[2 * x], w[2 * x + 1], a, b);
-            pf[t][kt / 2][kt % 2 * 2 + x] = a;
-            pr[t][kt / 2][kt % 2 * 2 + x] = b;
-          }
+          for (int x = 0; x < 2; ++x) W::split2(w[2 * x], w[2 * x + 1], hi[k][x], lo[k][x]);
         }
+#pragma unroll
+        for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            const bool own = SETS == 1 || set == kt / MT;
+            pf[t][kt / 2][kt % 2 * 2 + x] = own ? hi[kt % MT][x] : 0;
+            pr[t][kt / 2][kt % 2 * 2 + x] = own ? lo[kt % MT][x] : 0;
+          }
       }
       const uint8_t* v0 = vt + BUF * kStage * 16;
       const int in = l16 >> 1;                   // the lane's row of a transposing read
@@ -371,8 +410,14 @@ __global__ __launch_bounds__(64 * kWaves, (wgs_per_cu<D, NT>())) void decode_spl
       wait_all();
       __syncthreads();               // every wave is done with its tiles, or with the rows before
 #pragma unroll
-      for (int d = 0; d < DT; ++d) *(f32x4*)&mo[(wave * 16 + l16) * kPitch + 16 * d + 4 * g] = o[t][d] * back;
-      const float sum = over_query(l[t], [](float a, float x) { return a + x; }) * kUnscale;
+      for (int d = 0; d < DT; ++d) {
+        f32x4 x = o[t][d] * back;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) x[r] = over_sets<SETS>(x[r], [](float a, float y) { return a + y; });
+        *(f32x4*)&mo[(wave * 16 + l16) * kPitch + 16 * d + 4 * g] = x;
+      }
+      const float sum = over_query(over_sets<SETS>(l[t], [](float a, float x) { return a + x; }),
+                                   [](float a, float x) { return a + x; }) * kUnscale;
       if (g == 0) {
         ml[wave][0][l16] = m[t];
         ml[wave][1][l16] = sum;
@@ -403,13 +448,20 @@ Plan plan_of(int B, int H, int heads, int D, int W, int page, bool neighbours) {
   x.room = (int64_t)W * page;
   x.slots = (x.room + 255) / 256 * 256;
   const int64_t each = (int64_t)B * heads * x.gtiles;
-  x.whole = (x.room <= 256 || (x.room <= 512 && each >= 128)) && each <= (1 << 20);
+  // A workgroup per (sequence, head) and no join where no sequence is long: up to 512 slots
+  // always, up to 1024 where those workgroups go evenly on the CUs. us, split and joined /
+  // whole: 8 heads of one sequence of 500 slots 11.7 / 9.5, of 8 sequences 12.4 / 11.5; 32 x
+  // 8 heads of 1000 23.4 / 19.5, 64 x 8 of 800 35.8 / 28.8, of 20 to 1000 31.1 / 28.8, but
+  // 16 x 8 of 1000 16.9 / 17.7, 48 x 8 of 1000 30.3 / 32.3.
+  const int cus = compute_units();
+  const bool even = each >= cus && (each % cus == 0 || each >= 4 * cus);
+  x.whole = (x.room <= 512 || (x.room <= 1024 && even)) && each <= (1 << 20);
   x.hw = 1;
   if (!x.whole && neighbours)
     for (int hw = 4; hw > 1 && x.hw == 1; hw /= 2)
       if (heads % hw == 0 && (int64_t)B * (heads / hw) * x.gtiles >= 64) x.hw = hw;
   x.items = (int64_t)B * (heads / x.hw) * x.gtiles;
-  x.wgs = x.whole ? (int)x.items : 2 * compute_units();
+  x.wgs = x.whole ? (int)x.items : 2 * cus;
   const size_t parts = x.whole ? (size_t)x.items : (size_t)x.items + x.wgs;
   if (!x.whole) x.ml = (parts * x.hw * x.rows * 2 + 3) / 4 * 4;
   if (!x.whole) x.po = parts * x.hw * x.rows * D;
@@ -443,9 +495,11 @@ hipError_t run(const PagedAttnDesc& d, const QuantScales& q, hipStream_t s) {
                  x.whole ? "whole" : "split", x.hw);
   const dim3 grid(x.wgs), threads(64 * kWaves);
   auto go = [&](auto kern) { hipLaunchKernelGGL(kern, grid, threads, 0, s, qp); };
-  if (x.nt == 1) go(decode_split_i8<T, D, 1, true>);
-  else if (x.gtiles == 1) go(decode_split_i8<T, D, 2, true>);
-  else go(decode_split_i8<T, D, 2, false>);
+  if (p.group <= 4) go(decode_split_i8<T, D, 1, 4, true>);
+  else if (p.group <= 8) go(decode_split_i8<T, D, 1, 2, true>);
+  else if (x.nt == 1) go(decode_split_i8<T, D, 1, 1, true>);
+  else if (x.gtiles == 1) go(decode_split_i8<T, D, 2, 1, true>);
+  else go(decode_split_i8<T, D, 2, 1, false>);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess || x.whole) return e;
   const JoinPlan j = join_plan(x, p.B, p.H, p.heads, false);

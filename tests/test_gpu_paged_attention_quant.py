@@ -47,6 +47,10 @@ CASES = [
     (F16, 64, 2, 1, 16, 2, True, [9001]),
     (BF16, 128, 1, 1, 100, 50, False, [20000, 3, 12001]),
     (F16, 128, 64, 2, 32, 32, True, [3000, 63, 64, 65]),
+    (BF16, 128, 16, 2, 16, 16, True, [1100, 2, 64, 130]),
+    (F16, 64, 24, 3, 16, 1, False, [513, 200, 0]),
+    (BF16, 64, 16, 4, 64, 32, False, [4000, 33]),
+    (F16, 128, 8, 8, 16, 16, True, [1000 - 30 * i for i in range(32)]),      # a workgroup to each
 ]
 
 
