@@ -23,6 +23,7 @@ namespace grxk {
 namespace {
 
 constexpr int kThreads = 256;
+constexpr int64_t kStream = 32 << 20;     // bytes of 16 bits from which on stores go past the caches
 
 // A pool of codes as the kernels address it, strides in bytes, and its scales.
 struct Pool8 {
@@ -87,6 +88,8 @@ __device__ __forceinline__ uint32_t codes4(const float* x, float s, float r) {
   return lo | hi << 16;
 }
 
+typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+
 template <int CTRL> __device__ __forceinline__ uint32_t dpp_max(uint32_t v) {
   return max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, CTRL, 0xf, 0xf, false));
 }
@@ -108,8 +111,11 @@ template <int L> __device__ __forceinline__ uint32_t lanes_max(uint32_t v) {
 // One task: the block of one head's keys or values (blockIdx.z) that gets new rows, by L
 // threads with N chunks of 8 values each, held in registers between the maximum and the
 // codes: read once. Rows that the block already holds are rounded again, to the new scale,
-// where that is larger.
-template <NormType T, int C, int L, int N>   // C: chunks of a row
+// where that is larger. us, 8 sequences of 500 to 4000 tokens of 8 heads of 128, blocks of 32:
+// 23.9 (4.6 TB/s; stores through the caches 25.5), bound by memory with the VALU at work in
+// 60 % of the cycles (8 instructions a value); one token of 64 sequences 5.5, a launch and the
+// chain of length, table entry and rows.
+template <NormType T, int C, int L, int N, bool STREAM>   // C: chunks of a row
 __global__ __launch_bounds__(kThreads) void append_i8(AppendParams p) {
   __shared__ uint32_t most_of[kThreads / 64];
   const int tid = threadIdx.x, l = tid % L;
@@ -134,7 +140,7 @@ __global__ __launch_bounds__(kThreads) void append_i8(AppendParams p) {
       const float before = there && old > 0 ? *scale : 0.0f;
       const uint8_t* src = in.p + b * in.sb + h * in.sh;
       u32x4 x[N];
-      uint32_t most = 0;
+      u16x2 both = {0, 0};                                    // largest magnitudes of either half of a word
 #pragma unroll
       for (int i = 0; i < N; ++i) {
         const int c = i * L + l, r = c / C;
@@ -145,7 +151,9 @@ __global__ __launch_bounds__(kThreads) void append_i8(AppendParams p) {
 #pragma unroll
       for (int i = 0; i < N; ++i)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) most = max(max(most, x[i][e] & 0x7fffu), x[i][e] >> 16 & 0x7fffu);
+        for (int e = 0; e < 4; ++e)
+          both = __builtin_elementwise_max(both, __builtin_bit_cast(u16x2, x[i][e] & 0x7fff7fffu));
+      uint32_t most = max(both[0], both[1]);
       if constexpr (L <= 64) {
         most = lanes_max<L>(most);
       } else {
@@ -170,7 +178,9 @@ __global__ __launch_bounds__(kThreads) void append_i8(AppendParams p) {
         Io<T>::unpack(x[i], f);
         u32x2 w = {codes4(f, s, r1), codes4(f + 4, s, r1)};
         if (!fine) w = u32x2{0, 0};
-        *(u32x2*)(pool.row(page, h, row + r) + 8 * (c % C)) = w;
+        u32x2* to = (u32x2*)(pool.row(page, h, row + r) + 8 * (c % C));
+        if constexpr (STREAM) __builtin_nontemporal_store(w, to);
+        else *to = w;
       }
       if (old > 0 && s > before && fine) {
         for (int i = 0; i < N; ++i) {
@@ -189,7 +199,7 @@ __global__ __launch_bounds__(kThreads) void append_i8(AppendParams p) {
   }
 }
 
-template <NormType T, int C> hipError_t run_append(const AppendParams& p, hipStream_t s) {
+template <NormType T, int C, bool STREAM> hipError_t run_append(const AppendParams& p, hipStream_t s) {
   const int64_t blocks = ((int64_t)p.T + 2 * p.block - 2) / p.block;   // of a sequence, at most
   auto go = [&](auto kern, int lanes) {
     const int64_t tasks = blocks * p.heads, per = kThreads / lanes;
@@ -198,15 +208,19 @@ template <NormType T, int C> hipError_t run_append(const AppendParams& p, hipStr
     return hipGetLastError();
   };
   const int chunks = p.block * C;
-  if (p.block == 1) return go(append_i8<T, C, C, 1>, C);
-  if (chunks <= 64) return go(append_i8<T, C, 64, 1>, 64);
-  if (chunks <= 128) return go(append_i8<T, C, 64, 2>, 64);
-  if (chunks <= 256) return go(append_i8<T, C, 64, 4>, 64);
-  if (chunks <= 512) return go(append_i8<T, C, 64, 8>, 64);
-  if (chunks <= 1024) return go(append_i8<T, C, 256, 4>, 256);
-  if (chunks <= 2048) return go(append_i8<T, C, 256, 8>, 256);
-  if (chunks <= 4096) return go(append_i8<T, C, 256, 16>, 256);
+  if (p.block == 1) return go(append_i8<T, C, C, 1, STREAM>, C);
+  if (chunks <= 64) return go(append_i8<T, C, 64, 1, STREAM>, 64);
+  if (chunks <= 128) return go(append_i8<T, C, 64, 2, STREAM>, 64);
+  if (chunks <= 256) return go(append_i8<T, C, 64, 4, STREAM>, 64);
+  if (chunks <= 512) return go(append_i8<T, C, 64, 8, STREAM>, 64);
+  if (chunks <= 1024) return go(append_i8<T, C, 256, 4, STREAM>, 256);
+  if (chunks <= 2048) return go(append_i8<T, C, 256, 8, STREAM>, 256);
+  if (chunks <= 4096) return go(append_i8<T, C, 256, 16, STREAM>, 256);
   return hipErrorNotSupported;
+}
+
+template <NormType T, int C> hipError_t run_append(const AppendParams& p, hipStream_t s) {
+  return (int64_t)p.B * p.T * p.heads * C * 16 >= kStream ? run_append<T, C, true>(p, s) : run_append<T, C, false>(p, s);
 }
 
 // ---- read --------------------------------------------------------------------
@@ -217,26 +231,36 @@ struct ReadParams {
   uint8_t* out[2];
   int64_t sb[2], sh[2], st[2];   // bytes
   const int* first;
-  PageDiv by_heads, by_block;
+  PageDiv by_T, by_block;
   int B, T, heads;
 };
 
-// 8 codes times their scale; what is past the type's range is its largest value. zero: 0,
-// or NaN for a scale that is none.
-template <NormType T> __device__ __forceinline__ void put8(uint8_t* to, u32x2 w, float s, float zero) {
-  constexpr float kMost = T == NormType::F16 ? 65504.0f : T == NormType::BF16 ? 0x1.fep127f : __FLT_MAX__;
+// 8 codes times their scale s; `odd`: some of a wave's products may lie past the type's range,
+// where they are its largest value, or s may be no number.
+template <NormType T> constexpr float kMost = T == NormType::F16 ? 65504.0f : T == NormType::BF16 ? 0x1.fep127f : __FLT_MAX__;
+template <NormType T, bool STREAM> __device__ __forceinline__ void put8(uint8_t* to, u32x2 w, float s, bool odd) {
   float f[8];
 #pragma unroll
-  for (int e = 0; e < 8; ++e)
-    f[e] = fminf(fmaxf((float)(int8_t)(w[e / 4] >> 8 * (e % 4)) * s, -kMost), kMost) + zero;
+  for (int e = 0; e < 8; ++e) f[e] = (float)(int8_t)(w[e / 4] >> 8 * (e % 4)) * s;
+  if (odd)
 #pragma unroll
-  for (int i = 0; i < 8 / Io<T>::kVec; ++i) ((u32x4*)to)[i] = Io<T>::pack(f + i * Io<T>::kVec);
+    for (int e = 0; e < 8; ++e) f[e] = fminf(fmaxf(f[e], -kMost<T>), kMost<T>) + s * 0.0f;
+#pragma unroll
+  for (int i = 0; i < 8 / Io<T>::kVec; ++i) {
+    const u32x4 x = Io<T>::pack(f + i * Io<T>::kVec);
+    if constexpr (STREAM) __builtin_nontemporal_store(x, (u32x4*)to + i);
+    else ((u32x4*)to)[i] = x;
+  }
 }
 
-// U rows of a key and a value to a thread's chunk, all loaded before the first is stored.
-template <NormType T, int C>
+// U rows of a key and a value to a thread's chunk, all loaded before the first is stored; a
+// head's rows follow one another, as outputs mostly lie. us, 8 sequences of 5000 to 8192 slots
+// of 8 heads of 128 into bf16: 72.9 (5.2 TB/s, of which 72 % are writes); heads side by side
+// 73, stores through the caches 78. 3 sequences of 1001 to 1500 slots of 64 5.4 (with 4 rows
+// at a time 6.3).
+template <NormType T, int C, bool STREAM>
 __global__ __launch_bounds__(kThreads) void read_i8(ReadParams p) {
-  constexpr int R = kThreads / C, U = 4;
+  constexpr int R = kThreads / C, U = STREAM ? 4 : 2;
   constexpr int E = T == NormType::F32 ? 4 : 2;
   const int c = threadIdx.x % C, first = threadIdx.x / C;
   const int rows = p.T * p.heads;
@@ -250,8 +274,8 @@ __global__ __launch_bounds__(kThreads) void read_i8(ReadParams p) {
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         const int r = (int)min<int64_t>(r0 + u * R + first, rows - 1);
-        t[u] = div_page(p.by_heads, r);
-        h[u] = r - t[u] * p.heads;
+        h[u] = div_page(p.by_T, r);
+        t[u] = r - h[u] * p.T;
         const int64_t slot = from + t[u];
         int page, row;
         const bool there = find_slot(p.view, b, (int)min<int64_t>(slot, max(len - 1, 0)), &page, &row) & (slot < len);
@@ -260,7 +284,7 @@ __global__ __launch_bounds__(kThreads) void read_i8(ReadParams p) {
           w[x][u] = u32x2{0, 0};
           s[x][u] = 0.0f;
           if (there) {
-            w[x][u] = __builtin_nontemporal_load((const u32x2*)(p.pool[x].row(page, h[u], row) + 8 * c));
+            w[x][u] = *(const u32x2*)(p.pool[x].row(page, h[u], row) + 8 * c);
             s[x][u] = *p.pool[x].scale_of(page, h[u], div_page(p.by_block, row));
           }
         }
@@ -270,8 +294,9 @@ __global__ __launch_bounds__(kThreads) void read_i8(ReadParams p) {
         if (r0 + u * R + first >= rows) break;
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
+          const bool odd = __ballot(!(fabsf(s[x][u]) <= kMost<T> / 128.0f)) != 0;
           uint8_t* to = p.out[x] + b * p.sb[x] + h[u] * p.sh[x] + t[u] * p.st[x];
-          put8<T>(to + 8 * E * c, w[x][u], s[x][u], s[x][u] * 0.0f);
+          put8<T, STREAM>(to + 8 * E * c, w[x][u], s[x][u], odd);
         }
       }
     }
@@ -279,9 +304,12 @@ __global__ __launch_bounds__(kThreads) void read_i8(ReadParams p) {
 }
 
 template <NormType T, int C> hipError_t run_read(const ReadParams& p, hipStream_t s) {
-  const int64_t rows = (int64_t)p.T * p.heads, per = kThreads / C * 4;
+  const int64_t rows = (int64_t)p.T * p.heads;
+  const bool stream = p.B * rows * C * 16 >= kStream;
+  const int64_t per = kThreads / C * (stream ? 4 : 2);
   const dim3 grid((unsigned)std::min<int64_t>((rows + per - 1) / per, 1 << 20), (unsigned)std::min(p.B, 65535));
-  hipLaunchKernelGGL((read_i8<T, C>), grid, dim3(kThreads), 0, s, p);
+  if (stream) hipLaunchKernelGGL((read_i8<T, C, true>), grid, dim3(kThreads), 0, s, p);
+  else hipLaunchKernelGGL((read_i8<T, C, false>), grid, dim3(kThreads), 0, s, p);
   return hipGetLastError();
 }
 
@@ -317,7 +345,7 @@ hipError_t launch_paged_read_i8(NormType t, const PagedReadDesc& d, const QuantS
   p.out[0] = (uint8_t*)d.k; p.sb[0] = size * d.k_sb; p.sh[0] = size * d.k_sh; p.st[0] = size * d.k_st;
   p.out[1] = (uint8_t*)d.v; p.sb[1] = size * d.v_sb; p.sh[1] = size * d.v_sh; p.st[1] = size * d.v_st;
   p.first = d.first;
-  p.by_heads = page_div(d.c.heads);
+  p.by_T = page_div(d.T);
   p.by_block = page_div(q.block);
   p.B = d.c.B; p.T = d.T; p.heads = d.c.heads;
   if (d.c.D != 64 && d.c.D != 128) return hipErrorNotSupported;
