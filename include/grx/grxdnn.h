@@ -406,8 +406,8 @@ grxdnnStatus_t grxdnnPagedCacheAppendQuantized(grxdnnHandle_t handle,
  * first: B ints (below 0 counts as 0), or NULL for 0 each. k, v: [B, Hkv, T, D] of
  * GRX_R_16BF, GRX_R_16F or GRX_R_32F, strides multiples of 16 bytes, T * Hkv at most
  * 2^31 - 4096; rounded once; what is past the type's range comes back as its largest
- * value. A prompt's next chunk attends to them (grxdnnAttentionForward), or they go into
- * a cache of 16 bits. */
+ * value. For grxdnnAttentionForward over a whole prompt, or to go on in a cache of 16
+ * bits (grxdnnPagedCacheAppend), which eviction needs. */
 grxdnnStatus_t grxdnnPagedCacheReadQuantized(grxdnnHandle_t handle,
                                              grxdnnTensorDescriptor_t kCacheDesc, const void* kCache,
                                              grxdnnTensorDescriptor_t vCacheDesc, const void* vCache,
