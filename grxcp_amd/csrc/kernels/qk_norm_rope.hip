@@ -293,7 +293,7 @@ __global__ __launch_bounds__(kThreads, BWD ? 3 : 1) void qk_norm_rope(RParams p)
               }
             dot = row_sum<G>(dot) * (1.0f / D);
             const float by = inv * inv * dot;
-            if (__ballot(!(fabsf(by) <= __FLT_MAX__))) {   // (eps 0 and tiny rows, or no numbers)
+            if (!(fabsf(by) <= __FLT_MAX__)) {   // (eps 0 and tiny rows, or no numbers)
 #pragma unroll
               for (int c = 0; c < 2; ++c)
 #pragma unroll

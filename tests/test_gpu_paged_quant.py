@@ -322,3 +322,32 @@ def test_captured(gpu):
             assert torch.equal(a, b), f"replay {step}"
     del graph
     dnn.close()
+
+
+def test_pages_past_32_bits(dnn):
+    """Pools of more than 2^32 bytes, scales of more than 2^31 / 4: rows on the last pages."""
+    from quant_cases import attend, attention_ref
+    gen = torch.Generator().manual_seed(75)
+    c = QuantCache(gen, [0, 0], 8, 16, 4, 128, True, room=64)
+    pages = 270000
+    c.k, c.v = (torch.empty((pages, 16, 8, 128), dtype=torch.int8, device="cuda").transpose(1, 2) for _ in range(2))
+    c.ks, c.vs = (torch.empty((pages, 8, 4), device="cuda") for _ in range(2))
+    last = torch.arange(pages - 8, pages).flip(0).reshape(2, 4).int()
+    c.table = last.cuda()
+    for t in (c.k, c.v, c.ks, c.vs):
+        t[pages - 8:] = 1
+    small = QuantCache(gen, [0, 0], 8, 16, 4, 128, True, room=64)
+    k, v = rows(gen, 2, 8, 60, 128, BF16)
+    for x in (c, small):
+        append(dnn, x, k, v)
+        x.n, x.lengths = [60, 60], ints([60, 60])
+    out = [[torch.empty((2, 8, 60, 128), dtype=BF16, device="cuda") for _ in range(2)] for _ in range(2)]
+    q = torch.randn((2, 16, 1, 128), generator=gen).to(BF16).cuda()
+    o = [torch.empty_like(q) for _ in range(2)]
+    for x, (a, b), y in zip((c, small), out, o):
+        read(dnn, x, a, b)
+        attend(dnn, x, q, y, 0.1)
+    assert torch.equal(out[0][0], out[1][0]) and torch.equal(out[0][1], out[1][1]) and torch.equal(*o)
+    K, V, _ = small.rows(0)
+    ref, bound = attention_ref(q[0, :, 0].cpu(), K, V, 0.1)
+    assert ((o[0][0, :, 0].cpu().double() - ref).abs() <= bound).all()

@@ -404,3 +404,44 @@ def test_captured(gpu):
             assert torch.equal(a, b), f"replay {step}"
     del graph
     dnn.close()
+
+
+def test_a_row_does_not_depend_on_its_neighbours(dnn):
+    """NaN, infinities and tiny rows beside it (eps 0): the other rows' bits stay."""
+    c = Case(29, BF16, 1, 40, 8, 2, 64, 64, False, True, packed=False, eps=0.0)
+    runs = []
+    for odd in (False, True):
+        if odd:
+            c.q[0, 3, 5], c.q[0, 4, 5, 7], c.dyq[0, 2, 5, 1] = 2.0 ** -40, math.nan, math.inf
+        yq, yk, dq, dk = (torch.empty_like(t) for t in (c.q, c.k, c.q, c.k))
+        c.forward(dnn, yq, yk)
+        c.backward(dnn, dq, dk, None, None)
+        runs.append((yq, yk, dq, dk))
+    same = torch.ones(8, 40, dtype=torch.bool)
+    same[3, 5] = same[4, 5] = same[2, 5] = False
+    for i, (a, b) in enumerate(zip(*runs)):
+        if i % 2 == 0:
+            a, b = a[0, same], b[0, same]
+        assert torch.equal(a, b), i
+    # a row of 2^-40 alone is normalised like any other: dx is 2^40 times a row's of ones
+    assert torch.isfinite(runs[1][0][0, 3, 5]).all() and torch.isfinite(runs[1][2][0, 3, 5]).all()
+
+
+def test_rows_far_apart(dnn):
+    """A batch that lies 2^31 bytes behind the other."""
+    c = Case(30, BF16, 2, 3, 2, 1, 128, 128, False, True, packed=False)
+    far = torch.empty((1 << 31) + 4096, dtype=BF16, device="cuda")
+    wide = [(1 << 30) + 2048, 128, 512, 1]
+
+    def spread(t, at):
+        v = far.as_strided(t.shape, wide, at)
+        v.copy_(t)
+        return v
+
+    q, k = c.q, c.k
+    yq, yk = torch.empty_like(q), torch.empty_like(k)
+    c.forward(dnn, yq, yk)
+    c.q, c.k = spread(q, 0), spread(k, 256)
+    outs = (far.as_strided(q.shape, wide, 1024 * 1024), far.as_strided(k.shape, wide, 1024 * 1024 + 256))
+    c.forward(dnn, *outs)
+    assert torch.equal(outs[0], yq) and torch.equal(outs[1], yk)
