@@ -6,7 +6,7 @@
 //
 // The work is divided as over a cache of 16 bits (paged_attention.hip): units of a tile for
 // each of a workgroup's four waves, shares of equal size, parts joined in the order of the
-// slots. Half the bytes, so a wave's tile has 64 slots, 16 KB of codes again. What differs:
+// slots. Half the bytes, so a wave's tile has 64 slots where the work is shared, 16 KB of codes again. What differs:
 //
 //  * scores are S^T = K Q^T on the 8-bit matrix cores (v_mfma_i32_16x16x64_i8): the codes of
 //    K go in as they lie, with no conversion. A query's row is held as whole numbers of 23
@@ -25,7 +25,7 @@
 //    others through LDS.
 //
 // us, 32 query and 8 key heads of 128, bf16, a scale for 16 slots: 48 sequences of 33 to 4096
-// slots 51.9 (3.9 TB/s; the join 5), 48 of 8000 142 (5.5), 64 of 800 28.8, one of 201 7.5; 2 of
+// slots 51.4 (4.0 TB/s; the join 5), 48 of 8000 142 (5.5), 64 of 800 26.9, one of 201 7.4; 2 of
 // 131072 with 4 key heads, a scale each, 54 (5.1). What a call has above its bytes (6.3 TB/s
 // from one length to the next) are 11 us: launch, lengths, table, queries and the first tile
 // one after the other, and the join. Loads alone, without scales and products, take 48 of the
@@ -41,8 +41,11 @@
 namespace grxk {
 namespace {
 
-// Slots of a wave's tile: with two tiles of query heads half as many, for the registers.
-template <int NT> constexpr int tile() { return NT == 1 ? 64 : 32; }
+// Slots of a wave's tile: 64, and 32 with two tiles of query heads, for the registers, and where
+// a workgroup takes a whole sequence: three of them share a CU then, not two. us, 64 / 32:
+// whole sequences, 64 x 8 heads of 800 slots 28.9 / 26.9, 128 x 8 of 800 52.1 / 48.7, one of 201
+// 7.5 / 7.4; shares, 48 x 8 of 2000 45.3 / 48.1, 2 x 4 of 131072 52.7 / 55.3.
+constexpr int tile_of(int nt, bool whole) { return nt == 1 && !whole ? 64 : 32; }
 
 struct QParams {
   DParams d;                              // pools' strides in 16-byte chunks of codes
@@ -113,13 +116,12 @@ template <AttnType T> __device__ __forceinline__ void unpack8(u32x4 w, float* f)
   }
 }
 
-template <AttnType T, int D, int NT, int SETS, bool ONCE>
-__global__ __launch_bounds__(64 * kWaves, 2) void decode_split_i8(QParams qp) {
+template <AttnType T, int D, int NT, int SETS, int kTile, bool ONCE>
+__global__ __launch_bounds__(64 * kWaves, NT == 1 && kTile == 32 ? 3 : 2) void decode_split_i8(QParams qp) {
   using W = PIo<AttnType::F16>;      // the weights' type
   constexpr float kUnscale = 0x1p-11f;
   static_assert(W::kTop == 11.0f);
   const DParams& p = qp.d;
-  constexpr int kTile = tile<NT>();
   constexpr int F = D / 64;          // contraction steps of a score
   constexpr int DT = D / 16;         // tiles of the head dimension
   constexpr int CH = D / 16;         // chunks of a row
@@ -450,9 +452,9 @@ Plan plan_of(int B, int H, int heads, int D, int W, int page, bool neighbours) {
   const int64_t each = (int64_t)B * heads * x.gtiles;
   // A workgroup per (sequence, head) and no join where no sequence is long: up to 512 slots
   // always, up to 1024 where those workgroups go evenly on the CUs. us, split and joined /
-  // whole: 8 heads of one sequence of 500 slots 11.7 / 9.5, of 8 sequences 12.4 / 11.5; 32 x
-  // 8 heads of 1000 23.4 / 19.5, 64 x 8 of 800 35.8 / 28.8, of 20 to 1000 31.1 / 28.8, but
-  // 16 x 8 of 1000 16.9 / 17.7, 48 x 8 of 1000 30.3 / 32.3.
+  // whole (64-slot tiles): 8 heads of one sequence of 500 slots 11.7 / 9.5, of 8 sequences
+  // 12.4 / 11.5; 32 x 8 heads of 1000 23.4 / 19.5, 64 x 8 of 800 35.8 / 28.8, of 20 to 1000
+  // 31.1 / 28.8, but 16 x 8 of 1000 16.9 / 17.7, 48 x 8 of 1000 30.3 / 32.3.
   const int cus = compute_units();
   const bool even = each >= cus && (each % cus == 0 || each >= 4 * cus);
   x.whole = (x.room <= 512 || (x.room <= 1024 && even)) && each <= (1 << 20);
@@ -483,7 +485,7 @@ hipError_t run(const PagedAttnDesc& d, const QuantScales& q, hipStream_t s) {
   p.po = ws + x.ml;
   p.slots = x.slots;
   p.B = d.c.B; p.H = d.H; p.heads = d.c.heads; p.group = d.H / d.c.heads;
-  p.hw = x.hw; p.shift = (x.nt == 1 ? 6 : 5) + (x.hw == 4 ? 0 : x.hw == 2 ? 1 : 2);
+  p.hw = x.hw; p.shift = (tile_of(x.nt, x.whole) == 64 ? 6 : 5) + (x.hw == 4 ? 0 : x.hw == 2 ? 1 : 2);
   p.gtiles = x.gtiles; p.items = d.c.heads / x.hw * x.gtiles; p.rows = x.rows; p.wgs = x.wgs; p.whole = x.whole;
   p.c = d.scale * 1.4426950408889634f;
   qp.ks = q.k; qp.vs = q.v;
@@ -495,11 +497,17 @@ hipError_t run(const PagedAttnDesc& d, const QuantScales& q, hipStream_t s) {
                  x.whole ? "whole" : "split", x.hw);
   const dim3 grid(x.wgs), threads(64 * kWaves);
   auto go = [&](auto kern) { hipLaunchKernelGGL(kern, grid, threads, 0, s, qp); };
-  if (p.group <= 4) go(decode_split_i8<T, D, 1, 4, true>);
-  else if (p.group <= 8) go(decode_split_i8<T, D, 1, 2, true>);
-  else if (x.nt == 1) go(decode_split_i8<T, D, 1, 1, true>);
-  else if (x.gtiles == 1) go(decode_split_i8<T, D, 2, 1, true>);
-  else go(decode_split_i8<T, D, 2, 1, false>);
+  if (x.nt == 2) {
+    if (x.gtiles == 1) go(decode_split_i8<T, D, 2, 1, 32, true>);
+    else go(decode_split_i8<T, D, 2, 1, 32, false>);
+  } else if (x.whole) {
+    if (p.group <= 8) go(decode_split_i8<T, D, 1, 2, 32, true>);
+    else go(decode_split_i8<T, D, 1, 1, 32, true>);
+  } else {
+    if (p.group <= 4) go(decode_split_i8<T, D, 1, 4, 64, true>);
+    else if (p.group <= 8) go(decode_split_i8<T, D, 1, 2, 64, true>);
+    else go(decode_split_i8<T, D, 1, 1, 64, true>);
+  }
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess || x.whole) return e;
   const JoinPlan j = join_plan(x, p.B, p.H, p.heads, false);

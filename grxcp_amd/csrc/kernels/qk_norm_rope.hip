@@ -338,7 +338,7 @@ __global__ __launch_bounds__(kThreads, BWD ? 3 : 1) void qk_norm_rope(RParams p)
 // keys), 16 columns to a workgroup, in the same order every time.
 __global__ __launch_bounds__(1024) void gain_grad(const float* partial, int nq, int nk, int D, float* dq, float* dk) {
   constexpr int kAtOnce = 16;
-  __shared__ float red[64][17];
+  __shared__ float red[16][16];
   const int col = threadIdx.x & 15, lane = threadIdx.x >> 4;
   const bool keys = (int)blockIdx.x * 16 >= D;
   const int at = blockIdx.x * 16 + col - (keys ? D : 0), n = keys ? nk : nq;
@@ -353,14 +353,15 @@ __global__ __launch_bounds__(1024) void gain_grad(const float* partial, int nq, 
 #pragma unroll
     for (int u = 0; u < kAtOnce; ++u) v += i + 64 * u < n ? a[u] : 0.0f;
   }
-  red[lane][col] = v;
+  v += __shfl_xor(v, 16);
+  v += __shfl_xor(v, 32);
+  if ((threadIdx.x & 63) < 16) red[threadIdx.x >> 6][col] = v;
   __syncthreads();
+  if (threadIdx.x >= 16) return;
+  v = 0.0f;
 #pragma unroll
-  for (int o = 32; o > 0; o >>= 1) {
-    if (lane < o) red[lane][col] += red[lane + o][col];
-    __syncthreads();
-  }
-  if (lane == 0) out[at] = red[0][col];
+  for (int w = 0; w < 16; ++w) v += red[w][col];
+  out[at] = v;
 }
 
 struct RopePlan {
