@@ -22,17 +22,18 @@
 //    the tile's slots: the softmax is done once for every score. In the product with V a
 //    set's weights of the others' slots are 0, and the sets' results are added at the end;
 //  * a lane finds page, row and both scales of one slot of the tile, and hands them to the
-//    others through LDS.
+//    others through LDS;
+//  * K and V go to LDS without registers, 8 lanes to a row of 128 bytes. The products' operands
+//    need a row's bytes in four lanes 16 apart, and loads of K in that form straight from
+//    memory took the loads' unit four times as long: waves waited to issue in 45 % of their
+//    cycles (48 sequences of 33 to 4096 slots 50.6 for 47.7 us, 64 of 20 to 1000 26.6 for
+//    21.4). A tile that has come goes to registers whole, and the next one into its place.
 //
 // us, 32 query and 8 key heads of 128, bf16, a scale for 16 slots: 48 sequences of 33 to 4096
-// slots 51.4 (4.0 TB/s; the join 5), 48 of 8000 142 (5.5), 64 of 800 26.9, one of 201 7.4; 2 of
-// 131072 with 4 key heads, a scale each, 54 (5.1). What a call has above its bytes (6.3 TB/s
-// from one length to the next) are 11 us: launch, lengths, table, queries and the first tile
-// one after the other, and the join. Loads alone, without scales and products, take 48 of the
-// 52 that the batch took; 2 of them the sets of columns saved, 0.5 the digits made while the
-// first tile comes. Rows of K loaded by 8 neighbours together (128 bytes), each row as two of
-// the product's, were faster in few tiles (48 of 500 17.4 for 18.8) and slower in many (55.5
-// for 54.0 in the long ones).
+// slots 47.7 (4.3 TB/s; the join 5), 48 of 8000 137 (5.7), 64 of 800 23.7, one of 201 7.0; 2 of
+// 131072 with 4 key heads, a scale for each slot, 53 (5.2). What a call has above its bytes
+// (6.5 TB/s from one length to the next) are 11 us: launch, lengths, table, queries and the
+// first tile one after the other, and the join.
 
 #include "paged_split.h"
 
@@ -43,8 +44,8 @@ namespace {
 
 // Slots of a wave's tile: 64, and 32 with two tiles of query heads, for the registers, and where
 // a workgroup takes a whole sequence: three of them share a CU then, not two. us, 64 / 32:
-// whole sequences, 64 x 8 heads of 800 slots 28.9 / 26.9, 128 x 8 of 800 52.1 / 48.7, one of 201
-// 7.5 / 7.4; shares, 48 x 8 of 2000 45.3 / 48.1, 2 x 4 of 131072 52.7 / 55.3.
+// whole sequences, 64 x 8 heads of 800 slots 28.9 / 26.9, 128 x 8 of 800 52.1 / 48.7; shares (three
+// or two workgroups to a CU), 48 x 8 of 2000 43.1 / 45.5, 2 x 4 of 131072 51.8 / 53.2.
 constexpr int tile_of(int nt, bool whole) { return nt == 1 && !whole ? 64 : 32; }
 
 struct QParams {
@@ -61,9 +62,12 @@ template <int D> __device__ __forceinline__ int vswz(int row) {
   else return (row >> 1 & 1) | (row >> 3 & 2);
 }
 
-// Addresses come out of LDS, and the compiler takes a pointer that does for one of any memory:
-// such a load would hold up every later LDS access until it is back.
-typedef const __attribute__((address_space(1))) i32x4* global_i32x4_t;
+// The same of a K row: 8 neighbouring rows read at one chunk touch every bank once.
+template <int D> __device__ __forceinline__ int kswz(int row) {
+  if constexpr (D == 128) return row & 7;
+  else return row >> 1 & 3;
+}
+
 typedef int i32x2 __attribute__((ext_vector_type(2)));
 typedef __attribute__((address_space(3))) i32x2* lds_i32x2_t;
 
@@ -130,7 +134,7 @@ __global__ __launch_bounds__(64 * kWaves, NT == 1 && kTile == 32 ? 3 : 2) void d
   constexpr int HC = 16 / SETS;      // columns of a set: query heads
   constexpr int MT = KT / SETS;      // tiles of 16 slots that a lane looks after
   static_assert(NT == 1 || SETS == 1, "sets are for groups that leave columns empty");
-  constexpr int kStage = kTile * CH; // chunks of a V tile
+  constexpr int kStage = kTile * CH; // chunks of a tile of K or V
   constexpr int kPitch = D + 4;
   constexpr int kV = kWaves * 2 * kStage * 16, kMerge = kWaves * 16 * kPitch * 4;
   __shared__ __attribute__((aligned(1024))) uint8_t smem[kV > kMerge ? kV : kMerge];
@@ -146,7 +150,8 @@ __global__ __launch_bounds__(64 * kWaves, NT == 1 && kTile == 32 ? 3 : 2) void d
   int len64;
   if (!find_share(p, lane, b, it, i, share, left, len64)) return;
 
-  uint8_t* vt = smem + wave * 2 * kStage * 16;
+  uint8_t* ktile = smem + wave * 2 * kStage * 16;
+  uint8_t* vtile = ktile + kStage * 16;
   const int of = kWaves / p.hw;      // waves of a key head
   const int hd = wave / of, sub = wave - hd * of;
 
@@ -173,9 +178,8 @@ __global__ __launch_bounds__(64 * kWaves, NT == 1 && kTile == 32 ? 3 : 2) void d
     }
     float R = 0x1p-126f;             // o is in units of it
 
-    i32x4 kf[2][KT][F];
-    float ksr[2], vsr[2];            // the scales of the lane's slot
-    uint64_t live[2];
+    float ksr, vsr;                  // the scales of the lane's slot
+    uint64_t live;                   // the tile's slots that are there
     const int step = 1 << p.shift;
     int key = (int)(i << p.shift) + sub * kTile;                        // the wave's first slot
     const int end = (int)min((uint32_t)len, (i + take) << p.shift);
@@ -183,9 +187,8 @@ __global__ __launch_bounds__(64 * kWaves, NT == 1 && kTile == 32 ? 3 : 2) void d
       const int j = key0 + lane;
       return lane < kTile && j < end ? table[div_page(p.view.div, j)] : -1;
     };
-    // Loads of the tile at key0, whose table entries are e, into buffer BUF.
-    auto issue = [&](auto buf, int key0, int e) __attribute__((always_inline)) {
-      constexpr int BUF = decltype(buf)::value;
+    // Loads of the tile at key0, whose table entries are e.
+    auto issue = [&](int key0, int e) __attribute__((always_inline)) {
       const int j = key0 + lane;
       const int page = lane < kTile && j < end ? checked_page(e, p.view.pages) : -1;
       const int row = j - div_page(p.view.div, j) * p.view.page;
@@ -195,28 +198,23 @@ __global__ __launch_bounds__(64 * kWaves, NT == 1 && kTile == 32 ? 3 : 2) void d
         rows[wave][0][lane] = (uint64_t)(there ? kbase + 16 * (pg * p.k_sp + r64 * p.k_ss) : (const uint8_t*)zero_row);
         rows[wave][1][lane] = (uint64_t)(there ? vbase + 16 * (pg * p.v_sp + r64 * p.v_ss) : (const uint8_t*)zero_row);
       }
-      live[BUF] = __ballot(there);
-      ksr[BUF] = vsr[BUF] = 0.0f;
+      live = __ballot(there);
+      ksr = vsr = 0.0f;
       if (there) {
         const int64_t at = page * qp.cp + h * qp.ch + div_page(qp.by_block, row) * qp.cb;
-        ksr[BUF] = qp.ks[at];
-        vsr[BUF] = qp.vs[at];
+        ksr = qp.ks[at];
+        vsr = qp.vs[at];
       }
       __builtin_amdgcn_wave_barrier();
 #pragma unroll
-      for (int kt = 0; kt < KT; ++kt) {
-        const uint64_t src = rows[wave][0][16 * kt + l16] + 16 * g;
-#pragma unroll
-        for (int f = 0; f < F; ++f) {
-          if constexpr (ONCE) kf[BUF][kt][f] = __builtin_nontemporal_load((global_i32x4_t)(src + 64 * f));
-          else kf[BUF][kt][f] = *(global_i32x4_t)(src + 64 * f);
-        }
+      for (int x = 0; x < kTile / RPI; ++x) {
+        const int r = RPI * x + lane / CH;
+        dma16<ONCE>((const uint8_t*)rows[wave][0][r] + 16 * ((lane % CH) ^ kswz<D>(r)), lds_addr(ktile + 1024 * x));
       }
 #pragma unroll
       for (int x = 0; x < kTile / RPI; ++x) {
         const int r = RPI * x + lane / CH;
-        const uint8_t* src = (const uint8_t*)rows[wave][1][r] + 16 * ((lane % CH) ^ vswz<D>(r));
-        dma16<ONCE>(src, lds_addr(vt + (BUF * kStage + 64 * x) * 16));
+        dma16<ONCE>((const uint8_t*)rows[wave][1][r] + 16 * ((lane % CH) ^ vswz<D>(r)), lds_addr(vtile + 1024 * x));
       }
     };
     int e = entry(key);
@@ -232,7 +230,7 @@ __global__ __launch_bounds__(64 * kWaves, NT == 1 && kTile == 32 ? 3 : 2) void d
 #pragma unroll
         for (int x = 0; x < 2; ++x) raw[t][f][x] = *(const u32x4*)(src + 2 * (64 * f + 16 * g + 8 * x));
     }
-    issue(Buf<0>{}, key, e);         // (zeros where the wave has no slot)
+    issue(key, e);                   // (zeros where the wave has no slot)
     // The queries' digits, and what a sum of them stands for.
     i32x4 qd[NT][3][F];
     float unit[NT];
@@ -269,12 +267,11 @@ __global__ __launch_bounds__(64 * kWaves, NT == 1 && kTile == 32 ? 3 : 2) void d
         }
     }
 
-    auto compute = [&](auto buf) __attribute__((always_inline)) {
-      constexpr int BUF = decltype(buf)::value;
-      const uint64_t mask = live[BUF];
-      if (!mask) return;                         // nothing to add
-      if (__ballot(!(vsr[BUF] <= R))) {
-        const uint32_t top = __float_as_uint(fmaxf(wave_max(vsr[BUF]), 0.0f));
+    while (key < end) {
+      wait_all();
+      const uint64_t mask = live;
+      if (__ballot(!(vsr <= R))) {
+        const uint32_t top = __float_as_uint(fmaxf(wave_max(vsr), 0.0f));
         const float up = __uint_as_float(min((top + 0x7fffffu) & 0x7f800000u, 0x7e800000u));
         if (up > R) {
           const float f = R * inverse(up);
@@ -286,10 +283,38 @@ __global__ __launch_bounds__(64 * kWaves, NT == 1 && kTile == 32 ? 3 : 2) void d
         }
       }
       if (lane < kTile) {
-        scales[wave][0][lane] = ksr[BUF];
-        scales[wave][1][lane] = vsr[BUF] * inverse(R);
+        scales[wave][0][lane] = ksr;
+        scales[wave][1][lane] = vsr * inverse(R);
       }
-      __builtin_amdgcn_wave_barrier();
+      // The tile into registers; then its place takes the next one.
+      i32x4 kf[KT][F];
+#pragma unroll
+      for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+        for (int f = 0; f < F; ++f) {
+          const int r = 16 * kt + l16;
+          kf[kt][f] = *(const i32x4*)(ktile + r * D + 16 * ((4 * f + g) ^ kswz<D>(r)));
+        }
+      i32x2 vc[DT][KT / 2];
+      const int in = l16 >> 1;                   // the lane's row of a transposing read
+      const int r0 = in < 4 ? 4 * g + in : 12 + 4 * g + in;
+#pragma unroll
+      for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int x = 0; x < KT / 2; ++x) {
+          const int r = 32 * x + r0;
+          vc[d][x] = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
+              (lds_i32x2_t)(vtile + r * D + 16 * (d ^ vswz<D>(r)) + 8 * (lane & 1)));
+        }
+      if (key + step < end) {
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_s_waitcnt(0xc07f);      // lgkmcnt(0): the reads are done
+        asm volatile("" ::: "memory");
+        issue(key + step, next);
+        next = entry(key + 2 * step);
+      }
+      key += step;
+      if (!mask) continue;                       // nothing to add
       i32x4 pf[NT][KT / 2], pr[NT][KT / 2];      // the weights: leading bits, rest
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
@@ -304,7 +329,7 @@ __global__ __launch_bounds__(64 * kWaves, NT == 1 && kTile == 32 ? 3 : 2) void d
               i32x4 sum = {0, 0, 0, 0};
 #pragma unroll
               for (int f = 0; f < F; ++f)
-                sum = __builtin_amdgcn_mfma_i32_16x16x64_i8(kf[BUF][c * MT + k][f], qd[t][x][f], sum, 0, 0, 0);
+                sum = __builtin_amdgcn_mfma_i32_16x16x64_i8(kf[c * MT + k][f], qd[t][x][f], sum, 0, 0, 0);
               if (c == 0) a[x] = sum;
               else
 #pragma unroll
@@ -362,18 +387,11 @@ __global__ __launch_bounds__(64 * kWaves, NT == 1 && kTile == 32 ? 3 : 2) void d
             pr[t][kt / 2][kt % 2 * 2 + x] = own ? lo[kt % MT][x] : 0;
           }
       }
-      const uint8_t* v0 = vt + BUF * kStage * 16;
-      const int in = l16 >> 1;                   // the lane's row of a transposing read
-      const int r0 = in < 4 ? 4 * g + in : 12 + 4 * g + in;
 #pragma unroll
       for (int d = 0; d < DT; ++d) {
         i32x4 vf[KT / 2];
 #pragma unroll
-        for (int x = 0; x < KT / 2; ++x) {
-          const int r = 32 * x + r0;
-          vf[x] = to_half(__builtin_amdgcn_ds_read_tr8_b64_v2i32(
-              (lds_i32x2_t)(v0 + r * D + 16 * (d ^ vswz<D>(r)) + 8 * (lane & 1))));
-        }
+        for (int x = 0; x < KT / 2; ++x) vf[x] = to_half(vc[d][x]);
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
@@ -383,23 +401,6 @@ __global__ __launch_bounds__(64 * kWaves, NT == 1 && kTile == 32 ? 3 : 2) void d
 #pragma unroll
           for (int x = 0; x < KT / 2; ++x) o[t][d] = W::mma(vf[x], pr[t][x], o[t][d]);
       }
-    };
-    while (key < end) {
-      wait_all();
-      if (key + step < end) {
-        issue(Buf<1>{}, key + step, next);
-        next = entry(key + 2 * step);
-      }
-      compute(Buf<0>{});
-      key += step;
-      if (key >= end) break;
-      wait_all();
-      if (key + step < end) {
-        issue(Buf<0>{}, key + step, next);
-        next = entry(key + 2 * step);
-      }
-      compute(Buf<1>{});
-      key += step;
     }
 
     // The results of a key head's waves meet: 16 query heads at a time.
@@ -452,7 +453,7 @@ Plan plan_of(int B, int H, int heads, int D, int W, int page, bool neighbours) {
   const int64_t each = (int64_t)B * heads * x.gtiles;
   // A workgroup per (sequence, head) and no join where no sequence is long: up to 512 slots
   // always, up to 1024 where those workgroups go evenly on the CUs. us, split and joined /
-  // whole (64-slot tiles): 8 heads of one sequence of 500 slots 11.7 / 9.5, of 8 sequences
+  // whole: 8 heads of one sequence of 500 slots 11.7 / 9.5, of 8 sequences
   // 12.4 / 11.5; 32 x 8 heads of 1000 23.4 / 19.5, 64 x 8 of 800 35.8 / 28.8, of 20 to 1000
   // 31.1 / 28.8, but 16 x 8 of 1000 16.9 / 17.7, 48 x 8 of 1000 30.3 / 32.3.
   const int cus = compute_units();
