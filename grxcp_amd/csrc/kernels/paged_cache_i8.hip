@@ -10,7 +10,7 @@
 // = |2x - (2k + 1) s| / 2s is a whole number of the smaller last bit of 2x and s, and that
 // is at least 1 / 2S (S < 2^8 the significand of s) or 1 / X of the quotient (X < 2^11 that
 // of x; 2^15 for a code times an older scale). So codes are the same in every arithmetic
-// that keeps 2^-17, and ties go to the even code once the quotient is rounded correctly.
+// that keeps 2^-17 and tells a tie.
 
 #include "../launch.h"
 #include "device_common.h"
@@ -73,17 +73,23 @@ template <NormType T> __device__ __forceinline__ float scale_for(uint32_t bits) 
   return fmaxf(__uint_as_float(up), 0x1p-126f);
 }
 
-// The codes of 4 values: x / s rounded to the nearest whole number, ties to the even one.
-// r = 1 / s correctly rounded; the remainder x - y s is exact where the quotient has few
-// bits, so that a tie is one. Adding 1.5 * 2^23 rounds and leaves the code in the low byte.
-__device__ __forceinline__ uint32_t codes4(const float* x, float s, float r) {
+// 1 / s, less and more by 2^-21 of it: above what its rounding loses, far below the distance
+// of a quotient from a half that it is not.
+struct Inverse { float lo, hi; };
+__device__ __forceinline__ Inverse inverse(float s) {
+  const float r = 1.0f / s;
+  return {r * (1.0f - 0x1p-21f), r * (1.0f + 0x1p-21f)};
+}
+// The codes of 4 values: x / s rounded to the nearest whole number, ties to the even one. 1.5 *
+// 2^23 + x / s is rounded from either side of the quotient: to the same number, or, for a tie,
+// to its two neighbours. Their sum has one bit fewer, so that it rounds to twice the even one,
+// and the code is its low byte. (With the quotient's remainder, as a division corrects it,
+// 23.9 for 23.2 us in the case below.)
+__device__ __forceinline__ uint32_t codes4(const float* x, Inverse r) {
   uint32_t w[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float y = x[i] * r;
-    const float z = fmaf(fmaf(-y, s, x[i]), r, y);
-    w[i] = __float_as_uint(z + 12582912.0f);
-  }
+  for (int i = 0; i < 4; ++i)
+    w[i] = __float_as_uint(fmaf(x[i], r.lo, 12582912.0f) + fmaf(x[i], r.hi, 12582912.0f));
   const uint32_t lo = __builtin_amdgcn_perm(w[1], w[0], 0x0c0c0400u), hi = __builtin_amdgcn_perm(w[3], w[2], 0x0c0c0400u);
   return lo | hi << 16;
 }
@@ -112,8 +118,8 @@ template <int L> __device__ __forceinline__ uint32_t lanes_max(uint32_t v) {
 // threads with N chunks of 8 values each, held in registers between the maximum and the
 // codes: read once. Rows that the block already holds are rounded again, to the new scale,
 // where that is larger. us, 8 sequences of 500 to 4000 tokens of 8 heads of 128, blocks of 32:
-// 23.9 (4.6 TB/s; stores through the caches 25.5), bound by memory with the VALU at work in
-// 60 % of the cycles (8 instructions a value); one token of 64 sequences 5.5, a launch and the
+// 23.2 (4.8 TB/s; stores through the caches 1.6 more), bound by memory with the VALU at work in
+// 47 % of the cycles; one token of 64 sequences 5.5, a launch and the
 // chain of length, table entry and rows.
 template <NormType T, int C, int L, int N, bool STREAM>   // C: chunks of a row
 __global__ __launch_bounds__(kThreads) void append_i8(AppendParams p) {
@@ -169,14 +175,14 @@ __global__ __launch_bounds__(kThreads) void append_i8(AppendParams p) {
       if (s > 0.0f) s = fmaxf(s, 0x1p-126f);
       if (need != need || before != before) s = __uint_as_float(0x7fc00000u);
       const bool fine = s > 0.0f && s <= __FLT_MAX__;
-      const float r1 = fine ? 1.0f / s : 0.0f;
+      const Inverse inv = inverse(fine ? s : 1.0f);
 #pragma unroll
       for (int i = 0; i < N; ++i) {
         const int c = i * L + l, r = c / C;
         if (r < old || r >= end) continue;
         float f[8];
         Io<T>::unpack(x[i], f);
-        u32x2 w = {codes4(f, s, r1), codes4(f + 4, s, r1)};
+        u32x2 w = {codes4(f, inv), codes4(f + 4, inv)};
         if (!fine) w = u32x2{0, 0};
         u32x2* to = (u32x2*)(pool.row(page, h, row + r) + 8 * (c % C));
         if constexpr (STREAM) __builtin_nontemporal_store(w, to);
@@ -191,7 +197,7 @@ __global__ __launch_bounds__(kThreads) void append_i8(AppendParams p) {
           float f[8];
 #pragma unroll
           for (int e = 0; e < 8; ++e) f[e] = (float)(int8_t)(w[e / 4] >> 8 * (e % 4)) * before;
-          *to = u32x2{codes4(f, s, r1), codes4(f + 4, s, r1)};
+          *to = u32x2{codes4(f, inv), codes4(f + 4, inv)};
         }
       }
       if (l == 0) *scale = s;
@@ -255,8 +261,9 @@ template <NormType T, bool STREAM> __device__ __forceinline__ void put8(uint8_t*
 
 // U rows of a key and a value to a thread's chunk, all loaded before the first is stored; a
 // head's rows follow one another, as outputs mostly lie. us, 8 sequences of 5000 to 8192 slots
-// of 8 heads of 128 into bf16: 72.9 (5.2 TB/s, of which 72 % are writes); heads side by side
-// 73, stores through the caches 78. 3 sequences of 1001 to 1500 slots of 64 5.4 (with 4 rows
+// of 8 heads of 128 into bf16: 71.2 (5.3 TB/s, of which 72 % are writes); heads side by side
+// 73, stores through the caches 78, loads through them 72.3, keys and values by different workgroups
+// 75, 8 rows at a time 80. 3 sequences of 1001 to 1500 slots of 64 5.4 (with 4 rows
 // at a time 6.3).
 template <NormType T, int C, bool STREAM>
 __global__ __launch_bounds__(kThreads) void read_i8(ReadParams p) {
@@ -284,7 +291,9 @@ __global__ __launch_bounds__(kThreads) void read_i8(ReadParams p) {
           w[x][u] = u32x2{0, 0};
           s[x][u] = 0.0f;
           if (there) {
-            w[x][u] = *(const u32x2*)(p.pool[x].row(page, h[u], row) + 8 * c);
+            const u32x2* src = (const u32x2*)(p.pool[x].row(page, h[u], row) + 8 * c);
+            if constexpr (STREAM) w[x][u] = __builtin_nontemporal_load(src);
+            else w[x][u] = *src;
             s[x][u] = *p.pool[x].scale_of(page, h[u], div_page(p.by_block, row));
           }
         }

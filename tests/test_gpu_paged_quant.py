@@ -86,6 +86,29 @@ def test_ties_go_to_the_even_code(dnn):
         assert torch.equal(c.k[int(c.table[i, 0]), :, 0].cpu(), want[i, :, 0])
 
 
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_ties_of_every_scale(dnn, dtype):
+    """Scales of every odd significand of 8 bits: all halves of codes that the type holds, and their
+    neighbours; then a row that doubles the scale, so that the odd codes before lie half way."""
+    odd = torch.arange(1, 256, 2, dtype=torch.float64)
+    c = QuantCache(torch.Generator().manual_seed(44), [0] * len(odd), 2, 2, 2, 128, room=2)
+    for power, step in ((-9, 1), (-9, 2)):
+        s = (odd * 2.0 ** power * step)[:, None, None, None]
+        k = torch.stack([torch.arange(128.0) - 64, torch.arange(128.0)])[None, :, None].double()
+        x = ((k + 0.5) * s).to(dtype)
+        most = (127 * s).to(dtype)
+        bits = most.view(torch.int16)
+        most = torch.where(most.double() > 127 * s, (bits - 1).view(dtype), most)     # not above 127 scales
+        x[..., :1] = most
+        x = torch.minimum(x, most)
+        scale = least8(most.double() / 127)
+        assert torch.equal(scale, s)
+        assert ((x.double() / scale % 1).abs() == 0.5).sum() > 1000      # ties
+        check_append(dnn, c, x.cuda(), -x.cuda())
+        c.n = [n + 1 for n in c.n]
+        c.lengths += 1
+
+
 def test_every_value_of_the_types(dnn):
     """All finite bf16 and fp16 values as rows of blocks whose largest magnitude is of every
     size: the codes and scales of 64 bits."""
