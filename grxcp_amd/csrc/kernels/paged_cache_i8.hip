@@ -99,15 +99,17 @@ typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
 template <int CTRL> __device__ __forceinline__ uint32_t dpp_max(uint32_t v) {
   return max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, CTRL, 0xf, 0xf, false));
 }
-// The largest over L neighbouring lanes (8, 16 or 64), in each.
+// The largest over L neighbouring lanes (4 to 64), in each.
 template <int L> __device__ __forceinline__ uint32_t lanes_max(uint32_t v) {
   v = dpp_max<0xb1>(v);
   v = dpp_max<0x4e>(v);
-  v = dpp_max<0x141>(v);
+  if constexpr (L >= 8) v = dpp_max<0x141>(v);
   if constexpr (L >= 16) v = dpp_max<0x140>(v);
-  if constexpr (L == 64) {
+  if constexpr (L >= 32) {
     const auto a = __builtin_amdgcn_permlane16_swap(v, v, false, false);
     v = max(a[0], a[1]);
+  }
+  if constexpr (L == 64) {
     const auto b = __builtin_amdgcn_permlane32_swap(v, v, false, false);
     v = max(b[0], b[1]);
   }
@@ -116,13 +118,14 @@ template <int L> __device__ __forceinline__ uint32_t lanes_max(uint32_t v) {
 
 // One task: the block of one head's keys or values (blockIdx.z) that gets new rows, by L
 // threads with N chunks of 8 values each, held in registers between the maximum and the
-// codes: read once. Rows that the block already holds are rounded again, to the new scale,
+// codes: read once. The threads take M tasks at a time. Rows that the block already holds are rounded again, to the new scale,
 // where that is larger. us, 8 sequences of 500 to 4000 tokens of 8 heads of 128, blocks of 32:
-// 23.2 (4.8 TB/s; stores through the caches 1.6 more), bound by memory with the VALU at work in
-// 47 % of the cycles; one token of 64 sequences 5.5, a launch and the
-// chain of length, table entry and rows.
-template <NormType T, int C, int L, int N, bool STREAM>   // C: chunks of a row
-__global__ __launch_bounds__(kThreads) void append_i8(AppendParams p) {
+// 22.4 (4.9 TB/s; stores through the caches 1.6 more, registers for eight waves a SIMD, which
+// the loads then wait in turn for, 3.2), bound by memory with the VALU at work in 47 % of the
+// cycles; one token of 64 sequences 5.5, a launch and the chain of length, table entry and rows.
+template <NormType T, int C, int L, int N, int M, bool STREAM>   // C: chunks of a row
+__global__ __launch_bounds__(kThreads, 4) void append_i8(AppendParams p) {
+  constexpr int P = kThreads / L;
   __shared__ uint32_t most_of[kThreads / 64];
   const int tid = threadIdx.x, l = tid % L;
   const Pool8& pool = p.pool[blockIdx.z];
@@ -133,100 +136,130 @@ __global__ __launch_bounds__(kThreads) void append_i8(AppendParams p) {
     if (count <= 0) continue;
     const int b0 = div_page(p.by_block, n), blocks = div_page(p.by_block, n + count - 1) - b0 + 1;
     const int64_t tasks = (int64_t)blocks * p.heads;
-    for (int64_t t0 = (int64_t)blockIdx.x * (kThreads / L); t0 < tasks; t0 += (int64_t)gridDim.x * (kThreads / L)) {
-      const int64_t task = t0 + tid / L;
-      const bool mine = task < tasks;
-      const int at = mine ? (int)task : 0;
-      const int j = div_page(p.by_heads, at), h = at - j * p.heads;
-      const int lo = (b0 + j) * p.block;                      // its first slot
-      const int old = max(0, n - lo), end = min(p.block, n + count - lo);
-      int page, row;
-      const bool there = find_slot(p.view, b, lo, &page, &row) & mine;
-      float* scale = pool.scale_of(page, h, div_page(p.by_block, row));
-      const float before = there && old > 0 ? *scale : 0.0f;
-      const uint8_t* src = in.p + b * in.sb + h * in.sh;
-      u32x4 x[N];
-      u16x2 both = {0, 0};                                    // largest magnitudes of either half of a word
+    for (int64_t t0 = (int64_t)blockIdx.x * (P * M); t0 < tasks; t0 += (int64_t)gridDim.x * (P * M)) {
+      u32x4 x[M][N];
+      int h[M], lo[M], page[M], row[M];                       // head, first slot, its place
+      bool there[M];
+      float before[M];
 #pragma unroll
-      for (int i = 0; i < N; ++i) {
-        const int c = i * L + l, r = c / C;
-        x[i] = u32x4{0, 0, 0, 0};
-        if (there && r >= old && r < end)
-          x[i] = __builtin_nontemporal_load((const u32x4*)(src + (int64_t)(lo + r - n) * in.st) + c % C);
-      }
+      for (int m = 0; m < M; ++m) {
+        const int64_t task = t0 + m * P + tid / L;
+        const bool mine = task < tasks;
+        const int at = mine ? (int)task : 0;
+        const int j = div_page(p.by_heads, at);
+        h[m] = at - j * p.heads;
+        lo[m] = (b0 + j) * p.block;
+        const int old = max(0, n - lo[m]), end = min(p.block, n + count - lo[m]);
+        there[m] = find_slot(p.view, b, lo[m], &page[m], &row[m]) & mine;
+        before[m] = there[m] && old > 0 ? *pool.scale_of(page[m], h[m], div_page(p.by_block, row[m])) : 0.0f;
+        const uint8_t* src = in.p + b * in.sb + h[m] * in.sh;
 #pragma unroll
-      for (int i = 0; i < N; ++i)
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          both = __builtin_elementwise_max(both, __builtin_bit_cast(u16x2, x[i][e] & 0x7fff7fffu));
-      uint32_t most = max(both[0], both[1]);
-      if constexpr (L <= 64) {
-        most = lanes_max<L>(most);
-      } else {
-        most = lanes_max<64>(most);
-        __syncthreads();                                      // the task before has read
-        if ((tid & 63) == 0) most_of[tid >> 6] = most;
-        __syncthreads();
-        most = max(max(most_of[0], most_of[1]), max(most_of[2], most_of[3]));
-      }
-      if (!there) continue;                                   // (L = 256: of the whole workgroup)
-      const float need = scale_for<T>(most);
-      float s = fmaxf(need, before);
-      if (s > 0.0f) s = fmaxf(s, 0x1p-126f);
-      if (need != need || before != before) s = __uint_as_float(0x7fc00000u);
-      const bool fine = s > 0.0f && s <= __FLT_MAX__;
-      const Inverse inv = inverse(fine ? s : 1.0f);
-#pragma unroll
-      for (int i = 0; i < N; ++i) {
-        const int c = i * L + l, r = c / C;
-        if (r < old || r >= end) continue;
-        float f[8];
-        Io<T>::unpack(x[i], f);
-        u32x2 w = {codes4(f, inv), codes4(f + 4, inv)};
-        if (!fine) w = u32x2{0, 0};
-        u32x2* to = (u32x2*)(pool.row(page, h, row + r) + 8 * (c % C));
-        if constexpr (STREAM) __builtin_nontemporal_store(w, to);
-        else *to = w;
-      }
-      if (old > 0 && s > before && fine) {
         for (int i = 0; i < N; ++i) {
           const int c = i * L + l, r = c / C;
-          if (r >= old) continue;
-          u32x2* to = (u32x2*)(pool.row(page, h, row + r) + 8 * (c % C));
-          u32x2 w = *to;
-          float f[8];
-#pragma unroll
-          for (int e = 0; e < 8; ++e) f[e] = (float)(int8_t)(w[e / 4] >> 8 * (e % 4)) * before;
-          *to = u32x2{codes4(f, inv), codes4(f + 4, inv)};
+          x[m][i] = u32x4{0, 0, 0, 0};
+          if (there[m] && r >= old && r < end)
+            x[m][i] = __builtin_nontemporal_load((const u32x4*)(src + (int64_t)(lo[m] + r - n) * in.st) + c % C);
         }
       }
-      if (l == 0) *scale = s;
+#pragma unroll
+      for (int m = 0; m < M; ++m) {
+        const int old = max(0, n - lo[m]), end = min(p.block, n + count - lo[m]);
+        u16x2 both = {0, 0};                                  // largest magnitudes of either half of a word
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            both = __builtin_elementwise_max(both, __builtin_bit_cast(u16x2, x[m][i][e] & 0x7fff7fffu));
+        uint32_t most = max(both[0], both[1]);
+        if constexpr (L <= 64) {
+          most = lanes_max<L>(most);
+        } else {
+          most = lanes_max<64>(most);
+          __syncthreads();                                    // the task before has read
+          if ((tid & 63) == 0) most_of[tid >> 6] = most;
+          __syncthreads();
+          most = max(max(most_of[0], most_of[1]), max(most_of[2], most_of[3]));
+        }
+        if (!there[m]) continue;                              // (L = 256: of the whole workgroup)
+        const float need = scale_for<T>(most);
+        float s = fmaxf(need, before[m]);
+        if (s > 0.0f) s = fmaxf(s, 0x1p-126f);
+        if (need != need || before[m] != before[m]) s = __uint_as_float(0x7fc00000u);
+        const bool fine = s > 0.0f && s <= __FLT_MAX__;
+        const Inverse inv = inverse(fine ? s : 1.0f);
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          const int c = i * L + l, r = c / C;
+          if (r < old || r >= end) continue;
+          float f[8];
+          Io<T>::unpack(x[m][i], f);
+          u32x2 w = {codes4(f, inv), codes4(f + 4, inv)};
+          if (!fine) w = u32x2{0, 0};
+          u32x2* to = (u32x2*)(pool.row(page[m], h[m], row[m] + r) + 8 * (c % C));
+          if constexpr (STREAM) __builtin_nontemporal_store(w, to);
+          else *to = w;
+        }
+        if (old > 0 && s > before[m] && fine) {
+          for (int i = 0; i < N; ++i) {
+            const int c = i * L + l, r = c / C;
+            if (r >= old) continue;
+            u32x2* to = (u32x2*)(pool.row(page[m], h[m], row[m] + r) + 8 * (c % C));
+            u32x2 w = *to;
+            float f[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) f[e] = (float)(int8_t)(w[e / 4] >> 8 * (e % 4)) * before[m];
+            *to = u32x2{codes4(f, inv), codes4(f + 4, inv)};
+          }
+        }
+        if (l == 0) *pool.scale_of(page[m], h[m], div_page(p.by_block, row[m])) = s;
+      }
     }
   }
 }
 
-template <NormType T, int C, bool STREAM> hipError_t run_append(const AppendParams& p, hipStream_t s) {
-  const int64_t blocks = ((int64_t)p.T + 2 * p.block - 2) / p.block;   // of a sequence, at most
-  auto go = [&](auto kern, int lanes) {
-    const int64_t tasks = blocks * p.heads, per = kThreads / lanes;
-    const dim3 grid((unsigned)std::min<int64_t>((tasks + per - 1) / per, 1 << 20), (unsigned)std::min(p.B, 65535), 2);
-    hipLaunchKernelGGL(kern, grid, dim3(kThreads), 0, s, p);
-    return hipGetLastError();
-  };
-  const int chunks = p.block * C;
-  if (p.block == 1) return go(append_i8<T, C, C, 1, STREAM>, C);
-  if (chunks <= 64) return go(append_i8<T, C, 64, 1, STREAM>, 64);
-  if (chunks <= 128) return go(append_i8<T, C, 64, 2, STREAM>, 64);
-  if (chunks <= 256) return go(append_i8<T, C, 64, 4, STREAM>, 64);
-  if (chunks <= 512) return go(append_i8<T, C, 64, 8, STREAM>, 64);
-  if (chunks <= 1024) return go(append_i8<T, C, 256, 4, STREAM>, 256);
-  if (chunks <= 2048) return go(append_i8<T, C, 256, 8, STREAM>, 256);
-  if (chunks <= 4096) return go(append_i8<T, C, 256, 16, STREAM>, 256);
-  return hipErrorNotSupported;
+template <NormType T, int C, int L, int N, int M, bool STREAM>
+hipError_t go(const AppendParams& p, int64_t tasks, hipStream_t s) {
+  const int64_t per = (int64_t)kThreads / L * M;
+  const dim3 grid((unsigned)std::min<int64_t>((tasks + per - 1) / per, 1 << 20), (unsigned)std::min(p.B, 65535), 2);
+  hipLaunchKernelGGL((append_i8<T, C, L, N, M, STREAM>), grid, dim3(kThreads), 0, s, p);
+  return hipGetLastError();
+}
+
+// Blocks of up to CHUNKS chunks. Where that makes three workgroups per CU, a thread has four
+// chunks (two of the smallest blocks), of two tasks if need be: index arithmetic, maximum and
+// scale are for all of a task's threads, and a chunk alone does not keep the memory busy. One
+// chunk each is quicker for fewer. us, one chunk / so, 8 heads of 128: 8 sequences of 500 to 4000
+// tokens, blocks of 1, 45.2 / 24.7, of 2 77 / 24.1, of 4 44.2 / 22.4; 2 of 1000 in blocks of 1
+// 5.9 / 6.8, 8 of 500 10.3 / 7.2.
+template <NormType T, int C, int CHUNKS> hipError_t run_append(const AppendParams& p, hipStream_t s) {
+  const int64_t tasks = ((int64_t)p.T + 2 * p.block - 2) / p.block * p.heads;   // of a sequence, at most
+  const bool stream = (int64_t)p.B * p.T * p.heads * C * 16 >= kStream;
+  if constexpr (CHUNKS > 512) {
+    constexpr int N = CHUNKS / 256;
+    return stream ? go<T, C, 256, N, 1, true>(p, tasks, s) : go<T, C, 256, N, 1, false>(p, tasks, s);
+  } else {
+    constexpr int N = CHUNKS > 256 ? 8 : CHUNKS > 16 ? 4 : 2, L = CHUNKS / N, M = N == 2 ? 2 : 1;
+    constexpr int few = CHUNKS < 64 ? CHUNKS : 64;
+    if (stream) return go<T, C, L, N, M, true>(p, tasks, s);
+    if (2 * p.B * tasks >= 3 * 256 * (kThreads / L * M)) return go<T, C, L, N, M, false>(p, tasks, s);
+    return go<T, C, few, CHUNKS / few, 1, false>(p, tasks, s);
+  }
 }
 
 template <NormType T, int C> hipError_t run_append(const AppendParams& p, hipStream_t s) {
-  return (int64_t)p.B * p.T * p.heads * C * 16 >= kStream ? run_append<T, C, true>(p, s) : run_append<T, C, false>(p, s);
+  const int chunks = p.block * C;
+  if constexpr (C == 8)
+    if (chunks <= 8) return run_append<T, C, 8>(p, s);
+  if (chunks <= 16) return run_append<T, C, 16>(p, s);
+  if (chunks <= 32) return run_append<T, C, 32>(p, s);
+  if (chunks <= 64) return run_append<T, C, 64>(p, s);
+  if (chunks <= 128) return run_append<T, C, 128>(p, s);
+  if (chunks <= 256) return run_append<T, C, 256>(p, s);
+  if (chunks <= 512) return run_append<T, C, 512>(p, s);
+  if (chunks <= 1024) return run_append<T, C, 1024>(p, s);
+  if (chunks <= 2048) return run_append<T, C, 2048>(p, s);
+  if (chunks <= 4096) return run_append<T, C, 4096>(p, s);
+  return hipErrorNotSupported;
 }
 
 // ---- read --------------------------------------------------------------------

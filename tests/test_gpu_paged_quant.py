@@ -59,6 +59,19 @@ def test_append(dnn, case, spread):
     check_append(dnn, c, *rows(gen, len(lengths), heads, T, d, dtype, spread), counts)
 
 
+@pytest.mark.parametrize("stream", [False, True])
+@pytest.mark.parametrize("d, page, block", [(64, 16, 1), (128, 7, 1), (64, 6, 2), (128, 9, 3), (64, 14, 7), (128, 5, 5),
+                                            (64, 24, 12), (128, 16, 16), (128, 40, 20)])
+def test_append_of_many_rows(dnn, d, page, block, stream):
+    """As many blocks as give a thread more than one chunk, or task, at a time; blocks that hold
+    rows before, odd ones, pages that do not exist, and sequences that take fewer."""
+    T = 32 * 2 ** 20 // (2 * 40 * d * 2) + 19 if stream else 1300
+    gen = torch.Generator().manual_seed(17 * d + block)
+    c = QuantCache(gen, [3 * block + block // 2, block - 1], 40, page, block, d, block % 2 == 0, room=4 * block + T)
+    c.table[0, 5], c.table[1, 2] = -1, c.k.shape[0]
+    check_append(dnn, c, *rows(gen, 2, 40, T, d, (BF16, F16)[block % 2], 1.0), [T, T - 3 * block - 1])
+
+
 def test_tokens_one_at_a_time(dnn):
     """Blocks that fill row by row, their scales growing as they do; every step against 64 bits
     from the step before."""
