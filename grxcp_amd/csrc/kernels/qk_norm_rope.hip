@@ -15,7 +15,13 @@
 //  * a workgroup takes a few tokens with all of their heads, so that cosines and sines
 //    are computed once per token (into LDS) and not once per head. A backward call's
 //    workgroups take queries or keys, and keep the sums of their gains in registers;
-//  * what does not fit the caches is loaded and stored past them, two passes at a time.
+//  * what does not fit the caches is loaded and stored past them, two passes at a time, in
+//    whole lines of 128 bytes. Where a lane's chunks are not that (rows of 64, fp32, halves that
+//    turn only a part of the row) they go through LDS. us, direct / so, 16384 tokens of 40 heads
+//    of 128 bf16 of which 32 turn 85 / 60, of 64 39.7 / 33.8, 24 heads of 128 fp32 84 / 72; backward
+//    109 / 93.6, 59.6 / 53.5, 124 / 114. Whole lines already (128 bf16) 59.6 / 59.8, backward
+//    97.3 / 100, and through the caches, which put lines together (6000 tokens of 40 heads of 64)
+//    12.2 / 12.9.
 //    Every angle, sum and product left out makes 1 % of a difference (61.5 to 60.9 us at
 //    16384 tokens of 40 heads of 128): the order of loads and stores is what counts.
 //    Queries and keys by different workgroups in the forward call took 71 for 60;
@@ -104,30 +110,36 @@ template <int G> __device__ __forceinline__ float row_sum(float v) {
   return v;
 }
 
+template <bool STREAM> __device__ __forceinline__ u32x4 load1(const uint8_t* p) {
+  if constexpr (STREAM) return __builtin_nontemporal_load((const u32x4*)p);
+  else return *(const u32x4*)p;
+}
+template <bool STREAM> __device__ __forceinline__ void store1(uint8_t* p, u32x4 w) {
+  if constexpr (STREAM) __builtin_nontemporal_store(w, (u32x4*)p);
+  else *(u32x4*)p = w;
+}
 // 8 values at p.
 template <NormType T, bool STREAM>
 __device__ __forceinline__ void load8(const uint8_t* p, u32x4 (&w)[8 / Io<T>::kVec]) {
 #pragma unroll
-  for (int i = 0; i < 8 / Io<T>::kVec; ++i) {
-    const u32x4* q = (const u32x4*)p + i;
-    if constexpr (STREAM) w[i] = __builtin_nontemporal_load(q);
-    else w[i] = *q;
-  }
+  for (int i = 0; i < 8 / Io<T>::kVec; ++i) w[i] = load1<STREAM>(p + 16 * i);
 }
 template <NormType T> __device__ __forceinline__ void unpack8(const u32x4 (&w)[8 / Io<T>::kVec], float* f) {
 #pragma unroll
   for (int i = 0; i < 8 / Io<T>::kVec; ++i) Io<T>::unpack(w[i], f + i * Io<T>::kVec);
 }
-template <NormType T, bool STREAM> __device__ __forceinline__ void store8(uint8_t* p, const float* f) {
+template <NormType T> __device__ __forceinline__ void pack8(const float* f, u32x4 (&w)[8 / Io<T>::kVec]) {
 #pragma unroll
-  for (int i = 0; i < 8 / Io<T>::kVec; ++i) {
-    const u32x4 w = Io<T>::pack(f + i * Io<T>::kVec);
-    if constexpr (STREAM) __builtin_nontemporal_store(w, (u32x4*)p + i);
-    else ((u32x4*)p)[i] = w;
-  }
+  for (int i = 0; i < 8 / Io<T>::kVec; ++i) w[i] = Io<T>::pack(f + i * Io<T>::kVec);
+}
+template <NormType T, bool STREAM> __device__ __forceinline__ void store8(uint8_t* p, const float* f) {
+  u32x4 w[8 / Io<T>::kVec];
+  pack8<T>(f, w);
+#pragma unroll
+  for (int i = 0; i < 8 / Io<T>::kVec; ++i) store1<STREAM>(p + 16 * i, w[i]);
 }
 
-template <NormType T, int D, bool PAIRS, bool BWD, bool STREAM>
+template <NormType T, int D, bool PAIRS, bool BWD, bool STREAM, bool LINES>
 __global__ __launch_bounds__(kThreads, BWD ? 3 : 1) void qk_norm_rope(RParams p) {
   constexpr int G = D / 16, RW = 64 / G;   // lanes of a row, rows of a wave
   constexpr int W = 8 / Io<T>::kVec;
@@ -135,6 +147,9 @@ __global__ __launch_bounds__(kThreads, BWD ? 3 : 1) void qk_norm_rope(RParams p)
   constexpr int U = BWD ? (Io<T>::kVec == 8 ? 2 : 1) : STREAM ? 2 : 1;   // passes at a time
   __shared__ __attribute__((aligned(16))) float cs[2][kAngles];
   __shared__ float red[BWD ? kWaves : 1][BWD ? D : 1];
+  // LINES: a pass's rows lie here between memory, where a load takes whole rows, and the lanes
+  constexpr int PR = D * E / 16, PC = 2 * W;   // 16-byte pieces of a row, of a lane
+  __shared__ __attribute__((aligned(16))) uint8_t stage[LINES ? kWaves : 1][LINES ? 64 * 16 * PC : 16];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int g = lane / G, l = lane % G;
   const int half = p.rotary / 2, rc = p.rotary / 16;
@@ -144,10 +159,32 @@ __global__ __launch_bounds__(kThreads, BWD ? 3 : 1) void qk_norm_rope(RParams p)
   // the lane's two chunks of 8 values
   int c0 = l, c1 = l + G;
   if constexpr (!PAIRS) {
-    c0 = l < rc ? l : 2 * l;               // behind the rotated ones: 2 rc + 2 (l - rc)
-    c1 = l < rc ? l + rc : 2 * l + 1;
+    c0 = l < rc ? l : l + rc;              // behind the rotated ones: 2 rc + l - rc
+    c1 = l < rc ? l + rc : l + G;
   }
   const int o0 = 8 * E * c0, o1 = 8 * E * c1;
+  // A lane's pieces of the pass's memory (in: before, else after) for its two chunks' 16 bytes each.
+  auto turn = [&](u32x4 (&w)[2][W], bool in) __attribute__((always_inline)) {
+    uint8_t* rows = stage[LINES ? wave : 0];
+    u32x4* lines = (u32x4*)rows + lane;
+    u32x4* chunks[2] = {(u32x4*)(rows + g * D * E + o0), (u32x4*)(rows + g * D * E + o1)};
+    if (in) {
+#pragma unroll
+      for (int k = 0; k < PC; ++k) lines[64 * k] = w[k / W][k % W];
+    } else {
+#pragma unroll
+      for (int k = 0; k < PC; ++k) chunks[k / W][k % W] = w[k / W][k % W];
+    }
+    __builtin_amdgcn_wave_barrier();
+    if (in) {
+#pragma unroll
+      for (int k = 0; k < PC; ++k) w[k / W][k % W] = chunks[k / W][k % W];
+    } else {
+#pragma unroll
+      for (int k = 0; k < PC; ++k) w[k / W][k % W] = lines[64 * k];
+    }
+    __builtin_amdgcn_wave_barrier();
+  };
   float acc[2][8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) acc[0][i] = acc[1][i] = 0.0f;
@@ -174,7 +211,7 @@ __global__ __launch_bounds__(kThreads, BWD ? 3 : 1) void qk_norm_rope(RParams p)
     for (int first = w; first < passes; first += U * waves) {
       // U passes' rows are asked for before the first is waited for
       u32x4 wx[U][2][W], wd[U][2][W];
-      int64_t yo[U];
+      int64_t yo[U][LINES ? PC : 1];
       int toks[U];
       bool lives[U];
 #pragma unroll
@@ -187,6 +224,18 @@ __global__ __launch_bounds__(kThreads, BWD ? 3 : 1) void qk_norm_rope(RParams p)
         lives[u] = r < rows;
         const int row = min(r, rows - 1);
         toks[u] = div_page(q.by_heads, row);
+        if constexpr (LINES) {
+#pragma unroll
+          for (int k = 0; k < PC; ++k) {
+            const int at = min(r - g + (64 * k + lane) / PR, rows - 1), piece = 16 * (lane % PR);
+            const int tok = div_page(q.by_heads, at), h = at - tok * q.heads;
+            const int b = div_page(p.by_s, t0 + tok), s = t0 + tok - b * p.S;
+            if (!BWD || norm) wx[u][k / W][k % W] = load1<STREAM>(q.x.at(b, h, s) + piece);
+            if constexpr (BWD) wd[u][k / W][k % W] = load1<STREAM>(q.dy.at(b, h, s) + piece);
+            yo[u][k] = b * q.y.sb + h * q.y.sh + s * q.y.ss + piece;
+          }
+          continue;
+        }
         const int h = row - toks[u] * q.heads;
         const int b = div_page(p.by_s, t0 + toks[u]), s = t0 + toks[u] - b * p.S;
         if (!BWD || norm) {
@@ -199,7 +248,7 @@ __global__ __launch_bounds__(kThreads, BWD ? 3 : 1) void qk_norm_rope(RParams p)
           load8<T, STREAM>(pd + o0, wd[u][0]);
           load8<T, STREAM>(pd + o1, wd[u][1]);
         }
-        yo[u] = b * q.y.sb + h * q.y.sh + s * q.y.ss;
+        yo[u][0] = b * q.y.sb + h * q.y.sh + s * q.y.ss;
       }
 #pragma unroll
       for (int u = 0; u < U; ++u) {
@@ -228,7 +277,11 @@ __global__ __launch_bounds__(kThreads, BWD ? 3 : 1) void qk_norm_rope(RParams p)
             *(f32x4*)(si + 4) = *(const f32x4*)&cs[1][k + 4];
           }
         }
-        if (!lives[u]) continue;             // (whole rows: the others' sums are their own)
+        if constexpr (LINES) {
+          if (!BWD || norm) turn(wx[u], true);
+          if constexpr (BWD) turn(wd[u], true);
+        }
+        if (lives[u]) {                      // (whole rows: the others' sums are their own)
         float x[2][8], d[2][8], inv = 1.0f;
         if (!BWD || norm) {
           unpack8<T>(wx[u][0], x[0]);
@@ -305,9 +358,23 @@ __global__ __launch_bounds__(kThreads, BWD ? 3 : 1) void qk_norm_rope(RParams p)
                 for (int i = 0; i < 8; ++i) d[c][i] = fmaf(-x[c][i], by, d[c][i]);
             }
           }
-        uint8_t* py = q.y.p + yo[u];
-        store8<T, STREAM>(py + o0, v[0]);
-        store8<T, STREAM>(py + o1, v[1]);
+        if constexpr (!LINES) {
+          uint8_t* py = q.y.p + yo[u][0];
+          store8<T, STREAM>(py + o0, v[0]);
+          store8<T, STREAM>(py + o1, v[1]);
+        } else {
+          pack8<T>(v[0], wx[u][0]);
+          pack8<T>(v[1], wx[u][1]);
+        }
+        }
+        if constexpr (LINES) {
+          turn(wx[u], false);
+          const int r0 = (BWD || first + u * waves < passes0 ? first + u * waves : first + u * waves - passes0) * RW;
+          const int rows = n * q.heads;
+#pragma unroll
+          for (int k = 0; k < PC; ++k)
+            if (r0 + (64 * k + lane) / PR < rows) store1<STREAM>(q.y.p + yo[u][k], wx[u][k / W][k % W]);
+        }
       }
     }
   }
@@ -427,18 +494,28 @@ template <NormType T, int D> hipError_t run(const QkRopeDesc& d, bool bwd, hipSt
   if (r.group[0].wgs + r.group[1].wgs) {
     const dim3 grid(r.group[0].wgs + r.group[1].wgs, r.y), threads(kThreads);
     auto go = [&](auto kern) { hipLaunchKernelGGL(kern, grid, threads, 0, s, p); };
-    auto pick = [&](auto go, auto st) {
-      constexpr bool ST = decltype(st)::value;
+    auto pick = [&](auto st, auto li) {
+      constexpr bool ST = decltype(st)::value, LI = decltype(li)::value;
       if (bwd) {
-        if (d.pairs) go(qk_norm_rope<T, D, true, true, ST>);
-        else go(qk_norm_rope<T, D, false, true, ST>);
+        if (d.pairs) go(qk_norm_rope<T, D, true, true, ST, LI>);
+        else go(qk_norm_rope<T, D, false, true, ST, LI>);
       } else {
-        if (d.pairs) go(qk_norm_rope<T, D, true, false, ST>);
-        else go(qk_norm_rope<T, D, false, false, ST>);
+        if (d.pairs) go(qk_norm_rope<T, D, true, false, ST, LI>);
+        else go(qk_norm_rope<T, D, false, false, ST, LI>);
       }
     };
-    if (stream) pick(go, std::integral_constant<bool, true>{});
-    else pick(go, std::integral_constant<bool, false>{});
+    const std::integral_constant<bool, true> yes;
+    const std::integral_constant<bool, false> no;
+    // Whether a lane's loads and stores are of whole lines by themselves.
+    constexpr bool wide = T != NormType::F32 && D >= 128;
+    if (!stream) {
+      pick(no, no);
+    } else if constexpr (wide) {
+      if (d.pairs || d.rotary == D || d.rotary == 0) pick(yes, no);
+      else pick(yes, yes);
+    } else {
+      pick(yes, yes);
+    }
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
   }

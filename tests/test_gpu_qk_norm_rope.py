@@ -209,6 +209,41 @@ def test_backward_against_64_bits(dnn, case):
     check_backward(dnn, c, str(CASES[case]))
 
 
+LARGE = [
+    # calls past the caches: 48 MB and more, rows that end inside a pass
+    (BF16, 2, 2003, 40, 10, 128, 128, False, True, 0, True),
+    (BF16, 2, 4099, 40, 9, 64, 64, False, True, 0, True),
+    (F16, 1, 5003, 33, 7, 128, 48, False, True, 0, False),
+    (BF16, 3, 1111, 23, 7, 256, 96, False, True, 7, True),
+    (FP32, 1, 4999, 17, 3, 128, 128, False, True, 0, False),
+    (FP32, 2, 3001, 33, 0, 64, 32, True, True, 0, True),
+    (BF16, 1, 8193, 44, 5, 64, 48, True, False, 0, True),
+    (FP32, 5, 501, 15, 5, 256, 240, False, False, 0, False),
+]
+
+
+@pytest.mark.parametrize("case", range(len(LARGE)))
+def test_large_calls(dnn, case):
+    say(f"qk_norm_rope {LARGE[case]}")
+    c = Case(500 + case, *LARGE[case])
+    check_forward(dnn, c, str(LARGE[case]))
+    say(f"qk_norm_rope backward {LARGE[case]}")
+    check_backward(dnn, c, str(LARGE[case]))
+
+
+def test_large_calls_in_place(dnn):
+    args = (F16, 1, 8195, 41, 8, 64, 64, False, True, 0, True)
+    for where in (None, "x", "dy"):
+        say(f"qk_norm_rope in place, large: {where}")
+        c = Case(510, *args)
+        if where:
+            check_backward(dnn, c, "in place", inplace=where)
+        else:
+            v = c.packed[:, 49:].clone()
+            check_forward(dnn, c, "in place", inplace=True)
+            assert torch.equal(c.packed[:, 49:], v)
+
+
 def test_the_gradient_is_that_of_differences():
     """backward_ref against central differences of forward_ref (host, 64 bits)."""
     gen = torch.Generator().manual_seed(1)
