@@ -274,10 +274,11 @@ struct ReadParams {
   int B, T, heads;
 };
 
-// 8 codes times their scale s; `odd`: some of a wave's products may lie past the type's range,
+// 8 codes times their scale s, to memory; as fp32 the second four lie C pieces of 16 bytes behind
+// the first, so that the threads of a row write neighbouring ones; `odd`: some of a wave's products may lie past the type's range,
 // where they are its largest value, or s may be no number.
 template <NormType T> constexpr float kMost = T == NormType::F16 ? 65504.0f : T == NormType::BF16 ? 0x1.fep127f : __FLT_MAX__;
-template <NormType T, bool STREAM> __device__ __forceinline__ void put8(uint8_t* to, u32x2 w, float s, bool odd) {
+template <NormType T, int C, bool STREAM> __device__ __forceinline__ void put8(uint8_t* to, u32x2 w, float s, bool odd) {
   float f[8];
 #pragma unroll
   for (int e = 0; e < 8; ++e) f[e] = (float)(int8_t)(w[e / 4] >> 8 * (e % 4)) * s;
@@ -287,21 +288,22 @@ template <NormType T, bool STREAM> __device__ __forceinline__ void put8(uint8_t*
 #pragma unroll
   for (int i = 0; i < 8 / Io<T>::kVec; ++i) {
     const u32x4 x = Io<T>::pack(f + i * Io<T>::kVec);
-    if constexpr (STREAM) __builtin_nontemporal_store(x, (u32x4*)to + i);
-    else ((u32x4*)to)[i] = x;
+    if constexpr (STREAM) __builtin_nontemporal_store(x, (u32x4*)to + i * C);
+    else ((u32x4*)to)[i * C] = x;
   }
 }
 
 // U rows of a key and a value to a thread's chunk, all loaded before the first is stored; a
 // head's rows follow one another, as outputs mostly lie. us, 8 sequences of 5000 to 8192 slots
-// of 8 heads of 128 into bf16: 71.2 (5.3 TB/s, of which 72 % are writes); heads side by side
-// 73, stores through the caches 78, loads through them 72.3, keys and values by different workgroups
-// 75, 8 rows at a time 80. 3 sequences of 1001 to 1500 slots of 64 5.4 (with 4 rows
-// at a time 6.3).
+// of 8 heads of 128 into bf16: 71.4 (5.3 TB/s, of which 72 % are writes); heads side by side 73,
+// stores through the caches 78, loads through them 72.3, keys and values by different
+// workgroups 75, 8 rows at a time 80. Into fp32 120 (5.2 TB/s); 4 rows at a time 125, a thread's
+// eight values side by side, which leaves lines half written, 155. 3 sequences of 1001 to 1500
+// slots of 64 5.4 (with 4 rows at a time 6.3).
+constexpr int rows_of(NormType t, bool stream) { return stream && t != NormType::F32 ? 4 : 2; }
 template <NormType T, int C, bool STREAM>
 __global__ __launch_bounds__(kThreads) void read_i8(ReadParams p) {
-  constexpr int R = kThreads / C, U = STREAM ? 4 : 2;
-  constexpr int E = T == NormType::F32 ? 4 : 2;
+  constexpr int R = kThreads / C, U = rows_of(T, STREAM);
   const int c = threadIdx.x % C, first = threadIdx.x / C;
   const int rows = p.T * p.heads;
   for (int b = blockIdx.y; b < p.B; b += gridDim.y) {
@@ -324,9 +326,10 @@ __global__ __launch_bounds__(kThreads) void read_i8(ReadParams p) {
           w[x][u] = u32x2{0, 0};
           s[x][u] = 0.0f;
           if (there) {
-            const u32x2* src = (const u32x2*)(p.pool[x].row(page, h[u], row) + 8 * c);
-            if constexpr (STREAM) w[x][u] = __builtin_nontemporal_load(src);
-            else w[x][u] = *src;
+            const uint8_t* src = p.pool[x].row(page, h[u], row);
+            if constexpr (T == NormType::F32) w[x][u] = u32x2{((const uint32_t*)src)[c], ((const uint32_t*)src)[C + c]};
+            else if constexpr (STREAM) w[x][u] = __builtin_nontemporal_load((const u32x2*)src + c);
+            else w[x][u] = ((const u32x2*)src)[c];
             s[x][u] = *p.pool[x].scale_of(page, h[u], div_page(p.by_block, row));
           }
         }
@@ -338,7 +341,7 @@ __global__ __launch_bounds__(kThreads) void read_i8(ReadParams p) {
         for (int x = 0; x < 2; ++x) {
           const bool odd = __ballot(!(fabsf(s[x][u]) <= kMost<T> / 128.0f)) != 0;
           uint8_t* to = p.out[x] + b * p.sb[x] + h[u] * p.sh[x] + t[u] * p.st[x];
-          put8<T, STREAM>(to + 8 * E * c, w[x][u], s[x][u], odd);
+          put8<T, C, STREAM>(to + 16 * c, w[x][u], s[x][u], odd);
         }
       }
     }
@@ -348,7 +351,7 @@ __global__ __launch_bounds__(kThreads) void read_i8(ReadParams p) {
 template <NormType T, int C> hipError_t run_read(const ReadParams& p, hipStream_t s) {
   const int64_t rows = (int64_t)p.T * p.heads;
   const bool stream = p.B * rows * C * 16 >= kStream;
-  const int64_t per = kThreads / C * (stream ? 4 : 2);
+  const int64_t per = kThreads / C * rows_of(T, stream);
   const dim3 grid((unsigned)std::min<int64_t>((rows + per - 1) / per, 1 << 20), (unsigned)std::min(p.B, 65535));
   if (stream) hipLaunchKernelGGL((read_i8<T, C, true>), grid, dim3(kThreads), 0, s, p);
   else hipLaunchKernelGGL((read_i8<T, C, false>), grid, dim3(kThreads), 0, s, p);

@@ -269,6 +269,16 @@ def test_read(dnn, case):
     check_read(dnn, c, dtype, T, first)
 
 
+@pytest.mark.parametrize("dtype", [BF16, F16, FP32])
+@pytest.mark.parametrize("d, page, block", [(64, 32, 32), (128, 21, 21)])
+def test_large_reads(dnn, d, page, block, dtype):
+    """Calls past the caches, from the middle of the sequences to behind their ends."""
+    T = 32 * 2 ** 20 // (3 * 40 * d * 2) + 5
+    c = QuantCache(torch.Generator().manual_seed(59), [T + 7, 300, T + 40], 40, page, block, d, d == 64)
+    c.table[2, 3] = -1
+    check_read(dnn, c, dtype, T, [11, 0, 40])
+
+
 def test_read_outside_the_sequences(dnn):
     """First slots past the end and below 0, lengths outside the table, pages that do not exist."""
     gen = torch.Generator().manual_seed(70)
