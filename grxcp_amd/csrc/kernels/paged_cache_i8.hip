@@ -94,6 +94,15 @@ __device__ __forceinline__ uint32_t codes4(const float* x, Inverse r) {
   return lo | hi << 16;
 }
 
+// The same of scales of any bits, which only a caller sets: 64-bit quotients.
+__device__ __forceinline__ bool few_bits(float s) { return (__float_as_uint(s) & 0xffffu) == 0; }
+__device__ __forceinline__ u32x2 codes8(const float* x, double times, double s) {
+  u32x2 w = {0, 0};
+#pragma unroll
+  for (int e = 0; e < 8; ++e) w[e / 4] |= ((uint32_t)(int)rint(x[e] * times / s) & 255u) << 8 * (e % 4);
+  return w;
+}
+
 typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
 
 template <int CTRL> __device__ __forceinline__ uint32_t dpp_max(uint32_t v) {
@@ -140,7 +149,8 @@ __global__ __launch_bounds__(kThreads, 4) void append_i8(AppendParams p) {
       u32x4 x[M][N];
       int h[M], lo[M], page[M], row[M];                       // head, first slot, its place
       bool there[M];
-      float before[M];
+      float before[M], now[M];
+      int rest = 0;
 #pragma unroll
       for (int m = 0; m < M; ++m) {
         const int64_t task = t0 + m * P + tid / L;
@@ -187,6 +197,14 @@ __global__ __launch_bounds__(kThreads, 4) void append_i8(AppendParams p) {
         if (need != need || before[m] != before[m]) s = __uint_as_float(0x7fc00000u);
         const bool fine = s > 0.0f && s <= __FLT_MAX__;
         const Inverse inv = inverse(fine ? s : 1.0f);
+        const bool grew = old > 0 && s > before[m] && fine;
+        const bool many_bits = fine && !(few_bits(s) && (!grew || few_bits(before[m])));
+        if (l == 0) *pool.scale_of(page[m], h[m], div_page(p.by_block, row[m])) = s;
+        if (many_bits) {
+          rest |= 1 << m;
+          now[m] = s;
+          continue;
+        }
 #pragma unroll
         for (int i = 0; i < N; ++i) {
           const int c = i * L + l, r = c / C;
@@ -199,7 +217,7 @@ __global__ __launch_bounds__(kThreads, 4) void append_i8(AppendParams p) {
           if constexpr (STREAM) __builtin_nontemporal_store(w, to);
           else *to = w;
         }
-        if (old > 0 && s > before[m] && fine) {
+        if (grew) {
           for (int i = 0; i < N; ++i) {
             const int c = i * L + l, r = c / C;
             if (r >= old) continue;
@@ -211,7 +229,37 @@ __global__ __launch_bounds__(kThreads, 4) void append_i8(AppendParams p) {
             *to = u32x2{codes4(f, inv), codes4(f + 4, inv)};
           }
         }
-        if (l == 0) *pool.scale_of(page[m], h[m], div_page(p.by_block, row[m])) = s;
+      }
+      if (rest == 0) continue;
+      // tasks with scales of many bits, apart from what the others hold in registers
+#pragma unroll 1
+      for (int m = 0; m < M; ++m) {
+        if (!(rest >> m & 1)) continue;
+        const float s = m ? now[M - 1] : now[0], was = m ? before[M - 1] : before[0];
+        const int at = (int)(t0 + m * P + tid / L), j = div_page(p.by_heads, at), head = at - j * p.heads;
+        const int first = (b0 + j) * p.block, old = max(0, n - first), end = min(p.block, n + count - first);
+        int pg, slot;
+        find_slot(p.view, b, first, &pg, &slot);
+        const uint8_t* src = in.p + b * in.sb + head * in.sh;
+#pragma unroll 1
+        for (int c = l; c < N * L; c += L) {
+          const int r = c / C;
+          u32x2* to = (u32x2*)(pool.row(pg, head, slot + r) + 8 * (c % C));
+          float f[8];
+          double by = 1.0;
+          if (r < old) {
+            if (!(s > was)) continue;
+            const u32x2 w = *to;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) f[e] = (float)(int8_t)(w[e / 4] >> 8 * (e % 4));
+            by = was;
+          } else if (r < end) {
+            Io<T>::unpack(((const u32x4*)(src + (int64_t)(first + r - n) * in.st))[c % C], f);
+          } else {
+            continue;
+          }
+          *to = codes8(f, by, s);
+        }
       }
     }
   }

@@ -122,6 +122,26 @@ def test_ties_of_every_scale(dnn, dtype):
         c.lengths += 1
 
 
+@pytest.mark.parametrize("dtype, d, block, heads, T", [
+    (BF16, 64, 1, 2, 5), (F16, 128, 2, 2, 7), (BF16, 128, 16, 2, 35), (F16, 64, 32, 2, 67), (F16, 128, 64, 2, 131),
+    (BF16, 64, 7, 2, 17), (F16, 64, 2, 40, 150)])     # the last: two tasks to a thread
+def test_scales_that_the_caller_set(dnn, dtype, d, block, heads, T):
+    """Blocks with scales of 24 bits: larger than the new rows need, smaller (the rows before are
+    rounded again), and quotients so close to a half that fp32 would miss it."""
+    gen = torch.Generator().manual_seed(45)
+    n = 3 * block + block // 2
+    c = QuantCache(gen, [n] * 12, heads, 2 * block, block, d, block == 16, room=n + T, dtype=dtype, quick=True)
+    k, v = rows(gen, 12, heads, T, d, dtype, 1.0)
+    new = block - block // 2                 # rows that the block of each head still takes
+    page, at = c.table[:, 3 * block // c.page].long(), 3 * block % c.page // block
+    for t, scale in ((k, c.ks), (v, c.vs)):
+        by = scale[page, :, at][:, :, None, None] * (1 + 2.0 ** -20 * torch.randint(-9, 9, (12, heads, 1, 1), generator=gen).cuda())
+        scale[page, :, at] = by[:, :, 0, 0]
+        half = (torch.arange(new * d, device="cuda").reshape(new, d) % 100 + 0.5) * by
+        t[:6, :, :new] = half[:6].to(dtype)
+    check_append(dnn, c, k, v)
+
+
 def test_every_value_of_the_types(dnn):
     """All finite bf16 and fp16 values as rows of blocks whose largest magnitude is of every
     size: the codes and scales of 64 bits."""
