@@ -281,7 +281,7 @@ hipError_t go(const AppendParams& p, int64_t tasks, hipStream_t s) {
 // 5.9 / 6.8, 8 of 500 10.3 / 7.2.
 template <NormType T, int C, int CHUNKS> hipError_t run_append(const AppendParams& p, hipStream_t s) {
   const int64_t tasks = ((int64_t)p.T + 2 * p.block - 2) / p.block * p.heads;   // of a sequence, at most
-  const bool stream = (int64_t)p.B * p.T * p.heads * C * 16 >= kStream;
+  const bool stream = (double)p.B * p.T * p.heads * (C * 16) >= kStream;   // (rows may be broadcast: no limit but ints')
   if constexpr (CHUNKS > 512) {
     constexpr int N = CHUNKS / 256;
     return stream ? go<T, C, 256, N, 1, true>(p, tasks, s) : go<T, C, 256, N, 1, false>(p, tasks, s);
@@ -289,7 +289,7 @@ template <NormType T, int C, int CHUNKS> hipError_t run_append(const AppendParam
     constexpr int N = CHUNKS > 256 ? 8 : CHUNKS > 16 ? 4 : 2, L = CHUNKS / N, M = N == 2 ? 2 : 1;
     constexpr int few = CHUNKS < 64 ? CHUNKS : 64;
     if (stream) return go<T, C, L, N, M, true>(p, tasks, s);
-    if (2 * p.B * tasks >= 3 * 256 * (kThreads / L * M)) return go<T, C, L, N, M, false>(p, tasks, s);
+    if (2.0 * p.B * tasks >= 3 * 256 * (kThreads / L * M)) return go<T, C, L, N, M, false>(p, tasks, s);
     return go<T, C, few, CHUNKS / few, 1, false>(p, tasks, s);
   }
 }
