@@ -127,8 +127,8 @@ template <int L> __device__ __forceinline__ uint32_t lanes_max(uint32_t v) {
 
 // One task: the block of one head's keys or values (blockIdx.z) that gets new rows, by L
 // threads with N chunks of 8 values each, held in registers between the maximum and the
-// codes: read once. The threads take M tasks at a time. Rows that the block already holds are rounded again, to the new scale,
-// where that is larger. us, 8 sequences of 500 to 4000 tokens of 8 heads of 128, blocks of 32:
+// codes: read once. The threads take M tasks at a time. Rows that the block already holds are
+// rounded again, to the new scale, where that is larger. us, 8 sequences of 500 to 4000 tokens of 8 heads of 128, blocks of 32:
 // 22.4 (4.9 TB/s; stores through the caches 1.6 more, registers for eight waves a SIMD, which
 // the loads then wait in turn for, 3.2), bound by memory with the VALU at work in 47 % of the
 // cycles; one token of 64 sequences 5.5, a launch and the chain of length, table entry and rows.
@@ -281,7 +281,8 @@ hipError_t go(const AppendParams& p, int64_t tasks, hipStream_t s) {
 // 5.9 / 6.8, 8 of 500 10.3 / 7.2.
 template <NormType T, int C, int CHUNKS> hipError_t run_append(const AppendParams& p, hipStream_t s) {
   const int64_t tasks = ((int64_t)p.T + 2 * p.block - 2) / p.block * p.heads;   // of a sequence, at most
-  const bool stream = (double)p.B * p.T * p.heads * (C * 16) >= kStream;   // (rows may be broadcast: no limit but ints')
+  // (in floating point: broadcast rows may be any number)
+  const bool stream = (double)p.B * p.T * p.heads * (C * 16) >= kStream;
   if constexpr (CHUNKS > 512) {
     constexpr int N = CHUNKS / 256;
     return stream ? go<T, C, 256, N, 1, true>(p, tasks, s) : go<T, C, 256, N, 1, false>(p, tasks, s);
@@ -323,8 +324,8 @@ struct ReadParams {
 };
 
 // 8 codes times their scale s, to memory; as fp32 the second four lie C pieces of 16 bytes behind
-// the first, so that the threads of a row write neighbouring ones; `odd`: some of a wave's products may lie past the type's range,
-// where they are its largest value, or s may be no number.
+// the first, so that the threads of a row write neighbouring ones; `odd`: some of a wave's
+// products may lie past the type's range, where they are its largest value, or s may be no number.
 template <NormType T> constexpr float kMost = T == NormType::F16 ? 65504.0f : T == NormType::BF16 ? 0x1.fep127f : __FLT_MAX__;
 template <NormType T, int C, bool STREAM> __device__ __forceinline__ void put8(uint8_t* to, u32x2 w, float s, bool odd) {
   float f[8];

@@ -163,7 +163,7 @@ __global__ __launch_bounds__(kThreads, BWD ? 3 : 1) void qk_norm_rope(RParams p)
     c1 = l < rc ? l + rc : l + G;
   }
   const int o0 = 8 * E * c0, o1 = 8 * E * c1;
-  // A lane's pieces of the pass's memory (in: before, else after) for its two chunks' 16 bytes each.
+  // A lane's pieces of the pass's rows as they lie in memory against its two chunks: in, or back.
   auto turn = [&](u32x4 (&w)[2][W], bool in) __attribute__((always_inline)) {
     uint8_t* rows = stage[LINES ? wave : 0];
     u32x4* lines = (u32x4*)rows + lane;
@@ -282,90 +282,90 @@ __global__ __launch_bounds__(kThreads, BWD ? 3 : 1) void qk_norm_rope(RParams p)
           if constexpr (BWD) turn(wd[u], true);
         }
         if (lives[u]) {                      // (whole rows: the others' sums are their own)
-        float x[2][8], d[2][8], inv = 1.0f;
-        if (!BWD || norm) {
-          unpack8<T>(wx[u][0], x[0]);
-          unpack8<T>(wx[u][1], x[1]);
-        }
-        if (norm) {
-          float ss = 0.0f;
-#pragma unroll
-          for (int i = 0; i < 8; ++i) ss = fmaf(x[0][i], x[0][i], fmaf(x[1][i], x[1][i], ss));
-          inv = __builtin_amdgcn_rsqf(fmaf(row_sum<G>(ss), 1.0f / D, p.eps));
-        }
-        if constexpr (BWD) {
-          unpack8<T>(wd[u][0], d[0]);
-          unpack8<T>(wd[u][1], d[1]);
-        }
-        float gam[2][8];
-        if (norm) {
-          unpack8<T>(wg[0], gam[0]);
-          unpack8<T>(wg[1], gam[1]);
-        }
-        float (&v)[2][8] = BWD ? d : x;      // what is turned
-        if constexpr (!BWD)
-          if (norm)
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              v[0][i] *= inv * gam[0][i];
-              v[1][i] *= inv * gam[1][i];
-            }
-        if constexpr (PAIRS) {
-#pragma unroll
-          for (int c = 0; c < 2; ++c)
-            if ((c ? c1 : c0) < 2 * rc)
-#pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                const float a = v[c][2 * i], b = v[c][2 * i + 1];
-                const float k = co[4 * c + i], m = BWD ? -si[4 * c + i] : si[4 * c + i];
-                v[c][2 * i] = fmaf(a, k, -(b * m));
-                v[c][2 * i + 1] = fmaf(b, k, a * m);
-              }
-        } else {
-          if (l < rc)
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              const float a = v[0][i], b = v[1][i];
-              const float m = BWD ? -si[i] : si[i];
-              v[0][i] = fmaf(a, co[i], -(b * m));
-              v[1][i] = fmaf(b, co[i], a * m);
-            }
-        }
-        if constexpr (BWD)
+          float x[2][8], d[2][8], inv = 1.0f;
+          if (!BWD || norm) {
+            unpack8<T>(wx[u][0], x[0]);
+            unpack8<T>(wx[u][1], x[1]);
+          }
           if (norm) {
-            // with u = r g: dgamma += u x, dx = u gamma - x r^2 mean(u gamma x)
-            float dot = 0.0f;
+            float ss = 0.0f;
 #pragma unroll
-            for (int c = 0; c < 2; ++c)
+            for (int i = 0; i < 8; ++i) ss = fmaf(x[0][i], x[0][i], fmaf(x[1][i], x[1][i], ss));
+            inv = __builtin_amdgcn_rsqf(fmaf(row_sum<G>(ss), 1.0f / D, p.eps));
+          }
+          if constexpr (BWD) {
+            unpack8<T>(wd[u][0], d[0]);
+            unpack8<T>(wd[u][1], d[1]);
+          }
+          float gam[2][8];
+          if (norm) {
+            unpack8<T>(wg[0], gam[0]);
+            unpack8<T>(wg[1], gam[1]);
+          }
+          float (&v)[2][8] = BWD ? d : x;      // what is turned
+          if constexpr (!BWD)
+            if (norm)
 #pragma unroll
               for (int i = 0; i < 8; ++i) {
-                d[c][i] *= inv;
-                acc[c][i] = fmaf(d[c][i], x[c][i], acc[c][i]);
-                d[c][i] *= gam[c][i];
-                dot = fmaf(d[c][i], x[c][i], dot);
+                v[0][i] *= inv * gam[0][i];
+                v[1][i] *= inv * gam[1][i];
               }
-            dot = row_sum<G>(dot) * (1.0f / D);
-            const float by = inv * inv * dot;
-            if (!(fabsf(by) <= __FLT_MAX__)) {   // (eps 0 and tiny rows, or no numbers)
+          if constexpr (PAIRS) {
 #pragma unroll
-              for (int c = 0; c < 2; ++c)
+            for (int c = 0; c < 2; ++c)
+              if ((c ? c1 : c0) < 2 * rc)
 #pragma unroll
-                for (int i = 0; i < 8; ++i) d[c][i] = fmaf(-(x[c][i] * inv), inv * dot, d[c][i]);
-            } else {
+                for (int i = 0; i < 4; ++i) {
+                  const float a = v[c][2 * i], b = v[c][2 * i + 1];
+                  const float k = co[4 * c + i], m = BWD ? -si[4 * c + i] : si[4 * c + i];
+                  v[c][2 * i] = fmaf(a, k, -(b * m));
+                  v[c][2 * i + 1] = fmaf(b, k, a * m);
+                }
+          } else {
+            if (l < rc)
 #pragma unroll
-              for (int c = 0; c < 2; ++c)
-#pragma unroll
-                for (int i = 0; i < 8; ++i) d[c][i] = fmaf(-x[c][i], by, d[c][i]);
-            }
+              for (int i = 0; i < 8; ++i) {
+                const float a = v[0][i], b = v[1][i];
+                const float m = BWD ? -si[i] : si[i];
+                v[0][i] = fmaf(a, co[i], -(b * m));
+                v[1][i] = fmaf(b, co[i], a * m);
+              }
           }
-        if constexpr (!LINES) {
-          uint8_t* py = q.y.p + yo[u][0];
-          store8<T, STREAM>(py + o0, v[0]);
-          store8<T, STREAM>(py + o1, v[1]);
-        } else {
-          pack8<T>(v[0], wx[u][0]);
-          pack8<T>(v[1], wx[u][1]);
-        }
+          if constexpr (BWD)
+            if (norm) {
+              // with u = r g: dgamma += u x, dx = u gamma - x r^2 mean(u gamma x)
+              float dot = 0.0f;
+#pragma unroll
+              for (int c = 0; c < 2; ++c)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                  d[c][i] *= inv;
+                  acc[c][i] = fmaf(d[c][i], x[c][i], acc[c][i]);
+                  d[c][i] *= gam[c][i];
+                  dot = fmaf(d[c][i], x[c][i], dot);
+                }
+              dot = row_sum<G>(dot) * (1.0f / D);
+              const float by = inv * inv * dot;
+              if (!(fabsf(by) <= __FLT_MAX__)) {   // (eps 0 and tiny rows, or no numbers)
+#pragma unroll
+                for (int c = 0; c < 2; ++c)
+#pragma unroll
+                  for (int i = 0; i < 8; ++i) d[c][i] = fmaf(-(x[c][i] * inv), inv * dot, d[c][i]);
+              } else {
+#pragma unroll
+                for (int c = 0; c < 2; ++c)
+#pragma unroll
+                  for (int i = 0; i < 8; ++i) d[c][i] = fmaf(-x[c][i], by, d[c][i]);
+              }
+            }
+          if constexpr (!LINES) {
+            uint8_t* py = q.y.p + yo[u][0];
+            store8<T, STREAM>(py + o0, v[0]);
+            store8<T, STREAM>(py + o1, v[1]);
+          } else {
+            pack8<T>(v[0], wx[u][0]);
+            pack8<T>(v[1], wx[u][1]);
+          }
         }
         if constexpr (LINES) {
           turn(wx[u], false);

@@ -135,7 +135,8 @@ def test_scales_that_the_caller_set(dnn, dtype, d, block, heads, T):
     new = block - block // 2                 # rows that the block of each head still takes
     page, at = c.table[:, 3 * block // c.page].long(), 3 * block % c.page // block
     for t, scale in ((k, c.ks), (v, c.vs)):
-        by = scale[page, :, at][:, :, None, None] * (1 + 2.0 ** -20 * torch.randint(-9, 9, (12, heads, 1, 1), generator=gen).cuda())
+        nudge = torch.randint(-9, 9, (12, heads, 1, 1), generator=gen).cuda()
+        by = scale[page, :, at][:, :, None, None] * (1 + 2.0 ** -20 * nudge)
         scale[page, :, at] = by[:, :, 0, 0]
         half = (torch.arange(new * d, device="cuda").reshape(new, d) % 100 + 0.5) * by
         t[:6, :, :new] = half[:6].to(dtype)
