@@ -15,8 +15,9 @@
 //    the row's largest value. The slot's scale multiplies the sum;
 //  * O^T += V^T P^T on the fp16 matrix cores: the transposing LDS read of bytes brings 8
 //    slots of a value's dimension, and a code c becomes fp16 exactly, as the last bits of
-//    1024 + (c + 128) less 1152. The weights carry the slots' scales, relative to a power of
-//    two R not below any the wave has seen, and are split in two fp16 numbers;
+//    1024 + (c + 128) less 1152. The weights carry the slots' scales, in units of a power of
+//    two that follows the largest of those products (not the largest scale, whose slot may
+//    weigh nothing), and are split in two fp16 numbers;
 //  * a group of up to 4 (8) query heads leaves 12 (8) of a product's 16 columns empty. They
 //    get the same queries again, and each set of columns goes on with a quarter (half) of
 //    the tile's slots: the softmax is done once for every score. In the product with V a
@@ -97,8 +98,14 @@ __device__ __forceinline__ Digits digits4(const float* x, float scale) {
           (int)(__builtin_amdgcn_perm(b, a, 0x05040100u) ^ 0x80808080u)};
 }
 
-// 1 / x of a power of two, 2^-126 .. 2^126.
-__device__ __forceinline__ float inverse(float x) { return __uint_as_float((254u << 23) - __float_as_uint(x)); }
+// Two weights x, y of 0 .. 2^15 as a + b in fp16: 21 bits of each, and nothing below 2^-25. (b may
+// be 0, as codes are finite: no product of it needs to show.)
+__device__ __forceinline__ void split2(float x, float y, int& a, int& b) {
+  typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+  const f16x2 h = __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_pkrtz(x, y));
+  a = __builtin_bit_cast(int, h);
+  b = (int)pack_f16x2(x - (float)h[0], y - (float)h[1]);
+}
 
 // op over the sets of a group of 16 lanes, in each.
 template <int SETS, class Op> __device__ __forceinline__ float over_sets(float v, Op op) {
@@ -176,7 +183,12 @@ __global__ __launch_bounds__(64 * kWaves, NT == 1 && kTile == 32 ? 3 : 2) void d
 #pragma unroll
       for (int d = 0; d < DT; ++d) o[t][d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     }
-    float R = 0x1p-126f;             // o is in units of it
+    // A slot's product of weight and scale is held in units of 2^unit_o: the largest so far is 2^11
+    // .. 2^15 of them, whatever larger scales the slots without weight have. m is a whole number:
+    // where it rises, the weights' unit falls by a power of two, and o stays as it is.
+    int unit_o[NT];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) unit_o[t] = -4096;
 
     float ksr, vsr;                  // the scales of the lane's slot
     uint64_t live;                   // the tile's slots that are there
@@ -270,21 +282,9 @@ __global__ __launch_bounds__(64 * kWaves, NT == 1 && kTile == 32 ? 3 : 2) void d
     while (key < end) {
       wait_all();
       const uint64_t mask = live;
-      if (__ballot(!(vsr <= R))) {
-        const uint32_t top = __float_as_uint(fmaxf(wave_max(vsr), 0.0f));
-        const float up = __uint_as_float(min((top + 0x7fffffu) & 0x7f800000u, 0x7e800000u));
-        if (up > R) {
-          const float f = R * inverse(up);
-          R = up;
-#pragma unroll
-          for (int t = 0; t < NT; ++t)
-#pragma unroll
-            for (int d = 0; d < DT; ++d) o[t][d] *= f;
-        }
-      }
       if (lane < kTile) {
         scales[wave][0][lane] = ksr;
-        scales[wave][1][lane] = vsr * inverse(R);
+        scales[wave][1][lane] = vsr;
       }
       // The tile into registers; then its place takes the next one.
       i32x4 kf[KT][F];
@@ -357,27 +357,38 @@ __global__ __launch_bounds__(64 * kWaves, NT == 1 && kTile == 32 ? 3 : 2) void d
         mx = fmaxf(mx, kLowest);     // -inf scores weigh 0; a row of only such has l = 0 and is NaN
         const bool raise = mx - m[t] > kLazy;
         if (__ballot(raise)) {
-          const float top = raise ? mx : m[t];
-          const float alpha = raise ? __builtin_amdgcn_exp2f(m[t] - top) : 1.0f;
+          const float top = raise ? ceilf(mx) : m[t], drop = raise ? m[t] - top : 0.0f;
           m[t] = top;
-          l[t] *= alpha;
-#pragma unroll
-          for (int d = 0; d < DT; ++d) o[t][d] *= alpha;
+          l[t] *= __builtin_amdgcn_exp2f(drop);
+          unit_o[t] = max(unit_o[t] + (int)fmaxf(drop, -1024.0f), -4096);
         }
-        int hi[MT][2], lo[MT][2];
+        float most = 0.0f;
 #pragma unroll
         for (int k = 0; k < MT; ++k) {
           const f32x4 by = *(const f32x4*)&scales[wave][1][16 * (set * MT + k) + 4 * g];
-          float w[4];
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            w[r] = __builtin_amdgcn_exp2f((s[k][r] - m[t]) + W::kTop);
-            l[t] += w[r];
-            w[r] *= by[r];
+            const float w = __builtin_amdgcn_exp2f((s[k][r] - m[t]) + W::kTop);
+            l[t] += w;
+            s[k][r] = w * by[r];
+            most = fmaxf(most, s[k][r]);
           }
-#pragma unroll
-          for (int x = 0; x < 2; ++x) W::split2(w[2 * x], w[2 * x + 1], hi[k][x], lo[k][x]);
         }
+        if (__ballot(most > ldexpf(0x1p15f, unit_o[t]))) {
+          most = over_sets<SETS>(most, [](float a, float x) { return fmaxf(a, x); });
+          most = over_query(most, [](float a, float x) { return fmaxf(a, x); });
+          const int up = max(unit_o[t], (int)(__float_as_uint(most) >> 23) - 127 - 11);
+          const float f = ldexpf(1.0f, unit_o[t] - up);
+          unit_o[t] = up;
+#pragma unroll
+          for (int d = 0; d < DT; ++d) o[t][d] *= f;
+        }
+        int hi[MT][2], lo[MT][2];
+#pragma unroll
+        for (int k = 0; k < MT; ++k)
+#pragma unroll
+          for (int x = 0; x < 2; ++x)
+            split2(ldexpf(s[k][2 * x], -unit_o[t]), ldexpf(s[k][2 * x + 1], -unit_o[t]), hi[k][x], lo[k][x]);
 #pragma unroll
         for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
@@ -407,16 +418,16 @@ __global__ __launch_bounds__(64 * kWaves, NT == 1 && kTile == 32 ? 3 : 2) void d
     const bool whole = take == n;
     const int64_t part = p.whole ? share : (int64_t)b * p.items + it + share;
     float* mo = (float*)smem;
-    const float back = R * kUnscale;
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
       wait_all();
       __syncthreads();               // every wave is done with its tiles, or with the rows before
 #pragma unroll
       for (int d = 0; d < DT; ++d) {
-        f32x4 x = o[t][d] * back;
+        f32x4 x;
 #pragma unroll
-        for (int r = 0; r < 4; ++r) x[r] = over_sets<SETS>(x[r], [](float a, float y) { return a + y; });
+        for (int r = 0; r < 4; ++r)
+          x[r] = over_sets<SETS>(ldexpf(o[t][d][r], unit_o[t] - 11), [](float a, float y) { return a + y; });
         *(f32x4*)&mo[(wave * 16 + l16) * kPitch + 16 * d + 4 * g] = x;
       }
       const float sum = over_query(over_sets<SETS>(l[t], [](float a, float x) { return a + x; }),

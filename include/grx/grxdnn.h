@@ -422,9 +422,11 @@ grxdnnStatus_t grxdnnPagedCacheReadQuantized(grxdnnHandle_t handle,
  * without weights, with the slots' codes times their scales for keys and values.
  * q, o: [B, H, 1, D], GRX_R_16BF or GRX_R_16F; its rules and limits hold. A query's row is
  * taken to 2^-22 of its largest value (or to 2^-127), products with the codes are
- * exact, scores, softmax and sums fp32, the weights of the values keep 21 bits, and o is
- * rounded once. A row of q with NaN or infinities in it gives NaN, and so does a head
- * of a sequence with a scale of NaN among its slots' blocks. Values' scales up to 2^95.
+ * exact, scores, softmax and sums fp32 (a weight below 2^-126 of the largest counts as 0). A
+ * weight times its slot's scale of a value keeps 21 bits, or 2^-36 of the query's largest such
+ * product where that is more, and o is rounded once. A row of q with NaN or infinities in
+ * it gives NaN, and so does a head of a sequence with a scale of NaN among its slots'
+ * blocks. Values' scales up to 2^95.
  * workspace: as there, of grxdnnPagedAttentionQuantizedGetWorkspaceSize. */
 grxdnnStatus_t grxdnnPagedAttentionQuantizedGetWorkspaceSize(grxdnnHandle_t handle,
                                                              grxdnnTensorDescriptor_t qDesc,

@@ -300,3 +300,64 @@ def test_appended_rows_are_attended(dnn):
     append(dnn, c, k, v, ints([190, 77]))
     c.n, c.lengths = [190, 77], ints([190, 77])
     check(dnn, c, query(gen, 2, 4, 64, F16), 0.125)
+
+
+def weighed_ref(q, K, V, vs, scale):
+    """attention_ref with the weights held to what they are said to keep: a weight times its slot's
+    scale of a value, 21 bits, or half of fp16's least, 2^-25, where the largest such product of
+    the query has 2^11 or more: 2^-36 of that. vs [heads, n]: the slots' scales of values."""
+    H, d = q.shape
+    group = H // K.shape[0]
+    k, v, vs = (x.repeat_interleave(group, 0) for x in (K, V, vs.double()))
+    q64 = q.double()
+    p = torch.softmax(torch.matmul(k, q64[:, :, None])[..., 0] * scale, 1)
+    o = torch.matmul(p[:, None], v)[:, 0]
+    size = torch.matmul(k.abs(), q64.abs()[:, :, None])[..., 0]
+    off = 2.0 ** -22 * q64.abs().amax(1, keepdim=True) * k.abs().sum(2)
+    delta = (off + 8 * 2.0 ** -24 * size).amax(1, keepdim=True) * scale
+    rel = 2 * delta + 2.0 ** -18 + 2.0 ** -21
+    u = {BF16: 2.0 ** -8, F16: 2.0 ** -11}[q.dtype]
+    mass = torch.matmul(p[:, None], v.abs())[:, 0]
+    floor = k.shape[1] * 2.0 ** -36 * 127 * (p * vs).amax(1, keepdim=True)
+    return o, u * o.abs() + (1 + u) * (rel * mass + floor) + {BF16: 2.0 ** -134, F16: 2.0 ** -25}[q.dtype]
+
+
+def check_weighed(dnn, gen, dtype, d, H, heads, n, special, log_scale, ratios, block, what):
+    """The slots of `special` (multiples of block) have scores 26 below the others' (weights of
+    about 2^-37) and values 2^ratio times as large; a sequence to each ratio."""
+    b = len(ratios)
+    c = QuantCache(gen, [n] * b, heads, block, block, d, True, quick=True)
+    q = query(gen, b, H, d, dtype, 0.25)
+    q[..., 0] = 4.0
+    scales = torch.full((b, heads, n), 2.0 ** log_scale)
+    for i, ratio in enumerate(ratios):
+        at = torch.arange(n, device="cuda")
+        page, row = c.table[i, at // block].long(), at % block
+        c.ks[page] = 1.0 / 39
+        c.vs[page] = 2.0 ** log_scale
+        c.k[page, :, row, 0] = 127
+        odd = at[special[0]:special[1]]
+        c.k[c.table[i, odd // block].long(), :, odd % block, 0] = -127
+        c.vs[c.table[i, odd // block].long()] = 2.0 ** (log_scale + ratio)
+        scales[i, :, special[0]:special[1]] = 2.0 ** (log_scale + ratio)
+    o = torch.full_like(q, math.nan)
+    say(what)
+    attend(dnn, c, q, o, 1.0)
+    for i, ratio in enumerate(ratios):
+        K, V, _ = c.rows(i)
+        ref, bound = weighed_ref(q[i, :, 0].cpu(), K, V, scales[i], 1.0)
+        assert (bound < 0.02 * ref.abs().amax(1, keepdim=True)).all(), "a bound that holds nothing"
+        off = (o[i, :, 0].cpu().double() - ref).abs() - bound
+        assert not (off > 0).any(), f"{what}, 2^{ratio}: {off.max().item():.3g} past the bound"
+
+
+@pytest.mark.parametrize("H,heads,n", [(4, 1, 320), (8, 1, 320), (16, 1, 320), (33, 1, 320), (4, 1, 1600), (16, 2, 1600),
+                                       (13, 1, 1600), (64, 2, 1600)])
+@pytest.mark.parametrize("special", [(0, 16), (144, 160), (304, 320)])
+def test_values_of_little_weight_and_large_scale(dnn, H, heads, n, special):
+    """Whatever a slot's scale, o is made of what its slots weigh: from nothing to all of it."""
+    gen = torch.Generator().manual_seed(20)
+    for dtype, log_scale, ratios in ((BF16, -8, (10, 20, 25, 30, 34, 37, 40, 50, 70)), (F16, -6, (15, 25, 30, 34, 37, 40)),
+                                     (BF16, -100, (-20, 30, 60))):
+        check_weighed(dnn, gen, dtype, 128 if n > 1000 else 64, H, heads, n, special, log_scale, ratios, 16,
+                      f"values of little weight {dtype} {H} on {heads} heads, {n} slots, {special}, 2^{log_scale}")
