@@ -480,3 +480,21 @@ def test_rows_far_apart(dnn):
     outs = (far.as_strided(q.shape, wide, 1024 * 1024), far.as_strided(k.shape, wide, 1024 * 1024 + 256))
     c.forward(dnn, *outs)
     assert torch.equal(outs[0], yq) and torch.equal(outs[1], yk)
+
+
+@pytest.mark.parametrize("args", [CASES[i] for i in (1, 5, 11, 12, 13, 14)] + [c for c in LARGE if c[8]])
+def test_the_gains_gradients_hold_every_row(dnn, args):
+    """The sums over rows by their real depth: a lane adds 15 rows at most in these calls, then its
+    row's lanes (4 steps), the waves (3), and of up to 768 workgroups' parts 12 to a lane, two
+    steps over lanes, 15 over waves: 51 roundings of what is summed, where 64 are allowed. A
+    wave's rows, a 3072nd of them, make six times that or more of a difference."""
+    say(f"qk_norm_rope, gains {args}")
+    c = Case(600, *args)
+    angle = angles(c.positions.cpu(), c.freq.cpu())
+    gains = [torch.full((c.d,), math.nan, device="cuda") for _ in range(1 + (c.hk > 0))]
+    c.backward(dnn, torch.empty_like(c.q), torch.empty_like(c.k), gains[0], gains[1] if c.hk else None)
+    for got, (x, gain, dy) in zip(gains, c.sides()):
+        _, _, want, mass = backward_ref(x.cpu(), gain.cpu(), dy.cpu(), c.eps, angle, c.pairs, c.rotary)
+        bound = mass[0] * (mass[1] + 64 * F32)
+        within(got, want, bound, str(args))
+        assert bound.max() < 0.05 * want.abs().median()
