@@ -209,3 +209,11 @@ def test_refused_attention_calls(dnn):
     assert ask(dnn.h, None, pool.d, table.d, ctypes.byref(out)) == INVALID
     assert ask(dnn.h, T(BF16, [3, 6, 1, 64]).d, pool.d, table.d, ctypes.byref(out)) == INVALID
     assert ask(dnn.h, q.d, T(BF16, POOL).d, table.d, ctypes.byref(out)) == UNSUPPORTED
+
+
+def test_misaligned_attention_pointers(dnn):
+    """With room for 128 slots, where no workspace is needed and its alignment is not looked at."""
+    assert dnn.paged_attention_quantized_workspace(T(BF16, [3, 8, 1, 64]), T(I8, POOL), T(I32, TABLE)) == 0
+    for n in ("q", "kc", "vc", "o"):
+        for off in (2, 8):
+            assert attend(dnn, **{n: at(20) + off}) == UNSUPPORTED, (n, off)
