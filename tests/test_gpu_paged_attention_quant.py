@@ -361,3 +361,114 @@ def test_values_of_little_weight_and_large_scale(dnn, H, heads, n, special):
                                      (BF16, -100, (-20, 30, 60))):
         check_weighed(dnn, gen, dtype, 128 if n > 1000 else 64, H, heads, n, special, log_scale, ratios, 16,
                       f"values of little weight {dtype} {H} on {heads} heads, {n} slots, {special}, 2^{log_scale}")
+
+
+@pytest.mark.parametrize("dtype,b,H,heads,d,room,tokmajor,kernel", [
+    (BF16, 3, 8, 2, 64, 256, True, "whole1"),          # groups of 4, and so on
+    (F16, 20, 39, 3, 128, 500, False, "whole1"),       # 13
+    (BF16, 5, 42, 2, 128, 500, True, "whole1"),        # 21
+    (F16, 3, 70, 2, 64, 500, True, "whole1"),          # 35
+    (BF16, 3, 8, 2, 128, 1040, True, "split1"),        # 4
+    (F16, 20, 28, 4, 128, 1040, False, "split1"),      # 7
+    (BF16, 20, 36, 4, 64, 1040, False, "split1"),      # 9
+    (F16, 3, 32, 2, 128, 1200, True, "split1"),        # 16
+    (BF16, 2, 66, 2, 128, 1040, True, "split1"),       # 33
+    (F16, 40, 6, 6, 128, 1040, True, "split2"),        # 1
+    (BF16, 40, 30, 6, 64, 1040, True, "split2"),       # 5
+    (F16, 40, 72, 6, 128, 1040, True, "split2"),       # 12
+    (BF16, 40, 80, 2, 64, 1040, True, "split2"),       # 40
+    (BF16, 64, 16, 4, 128, 1040, True, "split4"),      # 4
+    (F16, 64, 32, 4, 64, 1040, True, "split4"),        # 8
+    (BF16, 64, 52, 4, 128, 1040, True, "split4"),      # 13
+    (F16, 64, 80, 4, 128, 1040, True, "split4"),       # 20
+    (F16, 40, 132, 4, 64, 1040, True, "split4"),       # 33
+])
+def test_every_kernel_choice(dnn, capfd, monkeypatch, dtype, b, H, heads, d, room, tokmajor, kernel):
+    """The choice that GRXDNN_LOG names, on ragged lengths from none to the room's."""
+    gen = torch.Generator().manual_seed(21)
+    lengths = [0, 1, room] + torch.randint(0, room + 1, (max(0, b - 3),), generator=gen).tolist()
+    c = QuantCache(gen, lengths[:b], heads, 20 if room % 20 == 0 else 16, 4, d, tokmajor, room=room, quick=True)
+    state = c.state()
+    c.state = lambda: state
+    capfd.readouterr()
+    monkeypatch.setenv("GRXDNN_LOG", "1")
+    check(dnn, c, query(gen, b, H, d, dtype, 2.0), d ** -0.5)
+    monkeypatch.delenv("GRXDNN_LOG")
+    log = [x for x in capfd.readouterr().err.splitlines() if x.startswith("grxdnn: paged attention i8 ")]
+    assert len(log) == 1 and log[0].endswith(f"kernel={kernel}"), log
+
+
+def test_the_same_bits_whatever_the_workspace_held(dnn):
+    """And, within the bound, the same next to other sequences as alone (where the work is
+    shared otherwise)."""
+    gen = torch.Generator().manual_seed(22)
+    c = QuantCache(gen, [3000, 10, 700], 2, 16, 16, 128, True, quick=True)
+    q = query(gen, 3, 8, 128, BF16)
+    args, qd, ad = c.args(), desc(q), g.AttnDesc(True, 0.1)
+    runs = []
+    for fill in (0, 0xFF, 0x7F):
+        o = torch.full_like(q, math.nan)
+        ws = Workspace(dnn.paged_attention_quantized_workspace(qd, args[0], args[7]))
+        ws.t.fill_(fill)
+        torch.cuda.synchronize()
+        g.check(dnn.paged_attention_quantized(ad, qd, q.data_ptr(), *args, qd, o.data_ptr(), ws.p, ws.size))
+        torch.cuda.synchronize()
+        runs.append(o)
+    assert torch.equal(runs[0], runs[1]) and torch.equal(runs[0], runs[2])
+    table, n = c.table, c.n
+    for i in range(3):
+        c.table, c.lengths, c.n = table[i:i + 1], ints(n[i:i + 1]), n[i:i + 1]
+        alone = check(dnn, c, q[i:i + 1].clone(), 0.1)
+        K, V, _ = c.rows(0)
+        ref, bound = attention_ref(q[i, :, 0].cpu(), K, V, 0.1)
+        assert ((runs[0][i, :, 0].cpu().double() - ref).abs() <= bound).all(), i
+        assert ((runs[0][i, :, 0] - alone[0, :, 0]).cpu().double().abs() <= 2 * bound).all(), i
+
+
+def test_captured_steps_with_new_rows(gpu):
+    """As test_captured_steps, with other keys, values and queries at every replay."""
+    dnn = g.Dnn()
+    caches = []
+    for _ in range(2):
+        gen = torch.Generator().manual_seed(23)
+        caches.append(QuantCache(gen, [30, 0, 700], 2, 16, 16, 128, True, room=1100))
+    gen = torch.Generator().manual_seed(24)
+    k, v, q = (torch.empty((3, h, 1, 128), dtype=F16, device="cuda") for h in (2, 2, 8))
+    kd, qd = desc(k), desc(q)
+    outs = [torch.zeros_like(q) for _ in range(2)]
+    args = [c.args() for c in caches]
+    ws = Workspace(dnn.paged_attention_quantized_workspace(qd, args[0][0], args[0][7]))
+    ad = g.AttnDesc(True, 128 ** -0.5)
+
+    def calls(i):
+        g.check(dnn.paged_append_quantized(kd, k.data_ptr(), kd, v.data_ptr(), *args[i]))
+        caches[i].lengths.add_(1)
+        g.check(dnn.paged_attention_quantized(ad, qd, q.data_ptr(), *args[i], qd, outs[i].data_ptr(), ws.p, ws.size))
+
+    graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    say("capturing append8 and attention, new rows")
+    with torch.cuda.graph(graph, stream=side):
+        dnn.set_stream(torch.cuda.current_stream().cuda_stream)
+        calls(1)
+    dnn.set_stream(None)
+    seen = []
+    for step in range(20):
+        for t in (k, v, q):
+            t.copy_(torch.randn(t.shape, generator=gen).mul(1.0 + 0.2 * step))
+        calls(0)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(*outs), f"replay {step}"
+        seen.append(outs[0].clone())
+        assert all(not torch.equal(outs[0], x) for x in seen[:-1])
+    caches[1].check(caches[0].state())
+    c = caches[0]
+    c.n = [n + 20 for n in c.n]
+    for i in range(3):
+        K, V, _ = c.rows(i)
+        ref, bound = attention_ref(q[i, :, 0].cpu(), K, V, 128 ** -0.5)
+        assert ((outs[1][i, :, 0].cpu().double() - ref).abs() <= bound).all(), i
+    del graph
+    dnn.close()
