@@ -116,6 +116,13 @@ __device__ __forceinline__ uint32_t wave_upto(uint32_t v) {
   return dpp_add<0x143, 0xc>(v);   // row_bcast 31
 }
 
+// A wave's LDS writes before this are there for its reads after it, whatever lane they are of (no
+// instruction: a wave's LDS accesses are done in order; the compiler is to keep it).
+__device__ __forceinline__ void wave_fence() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront", "local");
+  __builtin_amdgcn_wave_barrier();
+}
+
 // ---- cycle probe -------------------------------------------------------------
 // One grxCycleSlot per wave, written by lane 0 with an ordinary (vector)
 // global store. `core` = XCD id << 16 | CU-level hardware id bits, so slots

@@ -217,7 +217,7 @@ __global__ __launch_bounds__(64 * kWaves, NT == 1 && kTile == 32 ? 3 : 2) void d
         ksr = qp.ks[at];
         vsr = qp.vs[at];
       }
-      __builtin_amdgcn_wave_barrier();
+      wave_fence();
 #pragma unroll
       for (int x = 0; x < kTile / RPI; ++x) {
         const int r = RPI * x + lane / CH;
@@ -286,6 +286,7 @@ __global__ __launch_bounds__(64 * kWaves, NT == 1 && kTile == 32 ? 3 : 2) void d
         scales[wave][0][lane] = ksr;
         scales[wave][1][lane] = vsr;
       }
+      wave_fence();
       // The tile into registers; then its place takes the next one.
       i32x4 kf[KT][F];
 #pragma unroll

@@ -175,7 +175,7 @@ __global__ __launch_bounds__(kThreads, BWD ? 3 : 1) void qk_norm_rope(RParams p)
 #pragma unroll
       for (int k = 0; k < PC; ++k) chunks[k / W][k % W] = w[k / W][k % W];
     }
-    __builtin_amdgcn_wave_barrier();
+    wave_fence();
     if (in) {
 #pragma unroll
       for (int k = 0; k < PC; ++k) w[k / W][k % W] = chunks[k / W][k % W];
@@ -183,7 +183,7 @@ __global__ __launch_bounds__(kThreads, BWD ? 3 : 1) void qk_norm_rope(RParams p)
 #pragma unroll
       for (int k = 0; k < PC; ++k) w[k / W][k % W] = lines[64 * k];
     }
-    __builtin_amdgcn_wave_barrier();
+    wave_fence();
   };
   float acc[2][8];
 #pragma unroll
