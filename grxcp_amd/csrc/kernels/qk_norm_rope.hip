@@ -307,8 +307,8 @@ __global__ __launch_bounds__(kThreads, BWD ? 3 : 1) void qk_norm_rope(RParams p)
             if (norm)
 #pragma unroll
               for (int i = 0; i < 8; ++i) {
-                v[0][i] *= inv * gam[0][i];
-                v[1][i] *= inv * gam[1][i];
+                v[0][i] = v[0][i] * inv * gam[0][i];   // (inv * gam may be past fp32)
+                v[1][i] = v[1][i] * inv * gam[1][i];
               }
           if constexpr (PAIRS) {
 #pragma unroll

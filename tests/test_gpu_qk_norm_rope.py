@@ -498,3 +498,12 @@ def test_the_gains_gradients_hold_every_row(dnn, args):
         bound = mass[0] * (mass[1] + 64 * F32)
         within(got, want, bound, str(args))
         assert bound.max() < 0.05 * want.abs().median()
+
+
+def test_small_rows_with_large_gains(dnn):
+    """Gains whose product with 1 / root lies past fp32's range, either way, where y does not."""
+    for scale, gain in ((2.0 ** -60, 2.0 ** 75), (2.0 ** 55, 2.0 ** -85)):
+        c = Case(31, FP32, 1, 9, 3, 2, 128, 64, False, True, packed=False, scale=scale, eps=0.0)
+        for t in (c.qg, c.kg):
+            t.mul_(gain)
+        check_forward(dnn, c, f"rows of {scale}, gains of {gain}")
