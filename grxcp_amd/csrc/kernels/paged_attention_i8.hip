@@ -6,7 +6,8 @@
 //
 // The work is divided as over a cache of 16 bits (paged_attention.hip): units of a tile for
 // each of a workgroup's four waves, shares of equal size, parts joined in the order of the
-// slots. Half the bytes, so a wave's tile has 64 slots where the work is shared, 16 KB of codes again. What differs:
+// slots. Half the bytes, so a wave's tile has 64 slots where the work is shared, 16 KB of codes
+// again. What differs:
 //
 //  * scores are S^T = K Q^T on the 8-bit matrix cores (v_mfma_i32_16x16x64_i8): the codes of
 //    K go in as they lie, with no conversion. A query's row is held as whole numbers of 23

@@ -31,7 +31,9 @@ struct Pool8 {
   int64_t sp, sh, ss;
   float* scale;
   int64_t cp, ch, cb;
-  __device__ __forceinline__ uint8_t* row(int page, int h, int slot) const { return p + page * sp + h * sh + slot * ss; }
+  __device__ __forceinline__ uint8_t* row(int page, int h, int slot) const {
+    return p + page * sp + h * sh + slot * ss;
+  }
   __device__ __forceinline__ float* scale_of(int page, int h, int block) const {
     return scale + page * cp + h * ch + block * cb;
   }
@@ -90,7 +92,8 @@ __device__ __forceinline__ uint32_t codes4(const float* x, Inverse r) {
 #pragma unroll
   for (int i = 0; i < 4; ++i)
     w[i] = __float_as_uint(fmaf(x[i], r.lo, 12582912.0f) + fmaf(x[i], r.hi, 12582912.0f));
-  const uint32_t lo = __builtin_amdgcn_perm(w[1], w[0], 0x0c0c0400u), hi = __builtin_amdgcn_perm(w[3], w[2], 0x0c0c0400u);
+  const uint32_t lo = __builtin_amdgcn_perm(w[1], w[0], 0x0c0c0400u);
+  const uint32_t hi = __builtin_amdgcn_perm(w[3], w[2], 0x0c0c0400u);
   return lo | hi << 16;
 }
 
@@ -128,10 +131,11 @@ template <int L> __device__ __forceinline__ uint32_t lanes_max(uint32_t v) {
 // One task: the block of one head's keys or values (blockIdx.z) that gets new rows, by L
 // threads with N chunks of 8 values each, held in registers between the maximum and the
 // codes: read once. The threads take M tasks at a time. Rows that the block already holds are
-// rounded again, to the new scale, where that is larger. us, 8 sequences of 500 to 4000 tokens of 8 heads of 128, blocks of 32:
-// 22.4 (4.9 TB/s; stores through the caches 1.6 more, registers for eight waves a SIMD, which
-// the loads then wait in turn for, 3.2), bound by memory with the VALU at work in 47 % of the
-// cycles; one token of 64 sequences 5.5, a launch and the chain of length, table entry and rows.
+// rounded again, to the new scale, where that is larger. us, 8 sequences of 500 to 4000 tokens
+// of 8 heads of 128, blocks of 32: 22.4 (4.9 TB/s; stores through the caches 1.6 more,
+// registers for eight waves a SIMD, which the loads then wait in turn for, 3.2), bound by memory
+// with the VALU at work in 47 % of the cycles; one token of 64 sequences 5.5, a launch and the
+// chain of length, table entry and rows.
 template <NormType T, int C, int L, int N, int M, bool STREAM>   // C: chunks of a row
 __global__ __launch_bounds__(kThreads, 4) void append_i8(AppendParams p) {
   constexpr int P = kThreads / L;
@@ -326,8 +330,10 @@ struct ReadParams {
 // 8 codes times their scale s, to memory; as fp32 the second four lie C pieces of 16 bytes behind
 // the first, so that the threads of a row write neighbouring ones; `odd`: some of a wave's
 // products may lie past the type's range, where they are its largest value, or s may be no number.
-template <NormType T> constexpr float kMost = T == NormType::F16 ? 65504.0f : T == NormType::BF16 ? 0x1.fep127f : __FLT_MAX__;
-template <NormType T, int C, bool STREAM> __device__ __forceinline__ void put8(uint8_t* to, u32x2 w, float s, bool odd) {
+template <NormType T>
+constexpr float kMost = T == NormType::F16 ? 65504.0f : T == NormType::BF16 ? 0x1.fep127f : __FLT_MAX__;
+template <NormType T, int C, bool STREAM>
+__device__ __forceinline__ void put8(uint8_t* to, u32x2 w, float s, bool odd) {
   float f[8];
 #pragma unroll
   for (int e = 0; e < 8; ++e) f[e] = (float)(int8_t)(w[e / 4] >> 8 * (e % 4)) * s;

@@ -201,40 +201,41 @@ __device__ __forceinline__ void meet(const DParams& p, int tid, int of, int hg, 
                                      int64_t part, bool whole, const float* mo, const float (*ml)[2][16]) {
   using IO = PIo<T>;
   constexpr int kPitch = D + 4;
-        constexpr int E = D / 16;      // values of a thread, of 16 to a row
-        const int r = tid >> 4, d0 = (tid & 15) * E;
-        const int row = row0 + r;      // in the tile
-        if (q0 + row >= p.group) return;
-        for (int y = 0; y < p.hw; ++y) {
-          float top = -INFINITY;
-          for (int x = y * of; x < (y + 1) * of; ++x) top = fmaxf(top, ml[x][0][r]);
-          float lsum = 0.0f, acc[E];
-  #pragma unroll
-          for (int e = 0; e < E; ++e) acc[e] = 0.0f;
-          for (int x = y * of; x < (y + 1) * of; ++x) {
-            const float f = __builtin_amdgcn_exp2f(ml[x][0][r] - fmaxf(top, kLowest));
-            lsum = fmaf(f, ml[x][1][r], lsum);
-  #pragma unroll
-            for (int e = 0; e < E; ++e) acc[e] = fmaf(f, mo[(x * 16 + r) * kPitch + d0 + e], acc[e]);
-          }
-          const int64_t at = (part * p.hw + y) * p.rows + row;
-          if (whole) {
-            const float inv = top == -INFINITY ? 0.0f : 1.0f / lsum;   // no slot: 0; only -inf scores: 0 * inf
-            uint32_t out[E / 2];
-  #pragma unroll
-            for (int e = 0; e < E / 2; ++e) out[e] = IO::pack2(acc[2 * e] * inv, acc[2 * e + 1] * inv);
-            uint8_t* to = p.o + (int64_t)b * p.o_sb + ((hg * p.hw + y) * p.group + q0 + row) * p.o_sh + 2 * d0;
-            if constexpr (E == 8) *(u32x4*)to = u32x4{out[0], out[1], out[2], out[3]};
-            else *(u32x2*)to = u32x2{out[0], out[1]};
-          } else {
-  #pragma unroll
-            for (int e = 0; e < E; e += 4) *(f32x4*)(p.po + at * D + d0 + e) = f32x4{acc[e], acc[e + 1], acc[e + 2], acc[e + 3]};
-          }
-          if (d0 == 0 && (!whole || p.scores)) {
-            p.ml[2 * at] = top;
-            p.ml[2 * at + 1] = lsum;
-          }
-        }
+  constexpr int E = D / 16;      // values of a thread, of 16 to a row
+  const int r = tid >> 4, d0 = (tid & 15) * E;
+  const int row = row0 + r;      // in the tile
+  if (q0 + row >= p.group) return;
+  for (int y = 0; y < p.hw; ++y) {
+    float top = -INFINITY;
+    for (int x = y * of; x < (y + 1) * of; ++x) top = fmaxf(top, ml[x][0][r]);
+    float lsum = 0.0f, acc[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) acc[e] = 0.0f;
+    for (int x = y * of; x < (y + 1) * of; ++x) {
+      const float f = __builtin_amdgcn_exp2f(ml[x][0][r] - fmaxf(top, kLowest));
+      lsum = fmaf(f, ml[x][1][r], lsum);
+#pragma unroll
+      for (int e = 0; e < E; ++e) acc[e] = fmaf(f, mo[(x * 16 + r) * kPitch + d0 + e], acc[e]);
+    }
+    const int64_t at = (part * p.hw + y) * p.rows + row;
+    if (whole) {
+      const float inv = top == -INFINITY ? 0.0f : 1.0f / lsum;   // no slot: 0; only -inf scores: 0 * inf
+      uint32_t out[E / 2];
+#pragma unroll
+      for (int e = 0; e < E / 2; ++e) out[e] = IO::pack2(acc[2 * e] * inv, acc[2 * e + 1] * inv);
+      uint8_t* to = p.o + (int64_t)b * p.o_sb + ((hg * p.hw + y) * p.group + q0 + row) * p.o_sh + 2 * d0;
+      if constexpr (E == 8) *(u32x4*)to = u32x4{out[0], out[1], out[2], out[3]};
+      else *(u32x2*)to = u32x2{out[0], out[1]};
+    } else {
+#pragma unroll
+      for (int e = 0; e < E; e += 4)
+        *(f32x4*)(p.po + at * D + d0 + e) = f32x4{acc[e], acc[e + 1], acc[e + 2], acc[e + 3]};
+    }
+    if (d0 == 0 && (!whole || p.scores)) {
+      p.ml[2 * at] = top;
+      p.ml[2 * at + 1] = lsum;
+    }
+  }
 }
 
 // ---- the join ------------------------------------------------------------------
@@ -244,7 +245,8 @@ struct Parts {
   int64_t first;
   int count;
 };
-__device__ __forceinline__ Parts parts_of(const DParams& p, const Shares& sh, uint32_t before, uint32_t n, int b, int it) {
+__device__ __forceinline__ Parts parts_of(const DParams& p, const Shares& sh, uint32_t before, uint32_t n, int b,
+                                          int it) {
   const int64_t item = (int64_t)b * p.items + it;
   if (p.whole) return {item, 1};
   const uint32_t u = before + it * n, w0 = sh.of(u), w1 = sh.of(u + n - 1);

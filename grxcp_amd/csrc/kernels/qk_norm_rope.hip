@@ -486,7 +486,8 @@ template <NormType T, int D> hipError_t run(const QkRopeDesc& d, bool bwd, hipSt
   p.S = d.S;
   p.by_s = page_div(std::max(1, d.S));
   p.tokens = d.B * d.S;
-  const RopePlan r = p.tokens && d.heads[0] + d.heads[1] ? plan_of(p.tokens, d.heads[0], d.heads[1], D, bwd) : RopePlan{};
+  const RopePlan r =
+      p.tokens && d.heads[0] + d.heads[1] ? plan_of(p.tokens, d.heads[0], d.heads[1], D, bwd) : RopePlan{};
   p.group[0] = r.group[0];
   p.group[1] = r.group[1];
   p.partial = bwd && gains ? (float*)d.ws : nullptr;
