@@ -135,7 +135,9 @@ template <int L> __device__ __forceinline__ uint32_t lanes_max(uint32_t v) {
 // of 8 heads of 128, blocks of 32: 22.4 (4.9 TB/s; stores through the caches 1.6 more,
 // registers for eight waves a SIMD, which the loads then wait in turn for, 3.2), bound by memory
 // with the VALU at work in 47 % of the cycles; one token of 64 sequences 5.5, a launch and the
-// chain of length, table entry and rows.
+// chain of length, table entry and rows. Where every block's scale grows rows are loaded,
+// rounded and stored one after the other: one token of 64 sequences without / with, blocks of
+// 16 4.7 / 4.9, of 64 5.6 / 6.1, of 256 8.9 / 12.3.
 template <NormType T, int C, int L, int N, int M, bool STREAM>   // C: chunks of a row
 __global__ __launch_bounds__(kThreads, 4) void append_i8(AppendParams p) {
   constexpr int P = kThreads / L;

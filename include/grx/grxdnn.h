@@ -388,6 +388,8 @@ grxdnnStatus_t grxdnnPagedCacheEvict(grxdnnHandle_t handle,
  * behind the new ones are left as they are.
  * Slots of a block that another sequence shares must not be followed by rows of this
  * call (they would be rounded again): share whole blocks.
+ * A block that two written table entries name may hold codes of one and the scale of
+ * another: what it reads as is none of the values written.
  * k, v: [B, Hkv, T, D], GRX_R_16BF or GRX_R_16F, counts as in grxdnnPagedCacheAppend;
  * (T + 512) * Hkv below 2^31. Scales that the caller sets are finite and >= 0. */
 grxdnnStatus_t grxdnnPagedCacheAppendQuantized(grxdnnHandle_t handle,
@@ -406,8 +408,8 @@ grxdnnStatus_t grxdnnPagedCacheAppendQuantized(grxdnnHandle_t handle,
  * first: B ints (below 0 counts as 0), or NULL for 0 each. k, v: [B, Hkv, T, D] of
  * GRX_R_16BF, GRX_R_16F or GRX_R_32F, strides multiples of 16 bytes, T * Hkv at most
  * 2^31 - 4096; rounded once; what is past the type's range comes back as its largest
- * value. For grxdnnAttentionForward over a whole prompt, or to go on in a cache of 16
- * bits (grxdnnPagedCacheAppend), which eviction needs. */
+ * value. To go on in a cache of 16 bits (grxdnnPagedCacheAppend), which eviction needs, or
+ * for grxdnnAttentionForward over a whole prompt (as many heads and tokens as queries). */
 grxdnnStatus_t grxdnnPagedCacheReadQuantized(grxdnnHandle_t handle,
                                              grxdnnTensorDescriptor_t kCacheDesc, const void* kCache,
                                              grxdnnTensorDescriptor_t vCacheDesc, const void* vCache,
